@@ -135,7 +135,7 @@ def _parameters(case):
         for c in (width, width // 2, width // 4):
             tensors += [(c * c // 2, True), (9 * c * c // 2, True), (c, False), (c, False), (255 * c, True), (255, False)] * 3
         return tensors
-    return [((width + 7 * i) * (i % 5 + 1) ** 2 if i % 3 else width + i, i % 3 != 0) for i in range(blocks)]
+    return [((width + 7 * i) * (i % 5 + 1) ** 2 | 1 if i % 3 else width + i, i % 3 != 0) for i in range(blocks)]
 
 
 def _arena(case):
