@@ -96,7 +96,7 @@ def draw(rng):
     common = dict(kind=kind, model=model, bits=bits, gradients=gradients, copies=rng.random() < 0.5, max_norm=rng.choice([0.0, 0.5, 1.0]))
     if model == "tokens":
         width = _size(rng, 128, 1024, 80)
-        return dict(common, blocks=rng.randint(1, 12), width=width, wide=rng.choice([2, 4]) * width, vocab=_size(rng, 1000, 32768, 80))
+        return dict(common, blocks=rng.randint(1, 7), width=width, wide=rng.choice([2, 4]) * width, vocab=_size(rng, 1000, 32768, 80))
     if model == "detector":
         return dict(common, blocks=rng.randint(3, 23), width=rng.choice([256, 512, 1024]), wide=0, vocab=0)
     return dict(common, blocks=_log_int(rng, 2, 400), width=_log_int(rng, 9, 400), wide=0, vocab=0)
