@@ -38,6 +38,10 @@ enum pxh_activation {
     PXH_RELU, PXH_SOFTPLUS, PXH_SWISH, PXH_TANH
 };
 
+/* Types of values in memory, where an entry point takes `type` and void pointers: fp32, bfloat16, IEEE half, and the
+ * 8-bit e4m3 (4 exponent bits with bias 7, 3 mantissa bits, no infinities, largest value 448). */
+enum pxh_type { PXH_F32 = 0, PXH_BF16, PXH_F16, PXH_E4M3 };
+
 const char* pxh_last_error(void);
 /* library version, bumped when a signature changes or a declaration leaves this header
  * (2: the test hooks moved to a private header; the tensor tables, the norm-from-the-writer entry
@@ -591,6 +595,44 @@ int pxh_sgd_update_table(const pxh_tensor_table* table, int batch, float lr, flo
 int pxh_fill_f32_table(const pxh_tensor_table* table, float value, void* stream);
 int pxh_rescale_clip_table(const pxh_tensor_table* table, float threshold, float clip, float* norms,
                            void* stream);
+
+/* ------------------------------------------------------------------------
+ * Layers of token models: what stands between the matrix products of a network over tokens.  No counterpart in the
+ * reference, whose networks are convolutional; the products are not part of this library.
+ *
+ * Tensors here are rows of values of one type (pxh_type), the values of a row next to each other and the rows `*_stride`
+ * values apart (>= the row's length; 0 rows: nothing to do).  Nothing has to be aligned beyond its own values.  Sums,
+ * statistics and intermediate values are fp32; a result is rounded once, to nearest even, when it is stored.  As everywhere in
+ * this header what a backward pass leaves is ADDED to the parameters by the optimiser: hand in the gradient of what is to
+ * grow (a log likelihood).
+ * ---------------------------------------------------------------------- */
+
+/* Root-mean-square norm over the rows, with the residual's addition in front of it:
+ *   h = x + residual, rounded to `type` (h = x without one);  rstd = 1 / sqrt(mean(h^2) + eps);  y = h * rstd * weight
+ * residual, sum (receives h; only with a residual), scales and rstd are nullable.  weight holds `width` values of
+ * weight_type: `type` or PXH_F32.  y_type is `type`, or PXH_E4M3 with scales: `group` consecutive values of a row (128, or 0
+ * for the whole row; the last group of a row may be shorter) share
+ *   scale = max(largest |y| of the group / 448, 2^-126),  and y holds e4m3(y / scale);
+ * scales is [rows][width / group, rounded up], packed.  sum may be x or residual itself, and y (of `type`) may be x, residual or
+ * none of the others, where the strides are the same.  An infinity in a row makes its rstd 0 and the infinite values NaN, a NaN the
+ * whole row NaN, as the formulas have it. */
+int pxh_rms_norm_forward(const void* x, const void* residual, void* sum, const void* weight, void* y, float* scales,
+                         float* rstd, int type, int weight_type, int y_type, long long rows, int width, long long x_stride,
+                         long long residual_stride, long long sum_stride, long long y_stride, int group, float eps,
+                         void* stream);
+
+/* Its gradients, from h (the sum if there was a residual) and the forward's rstd:
+ *   c = mean(dy * weight * h * rstd) over the row;  dx = rstd * (dy * weight - h * rstd * c) + dsum;
+ *   dw (+)= sum over the rows of dy * h * rstd
+ * dsum (nullable) is what arrives along the residual stream; dx is then the gradient of x and of the residual alike.  dx may be dy
+ * or dsum where the strides are the same.  dw[width] is fp32, overwritten (accumulate == 0) or added to; it is summed in a fixed
+ * order.  workspace: pxh_rms_norm_workspace_bytes(rows, width), which serves fewer rows and shorter rows too, or NULL for the
+ * library's. */
+size_t pxh_rms_norm_workspace_bytes(long long rows, int width);
+int pxh_rms_norm_backward(const void* dy, const void* h, const void* weight, const float* rstd, const void* dsum, void* dx,
+                          float* dw, int type, int weight_type, long long rows, int width, long long dy_stride,
+                          long long h_stride, long long dsum_stride, long long dx_stride, int accumulate, void* workspace,
+                          size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -83,6 +83,8 @@ SIGNATURES = {
     "pxh_sgd_update_table": [P, I, F, F, F, P],
     "pxh_fill_f32_table": [P, F, P],
     "pxh_rescale_clip_table": [P, F, F, P, P],
+    "pxh_rms_norm_forward": [P, P, P, P, P, P, P, I, I, I, L, I, L, L, L, L, I, F, P],
+    "pxh_rms_norm_backward": [P, P, P, P, P, P, P, I, I, L, I, L, L, L, L, I, P, Z, P],
 }
 _OTHER_RETURNS = {
     "pxh_last_error": (ctypes.c_char_p, []),
@@ -98,6 +100,7 @@ _OTHER_RETURNS = {
     "pxh_nms_workspace_bytes": (Z, [I]),
     "pxh_reserve_workspace": (I, [Z]),
     "pxh_tensor_table_destroy": (None, [P]),
+    "pxh_rms_norm_workspace_bytes": (Z, [L, I]),
 }
 # test hooks (pixienn_amd/csrc/pixienn_hip_test.h): exported, but not part of the C ABI
 _TEST_HOOKS = {

@@ -1,0 +1,494 @@
+// Root-mean-square norm over rows, with the residual's addition in front of it and 8-bit results, and its gradients.
+#include "typed.h"
+
+namespace pxh {
+namespace {
+
+// ---------------------------------------------------------------- forward
+//   h = x + residual (rounded as it is kept);  rstd = 1 / sqrt(mean(h^2) + eps);  y = h * rstd * weight
+struct NormArgs {
+    const void* x;
+    const void* residual;
+    void* sum;
+    const void* weight;
+    void* y;
+    float* scales;
+    float* rstd;
+    long long rows, x_stride, residual_stride, sum_stride, y_stride;
+    int width, group;
+    bool weight_f32;
+    float eps;
+};
+
+// Rows of one launch: a grid has fewer than 2^32 work items.
+constexpr long long kLaunchRows = 1 << 21;
+
+template<int T>
+__host__ __device__ __forceinline__ const char* row_of(const void* p, long long row, long long stride)
+{
+    return static_cast<const char*>(p) + row * stride * kSize<T>;
+}
+
+template<int T>
+__host__ __device__ __forceinline__ char* row_of(void* p, long long row, long long stride)
+{
+    return static_cast<char*>(p) + row * stride * kSize<T>;
+}
+
+// V weights from column e on; zeros behind the last one.
+template<int T, int V>
+__device__ __forceinline__ void weights_at(const void* weight, bool f32, int e, int width, float (&w)[V])
+{
+    if (f32 && T != PXH_F32) {
+#pragma unroll
+        for (int q = 0; q < V; q += 4) {
+            float part[4];
+            load_row<PXH_F32, 4>(weight, e + q, width).get(part);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[q + k] = part[k];
+        }
+    } else {
+        load_row<T, V>(weight, e, width).get(w);
+    }
+}
+
+// The largest value among the lanes that hold one group of 128 values: 16 lanes of 8 values or 32 of 4.
+template<int V>
+__device__ __forceinline__ float scale_group_max(float v)
+{
+    v = fmaxf(v, lane_in_row<0xB1>(v));
+    v = fmaxf(v, lane_in_row<0x4E>(v));
+    v = fmaxf(v, lane_in_row<0x141>(v));
+    v = fmaxf(v, lane_in_row<0x140>(v));
+    if constexpr (V == 4) v = fmaxf(v, __shfl_xor(v, 16, kWave));
+    return v;
+}
+
+constexpr float kE4m3Max = 448.0f;
+constexpr float kLeastScale = 0x1p-126f;        // its reciprocal is finite, and a row of zeros has zeros
+
+__device__ __forceinline__ float scale_of(float peak) { return fmaxf(peak * (1.0f / kE4m3Max), kLeastScale); }
+
+// Four values no larger than 448 by more than a rounding: the conversion rounds to nearest even and leaves NaN.
+__device__ __forceinline__ uint32_t e4m3_of(float a, float b, float c, float d)
+{
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+    return static_cast<uint32_t>(w);
+}
+
+// V 8-bit values at column e of a row of n.
+template<int V>
+__device__ __forceinline__ void store_e4m3(char* y, int e, int n, const float (&q)[V])
+{
+    uint32_t w[V / 4];
+#pragma unroll
+    for (int k = 0; k < V / 4; ++k) w[k] = e4m3_of(q[4 * k], q[4 * k + 1], q[4 * k + 2], q[4 * k + 3]);
+    if (e + V <= n) {
+        typedef uint32_t words __attribute__((ext_vector_type(V / 4), aligned(1)));
+        *reinterpret_cast<words*>(y + e) = __builtin_bit_cast(words, w);
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+        if (e + k < n) y[e + k] = static_cast<char>(w[k / 4] >> (8 * (k & 3)));
+}
+
+// The values of a row are walked in vectors, lane by lane; K vectors per lane are kept in registers between the sum and
+// the result (K == 0: any width, the row is read again).
+template<int T, bool EIGHT, int LANES, int K>
+__global__ __launch_bounds__(LANES > kBlock ? LANES : kBlock) void rms_norm_kernel(NormArgs a)
+{
+    constexpr int V = kVec<T>;
+    constexpr int kRows = LANES < kBlock ? kBlock / LANES : 1;      // rows per workgroup, a wave each if several
+    __shared__ float slots[LANES / kWave + 1];
+    const int lane = threadIdx.x % LANES;
+    const long long row = static_cast<long long>(blockIdx.x) * kRows + threadIdx.x / LANES;
+    if (row >= a.rows) return;                                       // whole waves, and only where nothing is waited for
+    const char* x = row_of<T>(a.x, row, a.x_stride);
+    const char* residual = a.residual ? row_of<T>(a.residual, row, a.residual_stride) : nullptr;
+    char* sum = a.sum ? row_of<T>(a.sum, row, a.sum_stride) : nullptr;
+    const int n = a.width;
+    const int steps = K ? K : (n + LANES * V - 1) / (LANES * V);
+    constexpr int kUnroll = K ? K : 1;
+
+    const auto read = [&](int e, bool again) {
+        if (again && sum) return load_row<T, V>(sum, e, n);         // x may have been overwritten by it
+        Raw<T, V> h = load_row<T, V>(x, e, n);
+        if (residual) {
+            float p[V], q[V];
+            h.get(p);
+            load_row<T, V>(residual, e, n).get(q);
+#pragma unroll
+            for (int k = 0; k < V; ++k) p[k] += q[k];
+            h.set(p);
+        }
+        return h;
+    };
+
+    Raw<T, V> kept[K ? K : 1];
+    float squares = 0.0f, peak = 0.0f;
+#pragma unroll kUnroll
+    for (int s = 0; s < steps; ++s) {
+        const int e = (s * LANES + lane) * V;
+        if (e >= n) break;
+        const Raw<T, V> r = read(e, false);
+        float h[V];
+        r.get(h);
+#pragma unroll
+        for (int k = 0; k < V; ++k) squares = fmaf(h[k], h[k], squares);
+        if (EIGHT && a.group == 0) {
+            float w[V];
+            weights_at<T, V>(a.weight, a.weight_f32, e, n, w);
+#pragma unroll
+            for (int k = 0; k < V; ++k) peak = fmaxf(peak, fabsf(h[k] * w[k]));
+        }
+        if (sum) store_row<T, V>(sum, e, n, r);
+        if constexpr (K > 0) kept[s] = r;
+    }
+    squares = group_sum<LANES>(squares, slots);
+    const float rstd = 1.0f / sqrtf(squares / static_cast<float>(n) + a.eps);
+    if (a.rstd && lane == 0) a.rstd[row] = rstd;
+    float scale = 1.0f;
+    if (EIGHT && a.group == 0) {
+        scale = scale_of(group_max<LANES>(peak, slots) * rstd);
+        if (lane == 0) a.scales[row] = scale;
+    }
+    const int groups = (n + 127) / 128;
+#pragma unroll kUnroll
+    for (int s = 0; s < steps; ++s) {
+        const int e = (s * LANES + lane) * V;
+        // with a scale per group all lanes of a wave go on together
+        if (s * LANES * V + lane / kWave * kWave * V >= n) break;
+        float h[V] = {}, w[V] = {};
+        if (e < n) {
+            if constexpr (K > 0) kept[s].get(h);
+            else read(e, true).get(h);
+            weights_at<T, V>(a.weight, a.weight_f32, e, n, w);
+        }
+        float y[V];
+#pragma unroll
+        for (int k = 0; k < V; ++k) y[k] = h[k] * rstd * w[k];
+        if constexpr (EIGHT) {
+            if (a.group) {
+                float most = 0.0f;
+#pragma unroll
+                for (int k = 0; k < V; ++k) most = fmaxf(most, fabsf(y[k]));
+                scale = scale_of(scale_group_max<V>(most));
+                if (e % 128 == 0 && e < n) a.scales[row * groups + e / 128] = scale;
+            }
+            const float inverse = 1.0f / scale;
+#pragma unroll
+            for (int k = 0; k < V; ++k) y[k] *= inverse;
+            if (e < n) store_e4m3<V>(static_cast<char*>(a.y) + row * a.y_stride, e, n, y);
+        } else {
+            Raw<T, V> r;
+            r.set(y);
+            if (e < n) store_row<T, V>(row_of<T>(a.y, row, a.y_stride), e, n, r);
+        }
+    }
+}
+
+template<int T, bool EIGHT, int LANES, int K>
+int launch_norm(const NormArgs& a, hipStream_t s)
+{
+    constexpr int kRows = LANES < kBlock ? kBlock / LANES : 1;
+    for (long long done = 0; done < a.rows; done += kLaunchRows) {
+        NormArgs part = a;
+        part.x = row_of<T>(a.x, done, a.x_stride);
+        part.residual = a.residual ? row_of<T>(a.residual, done, a.residual_stride) : nullptr;
+        part.sum = a.sum ? row_of<T>(a.sum, done, a.sum_stride) : nullptr;
+        part.y = static_cast<char*>(a.y) + done * a.y_stride * (EIGHT ? 1 : kSize<T>);
+        part.scales = a.scales + (EIGHT ? done * (a.group ? (a.width + 127) / 128 : 1) : 0);
+        part.rstd = a.rstd ? a.rstd + done : nullptr;
+        part.rows = a.rows - done < kLaunchRows ? a.rows - done : kLaunchRows;
+        hipLaunchKernelGGL((rms_norm_kernel<T, EIGHT, LANES, K>), dim3(grid_for(part.rows, kRows)),
+                           dim3(LANES < kBlock ? kBlock : LANES), 0, s, part);
+        if (int rc = check_launch("pxh_rms_norm_forward")) return rc;
+    }
+    return PXH_OK;
+}
+
+template<int T, bool EIGHT>
+int norm_forward(const NormArgs& a, hipStream_t s)
+{
+    const int vectors = (a.width + kVec<T> - 1) / kVec<T>;
+    if (vectors <= 64) return launch_norm<T, EIGHT, 64, 1>(a, s);
+    if (vectors <= 256) return launch_norm<T, EIGHT, 256, 1>(a, s);
+    if (vectors <= 1024) return launch_norm<T, EIGHT, 256, 4>(a, s);
+    if (vectors <= 4096) return launch_norm<T, EIGHT, 1024, 4>(a, s);
+    return launch_norm<T, EIGHT, 1024, 0>(a, s);
+}
+
+// ---------------------------------------------------------------- backward
+struct NormBackwardArgs {
+    const void* dy;
+    const void* h;
+    const void* weight;
+    const float* rstd;
+    const void* dsum;
+    void* dx;
+    float* partial;         // [workers][width]
+    long long rows, dy_stride, h_stride, dsum_stride, dx_stride;
+    int width;
+    bool weight_f32;
+};
+
+// dx of every row, and the part of dw that this worker's rows give: a worker (LANES lanes) takes every workers-th row.
+template<int T, int LANES, int K>
+__global__ __launch_bounds__(LANES > kBlock ? LANES : kBlock) void rms_norm_backward_kernel(NormBackwardArgs a, int workers)
+{
+    constexpr int V = kVec<T>;
+    constexpr int kPer = LANES < kBlock ? kBlock / LANES : 1;
+    __shared__ float slots[LANES / kWave + 1];
+    const int lane = threadIdx.x % LANES;
+    const int worker = blockIdx.x * kPer + threadIdx.x / LANES;
+    if (worker >= workers) return;
+    const int n = a.width;
+    float w[K][V], dw[K][V];
+#pragma unroll
+    for (int s = 0; s < K; ++s) {
+        const int e = (s * LANES + lane) * V;
+#pragma unroll
+        for (int k = 0; k < V; ++k) dw[s][k] = w[s][k] = 0.0f;
+        if (e < n) weights_at<T, V>(a.weight, a.weight_f32, e, n, w[s]);
+    }
+    for (long long row = worker; row < a.rows; row += workers) {
+        const char* dy = row_of<T>(a.dy, row, a.dy_stride);
+        const char* h = row_of<T>(a.h, row, a.h_stride);
+        const float rstd = a.rstd[row];
+        Raw<T, V> rg[K], rh[K];
+        float dot = 0.0f;
+#pragma unroll
+        for (int s = 0; s < K; ++s) {
+            const int e = (s * LANES + lane) * V;
+            if (e >= n) break;
+            rg[s] = load_row<T, V>(dy, e, n);
+            rh[s] = load_row<T, V>(h, e, n);
+        }
+#pragma unroll
+        for (int s = 0; s < K; ++s) {
+            const int e = (s * LANES + lane) * V;
+            if (e >= n) break;
+            float g[V], x[V];
+            rg[s].get(g);
+            rh[s].get(x);
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const float xhat = x[k] * rstd;
+                dw[s][k] = fmaf(g[k], xhat, dw[s][k]);
+                dot = fmaf(g[k] * w[s][k], xhat, dot);
+            }
+        }
+        const float c = group_sum<LANES>(dot, slots) / static_cast<float>(n);
+#pragma unroll
+        for (int s = 0; s < K; ++s) {
+            const int e = (s * LANES + lane) * V;
+            if (e >= n) break;
+            float g[V], x[V], more[V] = {};
+            rg[s].get(g);
+            rh[s].get(x);
+            if (a.dsum) load_row<T, V>(row_of<T>(a.dsum, row, a.dsum_stride), e, n).get(more);
+#pragma unroll
+            for (int k = 0; k < V; ++k) g[k] = fmaf(rstd, g[k] * w[s][k] - x[k] * rstd * c, more[k]);
+            Raw<T, V> r;
+            r.set(g);
+            store_row<T, V>(row_of<T>(a.dx, row, a.dx_stride), e, n, r);
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < K; ++s) {
+        const int e = (s * LANES + lane) * V;
+#pragma unroll
+        for (int k = 0; k < V; ++k)
+            if (e + k < n) a.partial[static_cast<size_t>(worker) * n + e + k] = dw[s][k];
+    }
+}
+
+// Rows of any width: dx alone, the row is read twice.
+template<int T>
+__global__ __launch_bounds__(1024) void rms_norm_backward_wide_kernel(NormBackwardArgs a, long long first)
+{
+    constexpr int V = kVec<T>;
+    __shared__ float slots[1024 / kWave];
+    const int n = a.width;
+    const long long row = first + blockIdx.x;
+    const char* dy = row_of<T>(a.dy, row, a.dy_stride);
+    const char* h = row_of<T>(a.h, row, a.h_stride);
+    const float rstd = a.rstd[row];
+    float dot = 0.0f;
+    for (int e = threadIdx.x * V; e < n; e += 1024 * V) {
+        float g[V], x[V], w[V];
+        load_row<T, V>(dy, e, n).get(g);
+        load_row<T, V>(h, e, n).get(x);
+        weights_at<T, V>(a.weight, a.weight_f32, e, n, w);
+#pragma unroll
+        for (int k = 0; k < V; ++k) dot = fmaf(g[k] * w[k], x[k] * rstd, dot);
+    }
+    const float c = group_sum<1024>(dot, slots) / static_cast<float>(n);
+    for (int e = threadIdx.x * V; e < n; e += 1024 * V) {
+        float g[V], x[V], w[V], more[V] = {};
+        load_row<T, V>(dy, e, n).get(g);
+        load_row<T, V>(h, e, n).get(x);
+        weights_at<T, V>(a.weight, a.weight_f32, e, n, w);
+        if (a.dsum) load_row<T, V>(row_of<T>(a.dsum, row, a.dsum_stride), e, n).get(more);
+#pragma unroll
+        for (int k = 0; k < V; ++k) g[k] = fmaf(rstd, g[k] * w[k] - x[k] * rstd * c, more[k]);
+        Raw<T, V> r;
+        r.set(g);
+        store_row<T, V>(row_of<T>(a.dx, row, a.dx_stride), e, n, r);
+    }
+}
+
+// ... and the parts of dw, one column to a lane, before dx (which may be dy itself) is written.
+template<int T>
+__global__ __launch_bounds__(kBlock) void rms_norm_wide_dw_kernel(NormBackwardArgs a, int workers)
+{
+    const int e = blockIdx.x * kBlock + threadIdx.x;
+    if (e >= a.width) return;
+    float dw = 0.0f;
+    for (long long row = blockIdx.y; row < a.rows; row += workers)
+        dw = fmaf(load_one<T>(row_of<T>(a.dy, row, a.dy_stride), e), load_one<T>(row_of<T>(a.h, row, a.h_stride), e) * a.rstd[row], dw);
+    a.partial[static_cast<size_t>(blockIdx.y) * a.width + e] = dw;
+}
+
+// dw[column] (+)= the sum of the workers' parts.
+__global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const float* partial, int workers, int width, float* dw, int accumulate)
+{
+    __shared__ float sums[16][kWave];
+    const int column = blockIdx.x * kWave + threadIdx.x % kWave, part = threadIdx.x / kWave;
+    float sum = 0.0f;
+    if (column < width)
+        for (int w = part; w < workers; w += 16) sum += partial[static_cast<size_t>(w) * width + column];
+    sums[part][threadIdx.x % kWave] = sum;
+    __syncthreads();
+    if (part == 0 && column < width) {
+        float total = accumulate ? dw[column] : 0.0f;
+        float all = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) all += sums[k][threadIdx.x];
+        dw[column] = total + all;
+    }
+}
+
+// Workers that share the rows of the backward pass, each with a row of partial sums: fewer for wide rows, so that the
+// partial sums stay small beside the tensors.
+constexpr int kWideWorkers = 32;
+int workers_for(long long rows, int width)
+{
+    const int most = width <= 16384 ? 1024 : width <= 32768 ? 256 : kWideWorkers;
+    return static_cast<int>(rows < most ? rows : most);
+}
+
+template<int T, int LANES, int K>
+int launch_backward(const NormBackwardArgs& a, int workers, hipStream_t s)
+{
+    constexpr int kPer = LANES < kBlock ? kBlock / LANES : 1;
+    hipLaunchKernelGGL((rms_norm_backward_kernel<T, LANES, K>), dim3(grid_for(workers, kPer)), dim3(LANES < kBlock ? kBlock : LANES), 0, s, a, workers);
+    return check_launch("pxh_rms_norm_backward");
+}
+
+template<int T>
+int norm_backward(const NormBackwardArgs& a, int& workers, hipStream_t s)
+{
+    const int vectors = (a.width + kVec<T> - 1) / kVec<T>;
+    if (vectors <= 64) return launch_backward<T, 64, 1>(a, workers, s);
+    if (vectors <= 256) return launch_backward<T, 256, 1>(a, workers, s);
+    if (vectors <= 512) return launch_backward<T, 256, 2>(a, workers, s);
+    if (vectors <= 1024) return launch_backward<T, 512, 2>(a, workers, s);
+    if (vectors <= 4096) return launch_backward<T, 1024, 4>(a, workers, s);
+    if (workers > kWideWorkers) workers = kWideWorkers;
+    hipLaunchKernelGGL((rms_norm_wide_dw_kernel<T>), dim3(grid_for(a.width, kBlock), workers), dim3(kBlock), 0, s, a, workers);
+    if (int rc = check_launch("pxh_rms_norm_backward")) return rc;
+    for (long long done = 0; done < a.rows; done += kLaunchRows) {
+        const long long rows = a.rows - done < kLaunchRows ? a.rows - done : kLaunchRows;
+        hipLaunchKernelGGL((rms_norm_backward_wide_kernel<T>), dim3(static_cast<unsigned>(rows)), dim3(1024), 0, s, a, done);
+        if (int rc = check_launch("pxh_rms_norm_backward")) return rc;
+    }
+    return PXH_OK;
+}
+
+// What the two entry points refuse alike.
+int check_rows(const char* who, int type, int weight_type, long long rows, int width)
+{
+    if (type != PXH_F32 && type != PXH_BF16 && type != PXH_F16) return fail_invalid("%s: type %d is not fp32, bf16 or half", who, type);
+    if (weight_type != type && weight_type != PXH_F32)
+        return fail_invalid("%s: the weights are of the tensors' type or fp32 (got type %d)", who, weight_type);
+    if (rows < 0 || rows > 0x7fffffffll) return fail_invalid("%s: %lld rows", who, rows);
+    if (width <= 0 || width > 1 << 30) return fail_invalid("%s: rows of %d values", who, width);
+    return PXH_OK;
+}
+
+}  // namespace
+}  // namespace pxh
+
+using namespace pxh;
+
+extern "C" {
+
+int pxh_rms_norm_forward(const void* x, const void* residual, void* sum, const void* weight, void* y, float* scales,
+                         float* rstd, int type, int weight_type, int y_type, long long rows, int width, long long x_stride,
+                         long long residual_stride, long long sum_stride, long long y_stride, int group, float eps, void* stream)
+{
+    const char* who = "pxh_rms_norm_forward";
+    if (int rc = check_rows(who, type, weight_type, rows, width)) return rc;
+    const bool eight = y_type == PXH_E4M3;
+    if (!eight && y_type != type) return fail_invalid("%s: y is of the type of x or e4m3 (got type %d)", who, y_type);
+    if (group != 0 && group != 128) return fail_invalid("%s: a scale for 128 values or, with 0, for a row (got %d)", who, group);
+    if (sum && !residual) return fail_invalid("%s: a sum without a residual", who);
+    if (!(eps >= 0.0f)) return fail_invalid("%s: eps %g", who, static_cast<double>(eps));
+    if (rows == 0) return PXH_OK;
+    if (!x || !weight || !y) return fail_invalid("%s: null pointer", who);
+    if (eight && !scales) return fail_invalid("%s: 8-bit values without scales", who);
+    if (x_stride < width || y_stride < width || (residual && residual_stride < width) || (sum && sum_stride < width))
+        return fail_invalid("%s: rows of %d values that overlap", who, width);
+    const NormArgs a{ x, residual, sum, weight, y, scales, rstd, rows, x_stride, residual_stride, sum_stride, y_stride, width, group,
+                      weight_type == PXH_F32, eps };
+    int rc = PXH_OK;
+    dispatch_type(type, [&]<int T>() { rc = eight ? norm_forward<T, true>(a, as_stream(stream)) : norm_forward<T, false>(a, as_stream(stream)); });
+    return rc;
+}
+
+size_t pxh_rms_norm_workspace_bytes(long long rows, int width)
+{
+    if (rows <= 0 || width <= 0) return 0;
+    // the largest that any of the shapes up to this one takes
+    size_t most = 0;
+    for (int w: { 16384, 32768, width }) {
+        const int here = width < w ? width : w;
+        const size_t floats = static_cast<size_t>(workers_for(rows, here)) * static_cast<size_t>(here);
+        if (floats > most) most = floats;
+    }
+    return most * sizeof(float);
+}
+
+int pxh_rms_norm_backward(const void* dy, const void* h, const void* weight, const float* rstd, const void* dsum, void* dx,
+                          float* dw, int type, int weight_type, long long rows, int width, long long dy_stride,
+                          long long h_stride, long long dsum_stride, long long dx_stride, int accumulate, void* workspace,
+                          size_t workspace_bytes, void* stream)
+{
+    const char* who = "pxh_rms_norm_backward";
+    if (int rc = check_rows(who, type, weight_type, rows, width)) return rc;
+    if (!dw) return fail_invalid("%s: null pointer", who);
+    hipStream_t s = as_stream(stream);
+    if (rows > 0) {
+        if (!dy || !h || !weight || !rstd || !dx) return fail_invalid("%s: null pointer", who);
+        if (dy_stride < width || h_stride < width || dx_stride < width || (dsum && dsum_stride < width))
+            return fail_invalid("%s: rows of %d values that overlap", who, width);
+    }
+    int workers = rows > 0 ? workers_for(rows, width) : 0;
+    void* ws = nullptr;
+    if (rows > 0)
+        if (int rc = resolve_workspace(workspace, workspace_bytes, pxh_rms_norm_workspace_bytes(rows, width), &ws, s)) return rc;
+    const NormBackwardArgs a{ dy, h, weight, rstd, dsum, dx, static_cast<float*>(ws), rows, dy_stride, h_stride, dsum_stride, dx_stride,
+                              width, weight_type == PXH_F32 };
+    int rc = PXH_OK;
+    if (rows > 0) dispatch_type(type, [&]<int T>() { rc = norm_backward<T>(a, workers, s); });
+    if (rc) return rc;
+    // without rows the sum over them is zero
+    if (workers == 0 && accumulate) return PXH_OK;
+    hipLaunchKernelGGL(rms_norm_dw_kernel, dim3(grid_for(width, kWave)), dim3(1024), 0, s, a.partial, workers, width, dw, accumulate);
+    return check_launch(who);
+}
+
+}

@@ -619,6 +619,98 @@ def rescale_clip_from_groups(x, groups, threshold=0.0, clip=0.0, norm_out=None):
          None, 0, _stream())
 
 
+# ---------------------------------------------------------------- layers of token models
+# Types of values, as pxh_type numbers them.
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_E4M3 = torch.float8_e4m3fn
+
+
+def _rows(t, name):
+    """(rows, values of a row, values from row to row) of a tensor on the device: two dimensions, of which the last is
+    packed, or any number of packed ones, the leading ones being the rows."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        _chk(t, getattr(t, "dtype", None), name)
+    shape = t.shape
+    if len(shape) == 2:
+        rows, width = shape
+        stride, step = t.stride()
+        if step != 1 and width > 1:
+            raise PxError("%s must have the values of a row next to each other" % name)
+        return rows, width, stride if rows > 1 else max(stride, width)
+    if len(shape) == 0 or not t.is_contiguous():
+        raise PxError("%s must have two dimensions or be contiguous" % name)
+    width = shape[-1]
+    return (t.numel() // width if width else 0), width, width
+
+
+def _like(t, name, shape, dtype):
+    """The row stride of a further tensor of a call: of the shape and type that the first one has."""
+    if t is None:
+        return 0
+    stride = _rows(t, name)[2]
+    if t.shape != shape or t.dtype is not dtype:
+        raise PxError("%s must be %s of shape %s (got %s of %s)" % (name, dtype, tuple(shape), t.dtype, tuple(t.shape)))
+    return stride
+
+
+def _type(t, name):
+    kind = _TYPES.get(t.dtype)
+    if kind is None:
+        raise PxError("%s must be fp32, bfloat16 or half (got %s)" % (name, t.dtype))
+    return kind
+
+
+def _vector(t, name, n, dtype=None):
+    """A packed tensor of n values, or None."""
+    if t is None:
+        return
+    if dtype is not None or not isinstance(t, torch.Tensor) or not t.is_cuda or not t.is_contiguous():
+        _chk(t, dtype or getattr(t, "dtype", None), name)
+    if t.numel() != n:
+        raise PxError("%s must hold %d values (got %d)" % (name, n, t.numel()))
+
+
+def _bytes(workspace):
+    return 0 if workspace is None else workspace.numel() * workspace.element_size()
+
+
+def rms_norm_forward(x, y, weight, residual=None, sum=None, scales=None, rstd=None, eps=1e-6, group=0):
+    """y = h / sqrt(mean(h^2) + eps) * weight over the last dimension, h = x + residual (rounded to x's type; kept in `sum`).
+    y is of x's type, or float8_e4m3fn with `scales` [rows, 1] (group 0) or [rows, width / 128 rounded up] (group 128): the
+    value is scale * y.  rstd [rows] is what the backward pass needs."""
+    rows, width, x_stride = _rows(x, "x")
+    kind = _type(x, "x")
+    eight = _tensor(y).dtype is _E4M3
+    y_stride = _like(y, "y", x.shape, _E4M3 if eight else x.dtype)
+    _vector(weight, "weight", width)
+    if eight:
+        _vector(scales, "scales", rows * (-(-width // 128) if group else 1))
+    if rstd is not None:
+        _vector(rstd, "rstd", rows)
+    _run("pxh_rms_norm_forward", x.data_ptr(), ptr(residual), ptr(sum), weight.data_ptr(), y.data_ptr(), scales if eight else None,
+         rstd, kind, _type(weight, "weight"), 3 if eight else kind, rows, width, x_stride,
+         _like(residual, "residual", x.shape, x.dtype), _like(sum, "sum", x.shape, x.dtype), y_stride, group, float(eps))
+    return y
+
+
+def rms_norm_workspace_bytes(rows, width):
+    return int(capi.load().pxh_rms_norm_workspace_bytes(rows, width))
+
+
+def rms_norm_backward(dy, h, weight, rstd, dx, dw, dsum=None, accumulate=False, workspace=None):
+    """The gradients of rms_norm_forward from h (its `sum`, or x without a residual) and its rstd: dx of x and residual alike,
+    with dsum, what arrives along the residual stream, added; dw (fp32) overwritten or added to."""
+    rows, width, dy_stride = _rows(dy, "dy")
+    kind = _type(dy, "dy")
+    _vector(weight, "weight", width)
+    _vector(rstd, "rstd", rows)
+    _vector(dw, "dw", width)
+    _run("pxh_rms_norm_backward", dy.data_ptr(), ptr(h), weight.data_ptr(), rstd, ptr(dsum), ptr(dx), dw, kind,
+         _type(weight, "weight"), rows, width, dy_stride, _like(h, "h", dy.shape, dy.dtype), _like(dsum, "dsum", dy.shape, dy.dtype),
+         _like(dx, "dx", dy.shape, dy.dtype), int(bool(accumulate)), ptr(workspace), _bytes(workspace))
+    return dx
+
+
 DETECTION_DTYPE = workloads.DETECTION_DTYPE
 
 
