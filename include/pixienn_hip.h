@@ -634,6 +634,41 @@ int pxh_rms_norm_backward(const void* dy, const void* h, const void* weight, con
                           long long h_stride, long long dsum_stride, long long dx_stride, int accumulate, void* workspace,
                           size_t workspace_bytes, void* stream);
 
+/* Log probabilities of given tokens, entropy, and the most probable alternatives, one row of logits per token:
+ *   z = scale * logits;  lse = log sum exp z;  logp = z[target] - lse;  entropy = lse - sum softmax(z) * z
+ * targets: [rows], int32 (wide_targets == 0) or int64; one outside [0, vocab) gives a logp of 0 (a place at which nothing is to
+ * be learned).  targets and logp are given together or not at all; entropy and lse are nullable.  scale > 0.
+ * top_logp, top_ids [rows][top]: the `top` largest z (at most PXH_MOST_ALTERNATIVES, and vocab), descending, among equal ones the
+ * lowest index first; top == 0: none.  A logit of minus infinity has probability 0, and one of the type's lowest value is a number as
+ * any other.  A row of nothing but minus infinities has lse and logp minus infinity, entropy 0; one with a NaN or plus infinity
+ * has NaN in all three, and its NaNs come last among the alternatives.
+ * workspace: pxh_token_logprobs_workspace_bytes(rows, vocab, top), which serves fewer rows, fewer alternatives and smaller
+ * vocabularies too, or NULL for the library's. */
+#define PXH_MOST_ALTERNATIVES 64
+size_t pxh_token_logprobs_workspace_bytes(long long rows, int vocab, int top);
+int pxh_token_logprobs_forward(const void* logits, const void* targets, float* logp, float* entropy, float* lse,
+                               float* top_logp, int* top_ids, int type, int wide_targets, long long rows, int vocab,
+                               long long stride, int top, float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The gradient of the logits for gradients of logp and entropy (each nullable: none), from the forward's lse, and its entropy where
+ * d_entropy is given:
+ *   dlogits[j] = scale * (d_logp * ((j == target) - p[j]) - d_entropy * p[j] * (log p[j] + entropy)),  p = exp(z - lse)
+ * A row whose target is outside [0, vocab) has no gradient of logp; a row of nothing but minus infinities has zeros.  dlogits, of the
+ * logits' type, may be the logits themselves (with the same stride).  lse is taken as it is, rounded to fp32: its rounding, 2^-24 of
+ * |lse|, is in every probability (which matters where all logits of a row are huge, as in a row filled with the type's lowest
+ * value; the call below is exact there too). */
+int pxh_token_logprobs_backward(const void* logits, const void* targets, const float* lse, const float* entropy,
+                                const float* d_logp, const float* d_entropy, void* dlogits, int type, int wide_targets,
+                                long long rows, int vocab, long long stride, long long d_stride, float scale, void* stream);
+
+/* Both at once, for gradients that are known before (the weights of the tokens in a mean): what the two calls leave, the logits
+ * read once where a workgroup's registers hold a row (up to 163840 logits of 16 bits, half as many of fp32).  logp, entropy and lse
+ * are nullable. */
+int pxh_token_logprobs_forward_train(const void* logits, const void* targets, const float* d_logp, const float* d_entropy,
+                                     void* dlogits, float* logp, float* entropy, float* lse, int type, int wide_targets,
+                                     long long rows, int vocab, long long stride, long long d_stride, float scale,
+                                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

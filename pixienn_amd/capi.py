@@ -85,6 +85,9 @@ SIGNATURES = {
     "pxh_rescale_clip_table": [P, F, F, P, P],
     "pxh_rms_norm_forward": [P, P, P, P, P, P, P, I, I, I, L, I, L, L, L, L, I, F, P],
     "pxh_rms_norm_backward": [P, P, P, P, P, P, P, I, I, L, I, L, L, L, L, I, P, Z, P],
+    "pxh_token_logprobs_forward": [P, P, P, P, P, P, P, I, I, L, I, L, I, F, P, Z, P],
+    "pxh_token_logprobs_backward": [P, P, P, P, P, P, P, I, I, L, I, L, L, F, P],
+    "pxh_token_logprobs_forward_train": [P, P, P, P, P, P, P, P, I, I, L, I, L, L, F, P],
 }
 _OTHER_RETURNS = {
     "pxh_last_error": (ctypes.c_char_p, []),
@@ -101,6 +104,7 @@ _OTHER_RETURNS = {
     "pxh_reserve_workspace": (I, [Z]),
     "pxh_tensor_table_destroy": (None, [P]),
     "pxh_rms_norm_workspace_bytes": (Z, [L, I]),
+    "pxh_token_logprobs_workspace_bytes": (Z, [L, I, I]),
 }
 # test hooks (pixienn_amd/csrc/pixienn_hip_test.h): exported, but not part of the C ABI
 _TEST_HOOKS = {

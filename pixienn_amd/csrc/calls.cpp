@@ -113,6 +113,7 @@ Known entries[] = {
     ENTRY(pxh_route_backward), ENTRY(pxh_maxpool_forward), ENTRY(pxh_maxpool_backward), ENTRY(pxh_shortcut_backward_clipped),
     ENTRY(pxh_yolo_activate), ENTRY(pxh_yolo_detections_append), ENTRY(pxh_rescale_clip), ENTRY(pxh_adam_update),
     ENTRY(pxh_sgd_update), ENTRY(pxh_rms_norm_forward), ENTRY(pxh_rms_norm_backward),
+    ENTRY(pxh_token_logprobs_forward), ENTRY(pxh_token_logprobs_backward), ENTRY(pxh_token_logprobs_forward_train),
 };
 
 // bind(name, address) -> (callable, which arguments are tensors), or None for an entry point that is not made here

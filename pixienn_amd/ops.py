@@ -711,6 +711,64 @@ def rms_norm_backward(dy, h, weight, rstd, dx, dw, dsum=None, accumulate=False, 
     return dx
 
 
+def _targets(targets, rows):
+    """(address, whether of 64 bits) of the rows' tokens."""
+    if targets is None:
+        return None, 0
+    wide = getattr(targets, "dtype", None) is torch.int64
+    _vector(targets, "targets", rows, torch.int64 if wide else torch.int32)
+    return targets.data_ptr(), int(wide)
+
+
+def _per_row(rows, **tensors):
+    for name, t in tensors.items():
+        if t is not None:
+            _vector(t, name, rows)
+
+
+def token_logprobs_workspace_bytes(rows, vocab, top=0):
+    return int(capi.load().pxh_token_logprobs_workspace_bytes(rows, vocab, top))
+
+
+def token_logprobs_forward(logits, targets, logp, entropy=None, lse=None, top_logp=None, top_ids=None, scale=1.0, workspace=None):
+    """Per row of logits [rows, vocab], times `scale`: the log probability of its token (targets [rows], int32 or int64; 0 for one
+    outside the vocabulary), the entropy, the log of the sum of exponentials, and the most probable alternatives, top_logp and
+    top_ids (int32) [rows, top], the lowest index first among equal ones."""
+    rows, vocab, stride = _rows(logits, "logits")
+    at, wide = _targets(targets, rows)
+    _per_row(rows, logp=logp, entropy=entropy, lse=lse)
+    top = 0
+    if top_ids is not None:
+        if _tensor(top_ids).dim() == 0 or top_logp is None:
+            raise PxError("top_logp and top_ids go together, [rows, top]")
+        top = top_ids.shape[-1]
+        _vector(top_ids, "top_ids", rows * top, torch.int32)
+        _vector(top_logp, "top_logp", rows * top)
+    _run("pxh_token_logprobs_forward", logits.data_ptr(), at, logp, entropy, lse, top_logp if top else None, ptr(top_ids),
+         _type(logits, "logits"), wide, rows, vocab, stride, top, float(scale), ptr(workspace), _bytes(workspace))
+
+
+def token_logprobs_backward(logits, targets, lse, d_logp, dlogits, entropy=None, d_entropy=None, scale=1.0):
+    """The gradient of the logits for given gradients of logp and entropy (either may be None), from the forward's lse and, with
+    d_entropy, its entropy.  dlogits may be the logits."""
+    rows, vocab, stride = _rows(logits, "logits")
+    at, wide = _targets(targets, rows)
+    _per_row(rows, lse=lse, d_logp=d_logp, entropy=entropy, d_entropy=d_entropy)
+    _run("pxh_token_logprobs_backward", logits.data_ptr(), at, lse, entropy, d_logp, d_entropy, ptr(dlogits),
+         _type(logits, "logits"), wide, rows, vocab, stride, _like(dlogits, "dlogits", logits.shape, logits.dtype), float(scale))
+    return dlogits
+
+
+def token_logprobs_forward_train(logits, targets, d_logp, dlogits, logp=None, entropy=None, lse=None, d_entropy=None, scale=1.0):
+    """token_logprobs_forward and token_logprobs_backward at once, for gradients that are known before."""
+    rows, vocab, stride = _rows(logits, "logits")
+    at, wide = _targets(targets, rows)
+    _per_row(rows, d_logp=d_logp, logp=logp, entropy=entropy, lse=lse, d_entropy=d_entropy)
+    _run("pxh_token_logprobs_forward_train", logits.data_ptr(), at, d_logp, d_entropy, ptr(dlogits), logp, entropy, lse,
+         _type(logits, "logits"), wide, rows, vocab, stride, _like(dlogits, "dlogits", logits.shape, logits.dtype), float(scale))
+    return dlogits
+
+
 DETECTION_DTYPE = workloads.DETECTION_DTYPE
 
 
