@@ -669,6 +669,49 @@ int pxh_token_logprobs_forward_train(const void* logits, const void* targets, co
                                      long long rows, int vocab, long long stride, long long d_stride, float scale,
                                      void* stream);
 
+/* AdamW over all parameter tensors of a model at once, from a table kept on the device, with states in 32 or in 8 bits and the
+ * gradients clipped by their common norm:
+ *   norm = |d_scale * d|_2 over all tensors;  f = max_norm > 0 and norm > max_norm ? max_norm / norm : 1
+ *   g = d * d_scale * f;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+ *   w += lr * (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps) - lr * decay * w     (the decay where apply_decay says so)
+ *   copy = w, rounded to its type
+ * d is only read (unlike pxh_adam_update's).  d_scale: 1 / batch, the inverse of a loss scale, or both.
+ *
+ * States in 8 bits: m and the SQUARE ROOT of v are e4m3 values with a scale for each 256 of a tensor, its largest magnitude / 448
+ * (2^-126 at least): 2 + 1/32 bytes a value for both.  Each step's results are rounded stochastically, up with the
+ * probability of the part cut off: what a step changes of an average over 1000 steps is less than half a unit of such a value, and
+ * rounded to nearest it would never change.  A root that is not zero never rounds to zero (the quotient stays bounded).  The
+ * random bits come from `seed` (its low 31 bits) and the value's place in the table: another seed every step, the step's number
+ * for instance; the same seed gives the same bits.  A step reads the states as they were rounded, and applies its own before
+ * they are rounded.
+ *
+ * norm_out (nullable, device) receives the norm, also when max_norm is 0.  With max_norm > 0 and a norm that is not finite (an
+ * overflow of half-precision gradients) nothing is written but norm_out: the step is left out.
+ *
+ * pxh_adamw_table_create copies `tensors` (host memory); those of no values are left out; any number up to 2^20, of less than
+ * 2^31 values each.  state_bits is 32 (m, v: floats, the scales null) or 8.  The buffers need the alignment of their own values.
+ * Allocates device memory and uploads with a blocking copy: call it at set-up, not under graph capture.  The table belongs to
+ * the device that was current, and a step to a current device that is another is refused.  The norm's partial sums lie in the
+ * table: two steps of one table must not overlap in time. */
+typedef struct pxh_adamw_tensor {
+    float* w;
+    const void* d;          /* of d_type: PXH_F32, PXH_BF16 or PXH_F16 */
+    void* m;
+    void* v;
+    float* m_scale;         /* 8 bits: [n / 256, rounded up] */
+    float* v_scale;
+    void* copy;             /* nullable; of copy_type: PXH_BF16 or PXH_F16 */
+    size_t n;
+    int d_type, copy_type, apply_decay;
+} pxh_adamw_tensor;
+typedef struct pxh_adamw_table pxh_adamw_table;
+int pxh_adamw_table_create(int count, const pxh_adamw_tensor* tensors, int state_bits, pxh_adamw_table** table);
+void pxh_adamw_table_destroy(pxh_adamw_table* table);
+/* tensors in the table (those of no values are not counted) */
+int pxh_adamw_table_count(const pxh_adamw_table* table);
+int pxh_adamw_update_table(const pxh_adamw_table* table, int t, float lr, float beta1, float beta2, float eps, float decay,
+                           float d_scale, float max_norm, float* norm_out, unsigned seed, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -87,6 +87,9 @@ SIGNATURES = {
     "pxh_rms_norm_backward": [P, P, P, P, P, P, P, I, I, L, I, L, L, L, L, I, P, Z, P],
     "pxh_token_logprobs_forward": [P, P, P, P, P, P, P, I, I, L, I, L, I, F, P, Z, P],
     "pxh_token_logprobs_backward": [P, P, P, P, P, P, P, I, I, L, I, L, L, F, P],
+    "pxh_adamw_table_create": [I, P, I, P],
+    "pxh_adamw_table_count": [P],
+    "pxh_adamw_update_table": [P, I, F, F, F, F, F, F, F, P, U, P],
     "pxh_token_logprobs_forward_train": [P, P, P, P, P, P, P, P, I, I, L, I, L, L, F, P],
 }
 _OTHER_RETURNS = {
@@ -103,6 +106,7 @@ _OTHER_RETURNS = {
     "pxh_nms_workspace_bytes": (Z, [I]),
     "pxh_reserve_workspace": (I, [Z]),
     "pxh_tensor_table_destroy": (None, [P]),
+    "pxh_adamw_table_destroy": (None, [P]),
     "pxh_rms_norm_workspace_bytes": (Z, [L, I]),
     "pxh_token_logprobs_workspace_bytes": (Z, [L, I, I]),
 }
@@ -123,6 +127,12 @@ class YoloHead(ctypes.Structure):
     _fields_ = [("input", P), ("output", P), ("delta", P), ("masks", P), ("mask_count", I), ("width", I), ("height", I),
                 ("ignore_thresh", F), ("truth_thresh", F), ("coord_scale", F), ("object_scale", F),
                 ("noobject_scale", F), ("class_scale", F), ("stats", P), ("cost", P)]
+
+
+class AdamwTensor(ctypes.Structure):
+    """pxh_adamw_tensor of include/pixienn_hip.h."""
+    _fields_ = [("w", P), ("d", P), ("m", P), ("v", P), ("m_scale", P), ("v_scale", P), ("copy", P), ("n", Z), ("d_type", I),
+                ("copy_type", I), ("apply_decay", I)]
 
 
 class PxError(RuntimeError):

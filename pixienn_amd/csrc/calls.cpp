@@ -114,6 +114,7 @@ Known entries[] = {
     ENTRY(pxh_yolo_activate), ENTRY(pxh_yolo_detections_append), ENTRY(pxh_rescale_clip), ENTRY(pxh_adam_update),
     ENTRY(pxh_sgd_update), ENTRY(pxh_rms_norm_forward), ENTRY(pxh_rms_norm_backward),
     ENTRY(pxh_token_logprobs_forward), ENTRY(pxh_token_logprobs_backward), ENTRY(pxh_token_logprobs_forward_train),
+    ENTRY(pxh_adamw_update_table),
 };
 
 // bind(name, address) -> (callable, which arguments are tensors), or None for an entry point that is not made here

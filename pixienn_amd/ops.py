@@ -769,6 +769,91 @@ def token_logprobs_forward_train(logits, targets, d_logp, dlogits, logp=None, en
     return dlogits
 
 
+ADAMW_BLOCK = 256        # values with one scale, of an 8-bit state
+
+
+class AdamwTable:
+    """AdamW over lists of tensors (one entry per parameter tensor) in one call: w fp32, d (the gradient of what is to grow: it is
+    added) fp32, bfloat16 or half.  States m and v are fp32, or float8_e4m3fn with m_scales and v_scales, one fp32 for each 256
+    values of a tensor, where v holds the square root (adamw_states makes either kind).  copies: bfloat16 or half tensors that
+    receive the new weights, or None."""
+
+    def __init__(self, ws, ds, ms, vs, m_scales=None, v_scales=None, copies=None, apply_decay=None):
+        ws, ds, ms, vs = list(ws), list(ds), list(ms), list(vs)
+        count = len(ws)
+        eight = m_scales is not None
+        if eight != (v_scales is not None):
+            raise PxError("m_scales and v_scales go together")
+        m_scales, v_scales = (list(m_scales), list(v_scales)) if eight else ([None] * count, [None] * count)
+        copies = [None] * count if copies is None else list(copies)
+        flags = [False] * count if apply_decay is None else [bool(f) for f in apply_decay]
+        if any(len(group) != count for group in (ds, ms, vs, m_scales, v_scales, copies, flags)):
+            raise PxError("the lists of an AdamwTable have to be of one length")
+        state = _E4M3 if eight else torch.float32
+        table = (capi.AdamwTensor * max(1, count))()
+        device = None
+        for t, w, d, m, v, ms_, vs_, copy, flag in zip(table, ws, ds, ms, vs, m_scales, v_scales, copies, flags):
+            n = _tensor(w).numel()
+            blocks = -(-n // ADAMW_BLOCK)
+            for x, name, length, dtype in ((w, "w", n, torch.float32), (d, "d", n, None), (m, "m", n, state), (v, "v", n, state),
+                                           (ms_, "m_scale", blocks, torch.float32), (vs_, "v_scale", blocks, torch.float32), (copy, "copy", n, None)):
+                if x is None and (name == "copy" or not eight and name.endswith("scale")):
+                    continue
+                _chk(x, dtype or getattr(x, "dtype", None), name)
+                _vector(x, name, length, dtype)
+                device = x.device if device is None else device
+                if x.device != device:
+                    raise PxError("the tensors of an AdamwTable have to be on one device")
+            if copy is not None and copy.dtype not in (torch.bfloat16, torch.float16):
+                raise PxError("copy must be bfloat16 or half (got %s)" % copy.dtype)
+            t.w, t.d, t.m, t.v, t.m_scale, t.v_scale, t.copy = (ptr(x) for x in (w, d, m, v, ms_, vs_, copy))
+            t.n, t.d_type, t.apply_decay = n, _type(d, "d"), int(flag)
+            t.copy_type = 0 if copy is None else _type(copy, "copy")
+        self._keep = (ws, ds, ms, vs, m_scales, v_scales, copies)       # the tensors must outlive the table
+        self.handle = ctypes.c_void_p()
+        if device is None:
+            self._create(count, table, eight)
+        else:
+            with torch.cuda.device(device):
+                self._create(count, table, eight)
+        self.count = int(capi.load().pxh_adamw_table_count(self.handle))
+
+    def _create(self, count, table, eight):
+        call("pxh_adamw_table_create", count, ctypes.addressof(table), 8 if eight else 32, ctypes.byref(self.handle))
+
+    def close(self):
+        if self.handle:
+            capi.load().pxh_adamw_table_destroy(self.handle)
+            self.handle = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:      # noqa: BLE001 - interpreter shutdown
+            pass
+
+    def update(self, t, lr, beta1=0.9, beta2=0.999, eps=1e-8, decay=0.0, d_scale=1.0, max_norm=0.0, norm_out=None, seed=0):
+        """Step number t (from 1).  max_norm > 0 clips by the norm of all gradients, and leaves the step out where that is not
+        finite; norm_out (one fp32 value on the device) receives it.  seed: another one every step, for states in 8 bits."""
+        if norm_out is not None:
+            _vector(norm_out, "norm_out", 1)
+        _run("pxh_adamw_update_table", self.handle.value or 0, int(t), float(lr), float(beta1), float(beta2), float(eps), float(decay),
+             float(d_scale), float(max_norm), norm_out, int(seed) & 0x7FFFFFFF)
+
+
+def adamw_states(ws, bits=8):
+    """Zero states for tensors ws: the keyword arguments ms, vs (and m_scales, v_scales with 8 bits) of an AdamwTable."""
+    if bits not in (8, 32):
+        raise PxError("states of 8 or 32 bits (got %r)" % (bits,))
+    zeros = lambda w, dtype: torch.zeros(w.numel(), device=w.device, dtype=dtype)      # noqa: E731
+    states = {k: [zeros(w, torch.float32 if bits == 32 else torch.uint8) for w in ws] for k in ("ms", "vs")}
+    if bits == 8:
+        states = {k: [t.view(_E4M3) for t in v] for k, v in states.items()}
+        for k in ("m_scales", "v_scales"):
+            states[k] = [torch.zeros(-(-w.numel() // ADAMW_BLOCK), device=w.device) for w in ws]
+    return states
+
+
 DETECTION_DTYPE = workloads.DETECTION_DTYPE
 
 
