@@ -640,7 +640,8 @@ int pxh_rms_norm_backward(const void* dy, const void* h, const void* weight, con
  * be learned).  targets and logp are given together or not at all; entropy and lse are nullable.  scale > 0.
  * top_logp, top_ids [rows][top]: the `top` largest z (at most PXH_MOST_ALTERNATIVES, and vocab), descending, among equal ones the
  * lowest index first; top == 0: none.  A logit of minus infinity has probability 0, and one of the type's lowest value is a number as
- * any other.  A row of nothing but minus infinities has lse and logp minus infinity, entropy 0; one with a NaN or plus infinity
+ * any other.  A row of nothing but minus infinities has lse and logp minus infinity, entropy 0 (and NaN
+ * for its alternatives, which have no distribution); one with a NaN or plus infinity
  * has NaN in all three, and its NaNs come last among the alternatives.
  * workspace: pxh_token_logprobs_workspace_bytes(rows, vocab, top), which serves fewer rows, fewer alternatives and smaller
  * vocabularies too, or NULL for the library's. */

@@ -17,27 +17,32 @@ struct Sums {
 
     __device__ __forceinline__ float reference() const { return peak == -INFINITY ? 0.0f : peak; }
 
+    // Adds the sums of o, whose peak is not above this one's.
+    __device__ __forceinline__ void take(const Sums& o, float c)
+    {
+        const float t = (o.peak - reference()) * c;
+        const float f = __builtin_amdgcn_exp2f(t);
+        weighted += f * fmaf(fmaxf(t, kFar), o.sum, o.weighted);
+        sum += o.sum * f;
+    }
+
     // V more values
     template<int V>
     __device__ __forceinline__ void add(const float (&l)[V], float c)
     {
-        float most = l[0];
+        Sums r{ peak, 0.0f, 0.0f };
 #pragma unroll
-        for (int k = 1; k < V; ++k) most = fmaxf(most, l[k]);
-        const float next = fmaxf(peak, most);
-        const float ref = next == -INFINITY ? 0.0f : next;
-        const float t = (peak - ref) * c;
-        const float f = __builtin_amdgcn_exp2f(t);
-        weighted = f * fmaf(fmaxf(t, kFar), sum, weighted);
-        sum *= f;
-        peak = next;
+        for (int k = 0; k < V; ++k) r.peak = fmaxf(r.peak, l[k]);
+        r.take(*this, c);
+        const float ref = r.reference();
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             const float u = (l[k] - ref) * c;
             const float e = __builtin_amdgcn_exp2f(u);
-            sum += e;
-            weighted = fmaf(e, fmaxf(u, kFar), weighted);
+            r.sum += e;
+            r.weighted = fmaf(e, fmaxf(u, kFar), r.weighted);
         }
+        *this = r;
     }
 };
 
@@ -47,29 +52,18 @@ __device__ __forceinline__ Sums nothing() { return Sums{ -INFINITY, 0.0f, 0.0f }
 template<int LANES>
 __device__ __forceinline__ Sums group_join(Sums s, float c, Sums* slots)
 {
-    const float peak = wave_max_by_rows(s.peak);
-    Sums w{ peak, 0.0f, 0.0f };
-    {
-        const float t = (s.peak - w.reference()) * c;
-        const float f = __builtin_amdgcn_exp2f(t);
-        w.weighted = wave_sum_by_rows(f * fmaf(fmaxf(t, kFar), s.sum, s.weighted));
-        w.sum = wave_sum_by_rows(s.sum * f);
-    }
+    Sums w{ wave_max_by_rows(s.peak), 0.0f, 0.0f };
+    w.take(s, c);
+    w.sum = wave_sum_by_rows(w.sum);
+    w.weighted = wave_sum_by_rows(w.weighted);
     if constexpr (LANES > kWave) {
         if ((threadIdx.x & (kWave - 1)) == 0) slots[threadIdx.x / kWave] = w;
         __syncthreads();
         Sums all = nothing();
 #pragma unroll
         for (int k = 0; k < LANES / kWave; ++k) all.peak = fmaxf(all.peak, slots[k].peak);
-        const float ref = all.reference();
 #pragma unroll
-        for (int k = 0; k < LANES / kWave; ++k) {
-            const Sums o = slots[k];
-            const float t = (o.peak - ref) * c;
-            const float f = __builtin_amdgcn_exp2f(t);
-            all.weighted += f * fmaf(fmaxf(t, kFar), o.sum, o.weighted);
-            all.sum += o.sum * f;
-        }
+        for (int k = 0; k < LANES / kWave; ++k) all.take(slots[k], c);
         __syncthreads();
         w = all;
     }
@@ -125,53 +119,257 @@ __device__ __forceinline__ RowResult finish_row(const TokenArgs& a, long long ro
     return r;
 }
 
-// One number that orders by value, then by the lowest index; NaN below everything.
-__device__ __forceinline__ unsigned long long key_of(float z, uint32_t index)
+// ---------------------------------------------------------------- alternatives
+// One number that orders by value, then by the lowest index: the value's bits in their order in the upper half.  A NaN is below
+// everything, and 0 is no value at all.
+__device__ __forceinline__ uint32_t order_of(float z)
 {
-    const uint32_t bits = __float_as_uint(z + 0.0f);
-    const uint32_t order = z != z ? 0u : (bits & 0x80000000u) ? ~bits : bits | 0x80000000u;
-    return (static_cast<unsigned long long>(order) << 32) | ~index;
+    const uint32_t bits = __float_as_uint(z + 0.0f);        // one zero
+    return z != z ? 0u : (bits & 0x80000000u) ? ~bits : bits | 0x80000000u;
 }
 
-// ---------------------------------------------------------------- forward
-// A workgroup per row, one pass over it; then a pass for each alternative, over what the caches hold.
-template<int T, int LANES>
-__global__ __launch_bounds__(LANES) void token_logprobs_kernel(TokenArgs a)
+__device__ __forceinline__ unsigned long long key_of(float z, uint32_t index)
 {
-    constexpr int V = kVec<T>;
-    __shared__ Sums slots[LANES / kWave];
-    __shared__ unsigned long long best;
-    const long long row = blockIdx.x;
-    const char* logits = static_cast<const char*>(a.logits) + row * a.stride * kSize<T>;
-    const float c = a.scale * kLog2e;
-    const int target = target_of(a, row);
-    const float given = target < 0 ? 0.0f : load_one<T>(logits, target);
-    Sums s = nothing();
-    for (int e = threadIdx.x * V; e < a.vocab; e += LANES * V) {
-        float l[V];
-        load_row<T, V>(logits, e, a.vocab, -INFINITY).get(l);
-        s.add(l, c);
+    return (static_cast<unsigned long long>(order_of(z)) << 32) | ~index;
+}
+
+__device__ __forceinline__ float value_of(unsigned long long key)
+{
+    const uint32_t order = static_cast<uint32_t>(key >> 32);
+    if (order == 0) return __builtin_nanf("");
+    return __uint_as_float((order & 0x80000000u) ? order & 0x7fffffffu : ~order);
+}
+
+constexpr int kCandidates = 512;
+
+struct Selection {
+    uint32_t best[kWave];
+    unsigned long long list[kCandidates];
+    unsigned long long most;
+    int count;
+    uint32_t floor;
+};
+
+template<int CTRL>
+__device__ __forceinline__ uint32_t max_in_row(uint32_t v)
+{
+    const uint32_t o = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xF, 0xF, true));
+    return v > o ? v : o;
+}
+
+// The k largest keys of a workgroup, largest first: put(place, key), key 0 where there are fewer.  `best` is the largest order of
+// the lane's keys (0: none), each(f) calls f with every one of them.
+// The lanes' maxima, in 64 groups, are as many different values, so the k-th largest of those is not above the k-th largest of
+// all: only the lanes that reach it look at their values again, and little more than k values pass (8 of 16384 normal ones:
+// 9 on average).  They are ranked by counting.  Where too many values are equal for the list, each place takes a pass.
+template<int LANES, typename Each, typename Put>
+__device__ __forceinline__ void select_largest(int k, uint32_t best, const Each& each, const Put& put, Selection& s)
+{
+    static_assert(LANES == 256 || LANES == 1024, "64 groups of lanes of one row of 16");
+    uint32_t group = max_in_row<0x4E>(max_in_row<0xB1>(best));
+    if constexpr (LANES == 1024) group = max_in_row<0x140>(max_in_row<0x141>(group));
+    if (threadIdx.x % (LANES / kWave) == 0) s.best[threadIdx.x / (LANES / kWave)] = group;
+    if (threadIdx.x == 0) s.count = 0;
+    __syncthreads();
+    if (threadIdx.x < kWave) {
+        const uint32_t mine = s.best[threadIdx.x];
+        int above = 0;
+#pragma unroll
+        for (int j = 0; j < kWave; ++j) above += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), j)) > mine;
+        uint32_t low = above < k ? mine : ~0u;
+#pragma unroll
+        for (int off = kWave / 2; off > 0; off >>= 1) low = min(low, static_cast<uint32_t>(__shfl_xor(static_cast<int>(low), off, kWave)));
+        if (threadIdx.x == 0) s.floor = low;
     }
-    s = group_join<LANES>(s, c, slots);
-    const RowResult r = finish_row(a, row, s, target, given, threadIdx.x == 0);
+    __syncthreads();
+    const uint32_t floor = s.floor;
+    if (best >= floor)
+        each([&](unsigned long long key) {
+            if (static_cast<uint32_t>(key >> 32) < floor) return;
+            const int at = atomicAdd(&s.count, 1);
+            if (at < kCandidates) s.list[at] = key;
+        });
+    __syncthreads();
+    const int n = s.count;
+    if (n <= kCandidates) {
+        for (int t = threadIdx.x; t < n; t += LANES) {
+            const unsigned long long key = s.list[t];
+            int above = 0;
+            for (int j = 0; j < n; ++j) above += s.list[j] > key;
+            if (above < k) put(above, key);
+        }
+        for (int t = n + threadIdx.x; t < k; t += LANES) put(t, 0ull);
+        return;
+    }
     unsigned long long before = ~0ull;
-    for (int j = 0; j < a.top; ++j) {
-        if (threadIdx.x == 0) best = 0;
+    for (int place = 0; place < k; ++place) {
+        __syncthreads();
+        if (threadIdx.x == 0) s.most = 0;
         __syncthreads();
         unsigned long long mine = 0;
-        for (int e = threadIdx.x; e < a.vocab; e += LANES) {
-            const unsigned long long key = key_of(load_one<T>(logits, e) * a.scale, e);
+        each([&](unsigned long long key) {
             if (key < before && key > mine) mine = key;
-        }
-        atomicMax(&best, mine);
+        });
+        atomicMax(&s.most, mine);
         __syncthreads();
-        before = best;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            const uint32_t id = ~static_cast<uint32_t>(before);
-            a.top_ids[row * a.top + j] = static_cast<int>(id);
-            a.top_logp[row * a.top + j] = load_one<T>(logits, id) * a.scale - r.lse;
+        before = s.most;
+        if (threadIdx.x == 0) put(place, before);
+    }
+}
+
+// ---------------------------------------------------------------- a part of a row
+// Vectors first .. first + count of a row, K to a lane, and of the row's last values, which fill no vector, one to each of the
+// first lanes of the part that has them.  What is not there is minus infinity.
+template<int T, int LANES, int K>
+struct Part {
+    static constexpr int V = kVec<T>;
+    Raw<T, V> kept[K];
+    float extra;
+    int first, count, extra_at;
+
+    __device__ __forceinline__ bool has(int k) const { return k * LANES + static_cast<int>(threadIdx.x) < count; }
+    __device__ __forceinline__ int at(int k) const { return (first + k * LANES + static_cast<int>(threadIdx.x)) * V; }
+
+    __device__ __forceinline__ void load(const char* row, int vocab, int first_vector, int vectors)
+    {
+        constexpr uint32_t nothing = T == PXH_F32 ? 0xff800000u : T == PXH_BF16 ? 0xff80ff80u : 0xfc00fc00u;
+        const int whole = vocab / V;
+        first = first_vector;
+        count = min(vectors, whole - first_vector);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+#pragma unroll
+            for (int i = 0; i < Raw<T, V>::kWords; ++i) kept[k].w[i] = nothing;
+            if (has(k)) kept[k] = load_raw<T, V>(row, at(k));
         }
+        extra = -INFINITY;
+        extra_at = whole * V + static_cast<int>(threadIdx.x);
+        if (first_vector + vectors >= whole && extra_at < vocab) extra = load_one<T>(row, extra_at);
+        else extra_at = -1;
+    }
+
+    template<bool ENTROPY>
+    __device__ __forceinline__ Sums sums(float c) const
+    {
+        Sums s{ extra, 0.0f, 0.0f };
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            float l[V];
+            kept[k].get(l);
+#pragma unroll
+            for (int i = 0; i < V; ++i) s.peak = fmaxf(s.peak, l[i]);
+        }
+        const float ref = s.reference();
+        const auto take = [&](float l) {
+            const float u = (l - ref) * c;
+            const float e = __builtin_amdgcn_exp2f(u);
+            s.sum += e;
+            if (ENTROPY) s.weighted = fmaf(e, fmaxf(u, kFar), s.weighted);
+        };
+        take(extra);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            float l[V];
+            kept[k].get(l);
+#pragma unroll
+            for (int i = 0; i < V; ++i) take(l[i]);
+        }
+        return s;
+    }
+
+    template<typename F>
+    __device__ __forceinline__ void each(float scale, const F& f) const
+    {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            if (!has(k)) continue;
+            float l[V];
+            kept[k].get(l);
+#pragma unroll
+            for (int i = 0; i < V; ++i) f(key_of(l[i] * scale, at(k) + i));
+        }
+        if (extra_at >= 0) f(key_of(extra * scale, extra_at));
+    }
+};
+
+// ---------------------------------------------------------------- forward
+// A workgroup takes one part of a row into its registers; a row of several parts is put together by a second launch from
+// their sums and their largest values.
+struct Parts {
+    unsigned long long* keys;       // [rows][parts][top]
+    Sums* sums;                     // [rows][parts]
+    int parts, vectors;             // parts of a row, vectors of a part
+    FastDiv by_parts;
+};
+
+template<int T, bool ENTROPY, int LANES, int K>
+__global__ __launch_bounds__(LANES) void token_logprobs_kernel(TokenArgs a, Parts p)
+{
+    __shared__ Sums slots[LANES / kWave];
+    __shared__ Selection selection;
+    uint32_t row, part;
+    p.by_parts.divmod(blockIdx.x, row, part);
+    const char* logits = static_cast<const char*>(a.logits) + row * a.stride * kSize<T>;
+    const float c = a.scale * kLog2e;
+    const bool whole = p.parts == 1;
+    Part<T, LANES, K> mine;
+    mine.load(logits, a.vocab, static_cast<int>(part) * p.vectors, p.vectors);
+    const int target = whole ? target_of(a, row) : -1;
+    const float given = target < 0 ? 0.0f : load_one<T>(logits, target);
+    Sums s = mine.template sums<ENTROPY>(c);
+    const float peak = s.peak;
+    s = group_join<LANES>(s, c, slots);
+    float lse = 0.0f;
+    if (whole) lse = finish_row(a, row, s, target, given, threadIdx.x == 0).lse;
+    else if (threadIdx.x == 0) p.sums[blockIdx.x] = s;
+    if (a.top) {
+        const bool any = mine.has(0) || mine.extra_at >= 0;
+        const auto put = [&](int place, unsigned long long key) {
+            if (whole) {
+                a.top_ids[static_cast<long long>(row) * a.top + place] = static_cast<int>(~static_cast<uint32_t>(key));
+                a.top_logp[static_cast<long long>(row) * a.top + place] = value_of(key) - lse;
+            } else {
+                p.keys[static_cast<size_t>(blockIdx.x) * a.top + place] = key;
+            }
+        };
+        select_largest<LANES>(a.top, any ? order_of(peak * a.scale) : 0u, [&](const auto& f) { mine.each(a.scale, f); }, put, selection);
+    }
+}
+
+template<int T>
+__global__ __launch_bounds__(kBlock) void token_join_kernel(TokenArgs a, Parts p)
+{
+    __shared__ Sums slots[kBlock / kWave];
+    __shared__ Selection selection;
+    const long long row = blockIdx.x;
+    const float c = a.scale * kLog2e;
+    const int target = target_of(a, row);
+    const float given = target < 0 ? 0.0f : load_one<T>(static_cast<const char*>(a.logits) + row * a.stride * kSize<T>, target);
+    Sums s = nothing();
+    for (int k = threadIdx.x; k < p.parts; k += kBlock) {
+        const Sums o = p.sums[row * p.parts + k];
+        Sums r{ fmaxf(s.peak, o.peak), 0.0f, 0.0f };
+        r.take(s, c);
+        r.take(o, c);
+        s = r;
+    }
+    s = group_join<kBlock>(s, c, slots);
+    const float lse = finish_row(a, row, s, target, given, threadIdx.x == 0).lse;
+    if (a.top) {
+        const unsigned long long* keys = p.keys + static_cast<size_t>(row) * p.parts * a.top;
+        const int n = p.parts * a.top;
+        uint32_t best = 0;
+        for (int k = threadIdx.x; k < n; k += kBlock) best = max(best, static_cast<uint32_t>(keys[k] >> 32));
+        select_largest<kBlock>(a.top, best,
+                               [&](const auto& f) {
+                                   for (int k = threadIdx.x; k < n; k += kBlock)
+                                       if (keys[k]) f(keys[k]);
+                               },
+                               [&](int place, unsigned long long key) {
+                                   a.top_ids[row * a.top + place] = static_cast<int>(~static_cast<uint32_t>(key));
+                                   a.top_logp[row * a.top + place] = value_of(key) - lse;
+                               },
+                               selection);
     }
 }
 
@@ -255,8 +453,8 @@ __global__ __launch_bounds__(kBlock) void token_gradient_kernel(TokenArgs a, Fas
 }
 
 // ---------------------------------------------------------------- forward and gradient at once
-// A workgroup per row, which stays in registers, K vectors a lane, between its sums and its gradient (K == 0: a row of any
-// length, read again).  A lane writes the values that it has read, so the gradient may take the logits' place.
+// A workgroup per row, which stays in registers between its sums and its gradient.  A lane writes the values that it has read, so the
+// gradient may take the logits' place.
 template<int T, bool ENTROPY, int LANES, int K>
 __global__ __launch_bounds__(LANES) void token_train_kernel(TokenArgs a)
 {
@@ -266,62 +464,58 @@ __global__ __launch_bounds__(LANES) void token_train_kernel(TokenArgs a)
     const char* logits = static_cast<const char*>(a.logits) + row * a.stride * kSize<T>;
     char* out = static_cast<char*>(a.dlogits) + row * a.d_stride * kSize<T>;
     const float c = a.scale * kLog2e;
+    Part<T, LANES, K> mine;
+    mine.load(logits, a.vocab, 0, a.vocab);
     const int target = target_of(a, row);
     const float given = target < 0 ? 0.0f : load_one<T>(logits, target);        // before it is overwritten
-    Raw<T, V> kept[K ? K : 1];
-    Sums s = nothing();
-    if constexpr (K > 0) {
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int e = (k * LANES + threadIdx.x) * V;
-            kept[k] = load_row<T, V>(logits, e < a.vocab ? e : a.vocab, a.vocab, -INFINITY);
-        }
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            float l[V];
-            kept[k].get(l);
-#pragma unroll
-            for (int i = 0; i < V; ++i) s.peak = fmaxf(s.peak, l[i]);
-        }
-        const float ref = s.reference();
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            float l[V];
-            kept[k].get(l);
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float u = (l[i] - ref) * c;
-                const float e = __builtin_amdgcn_exp2f(u);
-                s.sum += e;
-                if (ENTROPY) s.weighted = fmaf(e, fmaxf(u, kFar), s.weighted);
-            }
-        }
-    } else {
-        for (int e = threadIdx.x * V; e < a.vocab; e += LANES * V) {
-            float l[V];
-            load_row<T, V>(logits, e, a.vocab, -INFINITY).get(l);
-            s.add(l, c);
-        }
-    }
-    s = group_join<LANES>(s, c, slots);
+    const Sums s = group_join<LANES>(mine.template sums<ENTROPY>(c), c, slots);
     const RowResult r = finish_row(a, row, s, target, given, threadIdx.x == 0);
     const auto gradient = gradient_of<T, true>(a, row, target, s.peak, r.log_sum, r.entropy);
-    const auto write = [&](int e, const Raw<T, V>& raw) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        if (!mine.has(k)) continue;
         float l[V], d[V];
-        raw.get(l);
+        mine.kept[k].get(l);
+        gradient.template apply<V>(l, mine.at(k), d);
+        Raw<T, V> o;
+        o.set(d);
+        store_raw<T, V>(out, mine.at(k), o);
+    }
+    if (mine.extra_at >= 0) {
+        float d[1];
+        gradient.template apply<1>({ mine.extra }, mine.extra_at, d);
+        store_one<T>(out, mine.extra_at, d[0]);
+    }
+}
+
+// Rows that no workgroup's registers hold are read twice.
+template<int T>
+__global__ __launch_bounds__(1024) void token_train_long_kernel(TokenArgs a)
+{
+    constexpr int V = kVec<T>;
+    __shared__ Sums slots[1024 / kWave];
+    const long long row = blockIdx.x;
+    const char* logits = static_cast<const char*>(a.logits) + row * a.stride * kSize<T>;
+    char* out = static_cast<char*>(a.dlogits) + row * a.d_stride * kSize<T>;
+    const float c = a.scale * kLog2e;
+    const int target = target_of(a, row);
+    const float given = target < 0 ? 0.0f : load_one<T>(logits, target);        // before it is overwritten
+    Sums s = nothing();
+    for (int e = threadIdx.x * V; e < a.vocab; e += 1024 * V) {
+        float l[V];
+        load_row<T, V>(logits, e, a.vocab, -INFINITY).get(l);
+        s.add(l, c);
+    }
+    s = group_join<1024>(s, c, slots);
+    const RowResult r = finish_row(a, row, s, target, given, threadIdx.x == 0);
+    const auto gradient = gradient_of<T, true>(a, row, target, s.peak, r.log_sum, r.entropy);
+    for (int e = threadIdx.x * V; e < a.vocab; e += 1024 * V) {
+        float l[V], d[V];
+        load_row<T, V>(logits, e, a.vocab).get(l);
         gradient.template apply<V>(l, e, d);
         Raw<T, V> o;
         o.set(d);
         store_row<T, V>(out, e, a.vocab, o);
-    };
-    if constexpr (K > 0) {
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int e = (k * LANES + threadIdx.x) * V;
-            if (e < a.vocab) write(e, kept[k]);
-        }
-    } else {
-        for (int e = threadIdx.x * V; e < a.vocab; e += LANES * V) write(e, load_row<T, V>(logits, e, a.vocab));
     }
 }
 
@@ -329,22 +523,54 @@ template<int T, bool ENTROPY>
 int launch_train(const char* who, const TokenArgs& a, hipStream_t s)
 {
     const dim3 grid(static_cast<unsigned>(a.rows));
-    const int vectors = a.vocab / kVec<T> + (a.vocab % kVec<T> != 0);
+    const int vectors = a.vocab / kVec<T>;
     if (vectors <= 256) hipLaunchKernelGGL((token_train_kernel<T, ENTROPY, 256, 1>), grid, dim3(256), 0, s, a);
     else if (vectors <= 1024) hipLaunchKernelGGL((token_train_kernel<T, ENTROPY, 256, 4>), grid, dim3(256), 0, s, a);
     else if (vectors <= 4096) hipLaunchKernelGGL((token_train_kernel<T, ENTROPY, 512, 8>), grid, dim3(512), 0, s, a);
     else if (vectors <= 8192) hipLaunchKernelGGL((token_train_kernel<T, ENTROPY, 1024, 8>), grid, dim3(1024), 0, s, a);
     else if (vectors <= 16384) hipLaunchKernelGGL((token_train_kernel<T, ENTROPY, 1024, 16>), grid, dim3(1024), 0, s, a);
     else if (vectors <= 20480) hipLaunchKernelGGL((token_train_kernel<T, ENTROPY, 1024, 20>), grid, dim3(1024), 0, s, a);
-    else hipLaunchKernelGGL((token_train_kernel<T, true, 1024, 0>), grid, dim3(1024), 0, s, a);
+    else hipLaunchKernelGGL((token_train_long_kernel<T>), grid, dim3(1024), 0, s, a);
     return check_launch(who);
 }
 
-template<int T>
-int launch_forward(const char* who, const TokenArgs& a, hipStream_t s)
+// Workgroups that fill the machine four times over: from there on a workgroup takes as much as its registers hold.
+constexpr long long kEnoughParts = 1024;
+constexpr int kMostVectors = 8;         // vectors of a lane
+
+// Parts of a row of `vectors`, with up to `k` vectors to a lane.
+inline int parts_of(long long vectors, int k) { return static_cast<int>((vectors + kBlock * k - 1) / (kBlock * k)); }
+
+int vectors_per_lane(long long rows, long long vectors)
 {
-    if (a.vocab <= 8192) hipLaunchKernelGGL((token_logprobs_kernel<T, 256>), dim3(static_cast<unsigned>(a.rows)), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((token_logprobs_kernel<T, 1024>), dim3(static_cast<unsigned>(a.rows)), dim3(1024), 0, s, a);
+    int k = kMostVectors;
+    while (k > 1 && rows * parts_of(vectors, k) < kEnoughParts) k /= 2;
+    return k;
+}
+
+template<int T, bool ENTROPY>
+int launch_forward(const char* who, const TokenArgs& a, void* workspace, hipStream_t s)
+{
+    const int vectors = a.vocab < kVec<T> ? 1 : a.vocab / kVec<T>;      // the values behind the last one go with it
+    const int k = vectors_per_lane(a.rows, vectors);
+    Parts p{};
+    p.parts = parts_of(vectors, k);
+    p.vectors = (vectors + p.parts - 1) / p.parts;
+    p.parts = (vectors + p.vectors - 1) / p.vectors;
+    p.by_parts = FastDiv(p.parts);
+    const size_t groups = static_cast<size_t>(a.rows) * p.parts;
+    p.keys = static_cast<unsigned long long*>(workspace);
+    p.sums = reinterpret_cast<Sums*>(static_cast<char*>(workspace) + groups * a.top * sizeof(unsigned long long));
+    const dim3 grid(static_cast<unsigned>(groups)), block(kBlock);
+    switch (k) {
+    case 1: hipLaunchKernelGGL((token_logprobs_kernel<T, ENTROPY, kBlock, 1>), grid, block, 0, s, a, p); break;
+    case 2: hipLaunchKernelGGL((token_logprobs_kernel<T, ENTROPY, kBlock, 2>), grid, block, 0, s, a, p); break;
+    case 4: hipLaunchKernelGGL((token_logprobs_kernel<T, ENTROPY, kBlock, 4>), grid, block, 0, s, a, p); break;
+    default: hipLaunchKernelGGL((token_logprobs_kernel<T, ENTROPY, kBlock, 8>), grid, block, 0, s, a, p); break;
+    }
+    if (int rc = check_launch(who)) return rc;
+    if (p.parts == 1) return PXH_OK;
+    hipLaunchKernelGGL((token_join_kernel<T>), dim3(static_cast<unsigned>(a.rows)), block, 0, s, a, p);
     return check_launch(who);
 }
 
@@ -407,8 +633,12 @@ extern "C" {
 
 size_t pxh_token_logprobs_workspace_bytes(long long rows, int vocab, int top)
 {
-    (void) rows; (void) vocab; (void) top;
-    return 0;
+    if (rows <= 0 || vocab <= 0 || top < 0) return 0;
+    // fp32 has the most vectors; a row whose parts are not the largest possible is one of few
+    const long long vectors = vocab < 4 ? 1 : vocab / 4;
+    const long long most = rows * parts_of(vectors, 1), least = rows * parts_of(vectors, kMostVectors);
+    const long long few = most < 2 * kEnoughParts ? most : 2 * kEnoughParts;
+    return static_cast<size_t>(least > few ? least : few) * (static_cast<size_t>(top) * sizeof(unsigned long long) + sizeof(Sums));
 }
 
 int pxh_token_logprobs_forward(const void* logits, const void* targets, float* logp, float* entropy, float* lse,
@@ -427,7 +657,14 @@ int pxh_token_logprobs_forward(const void* logits, const void* targets, float* l
     a.top = top; a.scale = scale;
     hipStream_t s = as_stream(stream);
     int rc = PXH_OK;
-    dispatch_type(type, [&]<int T>() { rc = by_rows(a, T, [&](const TokenArgs& p) { return launch_forward<T>(who, p, s); }); });
+    if (rows == 0) return PXH_OK;
+    void* ws = nullptr;
+    if ((rc = resolve_workspace(workspace, workspace_bytes, pxh_token_logprobs_workspace_bytes(rows, vocab, top), &ws, s))) return rc;
+    dispatch_type(type, [&]<int T>() {
+        rc = by_rows(a, T, [&](const TokenArgs& p) {
+            return entropy ? launch_forward<T, true>(who, p, ws, s) : launch_forward<T, false>(who, p, ws, s);
+        });
+    });
     return rc;
 }
 
