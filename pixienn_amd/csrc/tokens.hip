@@ -52,6 +52,7 @@ __device__ __forceinline__ Sums nothing() { return Sums{ -INFINITY, 0.0f, 0.0f }
 template<int LANES>
 __device__ __forceinline__ Sums group_join(Sums s, float c, Sums* slots)
 {
+    static_assert(LANES == kWave || LANES == 4 * kWave || LANES == 8 * kWave || LANES == 16 * kWave, "waves in part of a row of lanes");
     Sums w{ wave_max_by_rows(s.peak), 0.0f, 0.0f };
     w.take(s, c);
     w.sum = wave_sum_by_rows(w.sum);
@@ -59,11 +60,24 @@ __device__ __forceinline__ Sums group_join(Sums s, float c, Sums* slots)
     if constexpr (LANES > kWave) {
         if ((threadIdx.x & (kWave - 1)) == 0) slots[threadIdx.x / kWave] = w;
         __syncthreads();
-        Sums all = nothing();
-#pragma unroll
-        for (int k = 0; k < LANES / kWave; ++k) all.peak = fmaxf(all.peak, slots[k].peak);
-#pragma unroll
-        for (int k = 0; k < LANES / kWave; ++k) all.take(slots[k], c);
+        // a wave's sums to a lane, and over as many lanes of a row of 16 as there are waves
+        constexpr int kWaves = LANES / kWave;
+        const Sums o = slots[threadIdx.x % kWaves];
+        Sums all{ o.peak, 0.0f, 0.0f };
+        all.peak = fmaxf(all.peak, lane_in_row<0xB1>(all.peak));
+        all.peak = fmaxf(all.peak, lane_in_row<0x4E>(all.peak));
+        if constexpr (kWaves > 4) all.peak = fmaxf(all.peak, lane_in_row<0x141>(all.peak));
+        if constexpr (kWaves > 8) all.peak = fmaxf(all.peak, lane_in_row<0x140>(all.peak));
+        all.take(o, c);
+        const auto over_waves = [](float v) {
+            v += lane_in_row<0xB1>(v);
+            v += lane_in_row<0x4E>(v);
+            if constexpr (kWaves > 4) v += lane_in_row<0x141>(v);
+            if constexpr (kWaves > 8) v += lane_in_row<0x140>(v);
+            return v;
+        };
+        all.sum = over_waves(all.sum);
+        all.weighted = over_waves(all.weighted);
         __syncthreads();
         w = all;
     }
@@ -158,12 +172,13 @@ __device__ __forceinline__ uint32_t max_in_row(uint32_t v)
 }
 
 // The k largest keys of a workgroup, largest first: put(place, key), key 0 where there are fewer.  `best` is the largest order of
-// the lane's keys (0: none), each(f) calls f with every one of them.
+// the lane's keys (0: none); above(floor, f) calls f with those of its keys that reach `floor`, and may with others; each(f)
+// calls f with all keys of the workgroup, some by every lane.
 // The lanes' maxima, in 64 groups, are as many different values, so the k-th largest of those is not above the k-th largest of
 // all: only the lanes that reach it look at their values again, and little more than k values pass (8 of 16384 normal ones:
 // 9 on average).  They are ranked by counting.  Where too many values are equal for the list, each place takes a pass.
-template<int LANES, typename Each, typename Put>
-__device__ __forceinline__ void select_largest(int k, uint32_t best, const Each& each, const Put& put, Selection& s)
+template<int LANES, typename Above, typename Each, typename Put>
+__device__ __forceinline__ void select_largest(int k, uint32_t best, const Above& above, const Each& each, const Put& put, Selection& s)
 {
     static_assert(LANES == 256 || LANES == 1024, "64 groups of lanes of one row of 16");
     uint32_t group = max_in_row<0x4E>(max_in_row<0xB1>(best));
@@ -173,10 +188,10 @@ __device__ __forceinline__ void select_largest(int k, uint32_t best, const Each&
     __syncthreads();
     if (threadIdx.x < kWave) {
         const uint32_t mine = s.best[threadIdx.x];
-        int above = 0;
+        int larger = 0;
 #pragma unroll
-        for (int j = 0; j < kWave; ++j) above += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), j)) > mine;
-        uint32_t low = above < k ? mine : ~0u;
+        for (int j = 0; j < kWave; ++j) larger += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), j)) > mine;
+        uint32_t low = larger < k ? mine : ~0u;
 #pragma unroll
         for (int off = kWave / 2; off > 0; off >>= 1) low = min(low, static_cast<uint32_t>(__shfl_xor(static_cast<int>(low), off, kWave)));
         if (threadIdx.x == 0) s.floor = low;
@@ -184,7 +199,7 @@ __device__ __forceinline__ void select_largest(int k, uint32_t best, const Each&
     __syncthreads();
     const uint32_t floor = s.floor;
     if (best >= floor)
-        each([&](unsigned long long key) {
+        above(floor, [&](unsigned long long key) {
             if (static_cast<uint32_t>(key >> 32) < floor) return;
             const int at = atomicAdd(&s.count, 1);
             if (at < kCandidates) s.list[at] = key;
@@ -194,9 +209,9 @@ __device__ __forceinline__ void select_largest(int k, uint32_t best, const Each&
     if (n <= kCandidates) {
         for (int t = threadIdx.x; t < n; t += LANES) {
             const unsigned long long key = s.list[t];
-            int above = 0;
-            for (int j = 0; j < n; ++j) above += s.list[j] > key;
-            if (above < k) put(above, key);
+            int larger = 0;
+            for (int j = 0; j < n; ++j) larger += s.list[j] > key;
+            if (larger < k) put(larger, key);
         }
         for (int t = n + threadIdx.x; t < k; t += LANES) put(t, 0ull);
         return;
@@ -240,16 +255,26 @@ struct Part {
         for (int k = 0; k < K; ++k) {
 #pragma unroll
             for (int i = 0; i < Raw<T, V>::kWords; ++i) kept[k].w[i] = nothing;
-            if (has(k)) kept[k] = load_raw<T, V>(row, at(k));
+            if (has(k)) kept[k] = load_raw_at<T, V>(row + (static_cast<size_t>(first) + k * LANES) * 16, threadIdx.x * 16u);
         }
-        extra = -INFINITY;
         extra_at = whole * V + static_cast<int>(threadIdx.x);
-        if (first_vector + vectors >= whole && extra_at < vocab) extra = load_one<T>(row, extra_at);
-        else extra_at = -1;
+        if (first_vector + vectors < whole || extra_at >= vocab) extra_at = -1;
+        extra = load_one<T>(row, extra_at < 0 ? 0 : extra_at);      // without a branch, whose end would wait for all loads
+        if (extra_at < 0) extra = -INFINITY;
+    }
+
+    // Between two passes over the values: as fp32 numbers, which the compiler would keep from the first, they take twice the
+    // registers that they were read into (8 vectors of bf16: 169 in place of 60, two waves to a unit in place of eight).
+    __device__ __forceinline__ void again()
+    {
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < Raw<T, V>::kWords; ++i) asm volatile("" : "+v"(kept[k].w[i]));
     }
 
     template<bool ENTROPY>
-    __device__ __forceinline__ Sums sums(float c) const
+    __device__ __forceinline__ Sums sums(float c)
     {
         Sums s{ extra, 0.0f, 0.0f };
 #pragma unroll
@@ -259,6 +284,7 @@ struct Part {
 #pragma unroll
             for (int i = 0; i < V; ++i) s.peak = fmaxf(s.peak, l[i]);
         }
+        again();
         const float ref = s.reference();
         const auto take = [&](float l) {
             const float u = (l - ref) * c;
@@ -273,22 +299,38 @@ struct Part {
             kept[k].get(l);
 #pragma unroll
             for (int i = 0; i < V; ++i) take(l[i]);
+            __builtin_amdgcn_sched_barrier(0);      // a vector at a time, in few registers
         }
         return s;
     }
 
+    // f with the keys of all values that are not below `floor` (an order; a NaN is not below anything)
     template<typename F>
-    __device__ __forceinline__ void each(float scale, const F& f) const
+    __device__ __forceinline__ void above(float scale, uint32_t floor, const F& f)
     {
+        again();
+        const float least = value_of(static_cast<unsigned long long>(floor) << 32);
+        const auto look = [&](float l, int index) {
+            const float z = l * scale;
+            if (!(z < least)) f(key_of(z, index));
+        };
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             if (!has(k)) continue;
             float l[V];
             kept[k].get(l);
 #pragma unroll
-            for (int i = 0; i < V; ++i) f(key_of(l[i] * scale, at(k) + i));
+            for (int i = 0; i < V; ++i) look(l[i], at(k) + i);
         }
-        if (extra_at >= 0) f(key_of(extra * scale, extra_at));
+        if (extra_at >= 0) look(extra, extra_at);
+    }
+
+    // f with the keys of all values of the part, read from memory one by one
+    template<typename F>
+    __device__ __forceinline__ void each(const char* row, int vocab, float scale, const F& f) const
+    {
+        const int end = (first + count) * V + V > vocab ? vocab : (first + count) * V;
+        for (int e = first * V + static_cast<int>(threadIdx.x); e < end; e += LANES) f(key_of(load_one<T>(row, e) * scale, e));
     }
 };
 
@@ -312,10 +354,10 @@ __global__ __launch_bounds__(LANES) void token_logprobs_kernel(TokenArgs a, Part
     const char* logits = static_cast<const char*>(a.logits) + row * a.stride * kSize<T>;
     const float c = a.scale * kLog2e;
     const bool whole = p.parts == 1;
+    const int target = whole ? target_of(a, row) : -1;
+    const float given = load_one<T>(logits, target < 0 ? 0 : target);
     Part<T, LANES, K> mine;
     mine.load(logits, a.vocab, static_cast<int>(part) * p.vectors, p.vectors);
-    const int target = whole ? target_of(a, row) : -1;
-    const float given = target < 0 ? 0.0f : load_one<T>(logits, target);
     Sums s = mine.template sums<ENTROPY>(c);
     const float peak = s.peak;
     s = group_join<LANES>(s, c, slots);
@@ -332,7 +374,8 @@ __global__ __launch_bounds__(LANES) void token_logprobs_kernel(TokenArgs a, Part
                 p.keys[static_cast<size_t>(blockIdx.x) * a.top + place] = key;
             }
         };
-        select_largest<LANES>(a.top, any ? order_of(peak * a.scale) : 0u, [&](const auto& f) { mine.each(a.scale, f); }, put, selection);
+        select_largest<LANES>(a.top, any ? order_of(peak * a.scale) : 0u, [&](uint32_t floor, const auto& f) { mine.above(a.scale, floor, f); },
+                              [&](const auto& f) { mine.each(logits, a.vocab, a.scale, f); }, put, selection);
     }
 }
 
@@ -360,11 +403,11 @@ __global__ __launch_bounds__(kBlock) void token_join_kernel(TokenArgs a, Parts p
         const int n = p.parts * a.top;
         uint32_t best = 0;
         for (int k = threadIdx.x; k < n; k += kBlock) best = max(best, static_cast<uint32_t>(keys[k] >> 32));
-        select_largest<kBlock>(a.top, best,
-                               [&](const auto& f) {
-                                   for (int k = threadIdx.x; k < n; k += kBlock)
-                                       if (keys[k]) f(keys[k]);
-                               },
+        const auto each = [&](const auto& f) {
+            for (int k = threadIdx.x; k < n; k += kBlock)
+                if (keys[k]) f(keys[k]);
+        };
+        select_largest<kBlock>(a.top, best, [&](uint32_t, const auto& f) { each(f); }, each,
                                [&](int place, unsigned long long key) {
                                    a.top_ids[row * a.top + place] = static_cast<int>(~static_cast<uint32_t>(key));
                                    a.top_logp[row * a.top + place] = value_of(key) - lse;
@@ -464,11 +507,12 @@ __global__ __launch_bounds__(LANES) void token_train_kernel(TokenArgs a)
     const char* logits = static_cast<const char*>(a.logits) + row * a.stride * kSize<T>;
     char* out = static_cast<char*>(a.dlogits) + row * a.d_stride * kSize<T>;
     const float c = a.scale * kLog2e;
+    const int target = target_of(a, row);
+    const float given = load_one<T>(logits, target < 0 ? 0 : target);       // before it is overwritten
     Part<T, LANES, K> mine;
     mine.load(logits, a.vocab, 0, a.vocab);
-    const int target = target_of(a, row);
-    const float given = target < 0 ? 0.0f : load_one<T>(logits, target);        // before it is overwritten
     const Sums s = group_join<LANES>(mine.template sums<ENTROPY>(c), c, slots);
+    mine.again();
     const RowResult r = finish_row(a, row, s, target, given, threadIdx.x == 0);
     const auto gradient = gradient_of<T, true>(a, row, target, s.peak, r.log_sum, r.entropy);
 #pragma unroll
@@ -479,7 +523,8 @@ __global__ __launch_bounds__(LANES) void token_train_kernel(TokenArgs a)
         gradient.template apply<V>(l, mine.at(k), d);
         Raw<T, V> o;
         o.set(d);
-        store_raw<T, V>(out, mine.at(k), o);
+        store_raw_at<T, V>(out + static_cast<size_t>(k) * LANES * 16, threadIdx.x * 16u, o);
+        __builtin_amdgcn_sched_barrier(0);
     }
     if (mine.extra_at >= 0) {
         float d[1];
@@ -526,6 +571,7 @@ int launch_train(const char* who, const TokenArgs& a, hipStream_t s)
     const int vectors = a.vocab / kVec<T>;
     if (vectors <= 256) hipLaunchKernelGGL((token_train_kernel<T, ENTROPY, 256, 1>), grid, dim3(256), 0, s, a);
     else if (vectors <= 1024) hipLaunchKernelGGL((token_train_kernel<T, ENTROPY, 256, 4>), grid, dim3(256), 0, s, a);
+    else if (vectors <= 2048) hipLaunchKernelGGL((token_train_kernel<T, ENTROPY, 256, 8>), grid, dim3(256), 0, s, a);
     else if (vectors <= 4096) hipLaunchKernelGGL((token_train_kernel<T, ENTROPY, 512, 8>), grid, dim3(512), 0, s, a);
     else if (vectors <= 8192) hipLaunchKernelGGL((token_train_kernel<T, ENTROPY, 1024, 8>), grid, dim3(1024), 0, s, a);
     else if (vectors <= 16384) hipLaunchKernelGGL((token_train_kernel<T, ENTROPY, 1024, 16>), grid, dim3(1024), 0, s, a);

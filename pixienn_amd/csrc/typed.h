@@ -100,6 +100,20 @@ __device__ __forceinline__ void store_raw(void* p, size_t e, const Raw<T, V>& r)
     else *at = b;
 }
 
+// The same at a byte offset of the lane's own from a place that is the workgroup's: an address in scalar registers, one
+// register for the offset however many vectors a lane holds.
+template<int T, int V, bool NT = false>
+__device__ __forceinline__ Raw<T, V> load_raw_at(const char* place, uint32_t offset)
+{
+    return load_raw<T, V, NT>(place + offset, 0);
+}
+
+template<int T, int V, bool NT = false>
+__device__ __forceinline__ void store_raw_at(char* place, uint32_t offset, const Raw<T, V>& r)
+{
+    store_raw<T, V, NT>(place + offset, 0, r);
+}
+
 // One value.
 template<int T>
 __device__ __forceinline__ float load_one(const void* p, size_t e)
