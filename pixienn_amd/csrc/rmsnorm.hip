@@ -234,74 +234,115 @@ struct NormBackwardArgs {
     bool weight_f32;
 };
 
-// dx of every row, and the part of dw that this worker's rows give: a worker (LANES lanes) takes every workers-th row.
+// dx of every row, and the part of dw that this worker's rows give: a worker (LANES lanes) takes every workers-th row, and asks for
+// the next one before it waits for the sum over this one.  At four vectors a lane there are no registers for that, nor for
+// the weights, which are read again for every row.
 template<int T, int LANES, int K>
-__global__ __launch_bounds__(LANES > kBlock ? LANES : kBlock) void rms_norm_backward_kernel(NormBackwardArgs a, int workers)
+__global__ __launch_bounds__(LANES > kWave ? LANES : kBlock) void rms_norm_backward_kernel(NormBackwardArgs a, int workers)
 {
     constexpr int V = kVec<T>;
-    constexpr int kPer = LANES < kBlock ? kBlock / LANES : 1;
-    __shared__ float slots[LANES / kWave + 1];
+    constexpr int kPer = LANES > kWave ? 1 : kBlock / kWave;
+    constexpr int kWaves = LANES / kWave;
+    constexpr bool kAhead = K <= 2;
+    __shared__ float slots[2][kWaves];
     const int lane = threadIdx.x % LANES;
     const int worker = blockIdx.x * kPer + threadIdx.x / LANES;
-    if (worker >= workers) return;
+    if (worker >= workers) return;              // single waves, which wait for nobody
     const int n = a.width;
-    float w[K][V], dw[K][V];
+    float w[kAhead ? K : 1][V], dw[K][V];
 #pragma unroll
     for (int s = 0; s < K; ++s) {
         const int e = (s * LANES + lane) * V;
 #pragma unroll
-        for (int k = 0; k < V; ++k) dw[s][k] = w[s][k] = 0.0f;
-        if (e < n) weights_at<T, V>(a.weight, a.weight_f32, e, n, w[s]);
+        for (int k = 0; k < V; ++k) dw[s][k] = 0.0f;
+        if (kAhead) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) w[s][k] = 0.0f;
+            if (e < n) weights_at<T, V>(a.weight, a.weight_f32, e, n, w[s]);
+        }
     }
-    for (long long row = worker; row < a.rows; row += workers) {
+    struct Row {
+        Raw<T, V> g[K], h[K], more[K];
+        float rstd;
+    };
+    const auto ask = [&](long long row, Row& r) {
+        if (row >= a.rows) return;
         const char* dy = row_of<T>(a.dy, row, a.dy_stride);
         const char* h = row_of<T>(a.h, row, a.h_stride);
-        const float rstd = a.rstd[row];
-        Raw<T, V> rg[K], rh[K];
+        r.rstd = a.rstd[row];
+#pragma unroll
+        for (int s = 0; s < K; ++s) {
+            const int e = (s * LANES + lane) * V;
+            if (e >= n) break;
+            r.g[s] = load_row<T, V>(dy, e, n);
+            r.h[s] = load_row<T, V>(h, e, n);
+            if (kAhead && a.dsum) r.more[s] = load_row<T, V>(row_of<T>(a.dsum, row, a.dsum_stride), e, n);
+        }
+    };
+    Row next;
+    if (kAhead) ask(worker, next);
+    int turn = 0;
+    for (long long row = worker; row < a.rows; row += workers) {
+        if (!kAhead) ask(row, next);
+        const Row r = next;
         float dot = 0.0f;
 #pragma unroll
         for (int s = 0; s < K; ++s) {
             const int e = (s * LANES + lane) * V;
             if (e >= n) break;
-            rg[s] = load_row<T, V>(dy, e, n);
-            rh[s] = load_row<T, V>(h, e, n);
-        }
-#pragma unroll
-        for (int s = 0; s < K; ++s) {
-            const int e = (s * LANES + lane) * V;
-            if (e >= n) break;
-            float g[V], x[V];
-            rg[s].get(g);
-            rh[s].get(x);
+            float g[V], x[V], u[V];
+            r.g[s].get(g);
+            r.h[s].get(x);
+            if (!kAhead) weights_at<T, V>(a.weight, a.weight_f32, e, n, u);
 #pragma unroll
             for (int k = 0; k < V; ++k) {
-                const float xhat = x[k] * rstd;
+                const float xhat = x[k] * r.rstd;
                 dw[s][k] = fmaf(g[k], xhat, dw[s][k]);
-                dot = fmaf(g[k] * w[s][k], xhat, dot);
+                dot = fmaf(g[k] * (kAhead ? w[kAhead ? s : 0][k] : u[k]), xhat, dot);
             }
         }
-        const float c = group_sum<LANES>(dot, slots) / static_cast<float>(n);
+        if (kAhead) ask(row + workers, next);
+        dot = wave_sum_by_rows(dot);
+        if constexpr (kWaves > 1) {
+            // two places in turn: no wave is more than one row ahead of another
+            float* const slot = slots[turn];
+            turn ^= 1;
+            if ((lane & (kWave - 1)) == 0) slot[lane / kWave] = dot;
+            __syncthreads();
+            dot = slot[0];
+#pragma unroll
+            for (int k = 1; k < kWaves; ++k) dot += slot[k];
+        }
+        const float c = r.rstd * (dot / static_cast<float>(n));
 #pragma unroll
         for (int s = 0; s < K; ++s) {
             const int e = (s * LANES + lane) * V;
             if (e >= n) break;
-            float g[V], x[V], more[V] = {};
-            rg[s].get(g);
-            rh[s].get(x);
-            if (a.dsum) load_row<T, V>(row_of<T>(a.dsum, row, a.dsum_stride), e, n).get(more);
+            float g[V], x[V], u[V], more[V] = {};
+            r.g[s].get(g);
+            r.h[s].get(x);
+            if (!kAhead) weights_at<T, V>(a.weight, a.weight_f32, e, n, u);
+            if (a.dsum) {
+                if (kAhead) r.more[s].get(more);
+                else load_row<T, V>(row_of<T>(a.dsum, row, a.dsum_stride), e, n).get(more);
+            }
 #pragma unroll
-            for (int k = 0; k < V; ++k) g[k] = fmaf(rstd, g[k] * w[s][k] - x[k] * rstd * c, more[k]);
-            Raw<T, V> r;
-            r.set(g);
-            store_row<T, V>(row_of<T>(a.dx, row, a.dx_stride), e, n, r);
+            for (int k = 0; k < V; ++k) g[k] = fmaf(r.rstd, g[k] * (kAhead ? w[kAhead ? s : 0][k] : u[k]) - x[k] * c, more[k]);
+            Raw<T, V> out;
+            out.set(g);
+            store_row<T, V>(row_of<T>(a.dx, row, a.dx_stride), e, n, out);
         }
     }
 #pragma unroll
     for (int s = 0; s < K; ++s) {
         const int e = (s * LANES + lane) * V;
+        Raw<PXH_F32, 4> part;
 #pragma unroll
-        for (int k = 0; k < V; ++k)
-            if (e + k < n) a.partial[static_cast<size_t>(worker) * n + e + k] = dw[s][k];
+        for (int q = 0; q < V; q += 4) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) part.w[k] = __float_as_uint(dw[s][q + k]);
+            store_row<PXH_F32, 4>(a.partial + static_cast<size_t>(worker) * n, e + q, n, part);
+        }
     }
 }
 
@@ -352,39 +393,48 @@ __global__ __launch_bounds__(kBlock) void rms_norm_wide_dw_kernel(NormBackwardAr
     a.partial[static_cast<size_t>(blockIdx.y) * a.width + e] = dw;
 }
 
-// dw[column] (+)= the sum of the workers' parts.
+// dw[column] (+)= the sum of the workers' parts: 64 columns to a workgroup, whose waves share the workers.
 __global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const float* partial, int workers, int width, float* dw, int accumulate)
 {
-    __shared__ float sums[16][kWave];
-    const int column = blockIdx.x * kWave + threadIdx.x % kWave, part = threadIdx.x / kWave;
+    constexpr int kWaves = 16, kAhead = 8;
+    __shared__ float sums[kWaves][kWave];
+    const int column = blockIdx.x * kWave + threadIdx.x % kWave, wave = threadIdx.x / kWave;
     float sum = 0.0f;
-    if (column < width)
-        for (int w = part; w < workers; w += 16) sum += partial[static_cast<size_t>(w) * width + column];
-    sums[part][threadIdx.x % kWave] = sum;
+    if (column < width) {
+        int w = wave;
+        for (; w + (kAhead - 1) * kWaves < workers; w += kAhead * kWaves) {
+            float v[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) v[k] = partial[static_cast<size_t>(w + k * kWaves) * width + column];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) sum += v[k];
+        }
+        for (; w < workers; w += kWaves) sum += partial[static_cast<size_t>(w) * width + column];
+    }
+    sums[wave][threadIdx.x % kWave] = sum;
     __syncthreads();
-    if (part == 0 && column < width) {
-        float total = accumulate ? dw[column] : 0.0f;
+    if (wave == 0 && column < width) {
         float all = 0.0f;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) all += sums[k][threadIdx.x];
-        dw[column] = total + all;
+        for (int k = 0; k < kWaves; ++k) all += sums[k][threadIdx.x];
+        dw[column] = accumulate ? dw[column] + all : all;
     }
 }
 
-// Workers that share the rows of the backward pass, each with a row of partial sums: fewer for wide rows, so that the
-// partial sums stay small beside the tensors.
+// Workers that share the rows of the backward pass, each with a row of partial sums: two to four workgroups for each of 256
+// compute units, as wide as a row; fewer for the widest rows, so that the partial sums stay small beside the tensors.
 constexpr int kWideWorkers = 32;
 int workers_for(long long rows, int width)
 {
-    const int most = width <= 16384 ? 1024 : width <= 32768 ? 256 : kWideWorkers;
+    const int most = width <= 4096 ? 1024 : width <= 16384 ? 512 : width <= 32768 ? 256 : kWideWorkers;
     return static_cast<int>(rows < most ? rows : most);
 }
 
 template<int T, int LANES, int K>
 int launch_backward(const NormBackwardArgs& a, int workers, hipStream_t s)
 {
-    constexpr int kPer = LANES < kBlock ? kBlock / LANES : 1;
-    hipLaunchKernelGGL((rms_norm_backward_kernel<T, LANES, K>), dim3(grid_for(workers, kPer)), dim3(LANES < kBlock ? kBlock : LANES), 0, s, a, workers);
+    constexpr int kPer = LANES > kWave ? 1 : kBlock / kWave;
+    hipLaunchKernelGGL((rms_norm_backward_kernel<T, LANES, K>), dim3(grid_for(workers, kPer)), dim3(LANES * kPer), 0, s, a, workers);
     return check_launch("pxh_rms_norm_backward");
 }
 
@@ -393,9 +443,11 @@ int norm_backward(const NormBackwardArgs& a, int& workers, hipStream_t s)
 {
     const int vectors = (a.width + kVec<T> - 1) / kVec<T>;
     if (vectors <= 64) return launch_backward<T, 64, 1>(a, workers, s);
+    if (vectors <= 128) return launch_backward<T, 128, 1>(a, workers, s);
     if (vectors <= 256) return launch_backward<T, 256, 1>(a, workers, s);
-    if (vectors <= 512) return launch_backward<T, 256, 2>(a, workers, s);
-    if (vectors <= 1024) return launch_backward<T, 512, 2>(a, workers, s);
+    if (vectors <= 512) return launch_backward<T, 512, 1>(a, workers, s);
+    if (vectors <= 1024) return launch_backward<T, 1024, 1>(a, workers, s);
+    if (vectors <= 2048) return launch_backward<T, 1024, 2>(a, workers, s);
     if (vectors <= 4096) return launch_backward<T, 1024, 4>(a, workers, s);
     if (workers > kWideWorkers) workers = kWideWorkers;
     hipLaunchKernelGGL((rms_norm_wide_dw_kernel<T>), dim3(grid_for(a.width, kBlock), workers), dim3(kBlock), 0, s, a, workers);
@@ -454,7 +506,7 @@ size_t pxh_rms_norm_workspace_bytes(long long rows, int width)
     if (rows <= 0 || width <= 0) return 0;
     // the largest that any of the shapes up to this one takes
     size_t most = 0;
-    for (int w: { 16384, 32768, width }) {
+    for (int w: { 4096, 16384, 32768, width }) {
         const int here = width < w ? width : w;
         const size_t floats = static_cast<size_t>(workers_for(rows, here)) * static_cast<size_t>(here);
         if (floats > most) most = floats;
