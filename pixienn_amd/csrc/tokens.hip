@@ -1,4 +1,5 @@
 // Log probabilities of given tokens, entropy, the most probable alternatives, and the gradient of the logits.
+#include "stream.h"
 #include "typed.h"
 
 #include <cmath>
@@ -235,15 +236,18 @@ __device__ __forceinline__ void select_largest(int k, uint32_t best, const Above
 // ---------------------------------------------------------------- a part of a row
 // Vectors first .. first + count of a row, K to a lane, and of the row's last values, which fill no vector, one to each of the
 // first lanes of the part that has them.  What is not there is minus infinity.
-template<int T, int LANES, int K>
+template<int T, int LANES, int K, bool NT>
 struct Part {
     static constexpr int V = kVec<T>;
     Raw<T, V> kept[K];
-    float extra;
+    float extra, peak;          // peak: the largest of the lane's values, from sums()
     int first, count, extra_at;
 
     __device__ __forceinline__ bool has(int k) const { return k * LANES + static_cast<int>(threadIdx.x) < count; }
     __device__ __forceinline__ int at(int k) const { return (first + k * LANES + static_cast<int>(threadIdx.x)) * V; }
+
+    // of the part's values, in a row of `vocab`
+    __device__ __forceinline__ int end(int vocab) const { return (first + count) * V + V > vocab ? vocab : (first + count) * V; }
 
     __device__ __forceinline__ void load(const char* row, int vocab, int first_vector, int vectors)
     {
@@ -255,7 +259,7 @@ struct Part {
         for (int k = 0; k < K; ++k) {
 #pragma unroll
             for (int i = 0; i < Raw<T, V>::kWords; ++i) kept[k].w[i] = nothing;
-            if (has(k)) kept[k] = load_raw_at<T, V>(row + (static_cast<size_t>(first) + k * LANES) * 16, threadIdx.x * 16u);
+            if (has(k)) kept[k] = load_raw_at<T, V, NT>(row + (static_cast<size_t>(first) + k * LANES) * 16, threadIdx.x * 16u);
         }
         extra_at = whole * V + static_cast<int>(threadIdx.x);
         if (first_vector + vectors < whole || extra_at >= vocab) extra_at = -1;
@@ -267,40 +271,76 @@ struct Part {
     // registers that they were read into (8 vectors of bf16: 169 in place of 60, two waves to a unit in place of eight).
     __device__ __forceinline__ void again()
     {
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-#pragma unroll
-            for (int i = 0; i < Raw<T, V>::kWords; ++i) asm volatile("" : "+v"(kept[k].w[i]));
-    }
-
-    template<bool ENTROPY>
-    __device__ __forceinline__ Sums sums(float c)
-    {
-        Sums s{ extra, 0.0f, 0.0f };
+        typedef uint32_t words __attribute__((ext_vector_type(4)));
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            float l[V];
-            kept[k].get(l);
-#pragma unroll
-            for (int i = 0; i < V; ++i) s.peak = fmaxf(s.peak, l[i]);
+            words w = __builtin_bit_cast(words, kept[k]);
+            asm volatile("" : "+v"(w));
+            kept[k] = __builtin_bit_cast(Raw<T, V>, w);
         }
+    }
+
+    // The sums of the lane's values.  An exponent is one fused multiply-add, l * c - peak * c (which a half-precision value enters
+    // without being converted first), where the rounding of peak * c is less than 2^-4: it is the same in all of the lane's
+    // exponents, and taken out of the sums at the end.  Beyond that, in rows of huge values, (l - peak) * c, value by value
+    // from memory: two ways through the registers would hold them twice.
+    template<bool ENTROPY>
+    __device__ __forceinline__ Sums sums(const char* row, float c)
+    {
+        peak = largest();
         again();
+        Sums s{ peak, 0.0f, 0.0f };
         const float ref = s.reference();
-        const auto take = [&](float l) {
-            const float u = (l - ref) * c;
+        const float shift = ref * c;
+        if (!__all(fabsf(shift) < 0x1p20f)) return far_sums(row, c);
+        const auto add = [&](float l) {
+            const float u = fmaf(l, c, -shift);
             const float e = __builtin_amdgcn_exp2f(u);
             s.sum += e;
             if (ENTROPY) s.weighted = fmaf(e, fmaxf(u, kFar), s.weighted);
         };
-        take(extra);
+        add(extra);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             float l[V];
             kept[k].get(l);
 #pragma unroll
-            for (int i = 0; i < V; ++i) take(l[i]);
-            __builtin_amdgcn_sched_barrier(0);      // a vector at a time, in few registers
+            for (int i = 0; i < V; ++i) add(l[i]);
+            __builtin_amdgcn_sched_barrier(0);
         }
+        const float off = fmaf(ref, c, -shift), f = __builtin_amdgcn_exp2f(-off);
+        s.weighted = f * fmaf(-off, s.sum, s.weighted);
+        s.sum *= f;
+        return s;
+    }
+
+    __device__ __forceinline__ float largest() const
+    {
+        float most = extra;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            if constexpr (T == PXH_F16) {
+                typedef _Float16 two __attribute__((ext_vector_type(2)));
+                two pair = __builtin_bit_cast(two, kept[k].w[0]);
+#pragma unroll
+                for (int i = 1; i < Raw<T, V>::kWords; ++i) pair = __builtin_elementwise_max(pair, __builtin_bit_cast(two, kept[k].w[i]));
+                most = fmaxf(most, fmaxf(static_cast<float>(pair.x), static_cast<float>(pair.y)));
+            } else {
+                float l[V];
+                kept[k].get(l);
+#pragma unroll
+                for (int i = 0; i < V; ++i) most = fmaxf(most, l[i]);
+            }
+            __builtin_amdgcn_sched_barrier(0);          // a vector at a time, in few registers
+        }
+        return most;
+    }
+
+    __device__ __forceinline__ Sums far_sums(const char* row, float c) const
+    {
+        Sums s{ extra, extra == -INFINITY ? 0.0f : 1.0f, 0.0f };
+        for (int k = 0; k < K && has(k); ++k)
+            for (int i = 0; i < V; ++i) s.template add<1>({ load_one<T>(row, at(k) + i) }, c);
         return s;
     }
 
@@ -329,8 +369,7 @@ struct Part {
     template<typename F>
     __device__ __forceinline__ void each(const char* row, int vocab, float scale, const F& f) const
     {
-        const int end = (first + count) * V + V > vocab ? vocab : (first + count) * V;
-        for (int e = first * V + static_cast<int>(threadIdx.x); e < end; e += LANES) f(key_of(load_one<T>(row, e) * scale, e));
+        for (int e = first * V + static_cast<int>(threadIdx.x); e < end(vocab); e += LANES) f(key_of(load_one<T>(row, e) * scale, e));
     }
 };
 
@@ -344,7 +383,7 @@ struct Parts {
     FastDiv by_parts;
 };
 
-template<int T, bool ENTROPY, int LANES, int K>
+template<int T, bool ENTROPY, int LANES, int K, bool NT>
 __global__ __launch_bounds__(LANES) void token_logprobs_kernel(TokenArgs a, Parts p)
 {
     __shared__ Sums slots[LANES / kWave];
@@ -356,11 +395,9 @@ __global__ __launch_bounds__(LANES) void token_logprobs_kernel(TokenArgs a, Part
     const bool whole = p.parts == 1;
     const int target = whole ? target_of(a, row) : -1;
     const float given = load_one<T>(logits, target < 0 ? 0 : target);
-    Part<T, LANES, K> mine;
+    Part<T, LANES, K, NT> mine;
     mine.load(logits, a.vocab, static_cast<int>(part) * p.vectors, p.vectors);
-    Sums s = mine.template sums<ENTROPY>(c);
-    const float peak = s.peak;
-    s = group_join<LANES>(s, c, slots);
+    const Sums s = group_join<LANES>(mine.template sums<ENTROPY>(logits, c), c, slots);
     float lse = 0.0f;
     if (whole) lse = finish_row(a, row, s, target, given, threadIdx.x == 0).lse;
     else if (threadIdx.x == 0) p.sums[blockIdx.x] = s;
@@ -374,7 +411,7 @@ __global__ __launch_bounds__(LANES) void token_logprobs_kernel(TokenArgs a, Part
                 p.keys[static_cast<size_t>(blockIdx.x) * a.top + place] = key;
             }
         };
-        select_largest<LANES>(a.top, any ? order_of(peak * a.scale) : 0u, [&](uint32_t floor, const auto& f) { mine.above(a.scale, floor, f); },
+        select_largest<LANES>(a.top, any ? order_of(mine.peak * a.scale) : 0u, [&](uint32_t floor, const auto& f) { mine.above(a.scale, floor, f); },
                               [&](const auto& f) { mine.each(logits, a.vocab, a.scale, f); }, put, selection);
     }
 }
@@ -421,14 +458,31 @@ __global__ __launch_bounds__(kBlock) void token_join_kernel(TokenArgs a, Parts p
 // From the row's own sums log p = (l - peak) * scale - log(sum), which is right however large the logits are; from a stored lse,
 // which fp32 has rounded, log p = l * scale - lse.  The hardware's exp2 has no results below 2^-126; a type that has them
 // gets them from the square of half the exponent's power.
+// A 16-bit gradient of logp alone takes its exponent from one fused multiply-add, l * c - shift, where the shift is below 2^10 and
+// its rounding, below 2^-14, far less than the result's own: 8.5 instructions a value in place of 13 (an exponential counts four).
 template<int T, bool PEAK>
 struct RowGradient {
-    float peak, rest, scale, entropy, g, h;
+    float peak, rest, scale, entropy, g, h, c, shift;
     int target;
+    bool quick;
 
-    template<int V>
+    // QUICK where `quick` says so
+    template<int V, bool QUICK>
     __device__ __forceinline__ void apply(const float (&l)[V], int e, float (&d)[V]) const
     {
+        if constexpr (T != PXH_F32 && QUICK) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                if constexpr (T == PXH_F16) {
+                    d[k] = -g * __builtin_amdgcn_exp2f(fmaf(l[k], c, -shift));
+                } else {
+                    const float root = __builtin_amdgcn_exp2f(fmaf(l[k], c, -shift));
+                    d[k] = -g * root * root;
+                }
+            }
+            hit<V>(e, d);
+            return;
+        }
 #pragma unroll
         for (int k = 0; k < V; ++k) {
             const float logp = fmaf(PEAK ? l[k] - peak : l[k], scale, -rest);
@@ -442,6 +496,13 @@ struct RowGradient {
             d[k] = -g * p;
             if (h != 0.0f) d[k] -= h * p * (fmaxf(logp, kFar) + entropy);
         }
+        hit<V>(e, d);
+    }
+
+    // the given token's own part
+    template<int V>
+    __device__ __forceinline__ void hit(int e, float (&d)[V]) const
+    {
         if (static_cast<uint32_t>(target - e) < static_cast<uint32_t>(V)) {
 #pragma unroll
             for (int k = 0; k < V; ++k)
@@ -467,13 +528,18 @@ __device__ __forceinline__ RowGradient<T, PEAK> gradient_of(const TokenArgs& a, 
         r.rest = INFINITY;
         r.peak = r.g = r.h = 0.0f;
     }
+    r.c = a.scale * (T == PXH_F16 ? kLog2e : 0.5f * kLog2e);
+    r.shift = fmaf(r.peak, a.scale, r.rest) * (T == PXH_F16 ? kLog2e : 0.5f * kLog2e);
+    r.quick = __builtin_amdgcn_readfirstlane(r.h == 0.0f && fabsf(r.shift) < 0x1p10f);
     return r;
 }
 
-// A workgroup takes one part of a row.
-constexpr int kGradientSteps = 4;
+// A workgroup takes one part of a row.  Past the caches in short parts (1000 x 100001 fp32: 149 us with four steps through the caches, 144
+// with four past them, 137 with two), within them in longer ones (512 x 32768 bf16: 11.5 us, and 13 past them).
+template<bool NT>
+constexpr int kGradientSteps = NT ? 2 : 4;
 
-template<int T>
+template<int T, bool NT>
 __global__ __launch_bounds__(kBlock) void token_gradient_kernel(TokenArgs a, FastDiv parts)
 {
     constexpr int V = kVec<T>;
@@ -482,23 +548,27 @@ __global__ __launch_bounds__(kBlock) void token_gradient_kernel(TokenArgs a, Fas
     const auto r = gradient_of<T, false>(a, row, target_of(a, row), 0.0f, a.lse_in[row], a.d_entropy ? a.entropy_in[row] : 0.0f);
     const char* logits = static_cast<const char*>(a.logits) + row * a.stride * kSize<T>;
     char* out = static_cast<char*>(a.dlogits) + row * a.d_stride * kSize<T>;
+    const auto write = [&]<bool QUICK>() {
 #pragma unroll
-    for (int s = 0; s < kGradientSteps; ++s) {
-        const int e = ((part * kGradientSteps + s) * kBlock + threadIdx.x) * V;
-        if (e >= a.vocab) break;
-        float l[V], d[V];
-        load_row<T, V>(logits, e, a.vocab).get(l);
-        r.template apply<V>(l, e, d);
-        Raw<T, V> raw;
-        raw.set(d);
-        store_row<T, V>(out, e, a.vocab, raw);
-    }
+        for (int s = 0; s < kGradientSteps<NT>; ++s) {
+            const int e = ((part * kGradientSteps<NT> + s) * kBlock + threadIdx.x) * V;
+            if (e >= a.vocab) break;
+            float l[V], d[V];
+            load_row<T, V, NT>(logits, e, a.vocab).get(l);
+            r.template apply<V, QUICK>(l, e, d);
+            Raw<T, V> raw;
+            raw.set(d);
+            store_row<T, V, NT>(out, e, a.vocab, raw);
+        }
+    };
+    if (T != PXH_F32 && r.quick) write.template operator()<true>();
+    else write.template operator()<false>();
 }
 
 // ---------------------------------------------------------------- forward and gradient at once
 // A workgroup per row, which stays in registers between its sums and its gradient.  A lane writes the values that it has read, so the
 // gradient may take the logits' place.
-template<int T, bool ENTROPY, int LANES, int K>
+template<int T, bool ENTROPY, int LANES, int K, bool NT>
 __global__ __launch_bounds__(LANES) void token_train_kernel(TokenArgs a)
 {
     constexpr int V = kVec<T>;
@@ -509,27 +579,134 @@ __global__ __launch_bounds__(LANES) void token_train_kernel(TokenArgs a)
     const float c = a.scale * kLog2e;
     const int target = target_of(a, row);
     const float given = load_one<T>(logits, target < 0 ? 0 : target);       // before it is overwritten
-    Part<T, LANES, K> mine;
+    Part<T, LANES, K, NT> mine;
     mine.load(logits, a.vocab, 0, a.vocab);
-    const Sums s = group_join<LANES>(mine.template sums<ENTROPY>(c), c, slots);
-    mine.again();
+    const Sums s = group_join<LANES>(mine.template sums<ENTROPY>(logits, c), c, slots);
     const RowResult r = finish_row(a, row, s, target, given, threadIdx.x == 0);
     const auto gradient = gradient_of<T, true>(a, row, target, s.peak, r.log_sum, r.entropy);
+    mine.again();
+    const auto write = [&]<bool QUICK>() {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        if (!mine.has(k)) continue;
-        float l[V], d[V];
-        mine.kept[k].get(l);
-        gradient.template apply<V>(l, mine.at(k), d);
-        Raw<T, V> o;
-        o.set(d);
-        store_raw_at<T, V>(out + static_cast<size_t>(k) * LANES * 16, threadIdx.x * 16u, o);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int k = 0; k < K; ++k) {
+            if (!mine.has(k)) continue;
+            float l[V], d[V];
+            mine.kept[k].get(l);
+            gradient.template apply<V, QUICK>(l, mine.at(k), d);
+            Raw<T, V> o;
+            o.set(d);
+            store_raw_at<T, V>(out + static_cast<size_t>(k) * LANES * 16, threadIdx.x * 16u, o);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (mine.extra_at >= 0) {
+            float d[1];
+            gradient.template apply<1, QUICK>({ mine.extra }, mine.extra_at, d);
+            store_one<T>(out, mine.extra_at, d[0]);
+        }
+    };
+    if (T != PXH_F32 && gradient.quick) write.template operator()<true>();
+    else write.template operator()<false>();
+}
+
+// The same for a gradient of logp alone over rows of up to 4096 vectors: not the values stay in registers but their powers, so that
+// there is one exponential a value and not two (13 instructions a value of bf16 in place of 17, counting an exponential as four;
+// 8192 x 32768: 203 -> 192 us).  A type with results below 2^-126 keeps their roots.
+template<int T, bool ENTROPY, int LANES, int K, bool NT>
+__global__ __launch_bounds__(LANES) void token_powers_kernel(TokenArgs a)
+{
+    constexpr int V = kVec<T>;
+    constexpr bool kRoots = T != PXH_F16;
+    __shared__ Sums slots[LANES / kWave];
+    const long long row = blockIdx.x;
+    const char* logits = static_cast<const char*>(a.logits) + row * a.stride * kSize<T>;
+    char* out = static_cast<char*>(a.dlogits) + row * a.d_stride * kSize<T>;
+    const float c = a.scale * kLog2e;
+    const int target = target_of(a, row);
+    const float given = load_one<T>(logits, target < 0 ? 0 : target);       // before it is overwritten
+    float power[K][V], last;
+    float peak, shift, off;
+    Sums s;
+    bool near;
+    {
+        Part<T, LANES, K, NT> mine;
+        mine.load(logits, a.vocab, 0, a.vocab);
+        last = mine.extra;
+        peak = mine.largest();
+        s = Sums{ peak, 0.0f, 0.0f };
+        const float ref = s.reference();
+        shift = ref * c;
+        near = __all(fabsf(shift) < 0x1p20f);       // as in sums()
+        off = fmaf(ref, c, -shift);
+        if (near) {
+            const float c1 = kRoots ? 0.5f * c : c, shift1 = kRoots ? 0.5f * shift : shift;
+            const auto take = [&](float l) {
+                const float u = fmaf(l, c1, -shift1);
+                const float r = __builtin_amdgcn_exp2f(u);
+                const float e = kRoots ? r * r : r;
+                s.sum += e;
+                if (ENTROPY) s.weighted = fmaf(e, fmaxf(u, kFar), s.weighted);
+                return r;
+            };
+            last = take(last);
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                float l[V];
+                mine.kept[k].get(l);
+#pragma unroll
+                for (int i = 0; i < V; ++i) power[k][i] = take(l[i]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            if (kRoots) s.weighted *= 2.0f;
+            const float f = __builtin_amdgcn_exp2f(-off);
+            s.weighted = f * fmaf(-off, s.sum, s.weighted);
+            s.sum *= f;
+        } else {
+            s = mine.far_sums(logits, c);
+        }
     }
-    if (mine.extra_at >= 0) {
-        float d[1];
-        gradient.template apply<1>({ mine.extra }, mine.extra_at, d);
-        store_one<T>(out, mine.extra_at, d[0]);
+    s = group_join<LANES>(s, c, slots);
+    const RowResult r = finish_row(a, row, s, target, given, threadIdx.x == 0);
+    const auto gradient = gradient_of<T, true>(a, row, target, s.peak, r.log_sum, r.entropy);
+    const int count = a.vocab / V;
+    const int extra_at = count * V + static_cast<int>(threadIdx.x) < a.vocab ? count * V + static_cast<int>(threadIdx.x) : -1;
+    if (near) {
+        // p = power * 2^((lane's peak - row's peak) * c - off) / sum
+        float f = peak == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(((peak - s.peak) * c - off) * (kRoots ? 0.5f : 1.0f));
+        const float scaled = gradient.g == 0.0f ? 0.0f : -gradient.g / s.sum;
+        if (!kRoots) f *= scaled;
+        const auto result = [&](float r) {
+            const float q = r * f;
+            return kRoots ? scaled * q * q : q;
+        };
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            if (k * LANES + static_cast<int>(threadIdx.x) >= count) continue;
+            float d[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) d[i] = result(power[k][i]);
+            gradient.template hit<V>((k * LANES + static_cast<int>(threadIdx.x)) * V, d);
+            Raw<T, V> o;
+            o.set(d);
+            store_raw_at<T, V>(out + static_cast<size_t>(k) * LANES * 16, threadIdx.x * 16u, o);
+        }
+        if (extra_at >= 0) {
+            float d[1] = { result(last) };
+            gradient.template hit<1>(extra_at, d);
+            store_one<T>(out, extra_at, d[0]);
+        }
+    } else {
+        for (int v = threadIdx.x; v < count; v += LANES) {
+            float l[V], d[V];
+            load_raw<T, V>(logits, static_cast<size_t>(v) * V).get(l);
+            gradient.template apply<V, false>(l, v * V, d);
+            Raw<T, V> o;
+            o.set(d);
+            store_raw<T, V>(out, static_cast<size_t>(v) * V, o);
+        }
+        if (extra_at >= 0) {
+            float d[1];
+            gradient.template apply<1, false>({ last }, extra_at, d);
+            store_one<T>(out, extra_at, d[0]);
+        }
     }
 }
 
@@ -557,27 +734,40 @@ __global__ __launch_bounds__(1024) void token_train_long_kernel(TokenArgs a)
     for (int e = threadIdx.x * V; e < a.vocab; e += 1024 * V) {
         float l[V], d[V];
         load_row<T, V>(logits, e, a.vocab).get(l);
-        gradient.template apply<V>(l, e, d);
+        gradient.template apply<V, false>(l, e, d);
         Raw<T, V> o;
         o.set(d);
         store_row<T, V>(out, e, a.vocab, o);
     }
 }
 
-template<int T, bool ENTROPY>
+// The logits past the caches where they and the gradient do not fit (8192 x 32768 bf16 192 -> 187 us; 512 x 32768 would lose 8 %).
+template<int T, bool ENTROPY, bool NT>
 int launch_train(const char* who, const TokenArgs& a, hipStream_t s)
 {
     const dim3 grid(static_cast<unsigned>(a.rows));
     const int vectors = a.vocab / kVec<T>;
-    if (vectors <= 256) hipLaunchKernelGGL((token_train_kernel<T, ENTROPY, 256, 1>), grid, dim3(256), 0, s, a);
-    else if (vectors <= 1024) hipLaunchKernelGGL((token_train_kernel<T, ENTROPY, 256, 4>), grid, dim3(256), 0, s, a);
-    else if (vectors <= 2048) hipLaunchKernelGGL((token_train_kernel<T, ENTROPY, 256, 8>), grid, dim3(256), 0, s, a);
-    else if (vectors <= 4096) hipLaunchKernelGGL((token_train_kernel<T, ENTROPY, 512, 8>), grid, dim3(512), 0, s, a);
-    else if (vectors <= 8192) hipLaunchKernelGGL((token_train_kernel<T, ENTROPY, 1024, 8>), grid, dim3(1024), 0, s, a);
-    else if (vectors <= 16384) hipLaunchKernelGGL((token_train_kernel<T, ENTROPY, 1024, 16>), grid, dim3(1024), 0, s, a);
-    else if (vectors <= 20480) hipLaunchKernelGGL((token_train_kernel<T, ENTROPY, 1024, 20>), grid, dim3(1024), 0, s, a);
+    if (!a.d_entropy && vectors <= 4096) {
+        if (vectors <= 256) hipLaunchKernelGGL((token_powers_kernel<T, ENTROPY, 256, 1, NT>), grid, dim3(256), 0, s, a);
+        else if (vectors <= 1024) hipLaunchKernelGGL((token_powers_kernel<T, ENTROPY, 256, 4, NT>), grid, dim3(256), 0, s, a);
+        else if (vectors <= 2048) hipLaunchKernelGGL((token_powers_kernel<T, ENTROPY, 512, 4, NT>), grid, dim3(512), 0, s, a);
+        else hipLaunchKernelGGL((token_powers_kernel<T, ENTROPY, 512, 8, NT>), grid, dim3(512), 0, s, a);
+        return check_launch(who);
+    }
+    if (vectors <= 256) hipLaunchKernelGGL((token_train_kernel<T, ENTROPY, 256, 1, NT>), grid, dim3(256), 0, s, a);
+    else if (vectors <= 1024) hipLaunchKernelGGL((token_train_kernel<T, ENTROPY, 256, 4, NT>), grid, dim3(256), 0, s, a);
+    else if (vectors <= 4096) hipLaunchKernelGGL((token_train_kernel<T, ENTROPY, 512, 8, NT>), grid, dim3(512), 0, s, a);
+    else if (vectors <= 8192) hipLaunchKernelGGL((token_train_kernel<T, ENTROPY, 1024, 8, NT>), grid, dim3(1024), 0, s, a);
+    else if (vectors <= 16384) hipLaunchKernelGGL((token_train_kernel<T, ENTROPY, 1024, 16, NT>), grid, dim3(1024), 0, s, a);
+    else if (vectors <= 20480) hipLaunchKernelGGL((token_train_kernel<T, ENTROPY, 1024, 20, NT>), grid, dim3(1024), 0, s, a);
     else hipLaunchKernelGGL((token_train_long_kernel<T>), grid, dim3(1024), 0, s, a);
     return check_launch(who);
+}
+
+// Whether tensors of the logits' size, `tensors` of them, go past the caches.
+inline bool streams(const TokenArgs& a, int type, int tensors)
+{
+    return static_cast<size_t>(a.rows) * static_cast<size_t>(a.vocab) * size_of(type) * tensors >= kStreamingBytes;
 }
 
 // Workgroups that fill the machine four times over: from there on a workgroup takes as much as its registers hold.
@@ -609,10 +799,13 @@ int launch_forward(const char* who, const TokenArgs& a, void* workspace, hipStre
     p.sums = reinterpret_cast<Sums*>(static_cast<char*>(workspace) + groups * a.top * sizeof(unsigned long long));
     const dim3 grid(static_cast<unsigned>(groups)), block(kBlock);
     switch (k) {
-    case 1: hipLaunchKernelGGL((token_logprobs_kernel<T, ENTROPY, kBlock, 1>), grid, block, 0, s, a, p); break;
-    case 2: hipLaunchKernelGGL((token_logprobs_kernel<T, ENTROPY, kBlock, 2>), grid, block, 0, s, a, p); break;
-    case 4: hipLaunchKernelGGL((token_logprobs_kernel<T, ENTROPY, kBlock, 4>), grid, block, 0, s, a, p); break;
-    default: hipLaunchKernelGGL((token_logprobs_kernel<T, ENTROPY, kBlock, 8>), grid, block, 0, s, a, p); break;
+    case 1: hipLaunchKernelGGL((token_logprobs_kernel<T, ENTROPY, kBlock, 1, false>), grid, block, 0, s, a, p); break;
+    case 2: hipLaunchKernelGGL((token_logprobs_kernel<T, ENTROPY, kBlock, 2, false>), grid, block, 0, s, a, p); break;
+    case 4: hipLaunchKernelGGL((token_logprobs_kernel<T, ENTROPY, kBlock, 4, false>), grid, block, 0, s, a, p); break;
+    default:
+        // past the caches where the logits do not fit (4096 x 50001 half: 101.5 -> 99.5 us)
+        if (streams(a, T, 1)) hipLaunchKernelGGL((token_logprobs_kernel<T, ENTROPY, kBlock, 8, true>), grid, block, 0, s, a, p);
+        else hipLaunchKernelGGL((token_logprobs_kernel<T, ENTROPY, kBlock, 8, false>), grid, block, 0, s, a, p);
     }
     if (int rc = check_launch(who)) return rc;
     if (p.parts == 1) return PXH_OK;
@@ -620,12 +813,12 @@ int launch_forward(const char* who, const TokenArgs& a, void* workspace, hipStre
     return check_launch(who);
 }
 
-template<int T>
+template<int T, bool NT>
 int launch_gradient(const char* who, const TokenArgs& a, hipStream_t s)
 {
-    const int per = kGradientSteps * kBlock * kVec<T>;
+    const int per = kGradientSteps<NT> * kBlock * kVec<T>;
     const int parts = a.vocab / per + (a.vocab % per != 0);
-    hipLaunchKernelGGL((token_gradient_kernel<T>), dim3(static_cast<unsigned>(a.rows) * parts), dim3(kBlock), 0, s, a, FastDiv(parts));
+    hipLaunchKernelGGL((token_gradient_kernel<T, NT>), dim3(static_cast<unsigned>(a.rows) * parts), dim3(kBlock), 0, s, a, FastDiv(parts));
     return check_launch(who);
 }
 
@@ -728,7 +921,7 @@ int pxh_token_logprobs_backward(const void* logits, const void* targets, const f
     a.dlogits = dlogits; a.rows = rows; a.stride = stride; a.d_stride = d_stride; a.vocab = vocab; a.wide = wide_targets; a.scale = scale;
     hipStream_t s = as_stream(stream);
     int rc = PXH_OK;
-    dispatch_type(type, [&]<int T>() { rc = by_rows(a, T, [&](const TokenArgs& p) { return launch_gradient<T>(who, p, s); }); });
+    dispatch_type(type, [&]<int T>() { rc = by_rows(a, T, [&](const TokenArgs& p) { return streams(a, T, 2) ? launch_gradient<T, true>(who, p, s) : launch_gradient<T, false>(who, p, s); }); });
     return rc;
 }
 
@@ -749,7 +942,9 @@ int pxh_token_logprobs_forward_train(const void* logits, const void* targets, co
     int rc = PXH_OK;
     dispatch_type(type, [&]<int T>() {
         rc = by_rows(a, T, [&](const TokenArgs& p) {
-            return entropy || d_entropy ? launch_train<T, true>(who, p, s) : launch_train<T, false>(who, p, s);
+            const bool past = streams(a, T, 2);
+            if (entropy || d_entropy) return past ? launch_train<T, true, true>(who, p, s) : launch_train<T, true, false>(who, p, s);
+            return past ? launch_train<T, false, true>(who, p, s) : launch_train<T, false, false>(who, p, s);
         });
     });
     return rc;
