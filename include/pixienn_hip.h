@@ -676,7 +676,7 @@ int pxh_token_logprobs_forward_train(const void* logits, const void* targets, co
  *   g = d * d_scale * f;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
  *   w += lr * (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps) - lr * decay * w     (the decay where apply_decay says so)
  *   copy = w, rounded to its type
- * d is only read (unlike pxh_adam_update's).  d_scale: 1 / batch, the inverse of a loss scale, or both.
+ * beta1 and beta2 are taken in 64 bits (1 - beta is what an fp32 beta has lost).  d is only read (unlike pxh_adam_update's).  d_scale: 1 / batch, the inverse of a loss scale, or both.
  *
  * States in 8 bits: m and the SQUARE ROOT of v are e4m3 values with a scale for each 256 of a tensor, its largest magnitude / 448
  * (2^-126 at least): 2 + 1/32 bytes a value for both.  Each step's results are rounded stochastically, up with the
@@ -710,7 +710,7 @@ int pxh_adamw_table_create(int count, const pxh_adamw_tensor* tensors, int state
 void pxh_adamw_table_destroy(pxh_adamw_table* table);
 /* tensors in the table (those of no values are not counted) */
 int pxh_adamw_table_count(const pxh_adamw_table* table);
-int pxh_adamw_update_table(const pxh_adamw_table* table, int t, float lr, float beta1, float beta2, float eps, float decay,
+int pxh_adamw_update_table(const pxh_adamw_table* table, int t, float lr, double beta1, double beta2, float eps, float decay,
                            float d_scale, float max_norm, float* norm_out, unsigned seed, void* stream);
 
 #ifdef __cplusplus

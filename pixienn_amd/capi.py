@@ -17,6 +17,7 @@ ACTIVATIONS = {"leaky": 0, "linear": 1, "loggy": 2, "logistic": 3, "mish": 4,
 P = ctypes.c_void_p
 I = ctypes.c_int
 F = ctypes.c_float
+D = ctypes.c_double
 Z = ctypes.c_size_t
 L = ctypes.c_longlong
 U = ctypes.c_uint
@@ -89,7 +90,7 @@ SIGNATURES = {
     "pxh_token_logprobs_backward": [P, P, P, P, P, P, P, I, I, L, I, L, L, F, P],
     "pxh_adamw_table_create": [I, P, I, P],
     "pxh_adamw_table_count": [P],
-    "pxh_adamw_update_table": [P, I, F, F, F, F, F, F, F, P, U, P],
+    "pxh_adamw_update_table": [P, I, F, D, D, F, F, F, F, P, U, P],
     "pxh_token_logprobs_forward_train": [P, P, P, P, P, P, P, P, I, I, L, I, L, L, F, P],
 }
 _OTHER_RETURNS = {

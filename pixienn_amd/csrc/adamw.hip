@@ -12,8 +12,8 @@ namespace pxh {
 namespace {
 
 constexpr int kStateBlock = 256;            // values with one scale: four to a lane of a wave
-constexpr int kChunk = 16 * kStateBlock;    // values of a workgroup
-constexpr int kSteps = kChunk / (kBlock * 4);
+constexpr int kSteps = 4;                   // blocks of a wave
+constexpr int kChunk = kSteps * kBlock * 4; // values of a workgroup
 constexpr int kNormWorkers = 2048;
 constexpr float kE4m3Max = 448.0f;
 constexpr float kLeastScale = 0x1p-126f;
@@ -38,213 +38,283 @@ struct Chunk {
 struct AdamwStep {
     float beta1, beta2, a1, a2;         // a: 1 - beta
     float c1, c2;                       // 1 - beta^t, and the square root of 1 - beta2^t
-    float lr, eps, shrink, d_scale;
+    float lr, lr_c1, inverse_c2, eps, shrink, d_scale;
     uint32_t seed;
 };
 
 // Two rounds of an odd factor (of the golden ratio and the square root of two) and the high bits folded into the low ones.
-__host__ __device__ __forceinline__ uint32_t mixed(uint32_t x)
+constexpr uint32_t kMix1 = 0x9E3779B9u, kMix2 = 0x6A09E667u;
+
+__host__ __device__ __forceinline__ uint32_t second_round(uint32_t x)
 {
-    x *= 0x9E3779B9u;
     x ^= x >> 15;
-    x *= 0x6A09E667u;
+    x *= kMix2;
     x ^= x >> 13;
     return x;
 }
 
-// |x| / scale as e4m3 bits, rounded up with the probability of what is cut off: scaled by 2^-120 the value has e4m3's
-// exponent, its subnormals among fp32's own, and 20 random bits are added below the last place.  A NaN stays one.
-__device__ __forceinline__ uint32_t stochastic(float x, float inverse, uint32_t noise)
-{
-    const float small = fabsf(x) * inverse * 0x1p-120f;
-    const uint32_t code = (__float_as_uint(small) + noise) >> 20;
-    return x != x ? 0x7fu : code > 0x7eu ? 0x7eu : code;
-}
-
-__device__ __forceinline__ void from_e4m3(uint32_t codes, float scale, float (&x)[4])
-{
-    const auto low = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(codes), false);
-    const auto high = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(codes), true);
-    x[0] = low[0] * scale; x[1] = low[1] * scale; x[2] = high[0] * scale; x[3] = high[1] * scale;
-}
+__host__ __device__ __forceinline__ uint32_t mixed(uint32_t x) { return second_round(x * kMix1); }
 
 // Four values of a lane.
+template<int D>
 struct Quad {
-    float w[4], d[4], m[4], v[4];       // v: its root, with states in 8 bits
+    float w[4];
+    Raw<D, 4> d;
+    Raw<PXH_F32, 4> m32, v32;           // states in 32 bits
+    uint32_t m8, v8;                    // ... in 8
 };
 
 template<int BITS, int D, bool NT>
-__device__ __forceinline__ void load_quad(const AdamwRecord& r, uint32_t e, Quad& q)
+__device__ __forceinline__ void load_quad(const AdamwRecord& r, uint32_t e, Quad<D>& q)
 {
     load_raw<PXH_F32, 4, NT>(r.w, e).get(q.w);
-    load_raw<D, 4, NT>(r.d, e).get(q.d);
+    q.d = load_raw<D, 4, NT>(r.d, e);
     if constexpr (BITS == 32) {
-        load_raw<PXH_F32, 4, NT>(r.m, e).get(q.m);
-        load_raw<PXH_F32, 4, NT>(r.v, e).get(q.v);
+        q.m32 = load_raw<PXH_F32, 4, NT>(r.m, e);
+        q.v32 = load_raw<PXH_F32, 4, NT>(r.v, e);
     } else {
-        from_e4m3(load_raw<PXH_E4M3, 4, NT>(r.m, e).w[0], r.m_scale[e / kStateBlock], q.m);
-        from_e4m3(load_raw<PXH_E4M3, 4, NT>(r.v, e).w[0], r.v_scale[e / kStateBlock], q.v);
+        q.m8 = load_raw<PXH_E4M3, 4, NT>(r.m, e).w[0];
+        q.v8 = load_raw<PXH_E4M3, 4, NT>(r.v, e).w[0];
     }
 }
 
 // ... of which only those below n are there; zeros behind them.
 template<int BITS, int D>
-__device__ __forceinline__ void load_tail(const AdamwRecord& r, uint32_t e, Quad& q)
+__device__ __forceinline__ void load_last(const AdamwRecord& r, uint32_t e, Quad<D>& q)
 {
-    uint32_t m = 0, v = 0;
+    float d[4] = {}, m[4] = {}, v[4] = {};
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        const bool there = e + k < r.n;
-        q.w[k] = there ? r.w[e + k] : 0.0f;
-        q.d[k] = there ? load_one<D>(r.d, e + k) : 0.0f;
+        if (e + k >= r.n) continue;
+        q.w[k] = load_one<PXH_F32>(r.w, e + k);
+        d[k] = load_one<D>(r.d, e + k);
         if constexpr (BITS == 32) {
-            q.m[k] = there ? static_cast<const float*>(r.m)[e + k] : 0.0f;
-            q.v[k] = there ? static_cast<const float*>(r.v)[e + k] : 0.0f;
-        } else if (there) {
-            m |= static_cast<uint32_t>(static_cast<const uint8_t*>(r.m)[e + k]) << (8 * k);
-            v |= static_cast<uint32_t>(static_cast<const uint8_t*>(r.v)[e + k]) << (8 * k);
+            m[k] = load_one<PXH_F32>(r.m, e + k);
+            v[k] = load_one<PXH_F32>(r.v, e + k);
+        } else {
+            q.m8 |= static_cast<uint32_t>(global_memory<uint8_t>(r.m)[e + k]) << (8 * k);
+            q.v8 |= static_cast<uint32_t>(global_memory<uint8_t>(r.v)[e + k]) << (8 * k);
         }
     }
-    if constexpr (BITS == 8) {
-        const uint32_t block = min(e, r.n - 1) / kStateBlock;
-        from_e4m3(m, r.m_scale[block], q.m);
-        from_e4m3(v, r.v_scale[block], q.v);
-    }
+    q.d.set(d);
+    q.m32.set(m);
+    q.v32.set(v);
 }
 
-// One step of four values; the states as they are before they are rounded, v or its root.
-template<int BITS>
-__device__ __forceinline__ void step_quad(const AdamwStep& s, float factor, bool decay, Quad& q)
-{
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const float g = q.d[k] * factor;
-        const float m = fmaf(s.beta1, q.m[k], s.a1 * g);
-        const float before = BITS == 8 ? q.v[k] * q.v[k] : q.v[k];
-        const float v = fmaf(s.beta2, before, s.a2 * (g * g));
-        const float root = sqrtf(v);
-        const float step = (m / s.c1) / (root / s.c2 + s.eps);
-        const float w = q.w[k];
-        q.w[k] = fmaf(s.lr, step, w);
-        if (decay) q.w[k] = fmaf(-s.shrink, w, q.w[k]);
-        q.m[k] = m;
-        q.v[k] = BITS == 8 ? root : v;
-    }
-}
-
-// The largest magnitude of a wave's values, as a scale.
-__device__ __forceinline__ float block_scale(const float (&x)[4])
-{
-    const float most = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-    return fmaxf(wave_max_by_rows(most) * (1.0f / kE4m3Max), kLeastScale);
-}
-
-struct Codes {
-    uint32_t m, v;
-    float m_scale, v_scale;
-};
-
-// All lanes of a wave, with the values of one block.
-__device__ __forceinline__ Codes to_e4m3(const AdamwStep& s, uint32_t place, const Quad& q)
-{
-    Codes c{ 0, 0, block_scale(q.m), block_scale(q.v) };
-    const float mi = 1.0f / c.m_scale, vi = 1.0f / c.v_scale;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const uint32_t noise = mixed((place + k) ^ s.seed);
-        const uint32_t m = stochastic(q.m[k], mi, noise >> 12) | (q.m[k] < 0.0f ? 0x80u : 0u);
-        const uint32_t v = stochastic(q.v[k], vi, noise & 0xfffffu);
-        c.m |= m << (8 * k);
-        c.v |= (v == 0 && q.v[k] != 0.0f ? 1u : v) << (8 * k);
-    }
-    return c;
-}
-
+// What a lane writes of four values: all, or those below n.
 template<int BITS, bool NT>
-__device__ __forceinline__ void store_quad(const AdamwStep& s, const AdamwRecord& r, uint32_t e, const Quad& q)
+__device__ __forceinline__ void store_quad(const AdamwRecord& r, uint32_t e, const float (&w)[4], const float (&m)[4], const float (&v)[4],
+                                           uint32_t m8, uint32_t v8)
 {
-    Raw<PXH_F32, 4> f;
-    f.set(q.w);
-    store_raw<PXH_F32, 4, NT>(r.w, e, f);
-    if constexpr (BITS == 32) {
-        f.set(q.m);
-        store_raw<PXH_F32, 4, NT>(r.m, e, f);
-        f.set(q.v);
-        store_raw<PXH_F32, 4, NT>(r.v, e, f);
-    } else {
-        const Codes c = to_e4m3(s, r.place + e, q);
-        store_raw<PXH_E4M3, 4, NT>(r.m, e, Raw<PXH_E4M3, 4>{ { c.m } });
-        store_raw<PXH_E4M3, 4, NT>(r.v, e, Raw<PXH_E4M3, 4>{ { c.v } });
-        if (e % kStateBlock == 0) {
-            r.m_scale[e / kStateBlock] = c.m_scale;
-            r.v_scale[e / kStateBlock] = c.v_scale;
-        }
-    }
-    if (r.copy) {
-        if (r.copy_type == PXH_BF16) {
-            Raw<PXH_BF16, 4> h;
-            h.set(q.w);
-            store_raw<PXH_BF16, 4>(r.copy, e, h);
-        } else {
-            Raw<PXH_F16, 4> h;
-            h.set(q.w);
-            store_raw<PXH_F16, 4>(r.copy, e, h);
-        }
-    }
-}
-
-template<int BITS>
-__device__ __forceinline__ void store_tail(const AdamwStep& s, const AdamwRecord& r, uint32_t e, const Quad& q)
-{
-    Codes c{};
-    if constexpr (BITS == 8) {
-        c = to_e4m3(s, r.place + e, q);                 // the whole wave
-        if (e % kStateBlock == 0 && e < r.n) {
-            r.m_scale[e / kStateBlock] = c.m_scale;
-            r.v_scale[e / kStateBlock] = c.v_scale;
-        }
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        if (e + k >= r.n) break;
-        r.w[e + k] = q.w[k];
+    if (e + 4 <= r.n) {
+        Raw<PXH_F32, 4> f;
+        f.set(w);
+        store_raw<PXH_F32, 4, NT>(r.w, e, f);
         if constexpr (BITS == 32) {
-            static_cast<float*>(r.m)[e + k] = q.m[k];
-            static_cast<float*>(r.v)[e + k] = q.v[k];
+            f.set(m);
+            store_raw<PXH_F32, 4, NT>(r.m, e, f);
+            f.set(v);
+            store_raw<PXH_F32, 4, NT>(r.v, e, f);
         } else {
-            static_cast<uint8_t*>(r.m)[e + k] = static_cast<uint8_t>(c.m >> (8 * k));
-            static_cast<uint8_t*>(r.v)[e + k] = static_cast<uint8_t>(c.v >> (8 * k));
+            store_raw<PXH_E4M3, 4, NT>(r.m, e, Raw<PXH_E4M3, 4>{ { m8 } });
+            store_raw<PXH_E4M3, 4, NT>(r.v, e, Raw<PXH_E4M3, 4>{ { v8 } });
         }
         if (r.copy) {
-            if (r.copy_type == PXH_BF16) store_one<PXH_BF16>(r.copy, e + k, q.w[k]);
-            else store_one<PXH_F16>(r.copy, e + k, q.w[k]);
-        }
-    }
-}
-
-template<int BITS, int D, bool NT>
-__device__ __forceinline__ void step_chunk(const AdamwRecord& r, const AdamwStep& s, uint32_t first, float factor)
-{
-    const bool decay = r.decay != 0;
-    const uint32_t e = first + threadIdx.x * 4;
-    if (first + kChunk <= r.n) {
-        Quad q[kSteps];
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k) load_quad<BITS, D, NT>(r, e + k * kBlock * 4, q[k]);
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-            step_quad<BITS>(s, factor, decay, q[k]);
-            store_quad<BITS, NT>(s, r, e + k * kBlock * 4, q[k]);
+            if (r.copy_type == PXH_BF16) {
+                Raw<PXH_BF16, 4> h;
+                h.set(w);
+                store_raw<PXH_BF16, 4, NT>(r.copy, e, h);
+            } else {
+                Raw<PXH_F16, 4> h;
+                h.set(w);
+                store_raw<PXH_F16, 4, NT>(r.copy, e, h);
+            }
         }
         return;
     }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if (e + k >= r.n) continue;
+        store_one<PXH_F32>(r.w, e + k, w[k]);
+        if constexpr (BITS == 32) {
+            store_one<PXH_F32>(r.m, e + k, m[k]);
+            store_one<PXH_F32>(r.v, e + k, v[k]);
+        } else {
+            global_memory<uint8_t>(r.m)[e + k] = static_cast<uint8_t>(m8 >> (8 * k));
+            global_memory<uint8_t>(r.v)[e + k] = static_cast<uint8_t>(v8 >> (8 * k));
+        }
+        if (r.copy) {
+            if (r.copy_type == PXH_BF16) store_one<PXH_BF16>(r.copy, e + k, w[k]);
+            else store_one<PXH_F16>(r.copy, e + k, w[k]);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- states in 32 bits
+__device__ __forceinline__ void step_32(const AdamwStep& s, float clip, bool decay, const float (&d)[4], float (&w)[4], float (&m)[4],
+                                        float (&v)[4])
+{
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float g = d[k] * s.d_scale * clip;
+        m[k] = fmaf(s.beta1, m[k], s.a1 * g);
+        v[k] = fmaf(s.beta2, v[k], s.a2 * (g * g));
+        const float step = (m[k] / s.c1) / (sqrtf(v[k]) / s.c2 + s.eps);
+        const float old = w[k];
+        w[k] = fmaf(s.lr, step, old);
+        if (decay) w[k] = fmaf(-s.shrink, old, w[k]);
+    }
+}
+
+// ---------------------------------------------------------------- states in 8 bits
+// The states and their roots are formed operation by operation, each rounded to fp32, since a bit of theirs may turn what they are rounded
+// to; the quotient of the step, whose last bits are lost in the weight, by the hardware's reciprocal.
+__device__ __forceinline__ void step_8(const AdamwStep& s, float m_scale, float v_scale, float clip, bool decay, uint32_t m8, uint32_t v8,
+                                       const float (&d)[4], float (&w)[4], float (&m)[4], float (&root)[4])
+{
+    const auto m01 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(m8), false), m23 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(m8), true);
+    const auto v01 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(v8), false), v23 = __builtin_amdgcn_cvt_pk_f32_fp8(static_cast<int>(v8), true);
+    const float mc[4] = { m01[0], m01[1], m23[0], m23[1] }, vc[4] = { v01[0], v01[1], v23[0], v23[1] };
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float g = d[k] * s.d_scale * clip;
+        m[k] = s.beta1 * (mc[k] * m_scale) + s.a1 * g;
+        const float before = vc[k] * v_scale;
+        root[k] = sqrtf(s.beta2 * (before * before) + s.a2 * (g * g));
+        const float q = m[k] * __builtin_amdgcn_rcpf(fmaf(root[k], s.inverse_c2, s.eps));
+        const float old = w[k];
+        w[k] = fmaf(s.lr_c1, q, old);
+        if (decay) w[k] = fmaf(-s.shrink, old, w[k]);
+    }
+}
+
+__device__ __forceinline__ float largest(const float (&x)[4])
+{
+    return fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+}
+
+__device__ __forceinline__ float max_of_halves(float a, float b)
+{
+    // a's two halves of the wave against each other in the lower half, b's in the upper one
+    const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
+}
+
+__device__ __forceinline__ float max_of_rows(float a, float b)
+{
+    // the same for the even and odd rows of 16
+    const auto t = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return fmaxf(__uint_as_float(t[0]), __uint_as_float(t[1]));
+}
+
+// The maxima of eight values over the wave: lanes 8 j to 8 j + 7 have that of value j.  The lanes and the values are halved together, 18
+// instructions for all eight (one by one it is 14 for each, and as many scales to be formed).
+__device__ __forceinline__ float eight_maxima(const float (&x)[8])
+{
+    float y[4], z[2];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) y[k] = max_of_halves(x[k], x[k + 4]);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) z[k] = max_of_rows(y[k], y[k + 2]);
+    const bool upper = threadIdx.x & 8;
+    float v = fmaxf(upper ? z[1] : z[0], lane_in_row<0x128>(upper ? z[0] : z[1]));      // the lane eight further on in the row
+    v = fmaxf(v, lane_in_row<0xB1>(v));
+    v = fmaxf(v, lane_in_row<0x4E>(v));
+    return fmaxf(v, lane_in_row<0x141>(v));
+}
+
+// Four values over their block's scale as e4m3 (a NaN, which its weight has too, as the largest value): up with the probability of what
+// is cut off, by the upper 20 bits of the noise (the hardware's conversion, which is the addition of those bits below the last place,
+// subnormals among it).  The quotient from the rounded reciprocal and one correction by its remainder (Markstein), which
+// is the rounded quotient.
+__device__ __forceinline__ void to_e4m3(const AdamwStep& s, uint32_t place, const float (&m)[4], const float (&root)[4], float m_scale,
+                                        float m_inverse, float v_scale, float v_inverse, uint32_t& m8, uint32_t& v8)
+{
+    // the four places differ in their last two bits only: one product for all
+    const uint32_t base = ((place ^ s.seed) & ~3u) * kMix1;
+    const auto over = [](float x, float scale, float inverse) {
+        const float q = x * inverse;
+        return fmaf(fmaf(-q, scale, x), inverse, q);
+    };
+    int mw = 0, vw = 0;
+    const auto put = [&]<int K>() {
+        const uint32_t noise = second_round(base + ((K ^ s.seed) & 3u) * kMix1);
+        const float x = __builtin_amdgcn_fmed3f(over(m[K], m_scale, m_inverse), -kE4m3Max, kE4m3Max);
+        mw = __builtin_amdgcn_cvt_sr_fp8_f32(x, static_cast<int>(noise), mw, K);
+        // at least the least value there is, unless it is zero
+        const float v = __builtin_amdgcn_fmed3f(over(root[K], v_scale, v_inverse), fminf(root[K] * 0x1p100f, 0x1p-9f), kE4m3Max);
+        vw = __builtin_amdgcn_cvt_sr_fp8_f32(v, static_cast<int>(noise << 12), vw, K);
+    };
+    put.template operator()<0>();
+    put.template operator()<1>();
+    put.template operator()<2>();
+    put.template operator()<3>();
+    m8 = static_cast<uint32_t>(mw);
+    v8 = static_cast<uint32_t>(vw);
+}
+
+// ---------------------------------------------------------------- the step
+// A wave takes four blocks, 1024 values apart; all of their loads go out before the first is used.
+template<int BITS, int D, bool NT>
+__device__ __forceinline__ void step_chunk(const AdamwRecord& r, const AdamwStep& s, uint32_t first, float clip)
+{
+    const bool decay = r.decay != 0;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const uint32_t e = first + threadIdx.x * 4;
+    const uint32_t block = first / kStateBlock + wave;              // of the first step; the others four further on each
+    const uint32_t blocks = (r.n + kStateBlock - 1) / kStateBlock;
+    if (block >= blocks) return;                                    // a whole wave
+    Quad<D> q[kSteps];
+    float m_scale[kSteps], v_scale[kSteps];
+#pragma unroll
     for (int k = 0; k < kSteps; ++k) {
-        const uint32_t at = e + k * kBlock * 4;
-        if (at / kStateBlock * kStateBlock >= r.n) return;      // whole waves: a wave has a block of its own
-        Quad q;
-        load_tail<BITS, D>(r, at, q);
-        step_quad<BITS>(s, factor, decay, q);
-        store_tail<BITS>(s, r, at, q);
+        q[k] = Quad<D>{};
+        if (e + k * kBlock * 4 + 4 <= r.n) load_quad<BITS, D, NT>(r, e + k * kBlock * 4, q[k]);
+        if constexpr (BITS == 8) {
+            const uint32_t at = min(block + k * (kBlock / kWave), blocks - 1);
+            m_scale[k] = global_memory<float>(r.m_scale)[at];
+            v_scale[k] = global_memory<float>(r.v_scale)[at];
+        }
+    }
+    if (first + kChunk > r.n) {
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+            const uint32_t at = e + k * kBlock * 4;
+            if (at < r.n && at + 4 > r.n) load_last<BITS, D>(r, at, q[k]);
+        }
+    }
+    if constexpr (BITS == 32) {
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+            float d[4], m[4], v[4];
+            q[k].d.get(d);
+            q[k].m32.get(m);
+            q[k].v32.get(v);
+            step_32(s, clip, decay, d, q[k].w, m, v);
+            store_quad<BITS, NT>(r, e + k * kBlock * 4, q[k].w, m, v, 0, 0);
+        }
+    } else {
+        float m[kSteps][4], root[kSteps][4], most[2 * kSteps];
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+            float d[4];
+            q[k].d.get(d);
+            step_8(s, m_scale[k], v_scale[k], clip, decay, q[k].m8, q[k].v8, d, q[k].w, m[k], root[k]);
+            most[k] = largest(m[k]);
+            most[k + kSteps] = largest(root[k]);
+        }
+        // lanes 8 j and on: the scale of m in step j, and of the root in step j - 4
+        const uint32_t lane = threadIdx.x % kWave, j = lane / 8;
+        const float scale = fmaxf(eight_maxima(most) / kE4m3Max, kLeastScale), inverse = 1.0f / scale;
+        const uint32_t of = block + (j % kSteps) * (kBlock / kWave);
+        if (lane % 8 == 0 && of < blocks) global_memory<float>(j < kSteps ? r.m_scale : r.v_scale)[of] = scale;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+            uint32_t m8, v8;
+            to_e4m3(s, r.place + e + k * kBlock * 4, m[k], root[k], from_lane(scale, 8 * k), from_lane(inverse, 8 * k),
+                    from_lane(scale, 8 * (k + kSteps)), from_lane(inverse, 8 * (k + kSteps)), m8, v8);
+            store_quad<BITS, NT>(r, e + k * kBlock * 4, q[k].w, m[k], root[k], m8, v8);
+        }
     }
 }
 
@@ -253,38 +323,53 @@ __global__ __launch_bounds__(kBlock) void adamw_kernel(const AdamwRecord* record
 {
     const Chunk c = chunks[blockIdx.x];
     const AdamwRecord r = records[c.tensor];
-    float f = s.d_scale;
-    if (factor) {
-        const float clip = *factor;
-        if (clip != clip) return;               // the norm is not finite: the step is left out
-        f *= clip;
-    }
-    if (r.d_type == PXH_F32) step_chunk<BITS, PXH_F32, NT>(r, s, c.first, f);
-    else if (r.d_type == PXH_BF16) step_chunk<BITS, PXH_BF16, NT>(r, s, c.first, f);
-    else step_chunk<BITS, PXH_F16, NT>(r, s, c.first, f);
+    const float clip = factor ? *factor : 1.0f;
+    if (clip != clip) return;                   // the norm is not finite: the step is left out
+    if (r.d_type == PXH_F32) step_chunk<BITS, PXH_F32, NT>(r, s, c.first, clip);
+    else if (r.d_type == PXH_BF16) step_chunk<BITS, PXH_BF16, NT>(r, s, c.first, clip);
+    else step_chunk<BITS, PXH_F16, NT>(r, s, c.first, clip);
 }
 
 // ---------------------------------------------------------------- the norm of all gradients
 template<int D>
 __device__ __forceinline__ double squares_of_chunk(const AdamwRecord& r, uint32_t first)
 {
-    double sum = 0.0;
+    Raw<D, 4> raw[kSteps];
+    const uint32_t e = first + threadIdx.x * 4;
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
-        const uint32_t e = first + (k * kBlock + threadIdx.x) * 4;
-        float d[4] = {};
-        if (e + 4 <= r.n) load_raw<D, 4>(r.d, e).get(d);
-        else
-            for (int i = 0; i < 4; ++i)
-                if (e + i < r.n) d[i] = load_one<D>(r.d, e + i);
+        raw[k] = Raw<D, 4>{};
+        if (e + k * kBlock * 4 + 4 <= r.n) raw[k] = load_raw<D, 4>(r.d, e + k * kBlock * 4);
+    }
+    double sum = 0.0;
+    if (first + kChunk > r.n) {
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+            const uint32_t at = e + k * kBlock * 4;
+            if (at < r.n && at + 4 > r.n)
+                for (uint32_t i = at; i < r.n; ++i) {
+                    const float d = load_one<D>(r.d, i);
+                    sum += d * d;
+                }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+        float d[4];
+        raw[k].get(d);
         sum += fmaf(d[0], d[0], fmaf(d[1], d[1], fmaf(d[2], d[2], d[3] * d[3])));
     }
     return sum;
 }
 
-__global__ __launch_bounds__(kBlock) void adamw_squares_kernel(const AdamwRecord* records, const Chunk* chunks, uint32_t count, double* partial)
+// Each workgroup leaves the sum over its chunks, and the last one to be done makes the norm and the clipping factor of them, in their
+// order.  The sums cross from one die's cache to another's, as does the count of those that are done; that is zero again behind
+// the last.
+__global__ __launch_bounds__(kBlock) void adamw_squares_kernel(const AdamwRecord* records, const Chunk* chunks, uint32_t count, double* partial,
+                                                               uint32_t* done, float d_scale, float max_norm, float* factor, float* norm_out)
 {
     __shared__ double slots[kBlock / kWave];
+    __shared__ bool last;
     double sum = 0.0;
     for (uint32_t i = blockIdx.x; i < count; i += gridDim.x) {
         const Chunk c = chunks[i];
@@ -294,15 +379,14 @@ __global__ __launch_bounds__(kBlock) void adamw_squares_kernel(const AdamwRecord
         else sum += squares_of_chunk<PXH_F16>(r, c.first);
     }
     sum = block_sum(sum, slots);
-    if (threadIdx.x == 0) partial[blockIdx.x] = sum;
-}
-
-__global__ __launch_bounds__(kBlock) void adamw_norm_kernel(const double* partial, int count, float d_scale, float max_norm, float* factor,
-                                                            float* norm_out)
-{
-    __shared__ double slots[kBlock / kWave];
-    double sum = 0.0;
-    for (int i = threadIdx.x; i < count; i += kBlock) sum += partial[i];
+    if (threadIdx.x == 0) {
+        __hip_atomic_store(partial + blockIdx.x, sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last = __hip_atomic_fetch_add(done, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last) return;
+    sum = 0.0;
+    for (uint32_t i = threadIdx.x; i < gridDim.x; i += kBlock) sum += __hip_atomic_load(partial + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     sum = block_sum(sum, slots);
     if (threadIdx.x == 0) {
         const float norm = static_cast<float>(sqrt(sum) * fabs(static_cast<double>(d_scale)));
@@ -313,6 +397,7 @@ __global__ __launch_bounds__(kBlock) void adamw_norm_kernel(const double* partia
         }
         *factor = f;
         if (norm_out) *norm_out = norm;
+        __hip_atomic_store(done, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
 }
 
@@ -332,6 +417,7 @@ struct pxh_adamw_table {
     const Chunk* chunk_list;
     double* partial;
     float* factor;
+    uint32_t* done;             // workgroups of the norm that have left their sum; zero between launches
 };
 
 int pxh_adamw_table_create(int count, const pxh_adamw_tensor* tensors, int state_bits, pxh_adamw_table** table)
@@ -380,17 +466,18 @@ int pxh_adamw_table_create(int count, const pxh_adamw_tensor* tensors, int state
         }
         const auto align = [](size_t b) { return (b + 255) & ~static_cast<size_t>(255); };
         const size_t record_bytes = align(records.size() * sizeof(AdamwRecord)), chunk_bytes = align(chunks.size() * sizeof(Chunk));
+        const size_t head = record_bytes + chunk_bytes;
         hipError_t e = hipSuccess;
         std::vector<char> image;
         try {
-            image.resize(record_bytes + chunk_bytes);
+            image.resize(head + 256);       // behind them the factor and the count, which has to begin at zero
         } catch (...) {
             delete t;
             throw;
         }
         std::memcpy(image.data(), records.data(), records.size() * sizeof(AdamwRecord));
         std::memcpy(image.data() + record_bytes, chunks.data(), chunks.size() * sizeof(Chunk));
-        e = hipMalloc(&t->memory, image.size() + align(kNormWorkers * sizeof(double)) + 256);
+        e = hipMalloc(&t->memory, image.size() + kNormWorkers * sizeof(double));
         if (e == hipSuccess) {
             e = hipMemcpy(t->memory, image.data(), image.size(), hipMemcpyHostToDevice);
             if (e != hipSuccess) (void) hipFree(t->memory);
@@ -403,8 +490,9 @@ int pxh_adamw_table_create(int count, const pxh_adamw_tensor* tensors, int state
         char* base = static_cast<char*>(t->memory);
         t->records = reinterpret_cast<const AdamwRecord*>(base);
         t->chunk_list = reinterpret_cast<const Chunk*>(base + record_bytes);
+        t->factor = reinterpret_cast<float*>(base + head);
+        t->done = reinterpret_cast<uint32_t*>(base + head + 128);
         t->partial = reinterpret_cast<double*>(base + image.size());
-        t->factor = reinterpret_cast<float*>(base + image.size() + align(kNormWorkers * sizeof(double)));
         *table = t;
         return PXH_OK;
     } catch (const std::exception&) {
@@ -421,37 +509,34 @@ void pxh_adamw_table_destroy(pxh_adamw_table* table)
 
 int pxh_adamw_table_count(const pxh_adamw_table* table) { return table ? table->count : 0; }
 
-int pxh_adamw_update_table(const pxh_adamw_table* table, int t, float lr, float beta1, float beta2, float eps, float decay,
+int pxh_adamw_update_table(const pxh_adamw_table* table, int t, float lr, double beta1, double beta2, float eps, float decay,
                            float d_scale, float max_norm, float* norm_out, unsigned seed, void* stream)
 {
     const char* who = "pxh_adamw_update_table";
     if (!table) return fail_invalid("%s: null table", who);
     if (t < 1) return fail_invalid("%s: step %d", who, t);
-    if (!(beta1 >= 0.0f && beta1 < 1.0f && beta2 >= 0.0f && beta2 < 1.0f)) return fail_invalid("%s: beta %g, %g", who, static_cast<double>(beta1), static_cast<double>(beta2));
+    if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0)) return fail_invalid("%s: beta %g, %g", who, beta1, beta2);
     if (!(eps >= 0.0f) || !(max_norm >= 0.0f)) return fail_invalid("%s: eps %g, max_norm %g", who, static_cast<double>(eps), static_cast<double>(max_norm));
     if (table->count == 0 && !norm_out) return PXH_OK;
     int device = -1;
     if (hipGetDevice(&device) != hipSuccess || device != table->device)
         return fail_invalid("%s: the table is of device %d, the current one is %d", who, table->device, device);
     hipStream_t s = as_stream(stream);
-    if (table->count == 0) {
-        hipLaunchKernelGGL(adamw_norm_kernel, dim3(1), dim3(kBlock), 0, s, nullptr, 0, d_scale, 0.0f, norm_out, norm_out);
-        return check_launch(who);
-    }
+    if (table->count == 0) return pxh_fill_f32(norm_out, 1, 0.0f, stream);
     const bool clips = max_norm > 0.0f;
     if (clips || norm_out) {
         const unsigned workers = table->chunks < static_cast<uint32_t>(kNormWorkers) ? table->chunks : kNormWorkers;
-        hipLaunchKernelGGL(adamw_squares_kernel, dim3(workers), dim3(kBlock), 0, s, table->records, table->chunk_list, table->chunks, table->partial);
-        if (int rc = check_launch(who)) return rc;
-        hipLaunchKernelGGL(adamw_norm_kernel, dim3(1), dim3(kBlock), 0, s, table->partial, static_cast<int>(workers), d_scale, max_norm,
-                           table->factor, norm_out);
+        hipLaunchKernelGGL(adamw_squares_kernel, dim3(workers), dim3(kBlock), 0, s, table->records, table->chunk_list, table->chunks, table->partial,
+                           table->done, d_scale, max_norm, table->factor, norm_out);
         if (int rc = check_launch(who)) return rc;
     }
     AdamwStep step{};
-    step.beta1 = beta1; step.beta2 = beta2;
-    step.a1 = static_cast<float>(1.0 - static_cast<double>(beta1)); step.a2 = static_cast<float>(1.0 - static_cast<double>(beta2));
-    step.c1 = static_cast<float>(1.0 - std::pow(static_cast<double>(beta1), t));
-    step.c2 = static_cast<float>(std::sqrt(1.0 - std::pow(static_cast<double>(beta2), t)));
+    // constants from the arguments in 64 bits, each rounded once
+    const double c1 = 1.0 - std::pow(beta1, t), c2 = std::sqrt(1.0 - std::pow(beta2, t));
+    step.beta1 = static_cast<float>(beta1); step.beta2 = static_cast<float>(beta2);
+    step.a1 = static_cast<float>(1.0 - beta1); step.a2 = static_cast<float>(1.0 - beta2);
+    step.c1 = static_cast<float>(c1); step.c2 = static_cast<float>(c2);
+    step.lr_c1 = static_cast<float>(static_cast<double>(lr) / c1); step.inverse_c2 = static_cast<float>(1.0 / c2);
     step.lr = lr; step.eps = eps; step.d_scale = d_scale;
     step.shrink = static_cast<float>(static_cast<double>(lr) * static_cast<double>(decay));
     step.seed = mixed((seed & 0x7fffffffu) + 1u);

@@ -34,9 +34,9 @@ A argument(PyObject* o)
         void* p = PyLong_AsVoidPtr(o);
         if (PyErr_Occurred()) { PyErr_Clear(); throw NotHere{}; }
         return reinterpret_cast<A>(p);
-    } else if constexpr (std::is_same_v<A, float>) {
+    } else if constexpr (std::is_floating_point_v<A>) {
         if (!PyFloat_CheckExact(o)) throw NotHere{};
-        return static_cast<float>(PyFloat_AS_DOUBLE(o));
+        return static_cast<A>(PyFloat_AS_DOUBLE(o));
     } else {
         static_assert(std::is_integral_v<A>, "a kind of argument of its own");
         if (!PyLong_CheckExact(o)) throw NotHere{};

@@ -193,8 +193,9 @@ __device__ __forceinline__ void select_largest(int k, uint32_t best, const Above
 #pragma unroll
         for (int j = 0; j < kWave; ++j) larger += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), j)) > mine;
         uint32_t low = larger < k ? mine : ~0u;
-#pragma unroll
-        for (int off = kWave / 2; off > 0; off >>= 1) low = min(low, static_cast<uint32_t>(__shfl_xor(static_cast<int>(low), off, kWave)));
+        low = ~max_in_row<0x140>(max_in_row<0x141>(max_in_row<0x4E>(max_in_row<0xB1>(~low))));
+        const auto of_lane = [&](int lane) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(low), lane)); };
+        low = min(min(of_lane(0), of_lane(16)), min(of_lane(32), of_lane(48)));
         if (threadIdx.x == 0) s.floor = low;
     }
     __syncthreads();
@@ -302,6 +303,7 @@ struct Part {
         add(extra);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
+            if (k * LANES >= count) break;
             float l[V];
             kept[k].get(l);
 #pragma unroll
@@ -319,6 +321,7 @@ struct Part {
         float most = extra;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
+            if (k * LANES >= count) break;
             if constexpr (T == PXH_F16) {
                 typedef _Float16 two __attribute__((ext_vector_type(2)));
                 two pair = __builtin_bit_cast(two, kept[k].w[0]);
@@ -649,6 +652,7 @@ __global__ __launch_bounds__(LANES) void token_powers_kernel(TokenArgs a)
             last = take(last);
 #pragma unroll
             for (int k = 0; k < K; ++k) {
+                if (k * LANES >= mine.count) break;
                 float l[V];
                 mine.kept[k].get(l);
 #pragma unroll
@@ -774,6 +778,10 @@ inline bool streams(const TokenArgs& a, int type, int tensors)
 constexpr long long kEnoughParts = 1024;
 constexpr int kMostVectors = 8;         // vectors of a lane
 
+// From so many rows on a row that a workgroup of 1024 lanes holds is not split: two such workgroups to a compute unit (4096 x 50000
+// bf16 with three alternatives 98 -> 91 us).
+constexpr long long kRowsForWholeGroups = 512;
+
 // Parts of a row of `vectors`, with up to `k` vectors to a lane.
 inline int parts_of(long long vectors, int k) { return static_cast<int>((vectors + kBlock * k - 1) / (kBlock * k)); }
 
@@ -788,8 +796,16 @@ template<int T, bool ENTROPY>
 int launch_forward(const char* who, const TokenArgs& a, void* workspace, hipStream_t s)
 {
     const int vectors = a.vocab < kVec<T> ? 1 : a.vocab / kVec<T>;      // the values behind the last one go with it
-    const int k = vectors_per_lane(a.rows, vectors);
     Parts p{};
+    if (a.rows >= kRowsForWholeGroups && vectors > kBlock * kMostVectors && vectors <= 1024 * kMostVectors) {
+        p.parts = 1;
+        p.vectors = vectors;
+        const dim3 grid(static_cast<unsigned>(a.rows)), block(1024);
+        if (streams(a, T, 1)) hipLaunchKernelGGL((token_logprobs_kernel<T, ENTROPY, 1024, kMostVectors, true>), grid, block, 0, s, a, p);
+        else hipLaunchKernelGGL((token_logprobs_kernel<T, ENTROPY, 1024, kMostVectors, false>), grid, block, 0, s, a, p);
+        return check_launch(who);
+    }
+    const int k = vectors_per_lane(a.rows, vectors);
     p.parts = parts_of(vectors, k);
     p.vectors = (vectors + p.parts - 1) / p.parts;
     p.parts = (vectors + p.vectors - 1) / p.vectors;

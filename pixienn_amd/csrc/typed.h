@@ -74,6 +74,13 @@ struct Raw {
     }
 };
 
+// Global memory, whatever the compiler knows of a pointer: one that comes out of a table in memory would be accessed as one that
+// may as well lie in LDS, and waited for as such.
+template<typename W>
+__device__ __forceinline__ auto global_memory(const void* p) { return (const __attribute__((address_space(1))) W*) p; }
+template<typename W>
+__device__ __forceinline__ auto global_memory(void* p) { return (__attribute__((address_space(1))) W*) p; }
+
 // V values at element e of p, as one access of up to 128 bits; NT: past the caches.  The access takes any alignment: the
 // hardware has 128-bit accesses at every byte, and a row of an odd number of 16-bit values begins at a multiple of 2, so
 // that no row needs another form for where it begins.
@@ -83,7 +90,7 @@ __device__ __forceinline__ Raw<T, V> load_raw(const void* p, size_t e)
     constexpr int N = V * kSize<T>;
     static_assert(N <= 16, "one access");
     typedef uint32_t words __attribute__((ext_vector_type(N / 4), aligned(1)));
-    const words* at = reinterpret_cast<const words*>(static_cast<const char*>(p) + e * kSize<T>);
+    const auto at = global_memory<words>(static_cast<const char*>(p) + e * kSize<T>);
     const words b = NT ? __builtin_nontemporal_load(at) : *at;
     return __builtin_bit_cast(Raw<T, V>, b);
 }
@@ -94,7 +101,7 @@ __device__ __forceinline__ void store_raw(void* p, size_t e, const Raw<T, V>& r)
     constexpr int N = V * kSize<T>;
     static_assert(N <= 16, "one access");
     typedef uint32_t words __attribute__((ext_vector_type(N / 4), aligned(1)));
-    words* at = reinterpret_cast<words*>(static_cast<char*>(p) + e * kSize<T>);
+    const auto at = global_memory<words>(static_cast<char*>(p) + e * kSize<T>);
     const words b = __builtin_bit_cast(words, r);
     if constexpr (NT) __builtin_nontemporal_store(b, at);
     else *at = b;
@@ -118,9 +125,9 @@ __device__ __forceinline__ void store_raw_at(char* place, uint32_t offset, const
 template<int T>
 __device__ __forceinline__ float load_one(const void* p, size_t e)
 {
-    if constexpr (T == PXH_F32) return static_cast<const float*>(p)[e];
+    if constexpr (T == PXH_F32) return global_memory<float>(p)[e];
     else {
-        const uint32_t h = static_cast<const uint16_t*>(p)[e];
+        const uint32_t h = global_memory<uint16_t>(p)[e];
         if constexpr (T == PXH_BF16) return bf16_up(h);
         else return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(h)));
     }
@@ -129,8 +136,8 @@ __device__ __forceinline__ float load_one(const void* p, size_t e)
 template<int T>
 __device__ __forceinline__ void store_one(void* p, size_t e, float x)
 {
-    if constexpr (T == PXH_F32) static_cast<float*>(p)[e] = x;
-    else static_cast<uint16_t*>(p)[e] = static_cast<uint16_t>(pair_of<T>(x, x));
+    if constexpr (T == PXH_F32) global_memory<float>(p)[e] = x;
+    else global_memory<uint16_t>(p)[e] = static_cast<uint16_t>(pair_of<T>(x, x));
 }
 
 // x rounded to T and back.

@@ -85,7 +85,7 @@ class Model:
 def wanted(model, t, lr, beta1, beta2, eps, decay, d_scale, max_norm):
     """What a step leaves of every tensor in 64 bits, with the bounds."""
     f = lambda x: float(np.float32(x))  # noqa: E731
-    lr, beta1, beta2, eps, d_scale, max_norm, shrink = f(lr), f(beta1), f(beta2), f(eps), f(d_scale), f(max_norm), f(lr) * f(decay)
+    lr, eps, d_scale, max_norm, shrink = f(lr), f(eps), f(d_scale), f(max_norm), f(lr) * f(decay)
     norm = math.sqrt(sum(float((d.double() * d_scale).square().sum()) for d in model.d))
     factor = max_norm / norm if max_norm and norm > max_norm else 1.0
     ms, vs = model.states()
