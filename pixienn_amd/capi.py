@@ -145,6 +145,8 @@ _lib = None
 # The entry points that csrc/calls.cpp calls: name -> (callable that takes tensors for float buffers and answers None for a
 # call it does not make, which arguments are tensors).  Filled by bind_calls().
 native = {}
+# ... and those whose Python functions it takes whole, tensors of any type and stride: name -> callable.
+functions = {}
 
 
 def load():
@@ -188,6 +190,8 @@ def bind_calls():
                       "was built with" % e) from e
     native.update({name: _calls.bind(name, ctypes.cast(getattr(lib, name), ctypes.c_void_p).value)
                    for name in _calls.names()})
+    functions.update({name: _calls.bind_function(name, ctypes.cast(getattr(lib, name), ctypes.c_void_p).value)
+                      for name in _calls.functions()})
 
 
 def declared_symbols():

@@ -1,4 +1,5 @@
 // Root-mean-square norm over rows, with the residual's addition in front of it and 8-bit results, and its gradients.
+#include "stream.h"
 #include "typed.h"
 
 namespace pxh {
@@ -16,7 +17,6 @@ struct NormArgs {
     float* rstd;
     long long rows, x_stride, residual_stride, sum_stride, y_stride;
     int width, group;
-    bool weight_f32;
     float eps;
 };
 
@@ -94,14 +94,65 @@ __device__ __forceinline__ void store_e4m3(char* y, int e, int n, const float (&
         if (e + k < n) y[e + k] = static_cast<char>(w[k / 4] >> (8 * (k & 3)));
 }
 
-// The values of a row are walked in vectors, lane by lane; K vectors per lane are kept in registers between the sum and
-// the result (K == 0: any width, the row is read again).
-template<int T, bool EIGHT, int LANES, int K>
-__global__ __launch_bounds__(LANES > kBlock ? LANES : kBlock) void rms_norm_kernel(NormArgs a)
+// V values of a row and what goes with them: the residual and the weights.
+template<int T, bool WIDE>
+struct NormVector {
+    static constexpr int V = kVec<T>;
+    static constexpr int W = WIDE ? PXH_F32 : T;
+    static constexpr int kParts = V * kSize<W> / 16;                // accesses for the weights
+    static constexpr int kPart = V / kParts;
+    Raw<T, V> h, more;
+    Raw<W, kPart> w[kParts];
+
+    template<bool NT>
+    __device__ __forceinline__ void load(const NormArgs& a, const char* x, const char* residual, int e)
+    {
+        const int n = a.width;
+        if (e + V <= n) {
+            h = load_raw<T, V, NT>(x, e);
+            if (residual) more = load_raw<T, V, NT>(residual, e);
+#pragma unroll
+            for (int q = 0; q < kParts; ++q) w[q] = load_raw<W, kPart>(a.weight, e + q * kPart);
+        } else if (e < n) {
+            h = load_end<T, V>(x, e, n);
+            if (residual) more = load_end<T, V>(residual, e, n);
+#pragma unroll
+            for (int q = 0; q < kParts; ++q) w[q] = load_end<W, kPart>(a.weight, e + q * kPart, n);
+        }
+    }
+
+    // h with the residual, rounded as it is kept
+    __device__ __forceinline__ void add()
+    {
+        float p[V], q[V];
+        h.get(p);
+        more.get(q);
+#pragma unroll
+        for (int k = 0; k < V; ++k) p[k] += q[k];
+        h.set(p);
+    }
+
+    __device__ __forceinline__ void weights(float (&out)[V]) const
+    {
+#pragma unroll
+        for (int q = 0; q < kParts; ++q) {
+            float part[kPart];
+            w[q].get(part);
+#pragma unroll
+            for (int k = 0; k < kPart; ++k) out[q * kPart + k] = part[k];
+        }
+    }
+};
+
+// A row is walked in vectors, lane by lane.  K vectors a lane stay in registers between the sum and the result; the residual and the
+// weights are asked for with the row, so that there is one trip to memory.  K == 0: a row of any width, which is read again.
+template<int T, bool EIGHT, bool WIDE, int LANES, int K, bool NT>
+__global__ __launch_bounds__(LANES > kWave ? LANES : kBlock) void rms_norm_kernel(NormArgs a)
 {
     constexpr int V = kVec<T>;
-    constexpr int kRows = LANES < kBlock ? kBlock / LANES : 1;      // rows per workgroup, a wave each if several
-    __shared__ float slots[LANES / kWave + 1];
+    constexpr int kRows = LANES > kWave ? 1 : kBlock / kWave;       // rows per workgroup, a wave each if several
+    constexpr int kUnroll = K ? K : 1;
+    __shared__ float2 slots[LANES / kWave];
     const int lane = threadIdx.x % LANES;
     const long long row = static_cast<long long>(blockIdx.x) * kRows + threadIdx.x / LANES;
     if (row >= a.rows) return;                                       // whole waves, and only where nothing is waited for
@@ -110,48 +161,56 @@ __global__ __launch_bounds__(LANES > kBlock ? LANES : kBlock) void rms_norm_kern
     char* sum = a.sum ? row_of<T>(a.sum, row, a.sum_stride) : nullptr;
     const int n = a.width;
     const int steps = K ? K : (n + LANES * V - 1) / (LANES * V);
-    constexpr int kUnroll = K ? K : 1;
+    const bool whole_row = EIGHT && a.group == 0;
 
-    const auto read = [&](int e, bool again) {
-        if (again && sum) return load_row<T, V>(sum, e, n);         // x may have been overwritten by it
-        Raw<T, V> h = load_row<T, V>(x, e, n);
-        if (residual) {
-            float p[V], q[V];
-            h.get(p);
-            load_row<T, V>(residual, e, n).get(q);
+    NormVector<T, WIDE> kept[kUnroll];
+    if constexpr (K > 0) {
 #pragma unroll
-            for (int k = 0; k < V; ++k) p[k] += q[k];
-            h.set(p);
+        for (int s = 0; s < K; ++s) {
+            kept[s] = NormVector<T, WIDE>{};
+            kept[s].template load<NT>(a, x, residual, (s * LANES + lane) * V);
         }
-        return h;
-    };
-
-    Raw<T, V> kept[K ? K : 1];
+    }
     float squares = 0.0f, peak = 0.0f;
 #pragma unroll kUnroll
     for (int s = 0; s < steps; ++s) {
         const int e = (s * LANES + lane) * V;
         if (e >= n) break;
-        const Raw<T, V> r = read(e, false);
+        NormVector<T, WIDE>& v = kept[K ? s : 0];
+        if constexpr (K == 0) v.template load<NT>(a, x, residual, e);
+        if (residual) {
+            v.add();
+            if (sum) store_row<T, V, NT>(sum, e, n, v.h);
+        }
         float h[V];
-        r.get(h);
+        v.h.get(h);
 #pragma unroll
         for (int k = 0; k < V; ++k) squares = fmaf(h[k], h[k], squares);
-        if (EIGHT && a.group == 0) {
+        if (whole_row) {
             float w[V];
-            weights_at<T, V>(a.weight, a.weight_f32, e, n, w);
+            v.weights(w);
 #pragma unroll
             for (int k = 0; k < V; ++k) peak = fmaxf(peak, fabsf(h[k] * w[k]));
         }
-        if (sum) store_row<T, V>(sum, e, n, r);
-        if constexpr (K > 0) kept[s] = r;
     }
-    squares = group_sum<LANES>(squares, slots);
+    squares = wave_sum_by_rows(squares);
+    if (whole_row) peak = wave_max_by_rows(peak);
+    if constexpr (LANES > kWave) {
+        if ((lane & (kWave - 1)) == 0) slots[lane / kWave] = make_float2(squares, peak);
+        __syncthreads();
+        squares = 0.0f;
+#pragma unroll
+        for (int k = 0; k < LANES / kWave; ++k) {
+            squares += slots[k].x;
+            peak = fmaxf(peak, slots[k].y);
+        }
+    }
     const float rstd = 1.0f / sqrtf(squares / static_cast<float>(n) + a.eps);
     if (a.rstd && lane == 0) a.rstd[row] = rstd;
-    float scale = 1.0f;
-    if (EIGHT && a.group == 0) {
-        scale = scale_of(group_max<LANES>(peak, slots) * rstd);
+    float scale = 1.0f, inverse = 1.0f;
+    if (whole_row) {
+        scale = scale_of(peak * rstd);
+        inverse = 1.0f / scale;
         if (lane == 0) a.scales[row] = scale;
     }
     const int groups = (n + 127) / 128;
@@ -159,40 +218,46 @@ __global__ __launch_bounds__(LANES > kBlock ? LANES : kBlock) void rms_norm_kern
     for (int s = 0; s < steps; ++s) {
         const int e = (s * LANES + lane) * V;
         // with a scale per group all lanes of a wave go on together
-        if (s * LANES * V + lane / kWave * kWave * V >= n) break;
-        float h[V] = {}, w[V] = {};
-        if (e < n) {
-            if constexpr (K > 0) kept[s].get(h);
-            else read(e, true).get(h);
-            weights_at<T, V>(a.weight, a.weight_f32, e, n, w);
+        if ((s * LANES + lane / kWave * kWave) * V >= n) break;
+        NormVector<T, WIDE>& v = kept[K ? s : 0];
+        if constexpr (K == 0) {
+            v = NormVector<T, WIDE>{};
+            // x may have been overwritten by the sum, which is what is wanted
+            v.template load<NT>(a, sum ? sum : x, sum ? nullptr : residual, e);
+            if (residual && !sum) v.add();
         }
-        float y[V];
+        float y[V], w[V];
+        v.h.get(y);
+        v.weights(w);
 #pragma unroll
-        for (int k = 0; k < V; ++k) y[k] = h[k] * rstd * w[k];
+        for (int k = 0; k < V; ++k) y[k] = y[k] * rstd * w[k];
         if constexpr (EIGHT) {
             if (a.group) {
                 float most = 0.0f;
 #pragma unroll
                 for (int k = 0; k < V; ++k) most = fmaxf(most, fabsf(y[k]));
                 scale = scale_of(scale_group_max<V>(most));
+                inverse = 1.0f / scale;
                 if (e % 128 == 0 && e < n) a.scales[row * groups + e / 128] = scale;
             }
-            const float inverse = 1.0f / scale;
 #pragma unroll
             for (int k = 0; k < V; ++k) y[k] *= inverse;
             if (e < n) store_e4m3<V>(static_cast<char*>(a.y) + row * a.y_stride, e, n, y);
         } else {
             Raw<T, V> r;
             r.set(y);
-            if (e < n) store_row<T, V>(row_of<T>(a.y, row, a.y_stride), e, n, r);
+            if (e < n) store_row<T, V, NT>(row_of<T>(a.y, row, a.y_stride), e, n, r);
         }
     }
 }
 
-template<int T, bool EIGHT, int LANES, int K>
+template<int T, bool EIGHT, bool WIDE, int LANES, int K>
 int launch_norm(const NormArgs& a, hipStream_t s)
 {
-    constexpr int kRows = LANES < kBlock ? kBlock / LANES : 1;
+    constexpr int kRows = LANES > kWave ? 1 : kBlock / kWave;
+    // past the caches where the tensors do not fit
+    const size_t tensors = 1 + (a.residual != nullptr) + (a.sum != nullptr) + !EIGHT;
+    const bool past = K > 0 && static_cast<size_t>(a.rows) * static_cast<size_t>(a.width) * kSize<T> * tensors >= kStreamingBytes;
     for (long long done = 0; done < a.rows; done += kLaunchRows) {
         NormArgs part = a;
         part.x = row_of<T>(a.x, done, a.x_stride);
@@ -202,22 +267,26 @@ int launch_norm(const NormArgs& a, hipStream_t s)
         part.scales = a.scales + (EIGHT ? done * (a.group ? (a.width + 127) / 128 : 1) : 0);
         part.rstd = a.rstd ? a.rstd + done : nullptr;
         part.rows = a.rows - done < kLaunchRows ? a.rows - done : kLaunchRows;
-        hipLaunchKernelGGL((rms_norm_kernel<T, EIGHT, LANES, K>), dim3(grid_for(part.rows, kRows)),
-                           dim3(LANES < kBlock ? kBlock : LANES), 0, s, part);
+        const dim3 grid(grid_for(part.rows, kRows)), block(kRows * LANES);
+        if (past) hipLaunchKernelGGL((rms_norm_kernel<T, EIGHT, WIDE, LANES, K, K != 0>), grid, block, 0, s, part);
+        else hipLaunchKernelGGL((rms_norm_kernel<T, EIGHT, WIDE, LANES, K, false>), grid, block, 0, s, part);
         if (int rc = check_launch("pxh_rms_norm_forward")) return rc;
     }
     return PXH_OK;
 }
 
-template<int T, bool EIGHT>
+template<int T, bool EIGHT, bool WIDE>
 int norm_forward(const NormArgs& a, hipStream_t s)
 {
     const int vectors = (a.width + kVec<T> - 1) / kVec<T>;
-    if (vectors <= 64) return launch_norm<T, EIGHT, 64, 1>(a, s);
-    if (vectors <= 256) return launch_norm<T, EIGHT, 256, 1>(a, s);
-    if (vectors <= 1024) return launch_norm<T, EIGHT, 256, 4>(a, s);
-    if (vectors <= 4096) return launch_norm<T, EIGHT, 1024, 4>(a, s);
-    return launch_norm<T, EIGHT, 1024, 0>(a, s);
+    if (vectors <= 64) return launch_norm<T, EIGHT, WIDE, 64, 1>(a, s);
+    if (vectors <= 128) return launch_norm<T, EIGHT, WIDE, 128, 1>(a, s);
+    if (vectors <= 256) return launch_norm<T, EIGHT, WIDE, 256, 1>(a, s);
+    if (vectors <= 512) return launch_norm<T, EIGHT, WIDE, 256, 2>(a, s);
+    if (vectors <= 1024) return launch_norm<T, EIGHT, WIDE, 512, 2>(a, s);
+    if (vectors <= 2048) return launch_norm<T, EIGHT, WIDE, 1024, 2>(a, s);
+    if (vectors <= 4096) return launch_norm<T, EIGHT, WIDE, 1024, 4>(a, s);
+    return launch_norm<T, EIGHT, WIDE, 1024, 0>(a, s);
 }
 
 // ---------------------------------------------------------------- backward
@@ -494,10 +563,14 @@ int pxh_rms_norm_forward(const void* x, const void* residual, void* sum, const v
     if (eight && !scales) return fail_invalid("%s: 8-bit values without scales", who);
     if (x_stride < width || y_stride < width || (residual && residual_stride < width) || (sum && sum_stride < width))
         return fail_invalid("%s: rows of %d values that overlap", who, width);
-    const NormArgs a{ x, residual, sum, weight, y, scales, rstd, rows, x_stride, residual_stride, sum_stride, y_stride, width, group,
-                      weight_type == PXH_F32, eps };
+    const NormArgs a{ x, residual, sum, weight, y, scales, rstd, rows, x_stride, residual_stride, sum_stride, y_stride, width, group, eps };
     int rc = PXH_OK;
-    dispatch_type(type, [&]<int T>() { rc = eight ? norm_forward<T, true>(a, as_stream(stream)) : norm_forward<T, false>(a, as_stream(stream)); });
+    dispatch_type(type, [&]<int T>() {
+        constexpr bool kMayWiden = T != PXH_F32;
+        hipStream_t s = as_stream(stream);
+        if (kMayWiden && weight_type == PXH_F32) rc = eight ? norm_forward<T, true, kMayWiden>(a, s) : norm_forward<T, false, kMayWiden>(a, s);
+        else rc = eight ? norm_forward<T, true, false>(a, s) : norm_forward<T, false, false>(a, s);
+    });
     return rc;
 }
 

@@ -152,17 +152,28 @@ __device__ __forceinline__ float rounded(float x)
     }
 }
 
+// V values at element e < n of a row of n, the row's last ones, and `fill` behind them: without a branch, so that several such
+// loads go out together.
+template<int T, int V>
+__device__ __forceinline__ Raw<T, V> load_end(const void* p, int e, int n, float fill = 0.0f)
+{
+    float x[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        const float l = load_one<T>(p, min(e + k, n - 1));
+        x[k] = e + k < n ? l : fill;
+    }
+    Raw<T, V> r;
+    r.set(x);
+    return r;
+}
+
 // V values at element e of a row of n: whole vectors in one access, the row's last ones value by value, and `fill` behind them.
 template<int T, int V, bool NT = false>
 __device__ __forceinline__ Raw<T, V> load_row(const void* p, int e, int n, float fill = 0.0f)
 {
     if (e + V <= n) return load_raw<T, V, NT>(p, e);
-    float x[V];
-#pragma unroll
-    for (int k = 0; k < V; ++k) x[k] = e + k < n ? load_one<T>(p, e + k) : fill;
-    Raw<T, V> r;
-    r.set(x);
-    return r;
+    return load_end<T, V>(p, e, n, fill);
 }
 
 template<int T, int V, bool NT = false>

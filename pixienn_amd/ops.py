@@ -660,12 +660,11 @@ def _type(t, name):
     return kind
 
 
-def _vector(t, name, n, dtype=None):
-    """A packed tensor of n values, or None."""
+def _vector(t, name, n, dtype=_F32):
+    """A packed tensor of n values (dtype None: of any type), or None."""
     if t is None:
         return
-    if dtype is not None or not isinstance(t, torch.Tensor) or not t.is_cuda or not t.is_contiguous():
-        _chk(t, dtype or getattr(t, "dtype", None), name)
+    _chk(t, dtype or getattr(t, "dtype", None), name)
     if t.numel() != n:
         raise PxError("%s must hold %d values (got %d)" % (name, n, t.numel()))
 
@@ -674,22 +673,38 @@ def _bytes(workspace):
     return 0 if workspace is None else workspace.numel() * workspace.element_size()
 
 
+def _made(name, *args):
+    """Whether the native call has been made, with a function's own arguments; an error of the entry point is raised.  A call that
+    it leaves goes on through the function's checks, which say what is wrong with it."""
+    if not capi.functions:
+        capi.bind_calls()
+    try:
+        rc = capi.functions[name](*args, _raw_stream(_current_device()))
+    except RuntimeError:              # without a device: what is wrong with the tensors comes first
+        return False
+    if rc:
+        raise PxError("%s failed (status %d): %s" % (name, rc, capi.last_error()))
+    return rc == 0
+
+
 def rms_norm_forward(x, y, weight, residual=None, sum=None, scales=None, rstd=None, eps=1e-6, group=0):
     """y = h / sqrt(mean(h^2) + eps) * weight over the last dimension, h = x + residual (rounded to x's type; kept in `sum`).
     y is of x's type, or float8_e4m3fn with `scales` [rows, 1] (group 0) or [rows, width / 128 rounded up] (group 128): the
     value is scale * y.  rstd [rows] is what the backward pass needs."""
+    if _made("pxh_rms_norm_forward", x, y, weight, residual, sum, scales, rstd, eps, group):
+        return y
     rows, width, x_stride = _rows(x, "x")
     kind = _type(x, "x")
     eight = _tensor(y).dtype is _E4M3
     y_stride = _like(y, "y", x.shape, _E4M3 if eight else x.dtype)
-    _vector(weight, "weight", width)
+    _vector(weight, "weight", width, None)
     if eight:
         _vector(scales, "scales", rows * (-(-width // 128) if group else 1))
     if rstd is not None:
         _vector(rstd, "rstd", rows)
-    _run("pxh_rms_norm_forward", x.data_ptr(), ptr(residual), ptr(sum), weight.data_ptr(), y.data_ptr(), scales if eight else None,
-         rstd, kind, _type(weight, "weight"), 3 if eight else kind, rows, width, x_stride,
-         _like(residual, "residual", x.shape, x.dtype), _like(sum, "sum", x.shape, x.dtype), y_stride, group, float(eps))
+    call("pxh_rms_norm_forward", ptr(x), ptr(residual), ptr(sum), ptr(weight), ptr(y), ptr(scales) if eight else None, ptr(rstd),
+          kind, _type(weight, "weight"), 3 if eight else kind, rows, width, x_stride,
+         _like(residual, "residual", x.shape, x.dtype), _like(sum, "sum", x.shape, x.dtype), y_stride, group, float(eps), _stream())
     return y
 
 
@@ -700,14 +715,17 @@ def rms_norm_workspace_bytes(rows, width):
 def rms_norm_backward(dy, h, weight, rstd, dx, dw, dsum=None, accumulate=False, workspace=None):
     """The gradients of rms_norm_forward from h (its `sum`, or x without a residual) and its rstd: dx of x and residual alike,
     with dsum, what arrives along the residual stream, added; dw (fp32) overwritten or added to."""
+    if _made("pxh_rms_norm_backward", dy, h, weight, rstd, dx, dw, dsum, int(accumulate), workspace):
+        return dx
     rows, width, dy_stride = _rows(dy, "dy")
     kind = _type(dy, "dy")
-    _vector(weight, "weight", width)
+    _vector(weight, "weight", width, None)
     _vector(rstd, "rstd", rows)
     _vector(dw, "dw", width)
-    _run("pxh_rms_norm_backward", dy.data_ptr(), ptr(h), weight.data_ptr(), rstd, ptr(dsum), ptr(dx), dw, kind,
+    call("pxh_rms_norm_backward", ptr(dy), ptr(h), ptr(weight), ptr(rstd), ptr(dsum), ptr(dx), ptr(dw), kind,
          _type(weight, "weight"), rows, width, dy_stride, _like(h, "h", dy.shape, dy.dtype), _like(dsum, "dsum", dy.shape, dy.dtype),
-         _like(dx, "dx", dy.shape, dy.dtype), int(bool(accumulate)), ptr(workspace), _bytes(workspace))
+         _like(dx, "dx", dy.shape, dy.dtype), int(bool(accumulate)), ptr(workspace), _bytes(workspace),
+         _stream())
     return dx
 
 
@@ -734,6 +752,8 @@ def token_logprobs_forward(logits, targets, logp, entropy=None, lse=None, top_lo
     """Per row of logits [rows, vocab], times `scale`: the log probability of its token (targets [rows], int32 or int64; 0 for one
     outside the vocabulary), the entropy, the log of the sum of exponentials, and the most probable alternatives, top_logp and
     top_ids (int32) [rows, top], the lowest index first among equal ones."""
+    if _made("pxh_token_logprobs_forward", logits, targets, logp, entropy, lse, top_logp, top_ids, scale, workspace):
+        return
     rows, vocab, stride = _rows(logits, "logits")
     at, wide = _targets(targets, rows)
     _per_row(rows, logp=logp, entropy=entropy, lse=lse)
@@ -744,28 +764,32 @@ def token_logprobs_forward(logits, targets, logp, entropy=None, lse=None, top_lo
         top = top_ids.shape[-1]
         _vector(top_ids, "top_ids", rows * top, torch.int32)
         _vector(top_logp, "top_logp", rows * top)
-    _run("pxh_token_logprobs_forward", logits.data_ptr(), at, logp, entropy, lse, top_logp if top else None, ptr(top_ids),
-         _type(logits, "logits"), wide, rows, vocab, stride, top, float(scale), ptr(workspace), _bytes(workspace))
+    call("pxh_token_logprobs_forward", ptr(logits), at, ptr(logp), ptr(entropy), ptr(lse), ptr(top_logp) if top else None, ptr(top_ids),
+         _type(logits, "logits"), wide, rows, vocab, stride, top, float(scale), ptr(workspace), _bytes(workspace), _stream())
 
 
 def token_logprobs_backward(logits, targets, lse, d_logp, dlogits, entropy=None, d_entropy=None, scale=1.0):
     """The gradient of the logits for given gradients of logp and entropy (either may be None), from the forward's lse and, with
     d_entropy, its entropy.  dlogits may be the logits."""
+    if _made("pxh_token_logprobs_backward", logits, targets, lse, d_logp, dlogits, entropy, d_entropy, scale):
+        return dlogits
     rows, vocab, stride = _rows(logits, "logits")
     at, wide = _targets(targets, rows)
     _per_row(rows, lse=lse, d_logp=d_logp, entropy=entropy, d_entropy=d_entropy)
-    _run("pxh_token_logprobs_backward", logits.data_ptr(), at, lse, entropy, d_logp, d_entropy, ptr(dlogits),
-         _type(logits, "logits"), wide, rows, vocab, stride, _like(dlogits, "dlogits", logits.shape, logits.dtype), float(scale))
+    call("pxh_token_logprobs_backward", ptr(logits), at, ptr(lse), ptr(entropy), ptr(d_logp), ptr(d_entropy), ptr(dlogits),
+         _type(logits, "logits"), wide, rows, vocab, stride, _like(dlogits, "dlogits", logits.shape, logits.dtype), float(scale), _stream())
     return dlogits
 
 
 def token_logprobs_forward_train(logits, targets, d_logp, dlogits, logp=None, entropy=None, lse=None, d_entropy=None, scale=1.0):
     """token_logprobs_forward and token_logprobs_backward at once, for gradients that are known before."""
+    if _made("pxh_token_logprobs_forward_train", logits, targets, d_logp, dlogits, logp, entropy, lse, d_entropy, scale):
+        return dlogits
     rows, vocab, stride = _rows(logits, "logits")
     at, wide = _targets(targets, rows)
     _per_row(rows, d_logp=d_logp, logp=logp, entropy=entropy, lse=lse, d_entropy=d_entropy)
-    _run("pxh_token_logprobs_forward_train", logits.data_ptr(), at, d_logp, d_entropy, ptr(dlogits), logp, entropy, lse,
-         _type(logits, "logits"), wide, rows, vocab, stride, _like(dlogits, "dlogits", logits.shape, logits.dtype), float(scale))
+    call("pxh_token_logprobs_forward_train", ptr(logits), at, ptr(d_logp), ptr(d_entropy), ptr(dlogits), ptr(logp), ptr(entropy), ptr(lse),
+         _type(logits, "logits"), wide, rows, vocab, stride, _like(dlogits, "dlogits", logits.shape, logits.dtype), float(scale), _stream())
     return dlogits
 
 
@@ -799,8 +823,9 @@ class AdamwTable:
                                            (ms_, "m_scale", blocks, torch.float32), (vs_, "v_scale", blocks, torch.float32), (copy, "copy", n, None)):
                 if x is None and (name == "copy" or not eight and name.endswith("scale")):
                     continue
-                _chk(x, dtype or getattr(x, "dtype", None), name)
                 _vector(x, name, length, dtype)
+                if x is None:
+                    raise PxError("%s: torch.Tensor expected" % name)
                 device = x.device if device is None else device
                 if x.device != device:
                     raise PxError("the tensors of an AdamwTable have to be on one device")
