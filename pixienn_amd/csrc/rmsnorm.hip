@@ -306,7 +306,7 @@ struct NormBackwardArgs {
 // dx of every row, and the part of dw that this worker's rows give: a worker (LANES lanes) takes every workers-th row, and asks for
 // the next one before it waits for the sum over this one.  At four vectors a lane there are no registers for that, nor for
 // the weights, which are read again for every row.
-template<int T, int LANES, int K>
+template<int T, int LANES, int K, bool NT>
 __global__ __launch_bounds__(LANES > kWave ? LANES : kBlock) void rms_norm_backward_kernel(NormBackwardArgs a, int workers)
 {
     constexpr int V = kVec<T>;
@@ -343,9 +343,9 @@ __global__ __launch_bounds__(LANES > kWave ? LANES : kBlock) void rms_norm_backw
         for (int s = 0; s < K; ++s) {
             const int e = (s * LANES + lane) * V;
             if (e >= n) break;
-            r.g[s] = load_row<T, V>(dy, e, n);
-            r.h[s] = load_row<T, V>(h, e, n);
-            if (kAhead && a.dsum) r.more[s] = load_row<T, V>(row_of<T>(a.dsum, row, a.dsum_stride), e, n);
+            r.g[s] = load_row<T, V, NT>(dy, e, n);
+            r.h[s] = load_row<T, V, NT>(h, e, n);
+            if (kAhead && a.dsum) r.more[s] = load_row<T, V, NT>(row_of<T>(a.dsum, row, a.dsum_stride), e, n);
         }
     };
     Row next;
@@ -399,7 +399,7 @@ __global__ __launch_bounds__(LANES > kWave ? LANES : kBlock) void rms_norm_backw
             for (int k = 0; k < V; ++k) g[k] = fmaf(r.rstd, g[k] * (kAhead ? w[kAhead ? s : 0][k] : u[k]) - x[k] * c, more[k]);
             Raw<T, V> out;
             out.set(g);
-            store_row<T, V>(row_of<T>(a.dx, row, a.dx_stride), e, n, out);
+            store_row<T, V, NT>(row_of<T>(a.dx, row, a.dx_stride), e, n, out);
         }
     }
 #pragma unroll
@@ -490,12 +490,13 @@ __global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const float* partial,
     }
 }
 
-// Workers that share the rows of the backward pass, each with a row of partial sums: two to four workgroups for each of 256
-// compute units, as wide as a row; fewer for the widest rows, so that the partial sums stay small beside the tensors.
+// Workers that share the rows of the backward pass, each with a row of partial sums: a workgroup as wide as a row for each of 256 compute
+// units (16384 x 4096 bf16: 1024 workers 108 us, 512 96, 256 89.5; 777 x 5121 half 17.1 with 512, 14.9 with 256), more of them where
+// a row takes a few waves (16384 x 1024: 35 us with 512, 27 with 1024), fewer for rows of any width.
 constexpr int kWideWorkers = 32;
 int workers_for(long long rows, int width)
 {
-    const int most = width <= 4096 ? 1024 : width <= 16384 ? 512 : width <= 32768 ? 256 : kWideWorkers;
+    const int most = width <= 2048 ? 1024 : width <= 32768 ? 256 : kWideWorkers;
     return static_cast<int>(rows < most ? rows : most);
 }
 
@@ -503,7 +504,11 @@ template<int T, int LANES, int K>
 int launch_backward(const NormBackwardArgs& a, int workers, hipStream_t s)
 {
     constexpr int kPer = LANES > kWave ? 1 : kBlock / kWave;
-    hipLaunchKernelGGL((rms_norm_backward_kernel<T, LANES, K>), dim3(grid_for(workers, kPer)), dim3(LANES * kPer), 0, s, a, workers);
+    const dim3 grid(grid_for(workers, kPer)), block(LANES * kPer);
+    // past the caches where the tensors do not fit (16384 x 4096 bf16 105 -> 97 us; 2048 x 4096 would go from 17 to 20)
+    const size_t bytes = static_cast<size_t>(a.rows) * static_cast<size_t>(a.width) * kSize<T> * (a.dsum ? 4 : 3);
+    if (bytes >= kStreamingBytes) hipLaunchKernelGGL((rms_norm_backward_kernel<T, LANES, K, true>), grid, block, 0, s, a, workers);
+    else hipLaunchKernelGGL((rms_norm_backward_kernel<T, LANES, K, false>), grid, block, 0, s, a, workers);
     return check_launch("pxh_rms_norm_backward");
 }
 
@@ -579,7 +584,7 @@ size_t pxh_rms_norm_workspace_bytes(long long rows, int width)
     if (rows <= 0 || width <= 0) return 0;
     // the largest that any of the shapes up to this one takes
     size_t most = 0;
-    for (int w: { 4096, 16384, 32768, width }) {
+    for (int w: { 2048, 32768, width }) {
         const int here = width < w ? width : w;
         const size_t floats = static_cast<size_t>(workers_for(rows, here)) * static_cast<size_t>(here);
         if (floats > most) most = floats;
