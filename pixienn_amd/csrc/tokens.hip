@@ -778,9 +778,16 @@ inline bool streams(const TokenArgs& a, int type, int tensors)
 constexpr long long kEnoughParts = 1024;
 constexpr int kMostVectors = 8;         // vectors of a lane
 
-// From so many rows on a row that a workgroup of 1024 lanes holds is not split: two such workgroups to a compute unit (4096 x 50000
-// bf16 with three alternatives 98 -> 91 us).
-constexpr long long kRowsForWholeGroups = 512;
+// Whether a row goes to one workgroup of 1024 lanes, without a second launch: up to 4096 vectors whatever the rows (8 x 32768 bf16 8.0 us in
+// parts, 5.0 whole; 256 x 32768 with five alternatives 14.2 and 9.4), and up to the 8192 that it holds from 64 rows on (256 x 65536
+// with eight 18.2 and 13.5, 16 x 65536 9.9 and 11.1).  A row of up to 2048 vectors is not split anyway where the rows are many,
+// and then smaller workgroups have less to wait for.
+inline bool whole_rows(long long rows, long long vectors)
+{
+    if (vectors <= kBlock || vectors > 1024 * kMostVectors) return false;
+    if (vectors <= kBlock * kMostVectors && rows >= kEnoughParts) return false;
+    return vectors <= 512 * kMostVectors || rows >= 64;
+}
 
 // Parts of a row of `vectors`, with up to `k` vectors to a lane.
 inline int parts_of(long long vectors, int k) { return static_cast<int>((vectors + kBlock * k - 1) / (kBlock * k)); }
@@ -797,7 +804,7 @@ int launch_forward(const char* who, const TokenArgs& a, void* workspace, hipStre
 {
     const int vectors = a.vocab < kVec<T> ? 1 : a.vocab / kVec<T>;      // the values behind the last one go with it
     Parts p{};
-    if (a.rows >= kRowsForWholeGroups && vectors > kBlock * kMostVectors && vectors <= 1024 * kMostVectors) {
+    if (whole_rows(a.rows, vectors)) {
         p.parts = 1;
         p.vectors = vectors;
         const dim3 grid(static_cast<unsigned>(a.rows)), block(1024);

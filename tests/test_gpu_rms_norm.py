@@ -117,6 +117,26 @@ def test_eight_bits_are_the_scaled_values(ops, rows, width, kind, group, residua
 
 
 @gpu
+@pytest.mark.parametrize("rows,width,kind", [(9000, 4097, "bf16"), (70000, 500, "f16"), (2100, 16384, "f32")])
+def test_tensors_that_do_not_fit_the_caches(ops, rows, width, kind):
+    dtype, e, least = TYPES[kind]
+    x, r = (torch.randn(rows, width, device="cuda", generator=torch.Generator("cuda").manual_seed(i)).to(dtype) for i in (1, 2))
+    weight = draw(6, (1, width), 1.0, dtype)[0].contiguous()
+    y, total, rstd = torch.empty_like(x), torch.empty_like(x), torch.empty(rows, device="cuda")
+    ops.rms_norm_forward(x, y, weight, residual=r, sum=total, rstd=rstd, eps=1e-5)
+    h, want_rstd, want = formula(x, r, weight, 1e-5)
+    assert torch.equal(total, h)
+    held(rstd, want_rstd, want_rstd * U * (additions(width) / 2 + 3), "rstd")
+    held(y, want, want.abs() * (U * (additions(width) / 2 + 6) + e) + least, "y")
+    dx, dw = torch.empty_like(x), torch.empty(width, device="cuda")
+    ops.rms_norm_backward(r, h, weight, rstd, dx, dw, dsum=x)
+    want, dot, parts, want_dw, sum_dw = gradients(r, h, weight, rstd, x)
+    held(dx, want, dot * U * additions(width) + parts * 6 * U + want.abs() * (e + U) + least, "dx")
+    # the rows of one of 256 workers (of 1024 for narrow rows) in turn, then the workers
+    held(dw, want_dw, sum_dw * U * (rows / 256 + 64 + 20) + 1e-30, "dw")
+
+
+@gpu
 @pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("width", [96, 3000, 40000])
 def test_infinities_and_nan_stay_in_their_rows(ops, kind, width):

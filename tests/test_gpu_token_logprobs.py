@@ -265,6 +265,42 @@ def test_a_row_of_the_lowest_value_has_even_probabilities(ops, kind, vocab):
 
 
 @gpu
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [3000, 30001, 66001, 140000])
+def test_huge_logits(ops, kind, vocab):
+    """Exponents that one multiply-add does not hold, in all of a row or in some of its lanes only."""
+    dtype, e, least = TYPES[kind]
+    x = draw(vocab, 6, vocab, torch.float32)
+    x[0] *= 3e6
+    x[1, vocab // 2:] -= 5e6
+    x[2, : vocab // 3] = -2e30
+    x[3] += 7e6
+    x[4] = -3e7
+    x[4, 17] = -2.9e7
+    x = x.to(dtype)
+    targets = torch.tensor([0, 1, vocab - 1, 3, 17, vocab // 2], device="cuda")
+    got, want = check_forward(ops, x, targets, 5)
+    g = torch.ones(6, device="cuda")
+    for h in (None, g):
+        d, bound = want.gradient(targets, g, h, 1.0, want.lse_off, want.entropy_off, e, least)
+        for together in (True, False):
+            held(gradients(ops, x, targets, g, h, 1.0, together)[0], d, bound, "together %s" % together)
+
+
+@gpu
+@pytest.mark.parametrize("rows,vocab,kind", [(1100, 65536, "bf16"), (700, 100001, "f16"), (9000, 4003, "f32")])
+def test_logits_that_do_not_fit_the_caches(ops, rows, vocab, kind):
+    dtype, e, least = TYPES[kind]
+    x = draw(3, rows, vocab, dtype)
+    targets = torch.arange(rows, device="cuda")
+    got, want = check_forward(ops, x, targets, 2)
+    g = torch.ones(rows, device="cuda")
+    d, bound = want.gradient(targets, g, None, 1.0, want.lse_off, want.entropy_off, e, least)
+    for together in (True, False):
+        held(gradients(ops, x, targets, g, None, 1.0, together)[0], d, bound, "together %s" % together)
+
+
+@gpu
 def test_gradient_against_differences(ops):
     rows, vocab, scale = 3, 23, 0.75
     x = draw(1, rows, vocab, torch.float32)
