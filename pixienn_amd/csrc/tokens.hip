@@ -172,6 +172,13 @@ __device__ __forceinline__ uint32_t max_in_row(uint32_t v)
     return v > o ? v : o;
 }
 
+__device__ __forceinline__ uint32_t wave_max_of(uint32_t v)
+{
+    v = max_in_row<0x140>(max_in_row<0x141>(max_in_row<0x4E>(max_in_row<0xB1>(v))));
+    const auto of_lane = [&](int lane) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane)); };
+    return max(max(of_lane(0), of_lane(16)), max(of_lane(32), of_lane(48)));
+}
+
 // The k largest keys of a workgroup, largest first: put(place, key), key 0 where there are fewer.  `best` is the largest order of
 // the lane's keys (0: none); above(floor, f) calls f with those of its keys that reach `floor`, and may with others; each(f)
 // calls f with all keys of the workgroup, some by every lane.
@@ -189,13 +196,21 @@ __device__ __forceinline__ void select_largest(int k, uint32_t best, const Above
     __syncthreads();
     if (threadIdx.x < kWave) {
         const uint32_t mine = s.best[threadIdx.x];
-        int larger = 0;
+        uint32_t low;
+        if (k <= 8) {
+            // the k-th largest of different ones, which is no larger: round by round
+            uint32_t left = mine;
+            low = 0;
+            for (int j = 0; j < k; ++j) {
+                low = wave_max_of(left);
+                left = left == low ? 0u : left;
+            }
+        } else {
+            int larger = 0;
 #pragma unroll
-        for (int j = 0; j < kWave; ++j) larger += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), j)) > mine;
-        uint32_t low = larger < k ? mine : ~0u;
-        low = ~max_in_row<0x140>(max_in_row<0x141>(max_in_row<0x4E>(max_in_row<0xB1>(~low))));
-        const auto of_lane = [&](int lane) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(low), lane)); };
-        low = min(min(of_lane(0), of_lane(16)), min(of_lane(32), of_lane(48)));
+            for (int j = 0; j < kWave; ++j) larger += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), j)) > mine;
+            low = ~wave_max_of(larger < k ? ~mine : 0u);
+        }
         if (threadIdx.x == 0) s.floor = low;
     }
     __syncthreads();
