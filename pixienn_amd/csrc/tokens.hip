@@ -188,9 +188,10 @@ __device__ __forceinline__ uint32_t wave_max_of(uint32_t v)
 template<int LANES, typename Above, typename Each, typename Put>
 __device__ __forceinline__ void select_largest(int k, uint32_t best, const Above& above, const Each& each, const Put& put, Selection& s)
 {
-    static_assert(LANES == 256 || LANES == 1024, "64 groups of lanes of one row of 16");
+    static_assert(LANES == 256 || LANES == 512 || LANES == 1024, "64 groups of lanes of one row of 16");
     uint32_t group = max_in_row<0x4E>(max_in_row<0xB1>(best));
-    if constexpr (LANES == 1024) group = max_in_row<0x140>(max_in_row<0x141>(group));
+    if constexpr (LANES >= 512) group = max_in_row<0x141>(group);
+    if constexpr (LANES == 1024) group = max_in_row<0x140>(group);
     if (threadIdx.x % (LANES / kWave) == 0) s.best[threadIdx.x / (LANES / kWave)] = group;
     if (threadIdx.x == 0) s.count = 0;
     __syncthreads();
@@ -271,16 +272,18 @@ struct Part {
         const int whole = vocab / V;
         first = first_vector;
         count = min(vectors, whole - first_vector);
+        // before the vectors, which are waited for in their order (8000 x 17000 bf16 with five alternatives 106 -> 94 us), and without a
+        // branch, whose end would wait for all loads
+        extra_at = whole * V + static_cast<int>(threadIdx.x);
+        if (first_vector + vectors < whole || extra_at >= vocab) extra_at = -1;
+        extra = load_one<T>(row, extra_at < 0 ? 0 : extra_at);
+        if (extra_at < 0) extra = -INFINITY;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
 #pragma unroll
             for (int i = 0; i < Raw<T, V>::kWords; ++i) kept[k].w[i] = nothing;
             if (has(k)) kept[k] = load_raw_at<T, V, NT>(row + (static_cast<size_t>(first) + k * LANES) * 16, threadIdx.x * 16u);
         }
-        extra_at = whole * V + static_cast<int>(threadIdx.x);
-        if (first_vector + vectors < whole || extra_at >= vocab) extra_at = -1;
-        extra = load_one<T>(row, extra_at < 0 ? 0 : extra_at);      // without a branch, whose end would wait for all loads
-        if (extra_at < 0) extra = -INFINITY;
     }
 
     // Between two passes over the values: as fp32 numbers, which the compiler would keep from the first, they take twice the
@@ -431,6 +434,33 @@ __global__ __launch_bounds__(LANES) void token_logprobs_kernel(TokenArgs a, Part
         };
         select_largest<LANES>(a.top, any ? order_of(mine.peak * a.scale) : 0u, [&](uint32_t floor, const auto& f) { mine.above(a.scale, floor, f); },
                               [&](const auto& f) { mine.each(logits, a.vocab, a.scale, f); }, put, selection);
+    }
+}
+
+// A row's parts put together by one wave: at most 64 of them, and as many keys.
+template<int T>
+__global__ __launch_bounds__(kBlock) void token_join_few_kernel(TokenArgs a, Parts p)
+{
+    const int lane = threadIdx.x % kWave;
+    const long long row = static_cast<long long>(blockIdx.x) * (kBlock / kWave) + threadIdx.x / kWave;
+    if (row >= a.rows) return;                  // a whole wave, and none waits for another
+    const float c = a.scale * kLog2e;
+    const int target = target_of(a, row);
+    const float given = load_one<T>(static_cast<const char*>(a.logits) + row * a.stride * kSize<T>, target < 0 ? 0 : target);
+    const int n = p.parts * a.top;
+    const unsigned long long mine = lane < n ? p.keys[row * n + lane] : 0;
+    Sums s = nothing();
+    if (lane < p.parts) s = p.sums[row * p.parts + lane];
+    s = group_join<kWave>(s, c, nullptr);
+    const float lse = finish_row(a, row, s, target, given, lane == 0).lse;
+    int larger = 0;
+    for (int j = 0; j < n; ++j) {
+        const uint32_t low = __builtin_amdgcn_readlane(static_cast<int>(mine), j), high = __builtin_amdgcn_readlane(static_cast<int>(mine >> 32), j);
+        larger += (static_cast<unsigned long long>(high) << 32 | low) > mine;
+    }
+    if (lane < n && larger < a.top) {
+        a.top_ids[row * a.top + larger] = static_cast<int>(~static_cast<uint32_t>(mine));
+        a.top_logp[row * a.top + larger] = value_of(mine) - lse;
     }
 }
 
@@ -793,15 +823,19 @@ inline bool streams(const TokenArgs& a, int type, int tensors)
 constexpr long long kEnoughParts = 1024;
 constexpr int kMostVectors = 8;         // vectors of a lane
 
-// Whether a row goes to one workgroup of 1024 lanes, without a second launch: up to 4096 vectors whatever the rows (8 x 32768 bf16 8.0 us in
-// parts, 5.0 whole; 256 x 32768 with five alternatives 14.2 and 9.4), and up to the 8192 that it holds from 64 rows on (256 x 65536
-// with eight 18.2 and 13.5, 16 x 65536 9.9 and 11.1).  A row of up to 2048 vectors is not split anyway where the rows are many,
-// and then smaller workgroups have less to wait for.
-inline bool whole_rows(long long rows, long long vectors)
+// Lanes of the workgroup that takes a whole row, without a second launch, or 0.  1024 up to 4096 vectors whatever the rows (8 x 32768 bf16
+// 8.0 us in parts, 5.0 whole; 256 x 32768 with five alternatives 14.2 and 9.4), and up to the 8192 that they hold from 64 rows on
+// (256 x 65536 with eight 18.2 and 13.5; 16 x 65536 9.9 and 11.1).  Where there are rows enough for all units, as few as hold it: what
+// waits for a row's maximum, and for its alternatives, is then less of the machine (4096 x 32768 with five alternatives 1024 lanes 65 us,
+// 512 52; 8000 x 16000 97 and, with 256, 52).
+inline int lanes_for_whole_rows(long long rows, long long vectors)
 {
-    if (vectors <= kBlock || vectors > 1024 * kMostVectors) return false;
-    if (vectors <= kBlock * kMostVectors && rows >= kEnoughParts) return false;
-    return vectors <= 512 * kMostVectors || rows >= 64;
+    if (vectors <= kBlock || vectors > 1024 * kMostVectors) return 0;
+    if (rows >= kEnoughParts) {
+        if (vectors <= kBlock * kMostVectors) return 0;
+        if (vectors <= 512 * kMostVectors) return 512;
+    }
+    return vectors <= 512 * kMostVectors || rows >= 64 ? 1024 : 0;
 }
 
 // Parts of a row of `vectors`, with up to `k` vectors to a lane.
@@ -819,15 +853,19 @@ int launch_forward(const char* who, const TokenArgs& a, void* workspace, hipStre
 {
     const int vectors = a.vocab < kVec<T> ? 1 : a.vocab / kVec<T>;      // the values behind the last one go with it
     Parts p{};
-    if (whole_rows(a.rows, vectors)) {
+    const bool past = streams(a, T, 1);
+    if (const int lanes = lanes_for_whole_rows(a.rows, vectors)) {
         p.parts = 1;
         p.vectors = vectors;
-        const dim3 grid(static_cast<unsigned>(a.rows)), block(1024);
-        if (streams(a, T, 1)) hipLaunchKernelGGL((token_logprobs_kernel<T, ENTROPY, 1024, kMostVectors, true>), grid, block, 0, s, a, p);
-        else hipLaunchKernelGGL((token_logprobs_kernel<T, ENTROPY, 1024, kMostVectors, false>), grid, block, 0, s, a, p);
+        const dim3 grid(static_cast<unsigned>(a.rows)), block(lanes);
+        const auto launch = [&](auto* kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, a, p); };
+        if (lanes == 512) launch(past ? &token_logprobs_kernel<T, ENTROPY, 512, kMostVectors, true> : &token_logprobs_kernel<T, ENTROPY, 512, kMostVectors, false>);
+        else launch(past ? &token_logprobs_kernel<T, ENTROPY, 1024, kMostVectors, true> : &token_logprobs_kernel<T, ENTROPY, 1024, kMostVectors, false>);
         return check_launch(who);
     }
-    const int k = vectors_per_lane(a.rows, vectors);
+    // parts of 4096 vectors where they are enough, else of as many as make enough of them
+    const bool large = a.rows * parts_of(vectors, 2 * kMostVectors) >= kEnoughParts && vectors > kBlock * kMostVectors;
+    const int k = large ? 2 * kMostVectors : vectors_per_lane(a.rows, vectors);
     p.parts = parts_of(vectors, k);
     p.vectors = (vectors + p.parts - 1) / p.parts;
     p.parts = (vectors + p.vectors - 1) / p.vectors;
@@ -835,19 +873,22 @@ int launch_forward(const char* who, const TokenArgs& a, void* workspace, hipStre
     const size_t groups = static_cast<size_t>(a.rows) * p.parts;
     p.keys = static_cast<unsigned long long*>(workspace);
     p.sums = reinterpret_cast<Sums*>(static_cast<char*>(workspace) + groups * a.top * sizeof(unsigned long long));
-    const dim3 grid(static_cast<unsigned>(groups)), block(kBlock);
+    const auto launch = [&](auto* kernel, int lanes) { hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(groups)), dim3(lanes), 0, s, a, p); };
     switch (k) {
-    case 1: hipLaunchKernelGGL((token_logprobs_kernel<T, ENTROPY, kBlock, 1, false>), grid, block, 0, s, a, p); break;
-    case 2: hipLaunchKernelGGL((token_logprobs_kernel<T, ENTROPY, kBlock, 2, false>), grid, block, 0, s, a, p); break;
-    case 4: hipLaunchKernelGGL((token_logprobs_kernel<T, ENTROPY, kBlock, 4, false>), grid, block, 0, s, a, p); break;
-    default:
-        // past the caches where the logits do not fit (4096 x 50001 half: 101.5 -> 99.5 us)
-        if (streams(a, T, 1)) hipLaunchKernelGGL((token_logprobs_kernel<T, ENTROPY, kBlock, 8, true>), grid, block, 0, s, a, p);
-        else hipLaunchKernelGGL((token_logprobs_kernel<T, ENTROPY, kBlock, 8, false>), grid, block, 0, s, a, p);
+    case 1: launch(&token_logprobs_kernel<T, ENTROPY, kBlock, 1, false>, kBlock); break;
+    case 2: launch(&token_logprobs_kernel<T, ENTROPY, kBlock, 2, false>, kBlock); break;
+    case 4: launch(&token_logprobs_kernel<T, ENTROPY, kBlock, 4, false>, kBlock); break;
+    // past the caches where the logits do not fit (4096 x 50001 half: 101.5 -> 99.5 us)
+    case kMostVectors:
+        launch(past ? &token_logprobs_kernel<T, ENTROPY, kBlock, kMostVectors, true> : &token_logprobs_kernel<T, ENTROPY, kBlock, kMostVectors, false>, kBlock);
+        break;
+    default: launch(past ? &token_logprobs_kernel<T, ENTROPY, 512, kMostVectors, true> : &token_logprobs_kernel<T, ENTROPY, 512, kMostVectors, false>, 512);
     }
     if (int rc = check_launch(who)) return rc;
     if (p.parts == 1) return PXH_OK;
-    hipLaunchKernelGGL((token_join_kernel<T>), dim3(static_cast<unsigned>(a.rows)), block, 0, s, a, p);
+    if (p.parts <= kWave && p.parts * a.top <= kWave)
+        hipLaunchKernelGGL((token_join_few_kernel<T>), dim3(grid_for(a.rows, kBlock / kWave)), dim3(kBlock), 0, s, a, p);
+    else hipLaunchKernelGGL((token_join_kernel<T>), dim3(static_cast<unsigned>(a.rows)), dim3(kBlock), 0, s, a, p);
     return check_launch(who);
 }
 

@@ -288,7 +288,7 @@ def test_huge_logits(ops, kind, vocab):
 
 
 @gpu
-@pytest.mark.parametrize("rows,vocab,kind", [(1100, 65536, "bf16"), (700, 100001, "f16"), (9000, 4003, "f32")])
+@pytest.mark.parametrize("rows,vocab,kind", [(1100, 65536, "bf16"), (700, 100001, "f16"), (9000, 4003, "f32"), (3100, 20001, "bf16"), (2000, 16384, "f32")])
 def test_logits_that_do_not_fit_the_caches(ops, rows, vocab, kind):
     dtype, e, least = TYPES[kind]
     x = draw(3, rows, vocab, dtype)
