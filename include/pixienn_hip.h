@@ -613,9 +613,9 @@ int pxh_rescale_clip_table(const pxh_tensor_table* table, float threshold, float
  * weight_type: `type` or PXH_F32.  y_type is `type`, or PXH_E4M3 with scales: `group` consecutive values of a row (128, or 0
  * for the whole row; the last group of a row may be shorter) share
  *   scale = max(largest |y| of the group / 448, 2^-126),  and y holds e4m3(y / scale);
- * scales is [rows][width / group, rounded up], packed.  sum may be x or residual itself, and y (of `type`) may be x, residual or
- * none of the others, where the strides are the same.  An infinity in a row makes its rstd 0 and the infinite values NaN, a NaN the
- * whole row NaN, as the formulas have it. */
+ * scales is [rows][width / group, rounded up], packed.  sum may be x or residual itself, and y (of `type`) may be x or
+ * residual, where the strides are the same; nothing else that is written may overlap another tensor.  An infinity in a row makes
+ * its rstd 0 and the infinite values NaN, a NaN the whole row NaN, as the formulas have it. */
 int pxh_rms_norm_forward(const void* x, const void* residual, void* sum, const void* weight, void* y, float* scales,
                          float* rstd, int type, int weight_type, int y_type, long long rows, int width, long long x_stride,
                          long long residual_stride, long long sum_stride, long long y_stride, int group, float eps,
@@ -644,7 +644,7 @@ int pxh_rms_norm_backward(const void* dy, const void* h, const void* weight, con
  * for its alternatives, which have no distribution); one with a NaN or plus infinity
  * has NaN in all three, and its NaNs come last among the alternatives.
  * workspace: pxh_token_logprobs_workspace_bytes(rows, vocab, top), which serves fewer rows, fewer alternatives and smaller
- * vocabularies too, or NULL for the library's. */
+ * vocabularies too, or NULL for the library's (most calls write nothing to it: it is for rows in several parts). */
 #define PXH_MOST_ALTERNATIVES 64
 size_t pxh_token_logprobs_workspace_bytes(long long rows, int vocab, int top);
 int pxh_token_logprobs_forward(const void* logits, const void* targets, float* logp, float* entropy, float* lse,
@@ -676,15 +676,17 @@ int pxh_token_logprobs_forward_train(const void* logits, const void* targets, co
  *   g = d * d_scale * f;  m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
  *   w += lr * (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps) - lr * decay * w     (the decay where apply_decay says so)
  *   copy = w, rounded to its type
- * beta1 and beta2 are taken in 64 bits (1 - beta is what an fp32 beta has lost).  d is only read (unlike pxh_adam_update's).  d_scale: 1 / batch, the inverse of a loss scale, or both.
+ * beta1 and beta2 are taken in 64 bits (1 - beta is what an fp32 beta has lost).  d is only read (unlike pxh_adam_update's).
+ * d_scale: 1 / batch, the inverse of a loss scale, or both.  The norm is summed in 64 bits, in a fixed order, and rounded down
+ * to fp32.
  *
  * States in 8 bits: m and the SQUARE ROOT of v are e4m3 values with a scale for each 256 of a tensor, its largest magnitude / 448
  * (2^-126 at least): 2 + 1/32 bytes a value for both.  Each step's results are rounded stochastically, up with the
  * probability of the part cut off: what a step changes of an average over 1000 steps is less than half a unit of such a value, and
  * rounded to nearest it would never change.  A root that is not zero never rounds to zero (the quotient stays bounded).  The
  * random bits come from `seed` (its low 31 bits) and the value's place in the table: another seed every step, the step's number
- * for instance; the same seed gives the same bits.  A step reads the states as they were rounded, and applies its own before
- * they are rounded.
+ * for instance; the same seed gives the same bits.  A NaN is kept as the largest value of its block (its weight is the NaN).
+ * A step reads the states as they were rounded, and applies its own before they are rounded.
  *
  * norm_out (nullable, device) receives the norm, also when max_norm is 0.  With max_norm > 0 and a norm that is not finite (an
  * overflow of half-precision gradients) nothing is written but norm_out: the step is left out.

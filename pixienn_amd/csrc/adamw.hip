@@ -352,13 +352,14 @@ struct Gradients {
         for (int k = 0; k < kSteps; ++k) {
             float d[4];
             raw[k].get(d);
-            sum += fmaf(d[0], d[0], fmaf(d[1], d[1], fmaf(d[2], d[2], d[3] * d[3])));
+#pragma unroll
+            for (int j = 0; j < 4; ++j) sum = fma(static_cast<double>(d[j]), static_cast<double>(d[j]), sum);
         }
         if (first + kChunk > r.n) {             // the tensor's last values, which fill no vector
             const uint32_t e = r.n / 4 * 4 + threadIdx.x;
             if (threadIdx.x < 4 && e < r.n) {
-                const float d = load_one<D>(r.d, e);
-                sum += d * d;
+                const double d = load_one<D>(r.d, e);
+                sum = fma(d, d, sum);
             }
         }
         return sum;

@@ -202,7 +202,7 @@ inline bool dispatch_type(int type, F&& f)
     }
 }
 
-// Sums and maxima over a workgroup of LANES lanes, the same in every lane; `slots` is LDS of a float per wave.
+// The sum over a workgroup of LANES lanes, the same in every lane; `slots` is LDS of a float per wave.
 template<int LANES>
 __device__ __forceinline__ float group_sum(float v, float* slots)
 {
@@ -214,22 +214,6 @@ __device__ __forceinline__ float group_sum(float v, float* slots)
         v = slots[0];
 #pragma unroll
         for (int k = 1; k < LANES / kWave; ++k) v += slots[k];
-        __syncthreads();
-    }
-    return v;
-}
-
-template<int LANES>
-__device__ __forceinline__ float group_max(float v, float* slots)
-{
-    v = wave_max_by_rows(v);
-    if constexpr (LANES > kWave) {
-        const int wave = threadIdx.x / kWave;
-        if ((threadIdx.x & (kWave - 1)) == 0) slots[wave] = v;
-        __syncthreads();
-        v = slots[0];
-#pragma unroll
-        for (int k = 1; k < LANES / kWave; ++k) v = fmaxf(v, slots[k]);
         __syncthreads();
     }
     return v;

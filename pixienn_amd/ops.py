@@ -628,6 +628,8 @@ _E4M3 = torch.float8_e4m3fn
 def _rows(t, name):
     """(rows, values of a row, values from row to row) of a tensor on the device: two dimensions, of which the last is
     packed, or any number of packed ones, the leading ones being the rows."""
+    if t is None:
+        raise PxError("%s is required" % name)
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         _chk(t, getattr(t, "dtype", None), name)
     shape = t.shape

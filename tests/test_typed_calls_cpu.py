@@ -47,5 +47,5 @@ def test_the_functions_say_what_is_wrong():
     x = torch.zeros(2, 8)
     with pytest.raises(capi.PxError, match="must live on the GPU"):
         ops.rms_norm_forward(x, x, x[0])
-    with pytest.raises(capi.PxError, match="torch.Tensor expected"):
+    with pytest.raises(capi.PxError, match="logits is required"):
         ops.token_logprobs_forward(None, None, None)
