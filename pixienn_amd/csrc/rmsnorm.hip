@@ -251,13 +251,10 @@ __global__ __launch_bounds__(LANES > kWave ? LANES : kBlock) void rms_norm_kerne
     }
 }
 
-template<int T, bool EIGHT, bool WIDE, int LANES, int K>
+template<int T, bool EIGHT, bool WIDE, int LANES, int K, bool NT>
 int launch_norm(const NormArgs& a, hipStream_t s)
 {
     constexpr int kRows = LANES > kWave ? 1 : kBlock / kWave;
-    // past the caches where the tensors do not fit
-    const size_t tensors = 1 + (a.residual != nullptr) + (a.sum != nullptr) + !EIGHT;
-    const bool past = K > 0 && static_cast<size_t>(a.rows) * static_cast<size_t>(a.width) * kSize<T> * tensors >= kStreamingBytes;
     for (long long done = 0; done < a.rows; done += kLaunchRows) {
         NormArgs part = a;
         part.x = row_of<T>(a.x, done, a.x_stride);
@@ -268,25 +265,38 @@ int launch_norm(const NormArgs& a, hipStream_t s)
         part.rstd = a.rstd ? a.rstd + done : nullptr;
         part.rows = a.rows - done < kLaunchRows ? a.rows - done : kLaunchRows;
         const dim3 grid(grid_for(part.rows, kRows)), block(kRows * LANES);
-        if (past) hipLaunchKernelGGL((rms_norm_kernel<T, EIGHT, WIDE, LANES, K, K != 0>), grid, block, 0, s, part);
-        else hipLaunchKernelGGL((rms_norm_kernel<T, EIGHT, WIDE, LANES, K, false>), grid, block, 0, s, part);
+        hipLaunchKernelGGL((rms_norm_kernel<T, EIGHT, WIDE, LANES, K, NT>), grid, block, 0, s, part);
         if (int rc = check_launch("pxh_rms_norm_forward")) return rc;
     }
     return PXH_OK;
 }
 
-template<int T, bool EIGHT, bool WIDE>
+// Lanes and vectors a lane, by the vectors of a row: few vectors while the row is short, whose time is that of one trip through the chain
+// (1024 x 8192 bf16: 512 lanes of two 11.2 us, 1024 of one 12.5, 256 of four 11.5; 1111 x 1537 fp32: 256 of two 4.3, 512 of one
+// 4.8; 8 x 4096 bf16 128 of four 4.5, and 3.7).  Beyond 2048 vectors 512 lanes of eight would win some and lose some (2048 x 20001
+// with a residual 66.6 us in place of 72.6, 4000 x 32768 without one 104.8 in place of 101.1, 8 x 32768 6.5 in place of 5.9).
+// NT, past the caches, where the tensors do not fit: 4096 x 8192 to 8 bits 44.5 -> 39.7 us, 16384 x 4096 92.3 -> 88.7; 2048 x 4096 would go
+// from 11.3 to 13.5.
+template<int T, bool EIGHT, bool WIDE, bool NT>
 int norm_forward(const NormArgs& a, hipStream_t s)
 {
     const int vectors = (a.width + kVec<T> - 1) / kVec<T>;
-    if (vectors <= 64) return launch_norm<T, EIGHT, WIDE, 64, 1>(a, s);
-    if (vectors <= 128) return launch_norm<T, EIGHT, WIDE, 128, 1>(a, s);
-    if (vectors <= 256) return launch_norm<T, EIGHT, WIDE, 256, 1>(a, s);
-    if (vectors <= 512) return launch_norm<T, EIGHT, WIDE, 256, 2>(a, s);
-    if (vectors <= 1024) return launch_norm<T, EIGHT, WIDE, 512, 2>(a, s);
-    if (vectors <= 2048) return launch_norm<T, EIGHT, WIDE, 1024, 2>(a, s);
-    if (vectors <= 4096) return launch_norm<T, EIGHT, WIDE, 1024, 4>(a, s);
-    return launch_norm<T, EIGHT, WIDE, 1024, 0>(a, s);
+    if (vectors <= 64) return launch_norm<T, EIGHT, WIDE, 64, 1, NT>(a, s);
+    if (vectors <= 128) return launch_norm<T, EIGHT, WIDE, 128, 1, NT>(a, s);
+    if (vectors <= 256) return launch_norm<T, EIGHT, WIDE, 256, 1, NT>(a, s);
+    if (vectors <= 512) return launch_norm<T, EIGHT, WIDE, 256, 2, NT>(a, s);
+    if (vectors <= 1024) return launch_norm<T, EIGHT, WIDE, 512, 2, NT>(a, s);
+    if (vectors <= 2048) return launch_norm<T, EIGHT, WIDE, 1024, 2, NT>(a, s);
+    if (vectors <= 4096) return launch_norm<T, EIGHT, WIDE, 1024, 4, NT>(a, s);
+    return launch_norm<T, EIGHT, WIDE, 1024, 0, false>(a, s);           // read twice: through the caches
+}
+
+template<int T, bool EIGHT, bool WIDE>
+int norm_forward(const NormArgs& a, hipStream_t s)
+{
+    const size_t tensors = 1 + (a.residual != nullptr) + (a.sum != nullptr) + !EIGHT;
+    const bool past = static_cast<size_t>(a.rows) * static_cast<size_t>(a.width) * kSize<T> * tensors >= kStreamingBytes;
+    return past ? norm_forward<T, EIGHT, WIDE, true>(a, s) : norm_forward<T, EIGHT, WIDE, false>(a, s);
 }
 
 // ---------------------------------------------------------------- backward

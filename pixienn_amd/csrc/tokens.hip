@@ -822,18 +822,21 @@ inline bool streams(const TokenArgs& a, int type, int tensors)
 // Workgroups that fill the machine four times over: from there on a workgroup takes as much as its registers hold.
 constexpr long long kEnoughParts = 1024;
 constexpr int kMostVectors = 8;         // vectors of a lane
+// ... of one of 512 for a row that 1024 would hold otherwise: 76 registers, so that three such workgroups share a unit and not two
+// (4096 x 50001 half with three alternatives 92.6 -> 84.6 us; 16 vectors are 85 registers, two workgroups, and 101.7)
+constexpr int kThirdVectors = 14;
 
 // Lanes of the workgroup that takes a whole row, without a second launch, or 0.  1024 up to 4096 vectors whatever the rows (8 x 32768 bf16
 // 8.0 us in parts, 5.0 whole; 256 x 32768 with five alternatives 14.2 and 9.4), and up to the 8192 that they hold from 64 rows on
 // (256 x 65536 with eight 18.2 and 13.5; 16 x 65536 9.9 and 11.1).  Where there are rows enough for all units, as few as hold it: what
 // waits for a row's maximum, and for its alternatives, is then less of the machine (4096 x 32768 with five alternatives 1024 lanes 65 us,
-// 512 52; 8000 x 16000 97 and, with 256, 52).
+// 512 52; 8000 x 16000 97 and, with 256, 52; 300 x 50001 1024 lanes 15.2, 512 17.7).
 inline int lanes_for_whole_rows(long long rows, long long vectors)
 {
     if (vectors <= kBlock || vectors > 1024 * kMostVectors) return 0;
     if (rows >= kEnoughParts) {
         if (vectors <= kBlock * kMostVectors) return 0;
-        if (vectors <= 512 * kMostVectors) return 512;
+        if (vectors <= 512 * kThirdVectors) return 512;
     }
     return vectors <= 512 * kMostVectors || rows >= 64 ? 1024 : 0;
 }
@@ -859,7 +862,9 @@ int launch_forward(const char* who, const TokenArgs& a, void* workspace, hipStre
         p.vectors = vectors;
         const dim3 grid(static_cast<unsigned>(a.rows)), block(lanes);
         const auto launch = [&](auto* kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, a, p); };
-        if (lanes == 512) launch(past ? &token_logprobs_kernel<T, ENTROPY, 512, kMostVectors, true> : &token_logprobs_kernel<T, ENTROPY, 512, kMostVectors, false>);
+        if (lanes == 512 && vectors > 512 * kMostVectors)
+            launch(past ? &token_logprobs_kernel<T, ENTROPY, 512, kThirdVectors, true> : &token_logprobs_kernel<T, ENTROPY, 512, kThirdVectors, false>);
+        else if (lanes == 512) launch(past ? &token_logprobs_kernel<T, ENTROPY, 512, kMostVectors, true> : &token_logprobs_kernel<T, ENTROPY, 512, kMostVectors, false>);
         else launch(past ? &token_logprobs_kernel<T, ENTROPY, 1024, kMostVectors, true> : &token_logprobs_kernel<T, ENTROPY, 1024, kMostVectors, false>);
         return check_launch(who);
     }

@@ -300,6 +300,31 @@ def test_logits_that_do_not_fit_the_caches(ops, rows, vocab, kind):
         held(gradients(ops, x, targets, g, None, 1.0, together)[0], d, bound, "together %s" % together)
 
 
+# rows enough for every unit, taken whole by as few lanes as hold them
+@gpu
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("vectors,more,top", [(4097, 0, 1), (5000, 3, 64), (7168, 1, 8), (7169, 0, 3), (4096, 3, 5), (2049, 0, 0)])
+def test_rows_enough_to_be_taken_whole(ops, kind, vectors, more, top):
+    dtype, rows = TYPES[kind][0], 1027
+    vocab = vectors * (16 // dtype.itemsize) + more
+    x = draw(5, rows, vocab, dtype, pad=5)
+    x[::3] = x[::3].round()             # many equal values
+    x[7] = -math.inf
+    x[8, 5:] = -math.inf
+    x[9] = torch.finfo(dtype).min
+    x[10] = 0.0
+    targets = (torch.arange(rows, device="cuda") * 7919) % (vocab + 2) - 1
+    _, want = check_forward(ops, x, targets, 0, 0.8)
+    if top:
+        got = forward(ops, x, targets, top, 0.8)
+        some = torch.cat([torch.arange(16), torch.arange(rows - 5, rows)])
+        ids = torch.from_numpy(alternatives(x[some], np.float32(0.8), top).astype(np.int64)).cuda()
+        assert torch.equal(got["top_ids"][some].long(), ids)
+        z = want.z[some].gather(1, ids)
+        held(got["top_logp"][some], z - want.lse[some][:, None],
+             want.lse_off[some][:, None] + 4 * U * torch.nan_to_num(z, 0.0, 0.0, 0.0).abs().clamp(max=1e9), "top_logp")
+
+
 @gpu
 def test_gradient_against_differences(ops):
     rows, vocab, scale = 3, 23, 0.75
