@@ -254,7 +254,9 @@ __device__ __forceinline__ void to_e4m3(const AdamwStep& s, uint32_t place, cons
 }
 
 // ---------------------------------------------------------------- the step
-// A wave takes four blocks, 1024 values apart; all of their loads go out before the first is used.
+// A wave takes four blocks, 1024 values apart; all of their loads go out before the first is used.  Bound by its streams: 184.6 M values with
+// 8-bit states, bf16 gradients and copies are 2.97 GB in 457 us, 6.5 TB/s, beside 65 for the norm's read of the gradients; 50 M
+// with 32-bit ones 238 us for four streams in and three out, as a kernel that only moves those.
 template<int BITS, int D, bool NT>
 __device__ __forceinline__ void step_chunk(const AdamwRecord& r, const AdamwStep& s, uint32_t first, float clip)
 {

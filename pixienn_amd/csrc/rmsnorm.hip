@@ -146,6 +146,8 @@ struct NormVector {
 
 // A row is walked in vectors, lane by lane.  K vectors a lane stay in registers between the sum and the result; the residual and the
 // weights are asked for with the row, so that there is one trip to memory.  K == 0: a row of any width, which is read again.
+// Bound by its streams: 4096 x 8192 bf16 with a residual and the sum kept, to 8 bits with a scale for 128, is 236 MB in 39.7 us,
+// 5.9 TB/s where a copy has 6.6; 8 x 4096 is one launch, 3.8 us (an empty one 3.5).
 template<int T, bool EIGHT, bool WIDE, int LANES, int K, bool NT>
 __global__ __launch_bounds__(LANES > kWave ? LANES : kBlock) void rms_norm_kernel(NormArgs a)
 {
@@ -315,7 +317,8 @@ struct NormBackwardArgs {
 
 // dx of every row, and the part of dw that this worker's rows give: a worker (LANES lanes) takes every workers-th row, and asks for
 // the next one before it waits for the sum over this one.  At four vectors a lane there are no registers for that, nor for
-// the weights, which are read again for every row.
+// the weights, which are read again for every row.  16384 x 4096 bf16 with dsum: 537 MB in 88.7 us with the launch that adds up dw,
+// 6.05 TB/s, where a kernel that only moves three streams in and one out has 6.3.
 template<int T, int LANES, int K, bool NT>
 __global__ __launch_bounds__(LANES > kWave ? LANES : kBlock) void rms_norm_backward_kernel(NormBackwardArgs a, int workers)
 {

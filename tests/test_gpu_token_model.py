@@ -58,3 +58,46 @@ def test_it_learns_with_states_in_32_and_in_8_bits(example):
         assert float((ids[:, 0] == (5 * tokens + 7) % 512).double().mean()) > 0.99
         assert abs(float(logp[:, 0].exp().mean()) - 0.9) < 0.1 and float(entropy.mean()) < 2.0
     assert abs(means[8] - means[32]) < 0.1
+
+
+def test_a_pass_in_a_graph():
+    """Norm, log probabilities of rows in parts with their alternatives, gradient and the norm's gradient, captured and replayed with other
+    work between; every replay is the eager result to the bit."""
+    from pixienn_amd import ops
+    rows, width = 6, 20005
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(rows, width, device="cuda", generator=g).to(torch.bfloat16)
+    weight = torch.randn(width, device="cuda", generator=g).to(torch.bfloat16)
+    targets = torch.arange(rows, device="cuda") * 3001
+    d_logp = torch.ones(rows, device="cuda")
+    norm_space = torch.empty(ops.rms_norm_workspace_bytes(rows, width) // 4, device="cuda")
+    token_space = torch.empty(ops.token_logprobs_workspace_bytes(rows, width, 4) // 4 + 1, device="cuda")
+
+    def tensors():
+        t = {k: torch.zeros_like(x) for k in ("y", "dy", "dx")}
+        t.update({k: torch.zeros(rows, device="cuda") for k in ("rstd", "logp", "entropy", "lse", "logp2")})
+        return dict(t, dw=torch.zeros(width, device="cuda"), best=torch.zeros(rows, 4, device="cuda"), ids=torch.zeros(rows, 4, device="cuda", dtype=torch.int32))
+
+    def run(t):
+        ops.rms_norm_forward(x, t["y"], weight, rstd=t["rstd"])
+        ops.token_logprobs_forward(t["y"], targets, t["logp"], t["entropy"], t["lse"], t["best"], t["ids"], workspace=token_space)
+        ops.token_logprobs_forward_train(t["y"], targets, d_logp, t["dy"], t["logp2"])
+        ops.rms_norm_backward(t["dy"], x, weight, t["rstd"], t["dx"], t["dw"], workspace=norm_space)
+
+    captured, eager = tensors(), tensors()
+    run(captured)
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            run(captured)
+    for _ in range(4):
+        x.copy_(torch.randn(rows, width, device="cuda", generator=g))
+        for t in captured.values():
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        run(eager)
+        torch.cuda.synchronize()
+        for k in captured:
+            assert torch.equal(captured[k], eager[k]), k
