@@ -584,12 +584,14 @@ __device__ __forceinline__ RowGradient<T, PEAK> gradient_of(const TokenArgs& a, 
     return r;
 }
 
-// A workgroup takes one part of a row: 1000 x 100001 fp32 with the entropy's gradient is 800 MB in 138.5 us, 5.8 TB/s where a copy has 6.6
-// (rows of an odd length begin off the vectors' alignment).  Past the caches in short parts (1000 x 100001 fp32: 149 us with four steps through the caches, 144
+// A workgroup takes one part of a row: 1000 x 100001 fp32 with the entropy's gradient is 800 MB in 136 us, 5.9 TB/s where a copy has
+// 6.6.  Past the caches in short parts (1000 x 100001 fp32: 149 us with four steps through the caches, 144
 // with four past them, 137 with two), within them in longer ones (512 x 32768 bf16: 11.5 us, and 13 past them).
 template<bool NT>
 constexpr int kGradientSteps = NT ? 2 : 4;
 
+// A row's vectors begin at its first 16-byte boundary (4096 x 50001 half with the entropy's gradient 138 -> 134 us).  The passes that sum over a row
+// begin at its first value, so that a row's results are the same wherever it lies.
 template<int T, bool NT>
 __global__ __launch_bounds__(kBlock) void token_gradient_kernel(TokenArgs a, FastDiv parts)
 {
@@ -599,17 +601,27 @@ __global__ __launch_bounds__(kBlock) void token_gradient_kernel(TokenArgs a, Fas
     const auto r = gradient_of<T, false>(a, row, target_of(a, row), 0.0f, a.lse_in[row], a.d_entropy ? a.entropy_in[row] : 0.0f);
     const char* logits = static_cast<const char*>(a.logits) + row * a.stride * kSize<T>;
     char* out = static_cast<char*>(a.dlogits) + row * a.d_stride * kSize<T>;
+    const int head = min(static_cast<int>(-reinterpret_cast<uintptr_t>(logits) & 15) / kSize<T>, a.vocab);
+    const int whole = (a.vocab - head) / V;
     const auto write = [&]<bool QUICK>() {
 #pragma unroll
         for (int s = 0; s < kGradientSteps<NT>; ++s) {
-            const int e = ((part * kGradientSteps<NT> + s) * kBlock + threadIdx.x) * V;
-            if (e >= a.vocab) break;
+            const int v = (part * kGradientSteps<NT> + s) * kBlock + threadIdx.x;
+            if (v >= whole) break;
             float l[V], d[V];
-            load_row<T, V, NT>(logits, e, a.vocab).get(l);
-            r.template apply<V, QUICK>(l, e, d);
+            load_raw<T, V, NT>(logits, head + v * V).get(l);
+            r.template apply<V, QUICK>(l, head + v * V, d);
             Raw<T, V> raw;
             raw.set(d);
-            store_row<T, V, NT>(out, e, a.vocab, raw);
+            store_raw<T, V, NT>(out, head + v * V, raw);
+        }
+        // what fills no vector
+        int e = threadIdx.x;
+        if (e >= head) e += whole * V;
+        if (part == 0 && e < a.vocab) {
+            float d[1];
+            r.template apply<1, QUICK>({ load_one<T>(logits, e) }, e, d);
+            store_one<T>(out, e, d[0]);
         }
     };
     if (T != PXH_F32 && r.quick) write.template operator()<true>();
