@@ -253,12 +253,22 @@ __device__ __forceinline__ void select_largest(int k, uint32_t best, const Above
 // ---------------------------------------------------------------- a part of a row
 // Vectors first .. first + count of a row, K to a lane, and of the row's last values, which fill no vector, one to each of the
 // first lanes of the part that has them.  What is not there is minus infinity.
-template<int T, int LANES, int K, bool NT>
+constexpr int kMostVectors = 8;         // vectors of a lane
+// ... of one of 512 for a row that 1024 would hold otherwise: 76 registers, so that three such workgroups share a unit and not two
+// (4096 x 50001 half with three alternatives 92.6 -> 84.6 us; 16 vectors are 85 registers, two workgroups, and 101.7)
+constexpr int kThirdVectors = 14;
+
+// SETTLES: rows of 16-bit values off a 4-byte boundary are read from one value further on (below).  For the lanes of 14 vectors: 4096 x 50001 half,
+// every other row of which is, 85.0 -> 79.5 us, and 4096 x 50000 76.  The others lose (8000 x 17001 55.5 -> 58, 300 x 50001 14.8 -> 16.2).
+template<int T, int LANES, int K, bool NT, bool SETTLES = false>
 struct Part {
+    static constexpr bool kSettles = SETTLES && kSize<T> == 2;
     static constexpr int V = kVec<T>;
     Raw<T, V> kept[K];
     float extra, peak;          // peak: the largest of the lane's values, from sums()
     int first, count, extra_at;
+    uint32_t before;            // lane k: lane 0's first value in step k, where `odd`
+    bool odd;
 
     __device__ __forceinline__ bool has(int k) const { return k * LANES + static_cast<int>(threadIdx.x) < count; }
     __device__ __forceinline__ int at(int k) const { return (first + k * LANES + static_cast<int>(threadIdx.x)) * V; }
@@ -278,11 +288,40 @@ struct Part {
         if (first_vector + vectors < whole || extra_at >= vocab) extra_at = -1;
         extra = load_one<T>(row, extra_at < 0 ? 0 : extra_at);
         if (extra_at < 0) extra = -INFINITY;
+        const char* place = row;
+        if constexpr (kSettles) {
+            // Vectors off a 4-byte boundary are slow to load: one value further on they are not, and that value is the neighbour's to give.
+            // The last one reads the first of the values that fill no vector, so there have to be some.
+            odd = (reinterpret_cast<uintptr_t>(row) & 2) && whole * V < vocab;
+            const int lane = threadIdx.x % kWave, of = lane * LANES + static_cast<int>(threadIdx.x) - lane;
+            before = global_memory<uint16_t>(row)[odd && lane < K && of < count ? (first + of) * V : 0];
+            place += odd ? 2 : 0;
+        }
 #pragma unroll
         for (int k = 0; k < K; ++k) {
 #pragma unroll
             for (int i = 0; i < Raw<T, V>::kWords; ++i) kept[k].w[i] = nothing;
-            if (has(k)) kept[k] = load_raw_at<T, V, NT>(row + (static_cast<size_t>(first) + k * LANES) * 16, threadIdx.x * 16u);
+            if (has(k)) kept[k] = load_raw_at<T, V, NT>(place + (static_cast<size_t>(first) + k * LANES) * 16, threadIdx.x * 16u);
+        }
+        if constexpr (kSettles)
+            if (odd) settle();
+    }
+
+    // Values 1 to 8 of a vector become 0 to 7: the first is the last one of the lane in front, and lane 0's is in `before`.
+    __device__ __forceinline__ void settle()
+    {
+        constexpr int kBehind = 0x138;          // every lane the value of the lane in front; lane 0 keeps the old one
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            if (k * LANES >= count) break;
+            uint32_t (&w)[4] = kept[k].w;
+            const uint32_t given = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(before), k)) << 16;
+            const uint32_t front = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(given), static_cast<int>(w[3]), kBehind, 0xF, 0xF, false));
+            if (!has(k)) continue;
+            w[3] = __builtin_amdgcn_alignbit(w[3], w[2], 16);
+            w[2] = __builtin_amdgcn_alignbit(w[2], w[1], 16);
+            w[1] = __builtin_amdgcn_alignbit(w[1], w[0], 16);
+            w[0] = __builtin_amdgcn_alignbit(w[0], front, 16);
         }
     }
 
@@ -396,7 +435,7 @@ struct Part {
 
 // ---------------------------------------------------------------- forward
 // A workgroup takes one part of a row into its registers; a row of several parts is put together by a second launch from
-// their sums and their largest values.  4096 x 50001 half with entropy and three alternatives: 410 MB in 84.6 us, 4.8 TB/s.  The
+// their sums and their largest values.  4096 x 50001 half with entropy and three alternatives: 410 MB in 78.6 us, 5.2 TB/s.  The
 // arithmetic alone, 8.5 instructions a value counting an exponential as four, is 44 us; it waits for the row's maximum, so that the
 // next row's loads, another workgroup's, have to cover it.
 struct Parts {
@@ -418,7 +457,7 @@ __global__ __launch_bounds__(LANES) void token_logprobs_kernel(TokenArgs a, Part
     const bool whole = p.parts == 1;
     const int target = whole ? target_of(a, row) : -1;
     const float given = load_one<T>(logits, target < 0 ? 0 : target);
-    Part<T, LANES, K, NT> mine;
+    Part<T, LANES, K, NT, K == kThirdVectors> mine;
     mine.load(logits, a.vocab, static_cast<int>(part) * p.vectors, p.vectors);
     const Sums s = group_join<LANES>(mine.template sums<ENTROPY>(logits, c), c, slots);
     float lse = 0.0f;
@@ -630,9 +669,10 @@ __global__ __launch_bounds__(kBlock) void token_gradient_kernel(TokenArgs a, Fas
 
 // ---------------------------------------------------------------- forward and gradient at once
 // A workgroup per row, which stays in registers between its sums and its gradient.  A lane writes the values that it has read, so the
-// gradient may take the logits' place.
+// gradient may take the logits' place.  1024 lanes of 8 vectors are held to 64 registers, so that two rows share a unit and not one
+// (2000 x 65536 bf16 110 -> 102 us).
 template<int T, bool ENTROPY, int LANES, int K, bool NT>
-__global__ __launch_bounds__(LANES) void token_train_kernel(TokenArgs a)
+__global__ __launch_bounds__(LANES, LANES == 1024 && K == 8 ? 8 : 1) void token_train_kernel(TokenArgs a)
 {
     constexpr int V = kVec<T>;
     __shared__ Sums slots[LANES / kWave];
@@ -837,10 +877,6 @@ inline bool streams(const TokenArgs& a, int type, int tensors)
 
 // Workgroups that fill the machine four times over: from there on a workgroup takes as much as its registers hold.
 constexpr long long kEnoughParts = 1024;
-constexpr int kMostVectors = 8;         // vectors of a lane
-// ... of one of 512 for a row that 1024 would hold otherwise: 76 registers, so that three such workgroups share a unit and not two
-// (4096 x 50001 half with three alternatives 92.6 -> 84.6 us; 16 vectors are 85 registers, two workgroups, and 101.7)
-constexpr int kThirdVectors = 14;
 
 // Lanes of the workgroup that takes a whole row, without a second launch, or 0.  1024 up to 4096 vectors whatever the rows (8 x 32768 bf16
 // 8.0 us in parts, 5.0 whole; 256 x 32768 with five alternatives 14.2 and 9.4), and up to the 8192 that they hold from 64 rows on
