@@ -623,7 +623,7 @@ __device__ __forceinline__ RowGradient<T, PEAK> gradient_of(const TokenArgs& a, 
     return r;
 }
 
-// A workgroup takes one part of a row: 1000 x 100001 fp32 with the entropy's gradient is 800 MB in 136 us, 5.9 TB/s where a copy has
+// A workgroup takes one part of a row: 1000 x 100001 fp32 with the entropy's gradient is 800 MB in 134 us, 6.0 TB/s where a copy has
 // 6.6.  Past the caches in short parts (1000 x 100001 fp32: 149 us with four steps through the caches, 144
 // with four past them, 137 with two), within them in longer ones (512 x 32768 bf16: 11.5 us, and 13 past them).
 template<bool NT>
