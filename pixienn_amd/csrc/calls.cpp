@@ -197,6 +197,7 @@ struct Space {
     {
         if (o == Py_None) return;
         const at::Tensor& t = tensor_of(o);
+        if (!t.is_contiguous()) throw NotHere{};
         data = t.data_ptr();
         bytes = static_cast<size_t>(t.numel()) * t.element_size();
     }

@@ -671,8 +671,12 @@ def _vector(t, name, n, dtype=_F32):
         raise PxError("%s must hold %d values (got %d)" % (name, n, t.numel()))
 
 
-def _bytes(workspace):
-    return 0 if workspace is None else workspace.numel() * workspace.element_size()
+def _space(workspace):
+    """(address, bytes) of a workspace of the caller's."""
+    if workspace is None:
+        return None, 0
+    _chk(workspace, getattr(workspace, "dtype", None), "workspace")
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 def _made(name, *args):
@@ -726,8 +730,7 @@ def rms_norm_backward(dy, h, weight, rstd, dx, dw, dsum=None, accumulate=False, 
     _vector(dw, "dw", width)
     call("pxh_rms_norm_backward", ptr(dy), ptr(h), ptr(weight), ptr(rstd), ptr(dsum), ptr(dx), ptr(dw), kind,
          _type(weight, "weight"), rows, width, dy_stride, _like(h, "h", dy.shape, dy.dtype), _like(dsum, "dsum", dy.shape, dy.dtype),
-         _like(dx, "dx", dy.shape, dy.dtype), int(bool(accumulate)), ptr(workspace), _bytes(workspace),
-         _stream())
+         _like(dx, "dx", dy.shape, dy.dtype), int(bool(accumulate)), *_space(workspace), _stream())
     return dx
 
 
@@ -767,7 +770,7 @@ def token_logprobs_forward(logits, targets, logp, entropy=None, lse=None, top_lo
         _vector(top_ids, "top_ids", rows * top, torch.int32)
         _vector(top_logp, "top_logp", rows * top)
     call("pxh_token_logprobs_forward", ptr(logits), at, ptr(logp), ptr(entropy), ptr(lse), ptr(top_logp) if top else None, ptr(top_ids),
-         _type(logits, "logits"), wide, rows, vocab, stride, top, float(scale), ptr(workspace), _bytes(workspace), _stream())
+         _type(logits, "logits"), wide, rows, vocab, stride, top, float(scale), *_space(workspace), _stream())
 
 
 def token_logprobs_backward(logits, targets, lse, d_logp, dlogits, entropy=None, d_entropy=None, scale=1.0):

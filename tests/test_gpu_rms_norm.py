@@ -301,3 +301,14 @@ def test_tensors_that_do_not_fit_are_refused(ops):
               lambda: ops.rms_norm_backward(x, x, weight, rstd[:2], x, weight.clone())):
         with pytest.raises(capi.PxError):
             f()
+
+
+@gpu
+@pytest.mark.parametrize("bad", [lambda: torch.zeros(1 << 20), lambda: torch.zeros(1, device="cuda").expand(1 << 20), lambda: torch.zeros(1 << 21, device="cuda")[::2],
+                                 lambda: np.zeros(1 << 20)])
+def test_a_workspace_that_is_no_packed_memory_of_the_device_is_refused(ops, bad):
+    x, weight, rstd = torch.ones(4, 8, device="cuda"), torch.ones(8, device="cuda"), torch.ones(4, device="cuda")
+    with pytest.raises(capi.PxError, match="workspace"):
+        ops.rms_norm_backward(x, x, weight, rstd, torch.empty_like(x), torch.empty_like(weight), workspace=bad())
+    with pytest.raises(capi.PxError, match="workspace"):
+        ops.token_logprobs_forward(x, None, None, entropy=rstd, workspace=bad())

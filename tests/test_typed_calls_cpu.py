@@ -49,3 +49,12 @@ def test_the_functions_say_what_is_wrong():
         ops.rms_norm_forward(x, x, x[0])
     with pytest.raises(capi.PxError, match="logits is required"):
         ops.token_logprobs_forward(None, None, None)
+
+
+def test_a_workspace_is_packed_memory_of_the_device():
+    """Kernels write to it: anything else is refused before its address is taken."""
+    assert ops._space(None) == (None, 0)
+    with pytest.raises(capi.PxError, match="workspace must live on the GPU"):
+        ops._space(torch.zeros(1 << 20))
+    with pytest.raises(capi.PxError, match="workspace: torch.Tensor expected"):
+        ops._space(np.zeros(1 << 20))
