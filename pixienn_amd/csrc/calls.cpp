@@ -144,11 +144,13 @@ struct Rows {
     char* data = nullptr;
     long long rows = 0, width = 0, stride = 0;
     int type = 0;
+    bool given = false;         // a tensor of no values has no address either, and is not a missing one
 
     Rows() = default;
     explicit Rows(PyObject* o)
     {
         if (o == Py_None) return;
+        given = true;
         const at::Tensor& t = tensor_of(o);
         const auto dims = t.dim();
         if (dims == 0) throw NotHere{};
@@ -169,9 +171,7 @@ struct Rows {
     // of the same shape and, if asked, type
     const Rows& like(const Rows& o, int of_type) const
     {
-        if (data || rows) {
-            if (shape != o.shape || type != of_type) throw NotHere{};
-        }
+        if (given && (shape != o.shape || type != of_type)) throw NotHere{};
         return *this;
     }
 
@@ -223,7 +223,7 @@ int fits(long long v)
 }
 
 // The row stride of a tensor that may be None.
-long long stride_of(const Rows& r) { return r.data || r.rows ? r.stride : 0; }
+long long stride_of(const Rows& r) { return r.given ? r.stride : 0; }
 
 // f() with the interpreter free, its status as a number.
 template<typename F>

@@ -312,3 +312,16 @@ def test_a_workspace_that_is_no_packed_memory_of_the_device_is_refused(ops, bad)
         ops.rms_norm_backward(x, x, weight, rstd, torch.empty_like(x), torch.empty_like(weight), workspace=bad())
     with pytest.raises(capi.PxError, match="workspace"):
         ops.token_logprobs_forward(x, None, None, entropy=rstd, workspace=bad())
+
+
+@gpu
+@pytest.mark.parametrize("other", [lambda x: x[:0], lambda x: x[:0].half(), lambda x: x[:0].t(), lambda x: x.new_empty(0), lambda x: x[:, :0]])
+def test_an_empty_tensor_is_no_missing_one(ops, other):
+    x, weight, rstd = torch.ones(4, 8, device="cuda"), torch.ones(8, device="cuda"), torch.ones(4, device="cuda")
+    bad, dw = other(x), torch.ones(8, device="cuda")
+    y = torch.empty_like(x)
+    for f in (lambda: ops.rms_norm_forward(x, y, weight, residual=bad), lambda: ops.rms_norm_forward(x, y, weight, residual=x, sum=bad),
+              lambda: ops.rms_norm_forward(x, bad, weight), lambda: ops.rms_norm_backward(x, x, weight, rstd, y, dw, dsum=bad),
+              lambda: ops.rms_norm_backward(x, bad, weight, rstd, y, dw), lambda: ops.rms_norm_backward(x, x, weight, rstd, bad, dw)):
+        with pytest.raises(capi.PxError):
+            f()
