@@ -310,9 +310,10 @@ PyObject* token_logprobs_forward(PyObject* self, PyObject* const* args, Py_ssize
         float* const lse = floats(a[4], logits.rows);
         int top = 0, *ids = nullptr;
         float* best = nullptr;
+        if ((a[5] == Py_None) != (a[6] == Py_None)) throw NotHere{};
         if (a[6] != Py_None) {
             const at::Tensor& t = tensor_of(a[6]);
-            if (t.dim() == 0 || a[5] == Py_None) throw NotHere{};
+            if (t.dim() == 0) throw NotHere{};
             top = fits(t.size(t.dim() - 1));
             ids = packed<int>(a[6], logits.rows * top, at::kInt);
             best = floats(a[5], logits.rows * top);

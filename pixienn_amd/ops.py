@@ -763,9 +763,9 @@ def token_logprobs_forward(logits, targets, logp, entropy=None, lse=None, top_lo
     at, wide = _targets(targets, rows)
     _per_row(rows, logp=logp, entropy=entropy, lse=lse)
     top = 0
+    if (top_ids is None) != (top_logp is None) or top_ids is not None and _tensor(top_ids).dim() == 0:
+        raise PxError("top_logp and top_ids go together, [rows, top]")
     if top_ids is not None:
-        if _tensor(top_ids).dim() == 0 or top_logp is None:
-            raise PxError("top_logp and top_ids go together, [rows, top]")
         top = top_ids.shape[-1]
         _vector(top_ids, "top_ids", rows * top, torch.int32)
         _vector(top_logp, "top_logp", rows * top)

@@ -460,3 +460,12 @@ def test_tensors_that_do_not_fit_are_refused(ops):
               lambda: ops.token_logprobs_forward_train(x, t, v, None), lambda: ops.token_logprobs_forward_train(x, None, v, x)):
         with pytest.raises(capi.PxError):
             f()
+
+
+@gpu
+def test_alternatives_without_their_places_are_refused(ops):
+    x, t, v = torch.zeros(4, 9, device="cuda"), torch.zeros(4, device="cuda", dtype=torch.long), torch.zeros(4, device="cuda")
+    tops = torch.full((4, 3), 7.0, device="cuda")
+    for scale in (1.0, 1):          # by the native call, which leaves a whole number, and by the function's own checks
+        with pytest.raises(capi.PxError, match="go together"):
+            ops.token_logprobs_forward(x, t, v, top_logp=tops, scale=scale)
