@@ -677,8 +677,8 @@ int pxh_token_logprobs_forward_train(const void* logits, const void* targets, co
  *   w += lr * (m / (1 - beta1^t)) / (sqrt(v / (1 - beta2^t)) + eps) - lr * decay * w     (the decay where apply_decay says so)
  *   copy = w, rounded to its type
  * beta1 and beta2 are taken in 64 bits (1 - beta is what an fp32 beta has lost).  d is only read (unlike pxh_adam_update's).
- * d_scale: 1 / batch, the inverse of a loss scale, or both.  The norm is summed in 64 bits, in a fixed order, and rounded down
- * to fp32.
+ * d_scale: 1 / batch, the inverse of a loss scale, or both.  The norm is summed in 64 bits, in a fixed order; f is formed from it
+ * there, and both are rounded to fp32 once.
  *
  * States in 8 bits: m and the SQUARE ROOT of v are e4m3 values with a scale for each 256 of a tensor, its largest magnitude / 448
  * (2^-126 at least): 2 + 1/32 bytes a value for both.  Each step's results are rounded stochastically, up with the
@@ -688,8 +688,9 @@ int pxh_token_logprobs_forward_train(const void* logits, const void* targets, co
  * for instance; the same seed gives the same bits.  A NaN is kept as the largest value of its block (its weight is the NaN).
  * A step reads the states as they were rounded, and applies its own before they are rounded.
  *
- * norm_out (nullable, device) receives the norm, also when max_norm is 0.  With max_norm > 0 and a norm that is not finite (an
- * overflow of half-precision gradients) nothing is written but norm_out: the step is left out.
+ * norm_out (nullable, device) receives the norm, also when max_norm is 0.  With max_norm > 0 and a norm that is not finite as an fp32
+ * number (an overflow of half-precision gradients, or finite ones that are too large together) nothing is written but norm_out: the
+ * step is left out.
  *
  * pxh_adamw_table_create copies `tensors` (host memory); those of no values are left out; any number up to 2^20, of less than
  * 2^31 values each.  state_bits is 32 (m, v: floats, the scales null) or 8.  The buffers need the alignment of their own values.

@@ -436,12 +436,13 @@ __global__ __launch_bounds__(kBlock) void adamw_squares_kernel(const AdamwRecord
     for (uint32_t i = threadIdx.x; i < gridDim.x; i += kBlock) sum += __hip_atomic_load(partial + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     sum = block_sum(sum, slots);
     if (threadIdx.x == 0) {
-        // rounded down: a norm from sums in fp32, which lose what is small beside them, comes out there
-        const float norm = __double2float_rz(sqrt(sum) * fabs(static_cast<double>(d_scale)));
+        // rounded once, to nearest: one beyond the largest number becomes an infinity, and leaves the step out as any other
+        const double exact = sqrt(sum) * fabs(static_cast<double>(d_scale));
+        const float norm = static_cast<float>(exact);
         float f = 1.0f;
         if (max_norm > 0.0f) {
-            if (!(norm <= 3.4028234e38f)) f = __builtin_nanf("");
-            else if (norm > max_norm) f = max_norm / norm;
+            if (!(norm < INFINITY)) f = __builtin_nanf("");
+            else if (exact > max_norm) f = static_cast<float>(max_norm / exact);
         }
         *factor = f;
         if (norm_out) *norm_out = norm;

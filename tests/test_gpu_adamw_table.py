@@ -363,3 +363,36 @@ def test_tensors_that_do_not_fit_are_refused(ops):
     table.close()
     with pytest.raises(capi.PxError):
         table.update(1, 1e-3)
+
+
+@gpu
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("size,d_scale", [(1e38, 1.0), (3e38, 2.0), (2e38, -2.5)])
+def test_a_norm_beyond_the_largest_number_leaves_the_step_out(ops, bits, size, d_scale):
+    """Every gradient is a number, and so is their norm in 64 bits, but not as the fp32 value that clips them."""
+    model = Model(ops, bits, kinds=("f32",))
+    model.d[7].fill_(size)
+    before = model.everything()
+    norm = torch.zeros(1, device="cuda")
+    model.table.update(3, 1e-3, d_scale=d_scale, max_norm=1.0, norm_out=norm, seed=1)
+    for a, b in zip(before, model.everything()):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    assert float(norm) == math.inf
+    # the largest that is one clips as any other
+    model.d[7].fill_(0.0)
+    model.d[7][100] = 3.4e38
+    model.table.update(3, 1e-3, max_norm=1.0, norm_out=norm, seed=1)
+    assert float(norm) == float(np.float32(3.4e38))
+    assert all(bool(torch.isfinite(x.float()).all()) for group in (model.w, model.m, model.v) for x in group)
+    assert not torch.equal(model.w[7], before[7])
+
+
+@gpu
+def test_the_norm_is_the_nearest_number(ops):
+    """Sums that are exact in 64 bits: the norm is the fp32 number next to their root."""
+    norm = torch.zeros(1, device="cuda")
+    for n in range(1, 60):
+        w = torch.zeros(n, device="cuda")
+        table = ops.AdamwTable([w], [torch.ones(n, device="cuda")], **ops.adamw_states([w], 32))
+        table.update(1, 1e-3, d_scale=0.5, norm_out=norm)
+        assert float(norm) == float(np.float32(0.5 * math.sqrt(n))), n
