@@ -685,8 +685,9 @@ int pxh_token_logprobs_forward_train(const void* logits, const void* targets, co
  * probability of the part cut off: what a step changes of an average over 1000 steps is less than half a unit of such a value, and
  * rounded to nearest it would never change.  A root that is not zero never rounds to zero (the quotient stays bounded).  The
  * random bits come from `seed` (its low 31 bits) and the value's place in the table: another seed every step, the step's number
- * for instance; the same seed gives the same bits.  A NaN is kept as the largest value of its block (its weight is the NaN).
- * A step reads the states as they were rounded, and applies its own before they are rounded.
+ * for instance; the same seed gives the same bits.  A state that is no number, NaN or infinite, is kept as the largest value of its
+ * block, whose scale is that of the others: what is lost is its own weight.  A step reads the states as they were rounded, and
+ * applies its own before they are rounded.
  *
  * norm_out (nullable, device) receives the norm, also when max_norm is 0.  With max_norm > 0 and a norm that is not finite as an fp32
  * number (an overflow of half-precision gradients, or finite ones that are too large together) nothing is written but norm_out: the

@@ -223,10 +223,19 @@ __device__ __forceinline__ float eight_maxima(const float (&x)[8])
     return fmaxf(v, lane_in_row<0x141>(v));
 }
 
-// Four values over their block's scale as e4m3 (a NaN, which its weight has too, as the largest value): up with the probability of what
-// is cut off, by the upper 20 bits of the noise (the hardware's conversion, which is the addition of those bits below the last place,
-// subnormals among it).  The quotient from the rounded reciprocal and one correction by its remainder (Markstein), which
-// is the rounded quotient.
+// The same of values that are numbers: one that is not does not take its block's scale with it.
+__device__ __forceinline__ float largest_number(const float (&x)[4])
+{
+    float most = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) most = fmaxf(most, fabsf(x[k]) < INFINITY ? fabsf(x[k]) : 0.0f);
+    return most;
+}
+
+// Four values over their block's scale as e4m3, up with the probability of what is cut off, by the upper 20 bits of the noise (the
+// hardware's conversion, which is the addition of those bits below the last place, subnormals among it).  The quotient from the
+// rounded reciprocal and one correction by its remainder (Markstein), which is the rounded quotient; of what is no number, whose weight
+// is lost, it is a NaN, and kept as the largest value: the lesser of a NaN and a number is the number.
 __device__ __forceinline__ void to_e4m3(const AdamwStep& s, uint32_t place, const float (&m)[4], const float (&root)[4], float m_scale,
                                         float m_inverse, float v_scale, float v_inverse, uint32_t& m8, uint32_t& v8)
 {
@@ -239,10 +248,10 @@ __device__ __forceinline__ void to_e4m3(const AdamwStep& s, uint32_t place, cons
     int mw = 0, vw = 0;
     const auto put = [&]<int K>() {
         const uint32_t noise = second_round(base + ((K ^ s.seed) & 3u) * kMix1);
-        const float x = __builtin_amdgcn_fmed3f(over(m[K], m_scale, m_inverse), -kE4m3Max, kE4m3Max);
+        const float x = fmaxf(fminf(over(m[K], m_scale, m_inverse), kE4m3Max), -kE4m3Max);
         mw = __builtin_amdgcn_cvt_sr_fp8_f32(x, static_cast<int>(noise), mw, K);
         // at least the least value there is, unless it is zero
-        const float v = __builtin_amdgcn_fmed3f(over(root[K], v_scale, v_inverse), fminf(root[K] * 0x1p100f, 0x1p-9f), kE4m3Max);
+        const float v = fmaxf(fminf(over(root[K], v_scale, v_inverse), kE4m3Max), fminf(root[K] * 0x1p100f, 0x1p-9f));
         vw = __builtin_amdgcn_cvt_sr_fp8_f32(v, static_cast<int>(noise << 12), vw, K);
     };
     put.template operator()<0>();
@@ -307,7 +316,16 @@ __device__ __forceinline__ void step_chunk(const AdamwRecord& r, const AdamwStep
         }
         // lanes 8 j and on: the scale of m in step j, and of the root in step j - 4
         const uint32_t lane = threadIdx.x % kWave, j = lane / 8;
-        const float scale = fmaxf(eight_maxima(most) / kE4m3Max, kLeastScale), inverse = 1.0f / scale;
+        float peak = eight_maxima(most);
+        if (__any(peak == INFINITY)) {
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                most[k] = largest_number(m[k]);
+                most[k + kSteps] = largest_number(root[k]);
+            }
+            peak = eight_maxima(most);
+        }
+        const float scale = fmaxf(peak / kE4m3Max, kLeastScale), inverse = 1.0f / scale;
         const uint32_t of = block + (j % kSteps) * (kBlock / kWave);
         if (lane % 8 == 0 && of < blocks) global_memory<float>(j < kSteps ? r.m_scale : r.v_scale)[of] = scale;
 #pragma unroll

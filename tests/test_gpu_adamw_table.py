@@ -396,3 +396,30 @@ def test_the_norm_is_the_nearest_number(ops):
         table = ops.AdamwTable([w], [torch.ones(n, device="cuda")], **ops.adamw_states([w], 32))
         table.update(1, 1e-3, d_scale=0.5, norm_out=norm)
         assert float(norm) == float(np.float32(0.5 * math.sqrt(n))), n
+
+
+@gpu
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_a_value_that_is_no_number_is_kept_as_its_blocks_largest(ops, bad):
+    """States in 8 bits, without clipping: the value's own weight is lost and nothing beside it, in this step or in the next."""
+    model, clean = Model(ops, 8, kinds=("f32",)), Model(ops, 8, kinds=("f32",))
+    at = 300                                        # in the second block of 1000 values
+    for a in (model, clean):
+        for state in (a.m[7], a.v[7]):
+            state.view(torch.uint8)[at] = 0         # nothing that could be the block's largest
+        a.d[7][at] = 0.0
+    model.d[7][at] = bad
+    for a in (model, clean):
+        a.table.update(3, 1e-3, seed=1)
+    others = torch.arange(1000, device="cuda") != at
+    assert not bool(torch.isfinite(model.w[7][at])) and torch.equal(model.w[7][others], clean.w[7][others])
+    assert float(model.m[7][at]) == 448.0 and float(model.v[7][at]) == 448.0
+    for name in ("m", "v"):
+        got, want = getattr(model, name), getattr(clean, name)
+        assert torch.equal(got[7].view(torch.uint8)[others], want[7].view(torch.uint8)[others]), name
+        assert torch.equal(getattr(model, name + "s")[7], getattr(clean, name + "s")[7]), name
+    model.d[7][at] = 0.0
+    for t in (4, 5):
+        model.table.update(t, 1e-3, seed=t)
+    assert bool(torch.isfinite(model.w[7][others]).all()) and bool(torch.isfinite(model.v[7].float()).all())
+    assert bool(torch.isfinite(model.ms[7]).all()) and bool(torch.isfinite(model.vs[7]).all())
