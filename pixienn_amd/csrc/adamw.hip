@@ -512,15 +512,16 @@ int pxh_adamw_table_create(int count, const pxh_adamw_tensor* tensors, int state
             if (!t.w || !t.d || !t.m || !t.v || (state_bits == 8 && (!t.m_scale || !t.v_scale)))
                 return fail_invalid("%s: null pointer for tensor %d", who, i);
             const uint32_t n = static_cast<uint32_t>(t.n);
+            // before their list is made, which could be larger than memory
+            if (chunks.size() + (n + kChunk - 1) / kChunk > (1u << 24) - 1) {
+                set_error("%s: more values than one launch takes", who);
+                return PXH_ERR_UNSUPPORTED;
+            }
             const uint32_t tensor = static_cast<uint32_t>(records.size());
             records.push_back({ t.w, t.d, t.m, t.v, t.m_scale, t.v_scale, t.copy, n, place, t.d_type, t.copy_type, t.apply_decay != 0 });
             for (uint32_t at = 0; at < n; at += kChunk) chunks.push_back({ tensor, at });
             place += (n + kStateBlock - 1) / kStateBlock * kStateBlock;
             bytes += t.n * (8 + 2 * state_bits / 4 + size_of(t.d_type) + (t.copy ? 2 : 0));
-        }
-        if (chunks.size() > (1u << 24) - 1) {
-            set_error("%s: more values than one launch takes", who);
-            return PXH_ERR_UNSUPPORTED;
         }
         auto* t = new pxh_adamw_table{};
         t->count = static_cast<int>(records.size());

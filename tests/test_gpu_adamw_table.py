@@ -423,3 +423,15 @@ def test_a_value_that_is_no_number_is_kept_as_its_blocks_largest(ops, bad):
         model.table.update(t, 1e-3, seed=t)
     assert bool(torch.isfinite(model.w[7][others]).all()) and bool(torch.isfinite(model.v[7].float()).all())
     assert bool(torch.isfinite(model.ms[7]).all()) and bool(torch.isfinite(model.vs[7]).all())
+
+
+def test_more_values_than_a_launch_takes():
+    """Refused before a list of their chunks has been made, which would be larger than memory."""
+    count = 1 << 16
+    table = (capi.AdamwTensor * count)()
+    for t in table:
+        t.w = t.d = t.m = t.v = 256
+        t.n, t.d_type = (1 << 31) - 1, 0
+    handle = ctypes.c_void_p()
+    assert capi.call_raw("pxh_adamw_table_create", count, ctypes.addressof(table), 32, ctypes.byref(handle)) == -2
+    assert "one launch" in capi.last_error() and not handle.value
