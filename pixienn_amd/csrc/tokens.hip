@@ -118,7 +118,8 @@ struct RowResult {
 // What a row's sums say, with the given token's place (or -1) and logit.
 __device__ __forceinline__ RowResult finish_row(const TokenArgs& a, long long row, const Sums& s, int target, float given, bool writes)
 {
-    const bool empty = s.peak == -INFINITY;
+    // nothing but minus infinities; beside a NaN, which is above nothing, the sum is one
+    const bool empty = s.peak == -INFINITY && s.sum == 0.0f;
     const float log_sum = logf(s.sum);
     RowResult r;
     r.log_sum = log_sum;

@@ -469,3 +469,32 @@ def test_alternatives_without_their_places_are_refused(ops):
     for scale in (1.0, 1):          # by the native call, which leaves a whole number, and by the function's own checks
         with pytest.raises(capi.PxError, match="go together"):
             ops.token_logprobs_forward(x, t, v, top_logp=tops, scale=scale)
+
+
+# (rows, vocabulary): a row in one part of few lanes, in parts joined by a wave and by a workgroup, whole by 1024 lanes, and by 512 of 8 and of 14 vectors
+PLANS = [(2, 300), (3, 9000), (2, 131072), (70, 40001), (1030, 17001), (1030, 50001)]
+
+
+@gpu
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("rows,vocab", PLANS + [(1, 200001)])
+def test_rows_of_nothing_but_nan(ops, kind, rows, vocab):
+    x = draw(1, rows, vocab, TYPES[kind][0])
+    x[0] = math.nan
+    if rows > 2:
+        x[1] = math.nan
+        x[1, ::3] = -INF
+        x[rows - 1] = -INF
+        x[rows - 1, vocab - 1] = math.nan
+    bad = [0, 1, rows - 1] if rows > 2 else [0]
+    targets = torch.full((rows,), 3, device="cuda")
+    got = forward(ops, x, targets)
+    for k in got:
+        assert bool(torch.isnan(got[k][bad]).all()) and int(torch.isnan(got[k]).sum()) == len(bad), k
+    ones = torch.ones(rows, device="cuda")
+    for together in (True, False):
+        for h in (None, ones):
+            d, out = gradients(ops, x, targets, ones, h, 1.0, together)
+            assert bool(torch.isnan(d[bad]).all()) and int(torch.isnan(d).any(1).sum()) == len(bad)
+            for k in out:
+                assert bool(torch.isnan(out[k][bad]).all()), k
