@@ -465,7 +465,8 @@ __global__ __launch_bounds__(LANES) void token_logprobs_kernel(TokenArgs a, Part
     if (whole) lse = finish_row(a, row, s, target, given, threadIdx.x == 0).lse;
     else if (threadIdx.x == 0) p.sums[blockIdx.x] = s;
     if (a.top) {
-        const bool any = mine.has(0) || mine.extra_at >= 0;
+        // a lane of NaNs has minus infinity for its peak, which need not be a value of the row: no floor comes from there
+        const float peak = mine.peak * a.scale;
         const auto put = [&](int place, unsigned long long key) {
             if (whole) {
                 a.top_ids[static_cast<long long>(row) * a.top + place] = static_cast<int>(~static_cast<uint32_t>(key));
@@ -474,7 +475,7 @@ __global__ __launch_bounds__(LANES) void token_logprobs_kernel(TokenArgs a, Part
                 p.keys[static_cast<size_t>(blockIdx.x) * a.top + place] = key;
             }
         };
-        select_largest<LANES>(a.top, any ? order_of(mine.peak * a.scale) : 0u, [&](uint32_t floor, const auto& f) { mine.above(a.scale, floor, f); },
+        select_largest<LANES>(a.top, peak > -INFINITY ? order_of(peak) : 0u, [&](uint32_t floor, const auto& f) { mine.above(a.scale, floor, f); },
                               [&](const auto& f) { mine.each(logits, a.vocab, a.scale, f); }, put, selection);
     }
 }

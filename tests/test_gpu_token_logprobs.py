@@ -498,3 +498,58 @@ def test_rows_of_nothing_but_nan(ops, kind, rows, vocab):
             assert bool(torch.isnan(d[bad]).all()) and int(torch.isnan(d).any(1).sum()) == len(bad)
             for k in out:
                 assert bool(torch.isnan(out[k][bad]).all()), k
+
+
+def only(x, row, keep, values, fill):
+    """Row `row` holds `fill` but for `values` at the places `keep`."""
+    x[row] = fill
+    for at, value in zip(keep, values):
+        x[row, at] = value
+
+
+def check_alternatives(ops, x, some, top, scale=1.0):
+    """The places and log probabilities of rows `some`, on outputs that hold something else before."""
+    rows = len(x)
+    got = forward(ops, x, torch.zeros(rows, device="cuda", dtype=torch.long), top, scale)
+    some = torch.tensor(some)
+    ids = torch.from_numpy(alternatives(x[some.cuda()], np.float32(scale), top).astype(np.int64)).cuda()
+    assert torch.equal(got["top_ids"][some.cuda()].long(), ids), top
+    want = Want(x[some.cuda()], scale)
+    z = want.z.gather(1, ids)
+    held(got["top_logp"][some.cuda()], z - torch.where(want.empty, math.nan, want.lse)[:, None],
+         want.lse_off[:, None] + 4 * U * torch.nan_to_num(z, 0.0, 0.0, 0.0).abs().clamp(max=1e9), "top_logp")
+
+
+@gpu
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("rows,vocab", PLANS)
+@pytest.mark.parametrize("top", [1, 4, 9, 20])
+def test_alternatives_of_rows_with_nan(ops, kind, rows, vocab, top):
+    """NaNs come last, by their places, and every place is written."""
+    x = draw(2, rows, vocab, TYPES[kind][0])
+    last = rows - 1
+    x[0] = math.nan
+    only(x, last, [vocab // 3, 5], [1.5, -2.0], math.nan)
+    some = [0, last]
+    if rows > 2:
+        only(x, 1, [7], [1.0], math.nan)
+        x[1, vocab // 2:] = -INF
+        some.append(1)
+    if rows > 69:
+        x[2, 1::2] = math.nan
+        only(x, 3, [2, 3, vocab - 2], [math.nan, math.nan, 1.0], -INF)
+        only(x, 4, [vocab - 1], [math.nan], -INF)
+        some += [2, 3, 4]
+    check_alternatives(ops, x, some, top)
+
+
+@gpu
+def test_alternatives_of_a_row_in_seven_parts(ops):
+    """Seven parts with nine alternatives each are joined by a wave."""
+    x = draw(2, 300, 100001, torch.float32)
+    x[0] = math.nan
+    only(x, 1, [100000, 3], [1.0, 2.0], math.nan)
+    only(x, 2, [50000], [1.0], -INF)
+    x[3] = -INF
+    for top in (9, 20):
+        check_alternatives(ops, x, [0, 1, 2, 3, 299], top)
