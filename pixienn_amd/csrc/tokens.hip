@@ -156,14 +156,20 @@ __device__ __forceinline__ float value_of(unsigned long long key)
     return __uint_as_float((order & 0x80000000u) ? order & 0x7fffffffu : ~order);
 }
 
-constexpr int kCandidates = 512;
+constexpr uint32_t kNumber = 0x00800000u;       // the least order of a number: that of minus infinity is one less
+// for 64 of 65536 normal values 270 pass on average, more than 512 in a row of 50, and more than 1024 in one of 100000
+constexpr int kCandidates = 1024;
 
 struct Selection {
-    uint32_t best[kWave];
-    unsigned long long list[kCandidates];
-    unsigned long long most;
+    union {
+        uint32_t orders[1024];                  // of the lanes, wave by wave
+        unsigned long long list[kCandidates];
+    };
+    unsigned long long best[kWave];
+    unsigned long long floor, most;
+    uint32_t low;
     int count;
-    uint32_t floor;
+    bool mixed;
 };
 
 template<int CTRL>
@@ -180,32 +186,56 @@ __device__ __forceinline__ uint32_t wave_max_of(uint32_t v)
     return max(max(of_lane(0), of_lane(16)), max(of_lane(32), of_lane(48)));
 }
 
-// The k largest keys of a workgroup, largest first: put(place, key), key 0 where there are fewer.  `best` is the largest order of
-// the lane's keys (0: none); above(floor, f) calls f with those of its keys that reach `floor`, and may with others; each(f)
-// calls f with all keys of the workgroup, some by every lane.
-// The lanes' maxima, in 64 groups, are as many different values, so the k-th largest of those is not above the k-th largest of
-// all: only the lanes that reach it look at their values again, and little more than k values pass (8 of 16384 normal ones:
-// 9 on average).  They are ranked by counting.  Where too many values are equal for the list, each place takes a pass.
-template<int LANES, typename Above, typename Each, typename Put>
-__device__ __forceinline__ void select_largest(int k, uint32_t best, const Above& above, const Each& each, const Put& put, Selection& s)
+__device__ __forceinline__ unsigned long long key_of_lane(unsigned long long key, int lane)
 {
-    static_assert(LANES == 256 || LANES == 512 || LANES == 1024, "64 groups of lanes of one row of 16");
-    uint32_t group = max_in_row<0x4E>(max_in_row<0xB1>(best));
-    if constexpr (LANES >= 512) group = max_in_row<0x141>(group);
-    if constexpr (LANES == 1024) group = max_in_row<0x140>(group);
-    if (threadIdx.x % (LANES / kWave) == 0) s.best[threadIdx.x / (LANES / kWave)] = group;
-    if (threadIdx.x == 0) s.count = 0;
+    const uint32_t low = __builtin_amdgcn_readlane(static_cast<int>(key), lane), high = __builtin_amdgcn_readlane(static_cast<int>(key >> 32), lane);
+    return static_cast<unsigned long long>(high) << 32 | low;
+}
+
+// The key of a value that is no number, or 0.
+__device__ __forceinline__ unsigned long long key_of_masked(float z, uint32_t index) { return z > -INFINITY ? 0ull : key_of(z, index); }
+
+// The k largest keys of a workgroup, largest first: put(place, key), key 0 where there are fewer.  `best` is the largest order of
+// the lane's keys, or less than kNumber where none is a number's; largest() is its largest key; above(floor, f) calls f with those of its
+// keys that are not below `floor`, and may with others of its order; each(f) calls f with all keys of the workgroup, some by every lane; masked(i) is the
+// key of the i-th of `values` values by their places, or 0 where that is a number.  OWN: largest() is of the keys that above() goes through.
+// The lanes' maxima, in 64 columns (the lanes at one place in their waves), are as many different values, so the k-th largest of those
+// is not above the k-th largest of all: only the lanes that reach it look at their values again, and little more than k values pass
+// (8 of 16384 normal ones: 9 on average).  They are ranked by counting.
+// Where many values are equal, too many would pass, or do: the columns' floor is then formed once more from whole keys, of which the
+// lowest places are the largest, and what passes lies in the first vectors of a few columns (8 of 50001 values of one level: 57).
+// Minus infinity never passes: where fewer than k values are numbers, the other places go to the first that are masked, of which
+// there are enough among the first k.  Only where a NaN is among those, or too much passes all the same, does each place take a pass.
+template<int LANES, bool OWN, typename Largest, typename Above, typename Each, typename Masked, typename Put>
+__device__ __forceinline__ void select_largest(int k, int values, uint32_t best, const Largest& largest, const Above& above, const Each& each,
+                                               const Masked& masked, const Put& put, Selection& s)
+{
+    static_assert(LANES % kWave == 0 && LANES <= 1024, "whole waves");
+    const int lane = threadIdx.x % kWave;
+    const bool first_wave = threadIdx.x < kWave;
+    s.orders[threadIdx.x] = best;
     __syncthreads();
-    if (threadIdx.x < kWave) {
-        const uint32_t mine = s.best[threadIdx.x];
-        uint32_t low;
+    if (first_wave) {
+        uint32_t mine = best;
+#pragma unroll
+        for (int w = 1; w < LANES / kWave; ++w) mine = max(mine, s.orders[w * kWave + lane]);
+        uint32_t low = 0;
         if (k <= 8) {
-            // the k-th largest of different ones, which is no larger: round by round
+            // the k-th largest of different ones, which is no larger, or 0 where there are fewer: round by round
             uint32_t left = mine;
-            low = 0;
             for (int j = 0; j < k; ++j) {
                 low = wave_max_of(left);
                 left = left == low ? 0u : left;
+            }
+            if (static_cast<int>(__popcll(__ballot(mine >= max(low, kNumber)))) > 2 * k + 8) {
+                // far more of them: once more, with those that are equal
+                left = mine;
+                for (int need = k; need > 0;) {
+                    low = wave_max_of(left);
+                    if (low < kNumber) break;
+                    need -= __popcll(__ballot(left == low));
+                    left = left == low ? 0u : left;
+                }
             }
         } else {
             int larger = 0;
@@ -213,18 +243,48 @@ __device__ __forceinline__ void select_largest(int k, uint32_t best, const Above
             for (int j = 0; j < kWave; ++j) larger += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(mine), j)) > mine;
             low = ~wave_max_of(larger < k ? ~mine : 0u);
         }
-        if (threadIdx.x == 0) s.floor = low;
+        low = max(low, kNumber);
+        const int reach = __popcll(__ballot(mine >= low));
+        s.best[lane] = 0;
+        if (lane == 0) {
+            if (reach < k) low = kNumber;
+            s.floor = static_cast<unsigned long long>(low) << 32;
+            s.count = 0;
+            s.low = reach == kWave && k < kWave ? 0 : low;      // every column reaches it: there may be any number of them
+        }
     }
     __syncthreads();
-    const uint32_t floor = s.floor;
-    if (best >= floor)
-        above(floor, [&](unsigned long long key) {
-            if (static_cast<uint32_t>(key >> 32) < floor) return;
-            const int at = atomicAdd(&s.count, 1);
-            if (at < kCandidates) s.list[at] = key;
-        });
-    __syncthreads();
-    const int n = s.count;
+    int n = kCandidates + 1;
+    const auto pass = [&]<bool EXACT>(unsigned long long floor, bool reaches) {
+        if (reaches)
+            above(floor, [&](unsigned long long key) {
+                if (EXACT && key < floor) return;
+                const int at = atomicAdd(&s.count, 1);
+                if (at < kCandidates) s.list[at] = key;
+            });
+        __syncthreads();
+        n = __builtin_amdgcn_readfirstlane(s.count);
+    };
+    if (const uint32_t low = __builtin_amdgcn_readfirstlane(s.low)) pass.template operator()<false>(static_cast<unsigned long long>(low) << 32, !OWN || best >= low);
+    if (n > 12 * k + 24) {           // few as they are, they are ranked sooner than looked for again
+        const unsigned long long mine = !OWN || best >= static_cast<uint32_t>(s.floor >> 32) ? largest() : 0ull;
+        if (mine) atomicMax(&s.best[lane], mine);
+        __syncthreads();
+        if (first_wave) {
+            const unsigned long long column = s.best[lane];
+            int larger = 0;
+            for (int j = 0; j < kWave; ++j) larger += key_of_lane(column, j) > column;
+            const unsigned long long at = __ballot(column != 0 && larger == k - 1);
+            if (lane == 0) s.count = 0;
+            if (at != 0) {
+                const unsigned long long kth = key_of_lane(column, __ffsll(at) - 1);
+                if (lane == 0) s.floor = kth;
+            }
+        }
+        __syncthreads();
+        const unsigned long long floor = key_of_lane(s.floor, 0);
+        pass.template operator()<true>(floor, !OWN || mine >= floor);
+    }
     if (n <= kCandidates) {
         for (int t = threadIdx.x; t < n; t += LANES) {
             const unsigned long long key = s.list[t];
@@ -232,8 +292,21 @@ __device__ __forceinline__ void select_largest(int k, uint32_t best, const Above
             for (int j = 0; j < n; ++j) larger += s.list[j] > key;
             if (larger < k) put(larger, key);
         }
-        for (int t = n + threadIdx.x; t < k; t += LANES) put(t, 0ull);
-        return;
+        if (n >= k) return;
+        if (first_wave) {
+            const unsigned long long key = lane < min(k, values) ? masked(lane) : 0ull;
+            const bool infinity = static_cast<uint32_t>(key >> 32) == kNumber - 1;
+            const unsigned long long infinite = __ballot(infinity);
+            const bool mixed = __ballot(key != 0 && !infinity) != 0;
+            if (lane == 0) s.mixed = mixed;
+            if (!mixed) {
+                const int place = n + __popcll(infinite & ((1ull << lane) - 1));
+                if (infinity && place < k) put(place, key);
+                for (int t = n + __popcll(infinite) + lane; t < k; t += kWave) put(t, 0ull);
+            }
+        }
+        __syncthreads();
+        if (!s.mixed) return;
     }
     unsigned long long before = ~0ull;
     for (int place = 0; place < k; ++place) {
@@ -255,7 +328,7 @@ __device__ __forceinline__ void select_largest(int k, uint32_t best, const Above
 // Vectors first .. first + count of a row, K to a lane, and of the row's last values, which fill no vector, one to each of the
 // first lanes of the part that has them.  What is not there is minus infinity.
 constexpr int kMostVectors = 8;         // vectors of a lane
-// ... of one of 512 for a row that 1024 would hold otherwise: 76 registers, so that three such workgroups share a unit and not two
+// ... of one of 512 for a row that 1024 would hold otherwise: held to 80 registers, so that three such workgroups share a unit and not two
 // (4096 x 50001 half with three alternatives 92.6 -> 84.6 us; 16 vectors are 85 registers, two workgroups, and 101.7)
 constexpr int kThirdVectors = 14;
 
@@ -339,6 +412,16 @@ struct Part {
         }
     }
 
+    // The lane's number, so that the compiler does not keep a place for each value, or the eight or fourteen masks of the lanes that have a
+    // vector, from one look at them to the next: with more than 80 scalar registers a wave, one workgroup of 1024 lanes has a unit and not
+    // two (300 x 50001 bf16 with three alternatives 19.1 us in place of 14.1)
+    __device__ __forceinline__ int lane_again() const
+    {
+        int lane = threadIdx.x;
+        asm volatile("" : "+v"(lane));
+        return lane;
+    }
+
     // The sums of the lane's values.  An exponent is one fused multiply-add, l * c - peak * c (which a half-precision value enters
     // without being converted first), where the rounding of peak * c is less than 2^-4: it is the same in all of the lane's
     // exponents, and taken out of the sums at the end.  Beyond that, in rows of huge values, (l - peak) * c, value by value
@@ -374,24 +457,32 @@ struct Part {
         return s;
     }
 
+    // The largest of one vector.
+    __device__ __forceinline__ float largest_of(const Raw<T, V>& raw) const
+    {
+        if constexpr (T == PXH_F16) {
+            typedef _Float16 two __attribute__((ext_vector_type(2)));
+            two pair = __builtin_bit_cast(two, raw.w[0]);
+#pragma unroll
+            for (int i = 1; i < Raw<T, V>::kWords; ++i) pair = __builtin_elementwise_max(pair, __builtin_bit_cast(two, raw.w[i]));
+            return fmaxf(static_cast<float>(pair.x), static_cast<float>(pair.y));
+        } else {
+            float l[V];
+            raw.get(l);
+            float most = l[0];
+#pragma unroll
+            for (int i = 1; i < V; ++i) most = fmaxf(most, l[i]);
+            return most;
+        }
+    }
+
     __device__ __forceinline__ float largest() const
     {
         float most = extra;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             if (k * LANES >= count) break;
-            if constexpr (T == PXH_F16) {
-                typedef _Float16 two __attribute__((ext_vector_type(2)));
-                two pair = __builtin_bit_cast(two, kept[k].w[0]);
-#pragma unroll
-                for (int i = 1; i < Raw<T, V>::kWords; ++i) pair = __builtin_elementwise_max(pair, __builtin_bit_cast(two, kept[k].w[i]));
-                most = fmaxf(most, fmaxf(static_cast<float>(pair.x), static_cast<float>(pair.y)));
-            } else {
-                float l[V];
-                kept[k].get(l);
-#pragma unroll
-                for (int i = 0; i < V; ++i) most = fmaxf(most, l[i]);
-            }
+            most = fmaxf(most, largest_of(kept[k]));
             __builtin_amdgcn_sched_barrier(0);          // a vector at a time, in few registers
         }
         return most;
@@ -405,25 +496,48 @@ struct Part {
         return s;
     }
 
-    // f with the keys of all values that are not below `floor` (an order; a NaN is not below anything)
-    template<typename F>
-    __device__ __forceinline__ void above(float scale, uint32_t floor, const F& f)
+    // The largest key of the lane's values, one of which is a number: the first place of the peak.
+    __device__ __forceinline__ unsigned long long largest_key(float scale)
     {
         again();
-        const float least = value_of(static_cast<unsigned long long>(floor) << 32);
-        const auto look = [&](float l, int index) {
-            const float z = l * scale;
-            if (!(z < least)) f(key_of(z, index));
-        };
+        const float z = peak * scale;
+        const int lane = lane_again(), place = (first + lane) * V;
+        int index = -1;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            if (!has(k)) continue;
+            if (!__any(index < 0)) break;
+            if (index >= 0 || k * LANES + lane >= count) continue;
             float l[V];
             kept[k].get(l);
 #pragma unroll
-            for (int i = 0; i < V; ++i) look(l[i], at(k) + i);
+            for (int i = V - 1; i >= 0; --i)
+                if (l[i] * scale == z) index = place + k * LANES * V + i;
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if (extra_at >= 0) look(extra, extra_at);
+        return key_of(z, index < 0 ? extra_at : index);
+    }
+
+    // f with the keys of all values whose order is not below that of `floor`, which is a number's; of those that are equal to it, some of those
+    // behind its place may be left out.  A vector at a time: one whose largest value is not enough is passed over
+    template<typename F>
+    __device__ __forceinline__ void above(float scale, unsigned long long floor, const F& f)
+    {
+        again();
+        const float least = value_of(floor);
+        const uint32_t last = ~static_cast<uint32_t>(floor);
+        const int lane = lane_again(), place = (first + lane) * V;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            if (k * LANES + lane >= count) continue;
+            const float most = largest_of(kept[k]) * scale;
+            if (!(most > least || (most == least && static_cast<uint32_t>(place + k * LANES * V) <= last))) continue;
+            float l[V];
+            kept[k].get(l);
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if (l[i] * scale >= least) f(key_of(l[i] * scale, place + k * LANES * V + i));
+        }
+        if (extra_at >= 0 && extra * scale >= least) f(key_of(extra * scale, extra_at));
     }
 
     // f with the keys of all values of the part, read from memory one by one
@@ -447,7 +561,7 @@ struct Parts {
 };
 
 template<int T, bool ENTROPY, int LANES, int K, bool NT>
-__global__ __launch_bounds__(LANES) void token_logprobs_kernel(TokenArgs a, Parts p)
+__global__ __launch_bounds__(LANES, K == kThirdVectors ? 6 : 1) void token_logprobs_kernel(TokenArgs a, Parts p)
 {
     __shared__ Sums slots[LANES / kWave];
     __shared__ Selection selection;
@@ -475,8 +589,12 @@ __global__ __launch_bounds__(LANES) void token_logprobs_kernel(TokenArgs a, Part
                 p.keys[static_cast<size_t>(blockIdx.x) * a.top + place] = key;
             }
         };
-        select_largest<LANES>(a.top, peak > -INFINITY ? order_of(peak) : 0u, [&](uint32_t floor, const auto& f) { mine.above(a.scale, floor, f); },
-                              [&](const auto& f) { mine.each(logits, a.vocab, a.scale, f); }, put, selection);
+        const int begin = mine.first * kVec<T>;
+        const auto largest = [&] { return mine.largest_key(a.scale); };
+        const auto above = [&](unsigned long long floor, const auto& f) { mine.above(a.scale, floor, f); };
+        const auto each = [&](const auto& f) { mine.each(logits, a.vocab, a.scale, f); };
+        const auto masked = [&](int i) { return key_of_masked(load_one<T>(logits, begin + i) * a.scale, begin + i); };
+        select_largest<LANES, true>(a.top, mine.end(a.vocab) - begin, peak > -INFINITY ? order_of(peak) : 0u, largest, above, each, masked, put, selection);
     }
 }
 
@@ -497,10 +615,7 @@ __global__ __launch_bounds__(kBlock) void token_join_few_kernel(TokenArgs a, Par
     s = group_join<kWave>(s, c, nullptr);
     const float lse = finish_row(a, row, s, target, given, lane == 0).lse;
     int larger = 0;
-    for (int j = 0; j < n; ++j) {
-        const uint32_t low = __builtin_amdgcn_readlane(static_cast<int>(mine), j), high = __builtin_amdgcn_readlane(static_cast<int>(mine >> 32), j);
-        larger += (static_cast<unsigned long long>(high) << 32 | low) > mine;
-    }
+    for (int j = 0; j < n; ++j) larger += key_of_lane(mine, j) > mine;
     if (lane < n && larger < a.top) {
         a.top_ids[row * a.top + larger] = static_cast<int>(~static_cast<uint32_t>(mine));
         a.top_logp[row * a.top + larger] = value_of(mine) - lse;
@@ -529,18 +644,33 @@ __global__ __launch_bounds__(kBlock) void token_join_kernel(TokenArgs a, Parts p
     if (a.top) {
         const unsigned long long* keys = p.keys + static_cast<size_t>(row) * p.parts * a.top;
         const int n = p.parts * a.top;
-        uint32_t best = 0;
-        for (int k = threadIdx.x; k < n; k += kBlock) best = max(best, static_cast<uint32_t>(keys[k] >> 32));
+        unsigned long long best = 0;
+        // by places, so that the columns have the parts' first ones; where those are equal, by parts, whose first has the lowest places
         const auto each = [&](const auto& f) {
-            for (int k = threadIdx.x; k < n; k += kBlock)
-                if (keys[k]) f(keys[k]);
+            for (int k = threadIdx.x; k < n; k += kBlock) {
+                uint32_t place, part;
+                p.by_parts.divmod(k, place, part);
+                if (const unsigned long long key = keys[part * a.top + place]) f(key);
+            }
         };
-        select_largest<kBlock>(a.top, best, [&](uint32_t, const auto& f) { each(f); }, each,
-                               [&](int place, unsigned long long key) {
-                                   a.top_ids[row * a.top + place] = static_cast<int>(~static_cast<uint32_t>(key));
-                                   a.top_logp[row * a.top + place] = value_of(key) - lse;
-                               },
-                               selection);
+        each([&](unsigned long long key) { best = max(best, key); });
+        const auto first_keys = [&] {
+            unsigned long long most = 0;
+            for (int k = threadIdx.x; k < n; k += kBlock) most = max(most, keys[k]);
+            return most >> 32 < kNumber ? 0ull : most;
+        };
+        const char* logits = static_cast<const char*>(a.logits) + row * a.stride * kSize<T>;
+        const auto above = [&](unsigned long long floor, const auto& f) {
+            each([&](unsigned long long key) {
+                if (key >> 32 >= floor >> 32) f(key);
+            });
+        };
+        const auto masked = [&](int i) { return key_of_masked(load_one<T>(logits, i) * a.scale, i); };
+        const auto put = [&](int place, unsigned long long key) {
+            a.top_ids[row * a.top + place] = static_cast<int>(~static_cast<uint32_t>(key));
+            a.top_logp[row * a.top + place] = value_of(key) - lse;
+        };
+        select_largest<kBlock, false>(a.top, a.vocab, static_cast<uint32_t>(best >> 32), first_keys, above, each, masked, put, selection);
     }
 }
 

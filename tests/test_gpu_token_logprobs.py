@@ -553,3 +553,65 @@ def test_alternatives_of_a_row_in_seven_parts(ops):
     x[3] = -INF
     for top in (9, 20):
         check_alternatives(ops, x, [0, 1, 2, 3, 299], top)
+
+
+@gpu
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("rows,vocab", PLANS)
+@pytest.mark.parametrize("top", [1, 3, 8, 9, 64])
+def test_alternatives_of_few_allowed_or_equal_values(ops, kind, rows, vocab, top):
+    dtype = TYPES[kind][0]
+    x = draw(3, rows, vocab, dtype)
+    g = torch.Generator().manual_seed(vocab)
+    levels = lambda n: torch.randint(0, n, (vocab,), generator=g).to(dtype)          # noqa: E731
+    made = [lambda r: only(x, r, torch.randint(0, vocab, (5,), generator=g).tolist(), [1.0, 3.0, 2.0, 3.0, -4.0], -INF),
+            lambda r: x[r].copy_(levels(8)), lambda r: x[r].copy_(levels(3)), lambda r: x[r].fill_(-2.0),
+            lambda r: (x[r].fill_(-INF), x[r, vocab // 3:vocab // 3 + 90].copy_(levels(90)[:90])),
+            lambda r: (x[r].copy_(levels(2)), x[r, :vocab // 2].fill_(-INF)),
+lambda r: x[r].copy_((torch.randn(vocab, generator=g) * 3 + 100).to(torch.bfloat16)),
+            lambda r: only(x, r, [vocab - 1], [0.5], -INF), lambda r: only(x, r, [0, 1, 2], [-1.0, -1.0, -2.0], -INF),
+            lambda r: only(x, r, [0, vocab // 2], [torch.finfo(dtype).min, torch.finfo(dtype).min], -INF),
+            # a few columns of lanes hold a great many
+            lambda r: x[r].copy_(torch.where(torch.arange(vocab) % 512 < 24, levels(200).float(), -INF).to(dtype)),
+            lambda r: x[r].fill_(-INF)]
+    some = []
+    for r, make in zip(range(rows), made):
+        make(r)
+        some.append(r)
+    check_alternatives(ops, x, some, top)
+    if rows < 4:        # the others one by one
+        for make in made[rows:]:
+            make(0)
+            check_alternatives(ops, x, [0], top)
+
+
+def fastest(f, tries=5, calls=5):
+    f()
+    best = INF
+    for _ in range(tries):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        for _ in range(calls):
+            f()
+        b.record()
+        torch.cuda.synchronize()
+        best = min(best, a.elapsed_time(b) / calls)
+    return best
+
+
+@gpu
+@pytest.mark.parametrize("top", [3, 8])
+def test_masked_and_tied_rows_take_no_passes_of_their_own(ops, top):
+    """Rows of five allowed tokens, of four levels and of coarse values are not read `top` times over."""
+    rows, vocab = 2048, 50001
+    x = draw(4, rows, vocab, torch.float16)
+    targets = torch.zeros(rows, device="cuda", dtype=torch.long)
+    ordinary = fastest(lambda: forward(ops, x, targets, top))
+    g = torch.Generator("cuda").manual_seed(4)
+    levels = torch.randint(0, 4, (rows, vocab), device="cuda", generator=g).half()
+    coarse = (torch.randn(rows, vocab, device="cuda", generator=g) * 2.5 + 90).bfloat16()
+    allowed = torch.full_like(x, -INF)
+    allowed[:, [17, 4000, 20000, 33333, 50000]] = 1.0
+    for what, logits in (("levels", levels), ("coarse", coarse), ("allowed", allowed)):
+        taken = fastest(lambda: forward(ops, logits, targets, top))
+        assert taken < 2 * ordinary, (what, taken, ordinary)
