@@ -638,11 +638,12 @@ int pxh_rms_norm_backward(const void* dy, const void* h, const void* weight, con
  *   z = scale * logits;  lse = log sum exp z;  logp = z[target] - lse;  entropy = lse - sum softmax(z) * z
  * targets: [rows], int32 (wide_targets == 0) or int64; one outside [0, vocab) gives a logp of 0 (a place at which nothing is to
  * be learned).  targets and logp are given together or not at all; entropy and lse are nullable.  scale > 0.
- * top_logp, top_ids [rows][top]: the `top` largest z (at most PXH_MOST_ALTERNATIVES, and vocab), descending, among equal ones the
- * lowest index first; top == 0: none.  A logit of minus infinity has probability 0, and one of the type's lowest value is a number as
- * any other.  A row of nothing but minus infinities has lse and logp minus infinity, entropy 0 (and NaN
- * for its alternatives, which have no distribution); one with a NaN or plus infinity
- * has NaN in all three, and its NaNs come last among the alternatives.
+ * top_logp, top_ids [rows][top]: z - lse of the `top` largest z (at most PXH_MOST_ALTERNATIVES, and vocab) and their indices,
+ * descending, among equal ones the lowest index first; top == 0: none.  Like logp, top_logp is formed relative to the row's largest
+ * z, and so is right where lse, as an fp32 number, has lost the logarithm beside huge logits.
+ * A logit of minus infinity has probability 0, and one of the type's lowest value is a number as any other.  A row of nothing but
+ * minus infinities has lse and logp minus infinity, entropy 0 (and NaN for its alternatives, which have no distribution); one with a
+ * NaN or plus infinity has NaN in all three, and its NaNs come last among the alternatives.
  * workspace: pxh_token_logprobs_workspace_bytes(rows, vocab, top), which serves fewer rows, fewer alternatives and smaller
  * vocabularies too, or NULL for the library's (most calls write nothing to it: it is for rows in several parts). */
 #define PXH_MOST_ALTERNATIVES 64

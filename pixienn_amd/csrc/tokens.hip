@@ -113,6 +113,11 @@ __device__ __forceinline__ int target_of(const TokenArgs& a, long long row)
 
 struct RowResult {
     float lse, log_sum, entropy;        // log_sum: relative to the peak; minus infinity where there is nothing
+    float peak;                         // times the scale
+
+    // of an alternative, from its logit times the scale: as that of the given token it is right where lse has lost the logarithm of the
+    // sum beside huge logits
+    __device__ __forceinline__ float logp(float z) const { return (z - peak) - log_sum; }
 };
 
 // What a row's sums say, with the given token's place (or -1) and logit.
@@ -123,6 +128,7 @@ __device__ __forceinline__ RowResult finish_row(const TokenArgs& a, long long ro
     const float log_sum = logf(s.sum);
     RowResult r;
     r.log_sum = log_sum;
+    r.peak = s.peak * a.scale;
     r.lse = empty ? -INFINITY : fmaf(s.peak, a.scale, log_sum);
     r.entropy = empty ? 0.0f : log_sum - s.weighted / s.sum * kLn2;
     if (writes) {
@@ -575,8 +581,8 @@ __global__ __launch_bounds__(LANES, K == kThirdVectors ? 6 : 1) void token_logpr
     Part<T, LANES, K, NT, K == kThirdVectors> mine;
     mine.load(logits, a.vocab, static_cast<int>(part) * p.vectors, p.vectors);
     const Sums s = group_join<LANES>(mine.template sums<ENTROPY>(logits, c), c, slots);
-    float lse = 0.0f;
-    if (whole) lse = finish_row(a, row, s, target, given, threadIdx.x == 0).lse;
+    RowResult result{};
+    if (whole) result = finish_row(a, row, s, target, given, threadIdx.x == 0);
     else if (threadIdx.x == 0) p.sums[blockIdx.x] = s;
     if (a.top) {
         // a lane of NaNs has minus infinity for its peak, which need not be a value of the row: no floor comes from there
@@ -584,7 +590,7 @@ __global__ __launch_bounds__(LANES, K == kThirdVectors ? 6 : 1) void token_logpr
         const auto put = [&](int place, unsigned long long key) {
             if (whole) {
                 a.top_ids[static_cast<long long>(row) * a.top + place] = static_cast<int>(~static_cast<uint32_t>(key));
-                a.top_logp[static_cast<long long>(row) * a.top + place] = value_of(key) - lse;
+                a.top_logp[static_cast<long long>(row) * a.top + place] = result.logp(value_of(key));
             } else {
                 p.keys[static_cast<size_t>(blockIdx.x) * a.top + place] = key;
             }
@@ -613,12 +619,12 @@ __global__ __launch_bounds__(kBlock) void token_join_few_kernel(TokenArgs a, Par
     Sums s = nothing();
     if (lane < p.parts) s = p.sums[row * p.parts + lane];
     s = group_join<kWave>(s, c, nullptr);
-    const float lse = finish_row(a, row, s, target, given, lane == 0).lse;
+    const RowResult result = finish_row(a, row, s, target, given, lane == 0);
     int larger = 0;
     for (int j = 0; j < n; ++j) larger += key_of_lane(mine, j) > mine;
     if (lane < n && larger < a.top) {
         a.top_ids[row * a.top + larger] = static_cast<int>(~static_cast<uint32_t>(mine));
-        a.top_logp[row * a.top + larger] = value_of(mine) - lse;
+        a.top_logp[row * a.top + larger] = result.logp(value_of(mine));
     }
 }
 
@@ -640,7 +646,7 @@ __global__ __launch_bounds__(kBlock) void token_join_kernel(TokenArgs a, Parts p
         s = r;
     }
     s = group_join<kBlock>(s, c, slots);
-    const float lse = finish_row(a, row, s, target, given, threadIdx.x == 0).lse;
+    const RowResult result = finish_row(a, row, s, target, given, threadIdx.x == 0);
     if (a.top) {
         const unsigned long long* keys = p.keys + static_cast<size_t>(row) * p.parts * a.top;
         const int n = p.parts * a.top;
@@ -668,7 +674,7 @@ __global__ __launch_bounds__(kBlock) void token_join_kernel(TokenArgs a, Parts p
         const auto masked = [&](int i) { return key_of_masked(load_one<T>(logits, i) * a.scale, i); };
         const auto put = [&](int place, unsigned long long key) {
             a.top_ids[row * a.top + place] = static_cast<int>(~static_cast<uint32_t>(key));
-            a.top_logp[row * a.top + place] = value_of(key) - lse;
+            a.top_logp[row * a.top + place] = result.logp(value_of(key));
         };
         select_largest<kBlock, false>(a.top, a.vocab, static_cast<uint32_t>(best >> 32), first_keys, above, each, masked, put, selection);
     }

@@ -615,3 +615,17 @@ def test_masked_and_tied_rows_take_no_passes_of_their_own(ops, top):
     for what, logits in (("levels", levels), ("coarse", coarse), ("allowed", allowed)):
         taken = fastest(lambda: forward(ops, logits, targets, top))
         assert taken < 2 * ordinary, (what, taken, ordinary)
+
+
+@gpu
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("rows,vocab", PLANS)
+def test_alternatives_of_a_row_of_the_lowest_value(ops, kind, rows, vocab):
+    """All alike: every alternative has a vocabulary's share, though the logarithm of the sum is lost beside the logits."""
+    x = draw(5, rows, vocab, TYPES[kind][0])
+    x[0] = torch.finfo(x.dtype).min
+    got = forward(ops, x, torch.full((rows,), 4, device="cuda"), 5)
+    near = U * (vocab / 256 + 44 + 6 * math.log(vocab))
+    assert torch.equal(got["top_ids"][0], torch.arange(5, device="cuda", dtype=torch.int32))
+    for value in [*got["top_logp"][0].tolist(), float(got["logp"][0])]:
+        assert abs(value + math.log(vocab)) <= near
