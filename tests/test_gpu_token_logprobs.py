@@ -629,3 +629,45 @@ def test_alternatives_of_a_row_of_the_lowest_value(ops, kind, rows, vocab):
     assert torch.equal(got["top_ids"][0], torch.arange(5, device="cuda", dtype=torch.int32))
     for value in [*got["top_logp"][0].tolist(), float(got["logp"][0])]:
         assert abs(value + math.log(vocab)) <= near
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+@pytest.mark.parametrize("vectors,more,top", [(4097, 1, 0), (4097, 7, 3), (5600, 3, 8), (6250, 1, 64), (7168, 5, 3), (7168, 7, 9)])
+@pytest.mark.parametrize("begin", [0, 1])
+def test_rows_off_a_word_with_values_behind_the_last_vector(ops, kind, vectors, more, top, begin):
+    """Every other row begins between two words, and is read from its second value on: what a lane's first value is comes from the lane in
+    front, and at a wave's first lane from memory."""
+    dtype, rows = TYPES[kind][0], 1026
+    vocab = vectors * 8 + more
+    wide = draw(6, rows * vocab + begin, 1, dtype).view(-1)
+    x = wide[begin:].view(rows, vocab)
+    assert {(x.data_ptr() + 2 * vocab * r) % 4 for r in range(2)} == {0, 2}
+    for r in (2, 3):
+        x[r] = -INF
+        x[r, 512 * (r + 5)] = 1.0                   # a wave's first value alone
+        x[r + 2, 64 * 8::512 * 8] = math.nan        # ... no number
+        x[r + 4, ::512] = 9.0                       # ... the largest
+        x[r + 6, ::8] = 8.0
+        x[r + 8, 7::8] = 8.0
+        x[r + 10] = -INF
+        x[r + 12, vectors * 8:] = 12.0              # behind the last vector
+        x[r + 14] = torch.finfo(dtype).min
+        x[r + 16, vocab - 1] = math.nan
+        x[r + 18] = -INF
+        x[r + 18, vectors * 8 - 1] = 2.0            # the last vector's last
+        x[r + 20] = -INF
+        x[r + 20, vectors * 8] = 2.0                # the first behind it
+    targets = (torch.arange(rows, device="cuda") * 7919) % (vocab + 2) - 1
+    targets[2:4] = torch.tensor([512 * 7, 512 * 8])
+    clean = ~torch.isnan(x).any(1)
+    got = forward(ops, x, targets, top)
+    want = Want(x[clean], 1.0)
+    held(got["lse"][clean], want.lse, want.lse_off, "lse")
+    held(got["entropy"][clean], want.entropy, want.entropy_off, "entropy")
+    held(got["logp"][clean], *want.logp(targets[clean]), "logp")
+    for k in ("lse", "entropy"):
+        assert bool(torch.isnan(got[k][~clean]).all()), k
+    if top:
+        some = torch.cat([torch.arange(30), torch.arange(rows - 4, rows)]).cuda()
+        assert torch.equal(got["top_ids"][some].long().cpu(), torch.from_numpy(alternatives(x[some], np.float32(1), top).astype(np.int64)))
