@@ -682,7 +682,7 @@ int pxh_token_logprobs_forward_train(const void* logits, const void* targets, co
  * there, and both are rounded to fp32 once.
  *
  * States in 8 bits: m and the SQUARE ROOT of v are e4m3 values with a scale for each 256 of a tensor, its largest magnitude / 448
- * (2^-126 at least): 2 + 1/32 bytes a value for both.  Each step's results are rounded stochastically, up with the
+ * (as a product with 1/448, 2^-126 at least): 2 + 1/32 bytes a value for both.  Each step's results are rounded stochastically, up with the
  * probability of the part cut off: what a step changes of an average over 1000 steps is less than half a unit of such a value, and
  * rounded to nearest it would never change.  A root that is not zero never rounds to zero (the quotient stays bounded).  The
  * random bits come from `seed` (its low 31 bits) and the value's place in the table: another seed every step, the step's number

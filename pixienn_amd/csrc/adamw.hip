@@ -15,8 +15,6 @@ constexpr int kStateBlock = 256;            // values with one scale: four to a 
 constexpr int kSteps = 4;                   // blocks of a wave
 constexpr int kChunk = kSteps * kBlock * 4; // values of a workgroup
 constexpr int kNormWorkers = 2048;
-constexpr float kE4m3Max = 448.0f;
-constexpr float kLeastScale = 0x1p-126f;
 
 struct AdamwRecord {
     float* w;
@@ -325,7 +323,7 @@ __device__ __forceinline__ void step_chunk(const AdamwRecord& r, const AdamwStep
             }
             peak = eight_maxima(most);
         }
-        const float scale = fmaxf(peak / kE4m3Max, kLeastScale), inverse = 1.0f / scale;
+        const float scale = scale_of(peak), inverse = 1.0f / scale;
         const uint32_t of = block + (j % kSteps) * (kBlock / kWave);
         if (lane % 8 == 0 && of < blocks) global_memory<float>(j < kSteps ? r.m_scale : r.v_scale)[of] = scale;
 #pragma unroll

@@ -64,11 +64,6 @@ __device__ __forceinline__ float scale_group_max(float v)
     return v;
 }
 
-constexpr float kE4m3Max = 448.0f;
-constexpr float kLeastScale = 0x1p-126f;        // its reciprocal is finite, and a row of zeros has zeros
-
-__device__ __forceinline__ float scale_of(float peak) { return fmaxf(peak * (1.0f / kE4m3Max), kLeastScale); }
-
 // Four values no larger than 448 by more than a rounding: the conversion rounds to nearest even and leaves NaN.
 __device__ __forceinline__ uint32_t e4m3_of(float a, float b, float c, float d)
 {

@@ -190,6 +190,13 @@ __device__ __forceinline__ void store_row(void* p, int e, int n, const Raw<T, V>
         if (e + k < n) store_one<T>(p, e + k, x[k]);
 }
 
+// The scale of e4m3 values of which the largest magnitude is `peak`: a product with 1/448, as torch has a quotient by a number, so that
+// its operations give the same codes (a unit of a scale turns one code of 10^6 that are rounded stochastically, and as many at a tie).
+constexpr float kE4m3Max = 448.0f;
+constexpr float kLeastScale = 0x1p-126f;        // its reciprocal is finite, and zeros have zeros
+
+__device__ __forceinline__ float scale_of(float peak) { return fmaxf(peak * (1.0f / kE4m3Max), kLeastScale); }
+
 // Calls f.template operator()<T>() for a run-time type of values; false for another one.
 template<typename F>
 inline bool dispatch_type(int type, F&& f)

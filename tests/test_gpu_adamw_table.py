@@ -435,3 +435,18 @@ def test_more_values_than_a_launch_takes():
     handle = ctypes.c_void_p()
     assert capi.call_raw("pxh_adamw_table_create", count, ctypes.addressof(table), 32, ctypes.byref(handle)) == -2
     assert "one launch" in capi.last_error() and not handle.value
+
+
+@gpu
+def test_scales_are_the_largest_magnitude_times_a_448th(ops):
+    """To the bit what elementary operations in fp32 give, as the norm's scales are: an ulp of a scale turns single codes."""
+    n = 256 * 3000
+    g = torch.Generator().manual_seed(11)
+    w, d = torch.zeros(n, device="cuda"), normal(g, n, 1.0)
+    states = ops.adamw_states([w], 8)
+    ops.AdamwTable([w], [d], **states).update(1, 1e-3, 0.5, 0.75, seed=3)
+    m, root = 0.5 * d, (0.25 * (d * d)).cpu().numpy()
+    root = np.sqrt(root).reshape(-1, 256).max(1)                    # numpy's root is the rounded one
+    recip = np.float32(1.0) / np.float32(448.0)
+    assert np.array_equal(states["m_scales"][0].cpu().numpy(), m.abs().cpu().numpy().reshape(-1, 256).max(1) * recip)
+    assert np.array_equal(states["v_scales"][0].cpu().numpy(), root * recip)
