@@ -612,7 +612,7 @@ int pxh_rescale_clip_table(const pxh_tensor_table* table, float threshold, float
  * residual, sum (receives h; only with a residual), scales and rstd are nullable.  weight holds `width` values of
  * weight_type: `type` or PXH_F32.  y_type is `type`, or PXH_E4M3 with scales: `group` consecutive values of a row (128, or 0
  * for the whole row; the last group of a row may be shorter) share
- *   scale = max(largest |y| of the group / 448, 2^-126),  and y holds e4m3(y / scale);
+ *   scale = largest |y| of the group / 448 (as a product with 1/448; 2^-126 at least, and finite),  and y holds e4m3(y / scale);
  * scales is [rows][width / group, rounded up], packed.  sum may be x or residual itself, and y (of `type`) may be x or
  * residual, where the strides are the same; nothing else that is written may overlap another tensor.  An infinity in a row makes
  * its rstd 0 and the infinite values NaN, a NaN the whole row NaN, as the formulas have it. */

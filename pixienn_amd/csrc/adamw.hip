@@ -231,25 +231,20 @@ __device__ __forceinline__ float largest_number(const float (&x)[4])
 }
 
 // Four values over their block's scale as e4m3, up with the probability of what is cut off, by the upper 20 bits of the noise (the
-// hardware's conversion, which is the addition of those bits below the last place, subnormals among it).  The quotient from the
-// rounded reciprocal and one correction by its remainder (Markstein), which is the rounded quotient; of what is no number, whose weight
-// is lost, it is a NaN, and kept as the largest value: the lesser of a NaN and a number is the number.
+// hardware's conversion, which is the addition of those bits below the last place, subnormals among it).  What is no number, whose weight
+// is lost, has a NaN for its quotient, and is kept as the largest value: the lesser of a NaN and a number is the number.
 __device__ __forceinline__ void to_e4m3(const AdamwStep& s, uint32_t place, const float (&m)[4], const float (&root)[4], float m_scale,
                                         float m_inverse, float v_scale, float v_inverse, uint32_t& m8, uint32_t& v8)
 {
     // the four places differ in their last two bits only: one product for all
     const uint32_t base = ((place ^ s.seed) & ~3u) * kMix1;
-    const auto over = [](float x, float scale, float inverse) {
-        const float q = x * inverse;
-        return fmaf(fmaf(-q, scale, x), inverse, q);
-    };
     int mw = 0, vw = 0;
     const auto put = [&]<int K>() {
         const uint32_t noise = second_round(base + ((K ^ s.seed) & 3u) * kMix1);
-        const float x = fmaxf(fminf(over(m[K], m_scale, m_inverse), kE4m3Max), -kE4m3Max);
+        const float x = fmaxf(fminf(quotient_of(m[K], m_scale, m_inverse), kE4m3Max), -kE4m3Max);
         mw = __builtin_amdgcn_cvt_sr_fp8_f32(x, static_cast<int>(noise), mw, K);
         // at least the least value there is, unless it is zero
-        const float v = fmaxf(fminf(over(root[K], v_scale, v_inverse), kE4m3Max), fminf(root[K] * 0x1p100f, 0x1p-9f));
+        const float v = fmaxf(fminf(quotient_of(root[K], v_scale, v_inverse), kE4m3Max), fminf(root[K] * 0x1p100f, 0x1p-9f));
         vw = __builtin_amdgcn_cvt_sr_fp8_f32(v, static_cast<int>(noise << 12), vw, K);
     };
     put.template operator()<0>();

@@ -238,7 +238,7 @@ __global__ __launch_bounds__(LANES > kWave ? LANES : kBlock) void rms_norm_kerne
                 if (e % 128 == 0 && e < n) a.scales[row * groups + e / 128] = scale;
             }
 #pragma unroll
-            for (int k = 0; k < V; ++k) y[k] *= inverse;
+            for (int k = 0; k < V; ++k) y[k] = quotient_of(y[k], scale, inverse);
             if (e < n) store_e4m3<V>(static_cast<char*>(a.y) + row * a.y_stride, e, n, y);
         } else {
             Raw<T, V> r;

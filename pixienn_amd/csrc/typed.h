@@ -194,8 +194,16 @@ __device__ __forceinline__ void store_row(void* p, int e, int n, const Raw<T, V>
 // its operations give the same codes (a unit of a scale turns one code of 10^6 that are rounded stochastically, and as many at a tie).
 constexpr float kE4m3Max = 448.0f;
 constexpr float kLeastScale = 0x1p-126f;        // its reciprocal is finite, and zeros have zeros
+constexpr float kMostScale = 0x1.fffffep+127f;  // beside an infinity the others are zeros
 
-__device__ __forceinline__ float scale_of(float peak) { return fmaxf(peak * (1.0f / kE4m3Max), kLeastScale); }
+__device__ __forceinline__ float scale_of(float peak) { return __builtin_amdgcn_fmed3f(peak * (1.0f / kE4m3Max), kLeastScale, kMostScale); }
+
+// x / scale from the scale's rounded reciprocal and one correction by the remainder (Markstein), which is the rounded quotient.
+__device__ __forceinline__ float quotient_of(float x, float scale, float inverse)
+{
+    const float q = x * inverse;
+    return fmaf(fmaf(-q, scale, x), inverse, q);
+}
 
 // Calls f.template operator()<T>() for a run-time type of values; false for another one.
 template<typename F>

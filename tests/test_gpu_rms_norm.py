@@ -325,3 +325,44 @@ def test_an_empty_tensor_is_no_missing_one(ops, other):
               lambda: ops.rms_norm_backward(x, bad, weight, rstd, y, dw), lambda: ops.rms_norm_backward(x, x, weight, rstd, bad, dw)):
         with pytest.raises(capi.PxError):
             f()
+
+
+@gpu
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("width", [96, 1000, 4096, 20001, 40007])
+@pytest.mark.parametrize("group", [0, 128])
+def test_eight_bits_are_the_rounded_quotients(ops, kind, width, group):
+    """To the bit what elementary operations in fp32 make of the statistic that the call leaves."""
+    rows, dtype = 2000000 // width, TYPES[kind][0]
+    x = (torch.randn(rows, width, device="cuda", generator=torch.Generator("cuda").manual_seed(width)) * 3).to(dtype)
+    weight = draw(6, (1, width), 1.0, dtype)[0].contiguous()
+    groups = -(-width // 128) if group else 1
+    y, scales, rstd = torch.empty(rows, width, dtype=torch.float8_e4m3fn, device="cuda"), torch.empty(rows, groups, device="cuda"), torch.empty(rows, device="cuda")
+    ops.rms_norm_forward(x, y, weight, scales=scales, rstd=rstd, group=group)
+    h, w, r = x.float().cpu(), weight.float().cpu(), rstd.cpu()[:, None]
+    value = h * r * w
+    size = group or width
+    parts = lambda t: torch.nn.functional.pad(t, (0, groups * size - width)).view(rows, groups, size)      # noqa: E731
+    # a row's scale is found before its statistic
+    peak = parts(value).abs().amax(2) if group else (h * w).abs().amax(1, keepdim=True) * r
+    want = (peak * float(np.float32(1.0) / np.float32(448.0))).clamp(min=2.0 ** -126)
+    assert torch.equal(scales.cpu(), want)
+    codes = (parts(value) / want[:, :, None]).to(torch.float8_e4m3fn).view(rows, groups * size)[:, :width]
+    assert torch.equal(y.cpu().view(torch.uint8), codes.contiguous().view(torch.uint8))
+
+
+@gpu
+@pytest.mark.parametrize("group", [0, 128])
+def test_an_infinite_value_leaves_the_others_of_its_group(ops, group):
+    """A weight of infinity: NaN in its column, zeros beside it, and numbers where another scale is."""
+    x = draw(3, (5, 300), 1.0, torch.float32)
+    weight = torch.ones(300, device="cuda")
+    weight[140] = math.inf
+    y, scales = torch.empty(5, 300, dtype=torch.float8_e4m3fn, device="cuda"), torch.empty(5, 3 if group else 1, device="cuda")
+    ops.rms_norm_forward(x, y, weight, scales=scales, group=group)
+    y = y.float()
+    assert bool(torch.isnan(y[:, 140]).all()) and int(torch.isnan(y).sum()) == 5 and bool(torch.isfinite(scales).all())
+    beside = y[:, 128:256] if group else y
+    assert bool((beside.nan_to_num(0.0) == 0).all())
+    if group:
+        assert bool((y[:, :128] != 0).any(1).all()) and bool((y[:, 256:] != 0).any(1).all())
