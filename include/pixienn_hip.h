@@ -644,6 +644,8 @@ int pxh_rms_norm_backward(const void* dy, const void* h, const void* weight, con
  * A logit of minus infinity has probability 0, and one of the type's lowest value is a number as any other.  A row of nothing but
  * minus infinities has lse and logp minus infinity, entropy 0 (and NaN for its alternatives, which have no distribution); one with a
  * NaN or plus infinity has NaN in all three, and its NaNs come last among the alternatives.
+ * A row's results do not depend on where it lies or on the other rows' values; their last bits do on the number of rows, by which the
+ * workgroups of a row are chosen.
  * workspace: pxh_token_logprobs_workspace_bytes(rows, vocab, top), which serves fewer rows, fewer alternatives and smaller
  * vocabularies too, or NULL for the library's (most calls write nothing to it: it is for rows in several parts). */
 #define PXH_MOST_ALTERNATIVES 64

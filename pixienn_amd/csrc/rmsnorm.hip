@@ -312,7 +312,9 @@ struct NormBackwardArgs {
 
 // dx of every row, and the part of dw that this worker's rows give: a worker (LANES lanes) takes every workers-th row, and asks for
 // the next one before it waits for the sum over this one.  At four vectors a lane there are no registers for that, nor for
-// the weights, which are read again for every row.  16384 x 4096 bf16 with dsum: 537 MB in 88.7 us with the launch that adds up dw,
+// the weights, which are read again for every row.  The widest forms for 16 bits spill all the same, at two vectors 17 registers and at
+// four 142, most of them for the rows' ends, value by value in every step: 4096 x 16384 bf16 with dsum is 537 MB in 100.5 us, 5.3 TB/s, and
+// 2048 x 32768 takes 166.  16384 x 4096 bf16 with dsum: 537 MB in 88.7 us with the launch that adds up dw,
 // 6.05 TB/s, where a kernel that only moves three streams in and one out has 6.3.
 template<int T, int LANES, int K, bool NT>
 __global__ __launch_bounds__(LANES > kWave ? LANES : kBlock) void rms_norm_backward_kernel(NormBackwardArgs a, int workers)

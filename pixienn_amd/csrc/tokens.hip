@@ -335,11 +335,13 @@ __device__ __forceinline__ void select_largest(int k, int values, uint32_t best,
 // first lanes of the part that has them.  What is not there is minus infinity.
 constexpr int kMostVectors = 8;         // vectors of a lane
 // ... of one of 512 for a row that 1024 would hold otherwise: held to 80 registers, so that three such workgroups share a unit and not two
-// (4096 x 50001 half with three alternatives 92.6 -> 84.6 us; 16 vectors are 85 registers, two workgroups, and 101.7)
+// (4096 x 50001 half with three alternatives, when it was taken, 92.6 -> 84.6 us; 16 vectors are 85 registers, two workgroups, and 101.7)
 constexpr int kThirdVectors = 14;
 
-// SETTLES: rows of 16-bit values off a 4-byte boundary are read from one value further on (below).  For the lanes of 14 vectors: 4096 x 50001 half,
-// every other row of which is, 85.0 -> 79.5 us, and 4096 x 50000 76.  The others lose (8000 x 17001 55.5 -> 58, 300 x 50001 14.8 -> 16.2).
+// SETTLES: rows of 16-bit values off a 4-byte boundary are read from one value further on (below).  For the lanes of 14 vectors, where every
+// other row is: half with three alternatives, 4096 x 32777 59.0 -> 57.6 us, x 40001 67.9 -> 62.4, x 50001 83.2 -> 76.3, x 57345 94.1 -> 83.3;
+// at the short end with few rows it loses (1100 x 32777 bf16 16.4 -> 17.9, x 57351 35.9 -> 33.0).  The other forms lose (8000 x 17001
+// 55.5 -> 58, 300 x 50001 14.8 -> 16.2).
 template<int T, int LANES, int K, bool NT, bool SETTLES = false>
 struct Part {
     static constexpr bool kSettles = SETTLES && kSize<T> == 2;
@@ -556,7 +558,7 @@ struct Part {
 
 // ---------------------------------------------------------------- forward
 // A workgroup takes one part of a row into its registers; a row of several parts is put together by a second launch from
-// their sums and their largest values.  4096 x 50001 half with entropy and three alternatives: 410 MB in 78.6 us, 5.2 TB/s.  The
+// their sums and their largest values.  4096 x 50001 half with entropy and three alternatives: 410 MB in 74.5 us, 5.5 TB/s.  The
 // arithmetic alone, 8.5 instructions a value counting an exponential as four, is 44 us; it waits for the row's maximum, so that the
 // next row's loads, another workgroup's, have to cover it.
 struct Parts {
@@ -761,14 +763,15 @@ __device__ __forceinline__ RowGradient<T, PEAK> gradient_of(const TokenArgs& a, 
     return r;
 }
 
-// A workgroup takes one part of a row: 1000 x 100001 fp32 with the entropy's gradient is 800 MB in 134 us, 6.0 TB/s where a copy has
+// A workgroup takes one part of a row: 1000 x 100001 fp32 with the entropy's gradient is 800 MB in 137 us, 5.8 TB/s where a copy has
 // 6.6.  Past the caches in short parts (1000 x 100001 fp32: 149 us with four steps through the caches, 144
 // with four past them, 137 with two), within them in longer ones (512 x 32768 bf16: 11.5 us, and 13 past them).
 template<bool NT>
 constexpr int kGradientSteps = NT ? 2 : 4;
 
 // A row's vectors begin at its first 16-byte boundary (4096 x 50001 half with the entropy's gradient 138 -> 134 us).  The passes that sum over a row
-// begin at its first value, so that a row's results are the same wherever it lies.
+// begin at its first value, so that a row's results do not depend on its address (on the number of rows they do, by the last bits: the
+// lanes of a row and its parts are chosen by it).
 template<int T, bool NT>
 __global__ __launch_bounds__(kBlock) void token_gradient_kernel(TokenArgs a, FastDiv parts)
 {
