@@ -673,6 +673,44 @@ int pxh_token_logprobs_forward_train(const void* logits, const void* targets, co
                                      long long rows, int vocab, long long stride, long long d_stride, float scale,
                                      void* stream);
 
+/* Rows of a table by token: y[r] = scale * table[tokens[r]], zeros for a token outside [0, vocab).  tokens: [rows], int32
+ * (wide_tokens == 0) or int64.  table and y are of `type`. */
+int pxh_embedding_forward(const void* table, const void* tokens, void* y, int type, int wide_tokens, long long rows, int vocab,
+                          int width, long long table_stride, long long y_stride, float scale, void* stream);
+
+/* The gradient of the table: d[v] = scale * the sum of dy[r] over the rows r of token v (zeros for a token of no row), or, with
+ * accumulate, added to what d holds, of which rows without one are not touched.  d is of `type` or fp32 (d_type).  The rows are
+ * sorted by token and added up in fp32 in an order that the tokens alone decide: the same call gives the same bits.  Rows whose
+ * token is outside the vocabulary count nothing.  dy and d may not overlap.  workspace: pxh_embedding_workspace_bytes(rows, width),
+ * which serves fewer rows and shorter ones too, or NULL for the library's. */
+size_t pxh_embedding_workspace_bytes(long long rows, int width);
+int pxh_embedding_backward(const void* dy, const void* tokens, void* d, int type, int d_type, int wide_tokens, long long rows,
+                           int vocab, int width, long long dy_stride, long long d_stride, float scale, int accumulate,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* Layer norm over the rows, with the residual's addition in front of it:
+ *   h = x + residual, rounded to `type` (h = x without one);  mean = mean(h);  rstd = 1 / sqrt(mean((h - mean)^2) + eps)
+ *   y = (h - mean) * rstd * weight + bias
+ * residual, sum (receives h; only with a residual), bias, mean and rstd (each [rows], what the backward pass needs) are nullable.
+ * weight and bias hold `width` values of weight_type: `type` or PXH_F32.  sum may be x or residual itself, and y may be x or
+ * residual, where the strides are the same; nothing else that is written may overlap another tensor. */
+int pxh_layer_norm_forward(const void* x, const void* residual, void* sum, const void* weight, const void* bias, void* y,
+                           float* mean, float* rstd, int type, int weight_type, long long rows, int width, long long x_stride,
+                           long long residual_stride, long long sum_stride, long long y_stride, float eps, void* stream);
+
+/* Its gradients, from h (the sum if there was a residual) and the forward's mean and rstd:
+ *   g = dy * weight;  xhat = (h - mean) * rstd;  dx = rstd * (g - mean(g) - xhat * mean(g * xhat)) + dsum
+ *   dw (+)= sum over the rows of dy * xhat;  db (+)= sum over the rows of dy
+ * dsum (nullable) is what arrives along the residual stream; dx is then the gradient of x and of the residual alike, and may be dy
+ * or dsum where the strides are the same.  dw and db (nullable) are fp32, [width], overwritten (accumulate == 0) or added to, summed
+ * in a fixed order.  workspace: pxh_layer_norm_workspace_bytes(rows, width), which serves fewer rows and shorter rows too, or NULL
+ * for the library's. */
+size_t pxh_layer_norm_workspace_bytes(long long rows, int width);
+int pxh_layer_norm_backward(const void* dy, const void* h, const void* weight, const float* mean, const float* rstd,
+                            const void* dsum, void* dx, float* dw, float* db, int type, int weight_type, long long rows, int width,
+                            long long dy_stride, long long h_stride, long long dsum_stride, long long dx_stride, int accumulate,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
 /* AdamW over all parameter tensors of a model at once, from a table kept on the device, with states in 32 or in 8 bits and the
  * gradients clipped by their common norm:
  *   norm = |d_scale * d|_2 over all tensors;  f = max_norm > 0 and norm > max_norm ? max_norm / norm : 1

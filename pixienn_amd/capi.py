@@ -91,6 +91,10 @@ SIGNATURES = {
     "pxh_adamw_table_create": [I, P, I, P],
     "pxh_adamw_table_count": [P],
     "pxh_adamw_update_table": [P, I, F, D, D, F, F, F, F, P, U, P],
+    "pxh_embedding_forward": [P, P, P, I, I, L, I, I, L, L, F, P],
+    "pxh_embedding_backward": [P, P, P, I, I, I, L, I, I, L, L, F, I, P, Z, P],
+    "pxh_layer_norm_forward": [P, P, P, P, P, P, P, P, I, I, L, I, L, L, L, L, F, P],
+    "pxh_layer_norm_backward": [P, P, P, P, P, P, P, P, P, I, I, L, I, L, L, L, L, I, P, Z, P],
     "pxh_token_logprobs_forward_train": [P, P, P, P, P, P, P, P, I, I, L, I, L, L, F, P],
 }
 _OTHER_RETURNS = {
@@ -110,6 +114,8 @@ _OTHER_RETURNS = {
     "pxh_adamw_table_destroy": (None, [P]),
     "pxh_rms_norm_workspace_bytes": (Z, [L, I]),
     "pxh_token_logprobs_workspace_bytes": (Z, [L, I, I]),
+    "pxh_embedding_workspace_bytes": (Z, [L, I]),
+    "pxh_layer_norm_workspace_bytes": (Z, [L, I]),
 }
 # test hooks (pixienn_amd/csrc/pixienn_hip_test.h): exported, but not part of the C ABI
 _TEST_HOOKS = {
@@ -147,6 +153,8 @@ _lib = None
 native = {}
 # ... and those whose Python functions it takes whole, tensors of any type and stride: name -> callable.
 functions = {}
+# ... and those that look at the tensors' device as well, which is handed to them with the stream.
+layers = {}
 
 
 def load():
@@ -192,6 +200,8 @@ def bind_calls():
                    for name in _calls.names()})
     functions.update({name: _calls.bind_function(name, ctypes.cast(getattr(lib, name), ctypes.c_void_p).value)
                       for name in _calls.functions()})
+    layers.update({name: _calls.bind_function(name, ctypes.cast(getattr(lib, name), ctypes.c_void_p).value)
+                   for name in _calls.layers()})
 
 
 def declared_symbols():

@@ -374,11 +374,150 @@ PyObject* token_logprobs_forward_train(PyObject* self, PyObject* const* args, Py
     });
 }
 
+// ---------------------------------------------------------------- calls that look at the tensors' device too
+// The last arguments are the current device's index and its current stream: a tensor of another device is left to the caller.
+
+struct Device {
+    long long index;
+    void* stream;
+
+    const at::Tensor& tensor(PyObject* o) const
+    {
+        const at::Tensor& t = tensor_of(o);
+        if (t.get_device() != index) throw NotHere{};
+        return t;
+    }
+    Rows rows(PyObject* o) const
+    {
+        if (o != Py_None) tensor(o);
+        return Rows(o);
+    }
+    // A packed tensor of n values, or None.
+    template<typename V>
+    V* packed(PyObject* o, long long n, at::ScalarType type) const
+    {
+        if (o != Py_None) tensor(o);
+        return ::packed<V>(o, n, type);
+    }
+    float* floats(PyObject* o, long long n) const { return packed<float>(o, n, at::kFloat); }
+    Space space(PyObject* o) const
+    {
+        if (o != Py_None) tensor(o);
+        return Space(o);
+    }
+    // Weights of a norm and their type.
+    void* weights(PyObject* o, long long n, int& type) const
+    {
+        const at::Tensor& t = tensor(o);
+        type = type_of(t);
+        if (type == PXH_E4M3) throw NotHere{};
+        return packed<void>(o, n, t.scalar_type());
+    }
+    // Tokens that are there, of 32 or 64 bits.
+    Targets tokens(PyObject* o, long long n) const
+    {
+        tensor(o);
+        return Targets(o, n);
+    }
+};
+
+// body(args, device, entry point) where there are COUNT arguments and the device's two; None where it leaves the call.
+template<auto* F, size_t COUNT, typename B>
+PyObject* on_device(PyObject* self, PyObject* const* args, Py_ssize_t count, const B& body)
+{
+    return guarded<COUNT + 2>(args, count, [&](PyObject* const* a) {
+        const Device device{ argument<long long>(a[COUNT]), argument<void*>(a[COUNT + 1]) };
+        return body(a, device, reinterpret_cast<decltype(F)>(PyLong_AsVoidPtr(self)));
+    });
+}
+
+// (table, tokens, y, scale)
+PyObject* embedding_forward(PyObject* self, PyObject* const* args, Py_ssize_t count)
+{
+    return on_device<&pxh_embedding_forward, 4>(self, args, count, [](PyObject* const* a, const Device& d, auto f) {
+        const Rows table = d.rows(a[0]), y = d.rows(a[2]);
+        if (!table.given || !y.given || y.width != table.width || y.type != table.type) throw NotHere{};
+        const Targets tokens = d.tokens(a[1], y.rows);
+        const float scale = argument<float>(a[3]);
+        const int vocab = fits(table.rows), width = fits(table.width);
+        return status([&] {
+            return f(table.data, tokens.data, y.data, table.type, tokens.wide, y.rows, vocab, width, table.stride, y.stride, scale, d.stream);
+        });
+    });
+}
+
+// (dy, tokens, d, scale, accumulate, workspace)
+PyObject* embedding_backward(PyObject* self, PyObject* const* args, Py_ssize_t count)
+{
+    return on_device<&pxh_embedding_backward, 6>(self, args, count, [](PyObject* const* a, const Device& d, auto f) {
+        const Rows dy = d.rows(a[0]), table = d.rows(a[2]);
+        if (!dy.given || !table.given || dy.width != table.width || (table.type != dy.type && table.type != PXH_F32)) throw NotHere{};
+        const Targets tokens = d.tokens(a[1], dy.rows);
+        const float scale = argument<float>(a[3]);
+        const int accumulate = argument<int>(a[4]), vocab = fits(table.rows), width = fits(dy.width);
+        const Space space = d.space(a[5]);
+        return status([&] {
+            return f(dy.data, tokens.data, table.data, dy.type, table.type, tokens.wide, dy.rows, vocab, width, dy.stride, table.stride, scale,
+                     accumulate, space.data, space.bytes, d.stream);
+        });
+    });
+}
+
+// (x, y, weight, bias, residual, sum, mean, rstd, eps)
+PyObject* layer_norm_forward(PyObject* self, PyObject* const* args, Py_ssize_t count)
+{
+    return on_device<&pxh_layer_norm_forward, 9>(self, args, count, [](PyObject* const* a, const Device& d, auto f) {
+        const Rows x = d.rows(a[0]), y = d.rows(a[1]), residual = d.rows(a[4]), sum = d.rows(a[5]);
+        if (!x.given || !y.given) throw NotHere{};
+        y.like(x, x.type);
+        residual.like(x, x.type);
+        sum.like(x, x.type);
+        int type, bias_type;
+        void* const weight = d.weights(a[2], x.width, type);
+        void* const bias = a[3] == Py_None ? nullptr : d.weights(a[3], x.width, bias_type);
+        if (bias && bias_type != type) throw NotHere{};
+        float* const mean = d.floats(a[6], x.rows);
+        float* const rstd = d.floats(a[7], x.rows);
+        const float eps = argument<float>(a[8]);
+        const int width = fits(x.width);
+        return status([&] {
+            return f(x.data, residual.data, sum.data, weight, bias, y.data, mean, rstd, x.type, type, x.rows, width, x.stride, stride_of(residual),
+                     stride_of(sum), y.stride, eps, d.stream);
+        });
+    });
+}
+
+// (dy, h, weight, mean, rstd, dx, dw, db, dsum, accumulate, workspace)
+PyObject* layer_norm_backward(PyObject* self, PyObject* const* args, Py_ssize_t count)
+{
+    return on_device<&pxh_layer_norm_backward, 11>(self, args, count, [](PyObject* const* a, const Device& d, auto f) {
+        const Rows dy = d.rows(a[0]), h = d.rows(a[1]), dx = d.rows(a[5]), dsum = d.rows(a[8]);
+        if (!dy.given || !h.given || !dx.given) throw NotHere{};
+        h.like(dy, dy.type);
+        dx.like(dy, dy.type);
+        dsum.like(dy, dy.type);
+        int type;
+        void* const weight = d.weights(a[2], dy.width, type);
+        float* const mean = d.floats(a[3], dy.rows);
+        float* const rstd = d.floats(a[4], dy.rows);
+        float* const dw = d.floats(a[6], dy.width);
+        float* const db = d.floats(a[7], dy.width);
+        const int accumulate = argument<int>(a[9]), width = fits(dy.width);
+        const Space space = d.space(a[10]);
+        return status([&] {
+            return f(dy.data, h.data, weight, mean, rstd, dsum.data, dx.data, dw, db, dy.type, type, dy.rows, width, dy.stride, h.stride,
+                     stride_of(dsum), dx.stride, accumulate, space.data, space.bytes, d.stream);
+        });
+    });
+}
+
 #define FUNCTION(name) \
     PyMethodDef { "pxh_" #name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&name)), METH_FASTCALL, nullptr }
 
 PyMethodDef functions[] = { FUNCTION(rms_norm_forward), FUNCTION(rms_norm_backward), FUNCTION(token_logprobs_forward),
                             FUNCTION(token_logprobs_backward), FUNCTION(token_logprobs_forward_train) };
+
+PyMethodDef layers[] = { FUNCTION(embedding_forward), FUNCTION(embedding_backward), FUNCTION(layer_norm_forward), FUNCTION(layer_norm_backward) };
 
 // bind_function(name, address) -> the callable that takes a Python function's own arguments and the stream, or None
 PyObject* bind_function(PyObject*, PyObject* args)
@@ -388,20 +527,26 @@ PyObject* bind_function(PyObject*, PyObject* args)
     if (!PyArg_ParseTuple(args, "sO!", &name, &PyLong_Type, &address)) return nullptr;
     for (PyMethodDef& def: functions)
         if (std::string_view(def.ml_name) == name) return PyCFunction_New(&def, address);
+    for (PyMethodDef& def: layers)
+        if (std::string_view(def.ml_name) == name) return PyCFunction_New(&def, address);
     Py_RETURN_NONE;
 }
 
-// functions() -> their names
-PyObject* function_names(PyObject*, PyObject*)
+template<size_t N>
+PyObject* names_of(const PyMethodDef (&defs)[N])
 {
     PyObject* list = PyList_New(0);
-    for (const PyMethodDef& def: functions) {
+    for (const PyMethodDef& def: defs) {
         PyObject* s = list ? PyUnicode_FromString(def.ml_name) : nullptr;
         if (!s || PyList_Append(list, s)) { Py_XDECREF(s); Py_XDECREF(list); return nullptr; }
         Py_DECREF(s);
     }
     return list;
 }
+
+// functions(), layers() -> their names
+PyObject* function_names(PyObject*, PyObject*) { return names_of(functions); }
+PyObject* layer_names(PyObject*, PyObject*) { return names_of(layers); }
 
 // bind(name, address) -> (callable, which arguments are tensors), or None for an entry point that is not made here
 PyObject* bind(PyObject*, PyObject* args)
@@ -433,6 +578,7 @@ PyObject* names(PyObject*, PyObject*)
 
 PyMethodDef methods[] = { { "bind", bind, METH_VARARGS, nullptr }, { "names", names, METH_NOARGS, nullptr },
                           { "bind_function", bind_function, METH_VARARGS, nullptr }, { "functions", function_names, METH_NOARGS, nullptr },
+                          { "layers", layer_names, METH_NOARGS, nullptr },
                           { nullptr, nullptr, 0, nullptr } };
 PyModuleDef module = { PyModuleDef_HEAD_INIT, "_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr };
 

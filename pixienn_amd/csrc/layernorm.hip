@@ -1,0 +1,503 @@
+// Layer norm over rows, with the residual's addition in front of it, and its gradients.
+#include "rows.h"
+#include "stream.h"
+
+namespace pxh {
+namespace {
+
+// ---------------------------------------------------------------- forward
+//   h = x + residual (rounded as it is kept);  mean = mean(h);  rstd = 1 / sqrt(mean((h - mean)^2) + eps);  y = (h - mean) * rstd * weight + bias
+struct LayerNormArgs {
+    const void* x;
+    const void* residual;
+    void* sum;
+    const void* weight;
+    const void* bias;
+    void* y;
+    float* mean;
+    float* rstd;
+    long long rows, x_stride, residual_stride, sum_stride, y_stride;
+    int width;
+    float eps;
+    bool weight_f32;
+};
+
+// A row is walked in vectors, lane by lane.  K vectors a lane stay in registers from the sum over the squares of what is left
+// without the mean (not a difference of two sums, which loses what a large mean leaves of the digits) to the result.  K == 0: a row of
+// any width, which is read three times.
+template<int T, int LANES, int K, bool NT>
+__global__ __launch_bounds__(LANES > kWave ? LANES : kBlock) void layer_norm_kernel(LayerNormArgs a)
+{
+    constexpr int V = kVec<T>;
+    constexpr int kRows = LANES > kWave ? 1 : kBlock / kWave;       // rows per workgroup, a wave each if several
+    constexpr int kKept = K ? K : 1;
+    __shared__ float slots[LANES > kWave ? LANES / kWave : 1];
+    const int lane = threadIdx.x % LANES;
+    const long long row = static_cast<long long>(blockIdx.x) * kRows + threadIdx.x / LANES;
+    if (row >= a.rows) return;                                       // whole waves, and only where nothing is waited for
+    const char* x = row_of<T>(a.x, row, a.x_stride);
+    const char* residual = a.residual ? row_of<T>(a.residual, row, a.residual_stride) : nullptr;
+    char* sum = a.sum ? row_of<T>(a.sum, row, a.sum_stride) : nullptr;
+    char* y = row_of<T>(a.y, row, a.y_stride);
+    const int n = a.width;
+    const int steps = K ? K : (n + LANES * V - 1) / (LANES * V);
+
+    Raw<T, V> kept[kKept];
+    // h of step s
+    const auto ask = [&](int e, bool add) {
+        Raw<T, V> h = load_row<T, V, NT>(x, e, n);
+        if (add) {
+            float p[V], q[V];
+            h.get(p);
+            load_row<T, V, NT>(residual, e, n).get(q);
+#pragma unroll
+            for (int k = 0; k < V; ++k) p[k] += q[k];
+            h.set(p);
+        }
+        return h;
+    };
+    if constexpr (K > 0) {
+        Raw<T, V> more[K];
+#pragma unroll
+        for (int s = 0; s < K; ++s) {
+            const int e = (s * LANES + lane) * V;
+            kept[s] = more[s] = Raw<T, V>{};
+            if (e >= n) continue;
+            kept[s] = load_row<T, V, NT>(x, e, n);
+            if (residual) more[s] = load_row<T, V, NT>(residual, e, n);
+        }
+        if (residual) {
+#pragma unroll
+            for (int s = 0; s < K; ++s) {
+                const int e = (s * LANES + lane) * V;
+                float p[V], q[V];
+                kept[s].get(p);
+                more[s].get(q);
+#pragma unroll
+                for (int k = 0; k < V; ++k) p[k] += q[k];
+                kept[s].set(p);
+                if (sum && e < n) store_row<T, V, NT>(sum, e, n, kept[s]);
+            }
+        }
+    }
+    float total = 0.0f;
+#pragma unroll kKept
+    for (int s = 0; s < steps; ++s) {
+        const int e = (s * LANES + lane) * V;
+        if (e >= n) break;
+        if constexpr (K == 0) {
+            kept[0] = ask(e, residual != nullptr);
+            if (sum) store_row<T, V, NT>(sum, e, n, kept[0]);
+        }
+        float h[V];
+        kept[K ? s : 0].get(h);
+#pragma unroll
+        for (int k = 0; k < V; ++k) total += h[k];                   // zeros behind the row's last value
+    }
+    const float mean = group_sum<LANES>(total, slots) / static_cast<float>(n);
+    float squares = 0.0f;
+#pragma unroll kKept
+    for (int s = 0; s < steps; ++s) {
+        const int e = (s * LANES + lane) * V;
+        if (e >= n) break;
+        // x may have been overwritten by the sum, which is what is wanted
+        if constexpr (K == 0) kept[0] = sum ? load_row<T, V, NT>(sum, e, n) : ask(e, residual != nullptr);
+        float h[V];
+        kept[K ? s : 0].get(h);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const float d = e + V <= n || e + k < n ? h[k] - mean : 0.0f;
+            squares = fmaf(d, d, squares);
+        }
+    }
+    const float rstd = 1.0f / sqrtf(group_sum<LANES>(squares, slots) / static_cast<float>(n) + a.eps);
+    if (lane == 0) {
+        if (a.mean) a.mean[row] = mean;
+        if (a.rstd) a.rstd[row] = rstd;
+    }
+#pragma unroll kKept
+    for (int s = 0; s < steps; ++s) {
+        const int e = (s * LANES + lane) * V;
+        if (e >= n) break;
+        if constexpr (K == 0) kept[0] = sum ? load_row<T, V, NT>(sum, e, n) : ask(e, residual != nullptr);
+        float h[V], w[V], b[V] = {};
+        kept[K ? s : 0].get(h);
+        weights_at<T, V>(a.weight, a.weight_f32, e, n, w);
+        if (a.bias) weights_at<T, V>(a.bias, a.weight_f32, e, n, b);
+#pragma unroll
+        for (int k = 0; k < V; ++k) h[k] = fmaf((h[k] - mean) * rstd, w[k], b[k]);
+        Raw<T, V> r;
+        r.set(h);
+        store_row<T, V, NT>(y, e, n, r);
+    }
+}
+
+template<int T, int LANES, int K, bool NT>
+int launch_norm(const LayerNormArgs& a, hipStream_t s)
+{
+    constexpr int kRows = LANES > kWave ? 1 : kBlock / kWave;
+    for (long long done = 0; done < a.rows; done += kLaunchRows) {
+        LayerNormArgs part = a;
+        part.x = row_of<T>(a.x, done, a.x_stride);
+        part.residual = a.residual ? row_of<T>(a.residual, done, a.residual_stride) : nullptr;
+        part.sum = a.sum ? row_of<T>(a.sum, done, a.sum_stride) : nullptr;
+        part.y = row_of<T>(a.y, done, a.y_stride);
+        part.mean = a.mean ? a.mean + done : nullptr;
+        part.rstd = a.rstd ? a.rstd + done : nullptr;
+        part.rows = a.rows - done < kLaunchRows ? a.rows - done : kLaunchRows;
+        const dim3 grid(grid_for(part.rows, kRows)), block(kRows * LANES);
+        hipLaunchKernelGGL((layer_norm_kernel<T, LANES, K, NT>), grid, block, 0, s, part);
+        if (int rc = check_launch("pxh_layer_norm_forward")) return rc;
+    }
+    return PXH_OK;
+}
+
+// Lanes and vectors a lane by the vectors of a row, few vectors while the row is short.
+template<int T, bool NT>
+int norm_forward(const LayerNormArgs& a, hipStream_t s)
+{
+    const int vectors = (a.width + kVec<T> - 1) / kVec<T>;
+    if (vectors <= 64) return launch_norm<T, 64, 1, NT>(a, s);
+    if (vectors <= 128) return launch_norm<T, 128, 1, NT>(a, s);
+    if (vectors <= 256) return launch_norm<T, 256, 1, NT>(a, s);
+    if (vectors <= 512) return launch_norm<T, 256, 2, NT>(a, s);
+    if (vectors <= 1024) return launch_norm<T, 512, 2, NT>(a, s);
+    if (vectors <= 2048) return launch_norm<T, 1024, 2, NT>(a, s);
+    if (vectors <= 4096) return launch_norm<T, 1024, 4, NT>(a, s);
+    return launch_norm<T, 1024, 0, false>(a, s);        // read several times: through the caches
+}
+
+// ---------------------------------------------------------------- backward
+//   g = dy * weight;  xhat = (h - mean) * rstd;  dx = rstd * (g - mean(g) - xhat * mean(g * xhat)) + dsum
+//   dw (+)= sum over the rows of dy * xhat;  db (+)= sum of dy
+struct LayerNormBackwardArgs {
+    const void* dy;
+    const void* h;
+    const void* weight;
+    const float* mean;
+    const float* rstd;
+    const void* dsum;
+    void* dx;
+    float* partial;         // [workers][2][width]: of dw, of db
+    long long rows, dy_stride, h_stride, dsum_stride, dx_stride;
+    int width;
+    bool weight_f32, bias;
+};
+
+// Two sums over a workgroup, the same in every lane.  `slots` holds two places, used in turn from row to row: no wave is more
+// than one row ahead of another.
+template<int LANES>
+__device__ __forceinline__ float2 two_sums(float a, float b, float2* slot)
+{
+    a = wave_sum_by_rows(a);
+    b = wave_sum_by_rows(b);
+    if constexpr (LANES > kWave) {
+        if ((threadIdx.x & (kWave - 1)) == 0) slot[threadIdx.x / kWave] = make_float2(a, b);
+        __syncthreads();
+        float2 v = slot[0];
+#pragma unroll
+        for (int k = 1; k < LANES / kWave; ++k) {
+            v.x += slot[k].x;
+            v.y += slot[k].y;
+        }
+        return v;
+    }
+    return make_float2(a, b);
+}
+
+// dx of every row, and the part of dw and db that this worker's rows give: a worker (LANES lanes) takes every workers-th row, and
+// asks for the next one before it waits for the sums over this one.
+template<int T, int LANES, int K, bool NT>
+__global__ __launch_bounds__(LANES > kWave ? LANES : kBlock) void layer_norm_backward_kernel(LayerNormBackwardArgs a, int workers)
+{
+    constexpr int V = kVec<T>;
+    constexpr int kPer = LANES > kWave ? 1 : kBlock / kWave;
+    constexpr int kWaves = LANES / kWave;
+    constexpr bool kAhead = K <= 1;
+    __shared__ float2 slots[2][kWaves];
+    const int lane = threadIdx.x % LANES;
+    const int worker = blockIdx.x * kPer + threadIdx.x / LANES;
+    if (worker >= workers) return;              // single waves, which wait for nobody
+    const int n = a.width;
+    float w[kAhead ? K : 1][V], dw[K][V], db[K][V];
+#pragma unroll
+    for (int s = 0; s < K; ++s) {
+        const int e = (s * LANES + lane) * V;
+#pragma unroll
+        for (int k = 0; k < V; ++k) dw[s][k] = db[s][k] = 0.0f;
+        if (kAhead) {
+#pragma unroll
+            for (int k = 0; k < V; ++k) w[s][k] = 0.0f;
+            if (e < n) weights_at<T, V>(a.weight, a.weight_f32, e, n, w[s]);
+        }
+    }
+    struct Row {
+        Raw<T, V> g[K], h[K], more[K];
+        float mean, rstd;
+    };
+    const auto ask = [&](long long row, Row& r) {
+        if (row >= a.rows) return;
+        const char* dy = row_of<T>(a.dy, row, a.dy_stride);
+        const char* h = row_of<T>(a.h, row, a.h_stride);
+        r.mean = a.mean[row];
+        r.rstd = a.rstd[row];
+#pragma unroll
+        for (int s = 0; s < K; ++s) {
+            const int e = (s * LANES + lane) * V;
+            if (e >= n) break;
+            r.g[s] = load_row<T, V, NT>(dy, e, n);
+            r.h[s] = load_row<T, V, NT>(h, e, n);
+            if (kAhead && a.dsum) r.more[s] = load_row<T, V, NT>(row_of<T>(a.dsum, row, a.dsum_stride), e, n);
+        }
+    };
+    Row next;
+    if (kAhead) ask(worker, next);
+    int turn = 0;
+    for (long long row = worker; row < a.rows; row += workers) {
+        if (!kAhead) ask(row, next);
+        const Row r = next;
+        float plain = 0.0f, dot = 0.0f;
+#pragma unroll
+        for (int s = 0; s < K; ++s) {
+            const int e = (s * LANES + lane) * V;
+            if (e >= n) break;
+            float g[V], x[V], u[V];
+            r.g[s].get(g);
+            r.h[s].get(x);
+            if (!kAhead) weights_at<T, V>(a.weight, a.weight_f32, e, n, u);
+            // behind the row's last value g is zero
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const float xhat = (x[k] - r.mean) * r.rstd;
+                dw[s][k] = fmaf(g[k], xhat, dw[s][k]);
+                db[s][k] += g[k];
+                const float gw = g[k] * (kAhead ? w[kAhead ? s : 0][k] : u[k]);
+                plain += gw;
+                dot = fmaf(gw, xhat, dot);
+            }
+        }
+        if (kAhead) ask(row + workers, next);
+        const float2 sums = two_sums<LANES>(plain, dot, slots[turn]);
+        turn ^= 1;
+        const float c0 = sums.x / static_cast<float>(n), c1 = r.rstd * (sums.y / static_cast<float>(n));
+#pragma unroll
+        for (int s = 0; s < K; ++s) {
+            const int e = (s * LANES + lane) * V;
+            if (e >= n) break;
+            float g[V], x[V], u[V], more[V] = {};
+            r.g[s].get(g);
+            r.h[s].get(x);
+            if (!kAhead) weights_at<T, V>(a.weight, a.weight_f32, e, n, u);
+            if (a.dsum) {
+                if (kAhead) r.more[s].get(more);
+                else load_row<T, V>(row_of<T>(a.dsum, row, a.dsum_stride), e, n).get(more);
+            }
+#pragma unroll
+            for (int k = 0; k < V; ++k)
+                g[k] = fmaf(r.rstd, (g[k] * (kAhead ? w[kAhead ? s : 0][k] : u[k]) - c0) - (x[k] - r.mean) * c1, more[k]);
+            Raw<T, V> out;
+            out.set(g);
+            store_row<T, V, NT>(row_of<T>(a.dx, row, a.dx_stride), e, n, out);
+        }
+    }
+    float* const partial = a.partial + static_cast<size_t>(worker) * 2 * n;
+#pragma unroll
+    for (int s = 0; s < K; ++s) {
+        const int e = (s * LANES + lane) * V;
+        Raw<PXH_F32, 4> part;
+#pragma unroll
+        for (int q = 0; q < V; q += 4) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) part.w[k] = __float_as_uint(dw[s][q + k]);
+            store_row<PXH_F32, 4>(partial, e + q, n, part);
+            if (a.bias) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) part.w[k] = __float_as_uint(db[s][q + k]);
+                store_row<PXH_F32, 4>(partial + n, e + q, n, part);
+            }
+        }
+    }
+}
+
+// Rows of any width: dx alone, the row is read twice.
+template<int T>
+__global__ __launch_bounds__(1024) void layer_norm_backward_wide_kernel(LayerNormBackwardArgs a, long long first)
+{
+    constexpr int V = kVec<T>;
+    __shared__ float2 slot[1024 / kWave];
+    const int n = a.width;
+    const long long row = first + blockIdx.x;
+    const char* dy = row_of<T>(a.dy, row, a.dy_stride);
+    const char* h = row_of<T>(a.h, row, a.h_stride);
+    const float mean = a.mean[row], rstd = a.rstd[row];
+    float plain = 0.0f, dot = 0.0f;
+    for (int e = threadIdx.x * V; e < n; e += 1024 * V) {
+        float g[V], x[V], w[V];
+        load_row<T, V>(dy, e, n).get(g);
+        load_row<T, V>(h, e, n).get(x);
+        weights_at<T, V>(a.weight, a.weight_f32, e, n, w);
+#pragma unroll
+        for (int k = 0; k < V; ++k) {
+            const float gw = g[k] * w[k];
+            plain += gw;
+            dot = fmaf(gw, (x[k] - mean) * rstd, dot);
+        }
+    }
+    const float2 sums = two_sums<1024>(plain, dot, slot);
+    const float c0 = sums.x / static_cast<float>(n), c1 = rstd * (sums.y / static_cast<float>(n));
+    for (int e = threadIdx.x * V; e < n; e += 1024 * V) {
+        float g[V], x[V], w[V], more[V] = {};
+        load_row<T, V>(dy, e, n).get(g);
+        load_row<T, V>(h, e, n).get(x);
+        weights_at<T, V>(a.weight, a.weight_f32, e, n, w);
+        if (a.dsum) load_row<T, V>(row_of<T>(a.dsum, row, a.dsum_stride), e, n).get(more);
+#pragma unroll
+        for (int k = 0; k < V; ++k) g[k] = fmaf(rstd, (g[k] * w[k] - c0) - (x[k] - mean) * c1, more[k]);
+        Raw<T, V> r;
+        r.set(g);
+        store_row<T, V>(row_of<T>(a.dx, row, a.dx_stride), e, n, r);
+    }
+}
+
+// ... and the parts of dw and db, one column to a lane, before dx (which may be dy itself) is written.
+template<int T>
+__global__ __launch_bounds__(kBlock) void layer_norm_wide_sums_kernel(LayerNormBackwardArgs a, int workers)
+{
+    const int e = blockIdx.x * kBlock + threadIdx.x;
+    if (e >= a.width) return;
+    float dw = 0.0f, db = 0.0f;
+    for (long long row = blockIdx.y; row < a.rows; row += workers) {
+        const float g = load_one<T>(row_of<T>(a.dy, row, a.dy_stride), e);
+        dw = fmaf(g, (load_one<T>(row_of<T>(a.h, row, a.h_stride), e) - a.mean[row]) * a.rstd[row], dw);
+        db += g;
+    }
+    float* const partial = a.partial + static_cast<size_t>(blockIdx.y) * 2 * a.width;
+    partial[e] = dw;
+    partial[a.width + e] = db;
+}
+
+// The sums of the workers' parts: blockIdx.y 0 for dw, 1 for db.
+__global__ __launch_bounds__(kColumnLanes) void layer_norm_sums_kernel(const float* partial, int workers, int width, float* dw, float* db,
+                                                                        int accumulate)
+{
+    __shared__ float sums[kColumnWaves][kWave];
+    const int column = blockIdx.x * kWave + threadIdx.x % kWave;
+    const size_t which = blockIdx.y;
+    const float all = sum_of_workers(partial + which * width, workers, static_cast<size_t>(width) * 2, column, column < width, sums);
+    float* const out = which ? db : dw;
+    if (threadIdx.x < kWave && column < width) out[column] = accumulate ? out[column] + all : all;
+}
+
+// Workers that share the rows of the backward pass, each with two rows of partial sums.
+constexpr int kWideWorkers = 32;
+int workers_for(long long rows, int width)
+{
+    const int most = width <= 2048 ? 1024 : width <= 32768 ? 256 : kWideWorkers;
+    return static_cast<int>(rows < most ? rows : most);
+}
+
+template<int T, int LANES, int K>
+int launch_backward(const LayerNormBackwardArgs& a, int workers, hipStream_t s)
+{
+    constexpr int kPer = LANES > kWave ? 1 : kBlock / kWave;
+    const dim3 grid(grid_for(workers, kPer)), block(LANES * kPer);
+    // past the caches where the tensors do not fit
+    const size_t bytes = static_cast<size_t>(a.rows) * static_cast<size_t>(a.width) * kSize<T> * (a.dsum ? 4 : 3);
+    if (bytes >= kStreamingBytes) hipLaunchKernelGGL((layer_norm_backward_kernel<T, LANES, K, true>), grid, block, 0, s, a, workers);
+    else hipLaunchKernelGGL((layer_norm_backward_kernel<T, LANES, K, false>), grid, block, 0, s, a, workers);
+    return check_launch("pxh_layer_norm_backward");
+}
+
+template<int T>
+int norm_backward(const LayerNormBackwardArgs& a, int& workers, hipStream_t s)
+{
+    const int vectors = (a.width + kVec<T> - 1) / kVec<T>;
+    if (vectors <= 64) return launch_backward<T, 64, 1>(a, workers, s);
+    if (vectors <= 128) return launch_backward<T, 128, 1>(a, workers, s);
+    if (vectors <= 256) return launch_backward<T, 256, 1>(a, workers, s);
+    if (vectors <= 512) return launch_backward<T, 512, 1>(a, workers, s);
+    if (vectors <= 1024) return launch_backward<T, 1024, 1>(a, workers, s);
+    if (vectors <= 2048) return launch_backward<T, 1024, 2>(a, workers, s);
+    if (workers > kWideWorkers) workers = kWideWorkers;
+    hipLaunchKernelGGL((layer_norm_wide_sums_kernel<T>), dim3(grid_for(a.width, kBlock), workers), dim3(kBlock), 0, s, a, workers);
+    if (int rc = check_launch("pxh_layer_norm_backward")) return rc;
+    for (long long done = 0; done < a.rows; done += kLaunchRows) {
+        const long long rows = a.rows - done < kLaunchRows ? a.rows - done : kLaunchRows;
+        hipLaunchKernelGGL((layer_norm_backward_wide_kernel<T>), dim3(static_cast<unsigned>(rows)), dim3(1024), 0, s, a, done);
+        if (int rc = check_launch("pxh_layer_norm_backward")) return rc;
+    }
+    return PXH_OK;
+}
+
+}  // namespace
+}  // namespace pxh
+
+using namespace pxh;
+
+extern "C" {
+
+int pxh_layer_norm_forward(const void* x, const void* residual, void* sum, const void* weight, const void* bias, void* y, float* mean,
+                           float* rstd, int type, int weight_type, long long rows, int width, long long x_stride,
+                           long long residual_stride, long long sum_stride, long long y_stride, float eps, void* stream)
+{
+    const char* who = "pxh_layer_norm_forward";
+    if (int rc = check_norm_rows(who, type, weight_type, rows, width)) return rc;
+    if (sum && !residual) return fail_invalid("%s: a sum without a residual", who);
+    if (!(eps >= 0.0f)) return fail_invalid("%s: eps %g", who, static_cast<double>(eps));
+    if (rows == 0) return PXH_OK;
+    if (!x || !weight || !y) return fail_invalid("%s: null pointer", who);
+    if (x_stride < width || y_stride < width || (residual && residual_stride < width) || (sum && sum_stride < width))
+        return fail_invalid("%s: rows of %d values that overlap", who, width);
+    const LayerNormArgs a{ x, residual, sum, weight, bias, y, mean, rstd, rows, x_stride, residual_stride, sum_stride, y_stride, width, eps,
+                           weight_type == PXH_F32 };
+    const size_t tensors = 2 + (residual != nullptr) + (sum != nullptr);
+    const bool past = static_cast<size_t>(rows) * static_cast<size_t>(width) * size_of(type) * tensors >= kStreamingBytes;
+    int rc = PXH_OK;
+    dispatch_type(type, [&]<int T>() { rc = past ? norm_forward<T, true>(a, as_stream(stream)) : norm_forward<T, false>(a, as_stream(stream)); });
+    return rc;
+}
+
+size_t pxh_layer_norm_workspace_bytes(long long rows, int width)
+{
+    if (rows <= 0 || width <= 0) return 0;
+    // the largest that any of the shapes up to this one takes
+    size_t most = 0;
+    for (int w: { 2048, 32768, width }) {
+        const int here = width < w ? width : w;
+        const size_t floats = static_cast<size_t>(workers_for(rows, here)) * static_cast<size_t>(here) * 2;
+        if (floats > most) most = floats;
+    }
+    return most * sizeof(float);
+}
+
+int pxh_layer_norm_backward(const void* dy, const void* h, const void* weight, const float* mean, const float* rstd, const void* dsum,
+                            void* dx, float* dw, float* db, int type, int weight_type, long long rows, int width, long long dy_stride,
+                            long long h_stride, long long dsum_stride, long long dx_stride, int accumulate, void* workspace,
+                            size_t workspace_bytes, void* stream)
+{
+    const char* who = "pxh_layer_norm_backward";
+    if (int rc = check_norm_rows(who, type, weight_type, rows, width)) return rc;
+    if (!dw) return fail_invalid("%s: null pointer", who);
+    hipStream_t s = as_stream(stream);
+    int workers = 0;
+    void* ws = nullptr;
+    if (rows > 0) {
+        if (!dy || !h || !weight || !mean || !rstd || !dx) return fail_invalid("%s: null pointer", who);
+        if (dy_stride < width || h_stride < width || dx_stride < width || (dsum && dsum_stride < width))
+            return fail_invalid("%s: rows of %d values that overlap", who, width);
+        workers = workers_for(rows, width);
+        if (int rc = resolve_workspace(workspace, workspace_bytes, pxh_layer_norm_workspace_bytes(rows, width), &ws, s)) return rc;
+    }
+    const LayerNormBackwardArgs a{ dy, h, weight, mean, rstd, dsum, dx, static_cast<float*>(ws), rows, dy_stride, h_stride, dsum_stride,
+                                   dx_stride, width, weight_type == PXH_F32, db != nullptr };
+    int rc = PXH_OK;
+    if (rows > 0) dispatch_type(type, [&]<int T>() { rc = norm_backward<T>(a, workers, s); });
+    if (rc) return rc;
+    // without rows the sums over them are zero
+    if (workers == 0 && accumulate) return PXH_OK;
+    hipLaunchKernelGGL(layer_norm_sums_kernel, dim3(grid_for(width, kWave), db ? 2 : 1), dim3(kColumnLanes), 0, s, a.partial, workers, width, dw,
+                       db, accumulate);
+    return check_launch(who);
+}
+
+}

@@ -1,6 +1,6 @@
 // Root-mean-square norm over rows, with the residual's addition in front of it and 8-bit results, and its gradients.
+#include "rows.h"
 #include "stream.h"
-#include "typed.h"
 
 namespace pxh {
 namespace {
@@ -19,38 +19,6 @@ struct NormArgs {
     int width, group;
     float eps;
 };
-
-// Rows of one launch: a grid has fewer than 2^32 work items.
-constexpr long long kLaunchRows = 1 << 21;
-
-template<int T>
-__host__ __device__ __forceinline__ const char* row_of(const void* p, long long row, long long stride)
-{
-    return static_cast<const char*>(p) + row * stride * kSize<T>;
-}
-
-template<int T>
-__host__ __device__ __forceinline__ char* row_of(void* p, long long row, long long stride)
-{
-    return static_cast<char*>(p) + row * stride * kSize<T>;
-}
-
-// V weights from column e on; zeros behind the last one.
-template<int T, int V>
-__device__ __forceinline__ void weights_at(const void* weight, bool f32, int e, int width, float (&w)[V])
-{
-    if (f32 && T != PXH_F32) {
-#pragma unroll
-        for (int q = 0; q < V; q += 4) {
-            float part[4];
-            load_row<PXH_F32, 4>(weight, e + q, width).get(part);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) w[q + k] = part[k];
-        }
-    } else {
-        load_row<T, V>(weight, e, width).get(w);
-    }
-}
 
 // The largest value among the lanes that hold one group of 128 values: 16 lanes of 8 values or 32 of 4.
 template<int V>
@@ -473,31 +441,12 @@ __global__ __launch_bounds__(kBlock) void rms_norm_wide_dw_kernel(NormBackwardAr
 }
 
 // dw[column] (+)= the sum of the workers' parts: 64 columns to a workgroup, whose waves share the workers.
-__global__ __launch_bounds__(1024) void rms_norm_dw_kernel(const float* partial, int workers, int width, float* dw, int accumulate)
+__global__ __launch_bounds__(kColumnLanes) void rms_norm_dw_kernel(const float* partial, int workers, int width, float* dw, int accumulate)
 {
-    constexpr int kWaves = 16, kAhead = 8;
-    __shared__ float sums[kWaves][kWave];
-    const int column = blockIdx.x * kWave + threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    float sum = 0.0f;
-    if (column < width) {
-        int w = wave;
-        for (; w + (kAhead - 1) * kWaves < workers; w += kAhead * kWaves) {
-            float v[kAhead];
-#pragma unroll
-            for (int k = 0; k < kAhead; ++k) v[k] = partial[static_cast<size_t>(w + k * kWaves) * width + column];
-#pragma unroll
-            for (int k = 0; k < kAhead; ++k) sum += v[k];
-        }
-        for (; w < workers; w += kWaves) sum += partial[static_cast<size_t>(w) * width + column];
-    }
-    sums[wave][threadIdx.x % kWave] = sum;
-    __syncthreads();
-    if (wave == 0 && column < width) {
-        float all = 0.0f;
-#pragma unroll
-        for (int k = 0; k < kWaves; ++k) all += sums[k][threadIdx.x];
-        dw[column] = accumulate ? dw[column] + all : all;
-    }
+    __shared__ float sums[kColumnWaves][kWave];
+    const int column = blockIdx.x * kWave + threadIdx.x % kWave;
+    const float all = sum_of_workers(partial, workers, width, column, column < width, sums);
+    if (threadIdx.x < kWave && column < width) dw[column] = accumulate ? dw[column] + all : all;
 }
 
 // Workers that share the rows of the backward pass, each with a row of partial sums: a workgroup as wide as a row for each of 256 compute
@@ -544,17 +493,6 @@ int norm_backward(const NormBackwardArgs& a, int& workers, hipStream_t s)
     return PXH_OK;
 }
 
-// What the two entry points refuse alike.
-int check_rows(const char* who, int type, int weight_type, long long rows, int width)
-{
-    if (type != PXH_F32 && type != PXH_BF16 && type != PXH_F16) return fail_invalid("%s: type %d is not fp32, bf16 or half", who, type);
-    if (weight_type != type && weight_type != PXH_F32)
-        return fail_invalid("%s: the weights are of the tensors' type or fp32 (got type %d)", who, weight_type);
-    if (rows < 0 || rows > 0x7fffffffll) return fail_invalid("%s: %lld rows", who, rows);
-    if (width <= 0 || width > 1 << 30) return fail_invalid("%s: rows of %d values", who, width);
-    return PXH_OK;
-}
-
 }  // namespace
 }  // namespace pxh
 
@@ -567,7 +505,7 @@ int pxh_rms_norm_forward(const void* x, const void* residual, void* sum, const v
                          long long residual_stride, long long sum_stride, long long y_stride, int group, float eps, void* stream)
 {
     const char* who = "pxh_rms_norm_forward";
-    if (int rc = check_rows(who, type, weight_type, rows, width)) return rc;
+    if (int rc = check_norm_rows(who, type, weight_type, rows, width)) return rc;
     const bool eight = y_type == PXH_E4M3;
     if (!eight && y_type != type) return fail_invalid("%s: y is of the type of x or e4m3 (got type %d)", who, y_type);
     if (group != 0 && group != 128) return fail_invalid("%s: a scale for 128 values or, with 0, for a row (got %d)", who, group);
@@ -608,7 +546,7 @@ int pxh_rms_norm_backward(const void* dy, const void* h, const void* weight, con
                           size_t workspace_bytes, void* stream)
 {
     const char* who = "pxh_rms_norm_backward";
-    if (int rc = check_rows(who, type, weight_type, rows, width)) return rc;
+    if (int rc = check_norm_rows(who, type, weight_type, rows, width)) return rc;
     if (!dw) return fail_invalid("%s: null pointer", who);
     hipStream_t s = as_stream(stream);
     if (rows > 0) {
@@ -627,7 +565,7 @@ int pxh_rms_norm_backward(const void* dy, const void* h, const void* weight, con
     if (rc) return rc;
     // without rows the sum over them is zero
     if (workers == 0 && accumulate) return PXH_OK;
-    hipLaunchKernelGGL(rms_norm_dw_kernel, dim3(grid_for(width, kWave)), dim3(1024), 0, s, a.partial, workers, width, dw, accumulate);
+    hipLaunchKernelGGL(rms_norm_dw_kernel, dim3(grid_for(width, kWave)), dim3(kColumnLanes), 0, s, a.partial, workers, width, dw, accumulate);
     return check_launch(who);
 }
 

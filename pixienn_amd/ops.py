@@ -884,6 +884,119 @@ def adamw_states(ws, bits=8):
     return states
 
 
+def _on_device(**tensors):
+    """The tensors of a call lie on the current device, on whose stream its kernels run."""
+    here = _current_device()
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            _chk(t, getattr(t, "dtype", None), name)
+        if t.get_device() != here:
+            raise PxError("%s lies on %s and the current device is cuda:%d" % (name, t.device, here))
+
+
+def _layer(name, *args):
+    """_made() for the calls that also look at the tensors' device."""
+    if not capi.layers:
+        capi.bind_calls()
+    try:
+        here = _current_device()
+        rc = capi.layers[name](*args, here, _raw_stream(here))
+    except RuntimeError:              # without a device: what is wrong with the tensors comes first
+        return False
+    if rc:
+        raise PxError("%s failed (status %d): %s" % (name, rc, capi.last_error()))
+    return rc == 0
+
+
+def _tokens(tokens, rows, name="tokens"):
+    """(address, whether of 64 bits) of the rows' tokens."""
+    if tokens is None:
+        raise PxError("%s is required" % name)
+    wide = getattr(tokens, "dtype", None) is torch.int64
+    _vector(tokens, name, rows, torch.int64 if wide else torch.int32)
+    return tokens.data_ptr(), int(wide)
+
+
+def embedding_forward(table, tokens, y, scale=1.0):
+    """y[r] = scale * table[tokens[r]] (tokens int32 or int64, of y's leading dimensions; zeros for one outside the table)."""
+    if _layer("pxh_embedding_forward", table, tokens, y, scale):
+        return y
+    vocab, width, stride = _rows(table, "table")
+    kind = _type(table, "table")
+    rows, y_width, y_stride = _rows(y, "y")
+    if y_width != width or y.dtype is not table.dtype:
+        raise PxError("y must be %s in rows of %d values (got %s of %s)" % (table.dtype, width, y.dtype, tuple(y.shape)))
+    at, wide = _tokens(tokens, rows)
+    _on_device(table=table, tokens=tokens, y=y)
+    call("pxh_embedding_forward", ptr(table), at, ptr(y), kind, wide, rows, vocab, width, stride, y_stride, float(scale), _stream())
+    return y
+
+
+def embedding_workspace_bytes(rows, width):
+    return int(capi.load().pxh_embedding_workspace_bytes(rows, width))
+
+
+def embedding_backward(dy, tokens, d, scale=1.0, accumulate=False, workspace=None):
+    """The gradient of embedding_forward's table: d[v] = scale * the sum of dy's rows of token v, overwritten or added to; d is of
+    dy's type or fp32.  In a fixed order: the same call gives the same bits."""
+    if _layer("pxh_embedding_backward", dy, tokens, d, scale, int(accumulate), workspace):
+        return d
+    rows, width, stride = _rows(dy, "dy")
+    kind = _type(dy, "dy")
+    vocab, d_width, d_stride = _rows(d, "d")
+    if d_width != width or d.dtype not in (dy.dtype, _F32):
+        raise PxError("d must be %s or fp32 in rows of %d values (got %s of %s)" % (dy.dtype, width, d.dtype, tuple(d.shape)))
+    at, wide = _tokens(tokens, rows)
+    _on_device(dy=dy, tokens=tokens, d=d, workspace=workspace)
+    call("pxh_embedding_backward", ptr(dy), at, ptr(d), kind, _type(d, "d"), wide, rows, vocab, width, stride, d_stride, float(scale),
+         int(bool(accumulate)), *_space(workspace), _stream())
+    return d
+
+
+def layer_norm_forward(x, y, weight, bias=None, residual=None, sum=None, mean=None, rstd=None, eps=1e-5):
+    """y = (h - mean) / sqrt(variance + eps) * weight + bias over the last dimension, h = x + residual (rounded to x's type; kept in
+    `sum`).  mean and rstd [rows] are what the backward pass needs."""
+    if _layer("pxh_layer_norm_forward", x, y, weight, bias, residual, sum, mean, rstd, eps):
+        return y
+    rows, width, x_stride = _rows(x, "x")
+    kind = _type(x, "x")
+    y_stride = _like(_tensor(y), "y", x.shape, x.dtype)
+    _vector(_tensor(weight), "weight", width, None)
+    weight_kind = _type(weight, "weight")
+    _vector(bias, "bias", width, weight.dtype)
+    _per_row(rows, mean=mean, rstd=rstd)
+    strides = _like(residual, "residual", x.shape, x.dtype), _like(sum, "sum", x.shape, x.dtype)
+    _on_device(x=x, y=y, weight=weight, bias=bias, residual=residual, sum=sum, mean=mean, rstd=rstd)
+    call("pxh_layer_norm_forward", ptr(x), ptr(residual), ptr(sum), ptr(weight), ptr(bias), ptr(y), ptr(mean), ptr(rstd), kind, weight_kind,
+         rows, width, x_stride, *strides, y_stride, float(eps), _stream())
+    return y
+
+
+def layer_norm_workspace_bytes(rows, width):
+    return int(capi.load().pxh_layer_norm_workspace_bytes(rows, width))
+
+
+def layer_norm_backward(dy, h, weight, mean, rstd, dx, dw, db=None, dsum=None, accumulate=False, workspace=None):
+    """The gradients of layer_norm_forward from h (its `sum`, or x without a residual), its mean and rstd: dx of x and residual
+    alike, with dsum, what arrives along the residual stream, added; dw and db (fp32) overwritten or added to."""
+    if _layer("pxh_layer_norm_backward", dy, h, weight, mean, rstd, dx, dw, db, dsum, int(accumulate), workspace):
+        return dx
+    rows, width, dy_stride = _rows(dy, "dy")
+    kind = _type(dy, "dy")
+    _vector(_tensor(weight), "weight", width, None)
+    weight_kind = _type(weight, "weight")
+    _per_row(rows, mean=mean, rstd=rstd)
+    for name, t in (("dw", dw), ("db", db)):
+        _vector(t, name, width)
+    strides = [_like(t, name, dy.shape, dy.dtype) for name, t in (("h", h), ("dsum", dsum), ("dx", dx))]
+    _on_device(dy=dy, h=h, weight=weight, mean=mean, rstd=rstd, dx=dx, dw=dw, db=db, dsum=dsum, workspace=workspace)
+    call("pxh_layer_norm_backward", ptr(dy), ptr(h), ptr(weight), ptr(mean), ptr(rstd), ptr(dsum), ptr(dx), ptr(dw), ptr(db), kind,
+         weight_kind, rows, width, dy_stride, *strides, int(bool(accumulate)), *_space(workspace), _stream())
+    return dx
+
+
 DETECTION_DTYPE = workloads.DETECTION_DTYPE
 
 
