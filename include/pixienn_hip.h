@@ -711,6 +711,46 @@ int pxh_layer_norm_backward(const void* dy, const void* h, const void* weight, c
                             long long dy_stride, long long h_stride, long long dsum_stride, long long dx_stride, int accumulate,
                             void* workspace, size_t workspace_bytes, void* stream);
 
+/* A gated linear recurrence over sequences of tokens, channel by channel:
+ *   z = 1 / (1 + exp(-update));  h[t] = h[t - 1] + z * (x - h[t - 1]);  y = h, or with a gate (nullable) h * gate / (1 + exp(-gate))
+ * x, update, gate and y are [rows][width] of `type`; h is fp32 throughout.  The rows are the tokens of `sequences` sequences, one behind
+ * the other: starts[sequences + 1] (device, int32, not descending) says where each begins and the last one ends, or, where it is NULL,
+ * all are of rows / sequences tokens.  Rows in front of the first and behind the last sequence are not written.  Where starts descends
+ * or leaves the rows, the results are unspecified, but nothing beyond the tensors is touched.
+ * state, final (nullable, fp32 [slot_count][width]): a sequence begins with its row of state (zeros without), and leaves what h is behind
+ * its last token (without tokens: what it began with) in its row of final, which may be state itself.  slots[sequences] (device, int32)
+ * says which row is a sequence's, or, where it is NULL, row s is that of sequence s; one outside [0, slot_count) has no row: the sequence
+ * begins with zeros and leaves nothing.  Two sequences may not have the same row.
+ * saved (nullable, fp32 [rows / PXH_SCAN_SAVED, rounded up][width]) receives h in front of every PXH_SCAN_SAVED-th row, which is what
+ * the backward pass needs.  y may be x, update or gate where the strides are the same.
+ * A result depends on its sequence alone up to the last bits of h, which depend on where in the rows the sequence lies, and the same
+ * call gives the same bits.  Within a step h is rounded to 2^-23 of the larger of |h| and |x|.
+ * workspace: pxh_gated_scan_workspace_bytes(rows, width), which serves fewer rows and shorter rows too, or NULL for the library's. */
+#define PXH_SCAN_SAVED 16
+size_t pxh_gated_scan_workspace_bytes(long long rows, int width);
+int pxh_gated_scan_forward(const void* x, const void* update, const void* gate, void* y, const int* starts, const float* state,
+                           float* final, const int* slots, float* saved, int type, long long rows, int width, int sequences,
+                           int slot_count, long long x_stride, long long update_stride, long long gate_stride, long long y_stride,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* Its gradients, from the forward's inputs and what it saved:
+ *   G[t] = dy * g + (1 - z[t + 1]) * G[t + 1], with g = 1 or gate / (1 + exp(-gate)), and behind a sequence's last token its d_final
+ *   dx = z G;  dupdate = G (x - h[t - 1]) z (1 - z);  dgate = dy h s (1 + gate (1 - s)), s = 1 / (1 + exp(-gate));  d_state = (1 - z) G
+ * of a sequence's first token.  gate and dgate go together.  state: what the forward began with (it may not have been overwritten
+ * since).  d_final, d_state (nullable, fp32 [slot_count][width]) are the gradients of final and of state, by the forward's slots;
+ * d_state may be d_final.  dx may be dy or x, dupdate update and dgate gate, where the strides are the same. */
+int pxh_gated_scan_backward(const void* dy, const void* x, const void* update, const void* gate, const float* saved, void* dx,
+                            void* dupdate, void* dgate, const int* starts, const float* state, const float* d_final, float* d_state,
+                            const int* slots, int type, long long rows, int width, int sequences, int slot_count,
+                            long long dy_stride, long long x_stride, long long update_stride, long long gate_stride,
+                            long long dx_stride, long long dupdate_stride, long long dgate_stride, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* One new token of each of `rows` sequences, in one launch: as the forward with sequences of one token, the states in place. */
+int pxh_gated_scan_step(const void* x, const void* update, const void* gate, void* y, float* state, const int* slots, int type,
+                        long long rows, int width, int slot_count, long long x_stride, long long update_stride,
+                        long long gate_stride, long long y_stride, void* stream);
+
 /* AdamW over all parameter tensors of a model at once, from a table kept on the device, with states in 32 or in 8 bits and the
  * gradients clipped by their common norm:
  *   norm = |d_scale * d|_2 over all tensors;  f = max_norm > 0 and norm > max_norm ? max_norm / norm : 1

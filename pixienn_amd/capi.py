@@ -95,6 +95,9 @@ SIGNATURES = {
     "pxh_embedding_backward": [P, P, P, I, I, I, L, I, I, L, L, F, I, P, Z, P],
     "pxh_layer_norm_forward": [P, P, P, P, P, P, P, P, I, I, L, I, L, L, L, L, F, P],
     "pxh_layer_norm_backward": [P, P, P, P, P, P, P, P, P, I, I, L, I, L, L, L, L, I, P, Z, P],
+    "pxh_gated_scan_forward": [P, P, P, P, P, P, P, P, P, I, L, I, I, I, L, L, L, L, P, Z, P],
+    "pxh_gated_scan_backward": [P, P, P, P, P, P, P, P, P, P, P, P, P, I, L, I, I, I, L, L, L, L, L, L, L, P, Z, P],
+    "pxh_gated_scan_step": [P, P, P, P, P, P, I, L, I, I, L, L, L, L, P],
     "pxh_token_logprobs_forward_train": [P, P, P, P, P, P, P, P, I, I, L, I, L, L, F, P],
 }
 _OTHER_RETURNS = {
@@ -116,6 +119,7 @@ _OTHER_RETURNS = {
     "pxh_token_logprobs_workspace_bytes": (Z, [L, I, I]),
     "pxh_embedding_workspace_bytes": (Z, [L, I]),
     "pxh_layer_norm_workspace_bytes": (Z, [L, I]),
+    "pxh_gated_scan_workspace_bytes": (Z, [L, I]),
 }
 # test hooks (pixienn_amd/csrc/pixienn_hip_test.h): exported, but not part of the C ABI
 _TEST_HOOKS = {

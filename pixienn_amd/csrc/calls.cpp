@@ -511,13 +511,125 @@ PyObject* layer_norm_backward(PyObject* self, PyObject* const* args, Py_ssize_t 
     });
 }
 
+// A number that may be None.
+long long number_or(PyObject* o, long long none) { return o == Py_None ? none : argument<long long>(o); }
+
+// The sequences that a call's tokens belong to, and their states.
+struct Sequences {
+    const int* starts = nullptr;
+    int count = 0;
+
+    Sequences(const Device& d, const Rows& tokens, PyObject* starts_, PyObject* sequences)
+    {
+        if (starts_ != Py_None) {
+            const long long n = d.tensor(starts_).numel();
+            if (n < 1) throw NotHere{};
+            starts = d.packed<int>(starts_, n, at::kInt);
+            count = fits(n - 1);
+        } else {
+            const long long n = number_or(sequences, tokens.shape.size() == 3 ? tokens.shape[0] : tokens.rows > 0);
+            if (n < 0) throw NotHere{};
+            count = fits(n);
+        }
+    }
+};
+
+struct States {
+    const Device& d;
+    long long count, width, slot_count = -1;
+    const int* slots;
+
+    States(const Device& device, PyObject* slots_, long long sequences, long long width_)
+        : d(device), count(sequences), width(width_), slots(d.packed<int>(slots_, sequences, at::kInt)) {}
+    float* of(PyObject* o)
+    {
+        if (o == Py_None) return nullptr;
+        const at::Tensor& t = d.tensor(o);
+        if (t.dim() != 2 || t.size(1) != width || (slot_count >= 0 && t.size(0) != slot_count)) throw NotHere{};
+        slot_count = t.size(0);
+        return d.floats(o, slot_count * width);
+    }
+    int places() const { return slot_count < 0 ? 0 : fits(slot_count); }
+};
+
+const Rows& needed(const Rows& r)
+{
+    if (!r.given) throw NotHere{};
+    return r;
+}
+
+// (x, update, y, gate, starts, sequences, state, final, slots, saved, workspace)
+PyObject* gated_scan_forward(PyObject* self, PyObject* const* args, Py_ssize_t count)
+{
+    return on_device<&pxh_gated_scan_forward, 11>(self, args, count, [](PyObject* const* a, const Device& d, auto f) {
+        const Rows x = needed(d.rows(a[0])), u = needed(d.rows(a[1])), y = needed(d.rows(a[2])), gate = d.rows(a[3]);
+        u.like(x, x.type);
+        y.like(x, x.type);
+        gate.like(x, x.type);
+        const Sequences q(d, x, a[4], a[5]);
+        States states(d, a[8], q.count, x.width);
+        float* const state = states.of(a[6]);
+        float* const final = states.of(a[7]);
+        float* const saved = d.floats(a[9], (x.rows + PXH_SCAN_SAVED - 1) / PXH_SCAN_SAVED * x.width);
+        const Space space = d.space(a[10]);
+        const int width = fits(x.width), places = states.places();
+        return status([&] {
+            return f(x.data, u.data, gate.data, y.data, q.starts, state, final, states.slots, saved, x.type, x.rows, width, q.count, places,
+                     x.stride, u.stride, stride_of(gate), y.stride, space.data, space.bytes, d.stream);
+        });
+    });
+}
+
+// (dy, x, update, saved, dx, dupdate, gate, dgate, starts, sequences, state, d_final, d_state, slots, workspace)
+PyObject* gated_scan_backward(PyObject* self, PyObject* const* args, Py_ssize_t count)
+{
+    return on_device<&pxh_gated_scan_backward, 15>(self, args, count, [](PyObject* const* a, const Device& d, auto f) {
+        const Rows dy = needed(d.rows(a[0])), x = needed(d.rows(a[1])), u = needed(d.rows(a[2])), dx = needed(d.rows(a[4])),
+                   du = needed(d.rows(a[5])), gate = d.rows(a[6]), dgate = d.rows(a[7]);
+        for (const Rows* r: { &x, &u, &dx, &du, &gate, &dgate }) r->like(dy, dy.type);
+        const Sequences q(d, dy, a[8], a[9]);
+        States states(d, a[13], q.count, dy.width);
+        float* const state = states.of(a[10]);
+        float* const d_final = states.of(a[11]);
+        float* const d_state = states.of(a[12]);
+        float* const saved = d.floats(a[3], (dy.rows + PXH_SCAN_SAVED - 1) / PXH_SCAN_SAVED * dy.width);
+        const Space space = d.space(a[14]);
+        const int width = fits(dy.width), places = states.places();
+        return status([&] {
+            return f(dy.data, x.data, u.data, gate.data, saved, dx.data, du.data, dgate.data, q.starts, state, d_final, d_state, states.slots, dy.type,
+                     dy.rows, width, q.count, places, dy.stride, x.stride, u.stride, stride_of(gate), dx.stride, du.stride, stride_of(dgate),
+                     space.data, space.bytes, d.stream);
+        });
+    });
+}
+
+// (x, update, y, state, gate, slots)
+PyObject* gated_scan_step(PyObject* self, PyObject* const* args, Py_ssize_t count)
+{
+    return on_device<&pxh_gated_scan_step, 6>(self, args, count, [](PyObject* const* a, const Device& d, auto f) {
+        const Rows x = needed(d.rows(a[0])), u = needed(d.rows(a[1])), y = needed(d.rows(a[2])), gate = d.rows(a[4]);
+        u.like(x, x.type);
+        y.like(x, x.type);
+        gate.like(x, x.type);
+        States states(d, a[5], x.rows, x.width);
+        if (a[3] == Py_None) throw NotHere{};
+        float* const state = states.of(a[3]);
+        const int width = fits(x.width), places = states.places();
+        return status([&] {
+            return f(x.data, u.data, gate.data, y.data, state, states.slots, x.type, x.rows, width, places, x.stride, u.stride, stride_of(gate),
+                     y.stride, d.stream);
+        });
+    });
+}
+
 #define FUNCTION(name) \
     PyMethodDef { "pxh_" #name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&name)), METH_FASTCALL, nullptr }
 
 PyMethodDef functions[] = { FUNCTION(rms_norm_forward), FUNCTION(rms_norm_backward), FUNCTION(token_logprobs_forward),
                             FUNCTION(token_logprobs_backward), FUNCTION(token_logprobs_forward_train) };
 
-PyMethodDef layers[] = { FUNCTION(embedding_forward), FUNCTION(embedding_backward), FUNCTION(layer_norm_forward), FUNCTION(layer_norm_backward) };
+PyMethodDef layers[] = { FUNCTION(embedding_forward), FUNCTION(embedding_backward), FUNCTION(layer_norm_forward), FUNCTION(layer_norm_backward),
+                         FUNCTION(gated_scan_forward), FUNCTION(gated_scan_backward), FUNCTION(gated_scan_step) };
 
 // bind_function(name, address) -> the callable that takes a Python function's own arguments and the stream, or None
 PyObject* bind_function(PyObject*, PyObject* args)

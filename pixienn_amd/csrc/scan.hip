@@ -1,0 +1,717 @@
+// A gated linear recurrence over sequences of tokens, its gradients, and the step for one new token of each sequence.
+//   z = 1 / (1 + exp(-update));  h[t] = h[t - 1] + z * (x - h[t - 1]);  y = h, or with a gate h * gate / (1 + exp(-gate))
+#include "rows.h"
+#include "stream.h"
+
+namespace pxh {
+namespace {
+
+// A range of tokens takes a state s to (1 - Z) * s + H.  1 - z is never kept: of a z of 2^-13 it has only half the digits in fp32, which
+// thousands of tokens would add up, while Z = z + z' - z z' has them all.  Z == 1 says that nothing in front of the range counts
+// any more; then the state behind it is H to the bit, whatever came before.
+struct Range {
+    float z, h;
+};
+
+__device__ __forceinline__ float behind(float s, Range r) { return r.z == 1.0f ? r.h : s + fmaf(-r.z, s, r.h); }
+
+__device__ __forceinline__ Range joined(Range first, Range then)
+{
+    return Range{ then.z == 1.0f ? 1.0f : first.z + fmaf(-then.z, first.z, then.z), behind(first.h, then) };
+}
+
+// z = 1 / (1 + e) with e = exp(-u), and 1 - z to all its digits: e z where z is near 1.  16-bit values: the hardware's exp2 of the
+// product, an error of 2^-24 |u| and less.  An update of minus infinity has z = 0.
+template<int T>
+__device__ __forceinline__ void gate_of(float u, float& z, float& rest)
+{
+    float e;
+    if constexpr (T == PXH_F32) {
+        const float a = u < -87.0f ? -87.0f : u > 110.0f ? 110.0f : u;
+        e = exp_by_exp2(-a);
+        z = u < -87.0f ? 0.0f : quotient(1.0f, 1.0f + e);
+    } else {
+        e = __builtin_amdgcn_exp2f(u * -1.44269504f);
+        z = __builtin_amdgcn_rcpf(1.0f + e);
+    }
+    rest = z < 0.5f ? 1.0f - z : e * z;
+}
+
+// h times the gate's factor o s, rounded to fp32 before it is rounded to the type: the compiler would round some products to half at
+// once, and a step would not have the bits of the forward pass.
+template<int T>
+__device__ __forceinline__ float gated(float h, float o)
+{
+    float s, rest;
+    gate_of<T>(o, s, rest);
+    float y = h * (o * s);
+    if constexpr (T == PXH_F16) asm("" : "+v"(y));
+    return y;
+}
+
+constexpr int kSteps = 16;              // tokens of a wave, and from one saved state to the next
+constexpr int kWaves = 8;               // of a workgroup, one behind the other along the tokens
+constexpr int kChunk = kSteps * kWaves; // tokens of a workgroup
+constexpr int kV = 2;                   // channels of a lane
+constexpr int kTile = kV * kWave;       // ... and of a workgroup
+constexpr int kScanLanes = kWaves * kWave;
+constexpr uint32_t kAll = (1u << kSteps) - 1;
+
+// Where sequences begin: starts[sequences + 1], or all of one length.
+struct Sequences {
+    const int* starts;
+    FastDiv length;
+    int count, rows;
+};
+
+// States of sequences: a row of `width` fp32 for each slot.
+struct Slots {
+    const int* of;          // [sequences], or null: a sequence's own number
+    int count;
+};
+
+// The place of sequence s in the states, or -1 where none is kept.
+__device__ __forceinline__ int slot_of(const Slots& slots, int s)
+{
+    const int slot = slots.of ? slots.of[s] : s;
+    return slot >= 0 && slot < slots.count ? slot : -1;
+}
+
+// What the wave has to know of its tokens first .. first + kSteps: a bit each, for those that begin a sequence, end one, and lie in
+// one; lane i knows the sequence of token i.
+struct Borders {
+    uint32_t begins, ends, active;
+    int sequence;
+};
+
+__device__ __forceinline__ Borders borders_of(const Sequences& q, int first)
+{
+    const int lane = threadIdx.x % kWave;
+    const int t = first + lane;
+    const bool mine = lane < kSteps && t < q.rows;
+    bool begins = false, ends = false, active = false;
+    int s = 0;
+    if (mine) {
+        if (q.starts) {
+            // the last sequence that begins at or in front of t
+            int low = 0, n = q.count + 1;
+            while (n > 0) {
+                const int half = n / 2;
+                if (q.starts[low + half] <= t) {
+                    low += half + 1;
+                    n -= half + 1;
+                } else {
+                    n = half;
+                }
+            }
+            s = low - 1;
+            if (s >= 0 && s < q.count) {
+                active = true;
+                begins = q.starts[s] == t;
+                ends = q.starts[s + 1] == t + 1 || t + 1 == q.rows;
+            } else {
+                s = 0;
+            }
+        } else {
+            uint32_t which, place;
+            q.length.divmod(t, which, place);
+            s = static_cast<int>(which);
+            active = true;
+            begins = place == 0;
+            ends = place + 1 == q.length.d;
+        }
+    }
+    return Borders{ static_cast<uint32_t>(__ballot(begins)), static_cast<uint32_t>(__ballot(ends)), static_cast<uint32_t>(__ballot(active)), s };
+}
+
+// ---------------------------------------------------------------- from chunk to chunk
+// Workgroups take numbers, chunk by chunk along the tokens (for the gradients against them).  Each leaves what its chunk does to a
+// state, channel by channel, as one 64-bit word, and once it knows the state in front of it the one behind it as a range with Z = 1.  It
+// looks back at the words of up to kWindow chunks, until one of them has Z = 1 and none nearer is missing, and goes on
+// from there: s + (H - Z s) chunk by chunk is the same to the bit wherever it begins.
+// A workgroup waits for lower numbers only, which are running or done: the lowest of those running waits for none.  The bound on the looks
+// makes the exit unconditional all the same; where it was reached (two launches at once on one workspace, which the interface
+// forbids) the states are NaN.
+constexpr unsigned long long kNotThere = ~0ull;     // no range: a Z that is no number is left as 1, with its H
+constexpr int kWindow = 8;
+constexpr uint32_t kLooks = 1u << 22;
+
+struct Exchange {
+    unsigned long long* words;      // [chunks][width]; null where no chunk needs another's
+    uint32_t* counter;
+    uint32_t chunks;
+    FastDiv by_tiles;
+};
+
+__device__ __forceinline__ unsigned long long word_of(Range r)
+{
+    return static_cast<unsigned long long>(__float_as_uint(r.z != r.z ? 1.0f : r.z)) << 32 | __float_as_uint(r.h);
+}
+
+__device__ __forceinline__ Range range_of(unsigned long long w)
+{
+    return Range{ __uint_as_float(static_cast<uint32_t>(w >> 32)), __uint_as_float(static_cast<uint32_t>(w)) };
+}
+
+__device__ __forceinline__ void leave_word(unsigned long long* at, Range r)
+{
+    __hip_atomic_store(at, word_of(r), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// The state behind the chunk in front of `chunk`, of one channel (there: one that exists); chunk > 0, all lanes of the wave.
+__device__ __forceinline__ float look_back(const unsigned long long* words, uint32_t chunk, size_t width, bool there)
+{
+    unsigned long long w[kWindow];
+    int found = -1;
+    for (uint32_t looks = kLooks; looks; --looks) {
+#pragma unroll
+        for (int d = 0; d < kWindow; ++d) {
+            w[d] = word_of(Range{ 1.0f, 0.0f });         // in front of the first chunk
+            if (there && chunk > static_cast<uint32_t>(d))
+                w[d] = __hip_atomic_load(words + (chunk - 1 - d) * width, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        bool whole = true;
+        found = -1;
+#pragma unroll
+        for (int d = 0; d < kWindow; ++d) {
+            whole = whole && w[d] != kNotThere;
+            if (whole && found < 0 && range_of(w[d]).z == 1.0f) found = d;
+        }
+        if (!__any(found < 0)) break;
+        __builtin_amdgcn_s_sleep(1);
+    }
+    float s = __builtin_nanf("");
+#pragma unroll
+    for (int d = kWindow - 1; d >= 0; --d) {
+        if (d < found) s = behind(s, range_of(w[d]));
+        else if (d == found) s = range_of(w[d]).h;
+    }
+    return s;
+}
+
+struct ScanShared {
+    Range ranges[kWaves][kTile];
+    float states[kWaves][kTile];        // in front of each wave's tokens
+    uint32_t number, fresh;             // fresh: no state reaches the chunk
+};
+
+// Takes the workgroup's number: chunk and tile.
+__device__ __forceinline__ void take_number(const Exchange& x, ScanShared& lds, uint32_t& chunk, uint32_t& tile)
+{
+    uint32_t number = blockIdx.x;
+    if (x.words) {
+        if (threadIdx.x == 0) lds.number = atomicAdd(x.counter, 1u);
+        __syncthreads();
+        number = lds.number;
+    }
+    x.by_tiles.divmod(number, chunk, tile);
+}
+
+// From the waves' ranges, in the order `order(0 .. kWaves - 1)`, and the chunks in front of `chunk`: the state in front of every wave.
+template<typename Order>
+__device__ __forceinline__ void join_waves(const Exchange& x, ScanShared& lds, uint32_t chunk, uint32_t tile, int width, const Order& order)
+{
+    __syncthreads();
+    const int c = threadIdx.x;
+    if (c < kTile) {            // whole waves
+        const int e = static_cast<int>(tile) * kTile + c;
+        const bool there = e < width;
+        Range own[kWaves], all{ 0.0f, 0.0f };
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            own[w] = lds.ranges[order(w)][c];
+            all = joined(all, own[w]);
+        }
+        float s = 0.0f;
+        if (x.words) {
+            unsigned long long* const word = x.words + e;
+            const bool leaves = there && chunk + 1 < x.chunks;
+            const bool fresh = chunk == 0 || lds.fresh;
+            if (fresh) all.z = 1.0f;
+            if (leaves) leave_word(word + chunk * static_cast<size_t>(width), all);
+            if (!fresh) {
+                s = look_back(word, chunk, width, there);
+                if (leaves && all.z != 1.0f) leave_word(word + chunk * static_cast<size_t>(width), Range{ 1.0f, behind(s, all) });
+            }
+        }
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            lds.states[order(w)][c] = s;
+            s = behind(s, own[w]);
+        }
+    }
+    __syncthreads();
+}
+
+// ---- the launch in front: empties the words, and hands the states of sequences without tokens on.
+__global__ __launch_bounds__(kBlock) void scan_start_kernel(unsigned long long* words, size_t count, uint32_t* counter, Sequences q, Slots slots, const float* from,
+                                                            float* to, int width)
+{
+    const size_t i = static_cast<size_t>(blockIdx.x) * kBlock + threadIdx.x;
+    const size_t lanes = static_cast<size_t>(gridDim.x) * kBlock;
+    if (i == 0 && counter) *counter = 0;
+    for (size_t k = i; k < count; k += lanes) words[k] = kNotThere;
+    if (!to) return;
+    for (int s = blockIdx.x; s < q.count; s += gridDim.x) {
+        if (q.starts && q.starts[s] != q.starts[s + 1]) continue;
+        const int slot = slot_of(slots, s);
+        if (slot < 0) continue;
+        for (int e = threadIdx.x; e < width; e += kBlock)
+            to[static_cast<size_t>(slot) * width + e] = from ? from[static_cast<size_t>(slot) * width + e] : 0.0f;
+    }
+}
+
+// kV channels of a row of fp32 states.
+__device__ __forceinline__ void load_state(const float* states, int slot, int e, int width, float (&s)[kV])
+{
+#pragma unroll
+    for (int k = 0; k < kV; ++k) s[k] = states && slot >= 0 && e + k < width ? states[static_cast<size_t>(slot) * width + e + k] : 0.0f;
+}
+
+__device__ __forceinline__ void store_state(float* states, int slot, int e, int width, const float (&s)[kV])
+{
+#pragma unroll
+    for (int k = 0; k < kV; ++k)
+        if (slot >= 0 && e + k < width) states[static_cast<size_t>(slot) * width + e + k] = s[k];
+}
+
+// The wave's kSteps tokens of a tensor, kV channels a lane; tokens behind the last row repeat it, channels behind the last one are
+// zeros.  No branch around a load.
+template<int T>
+__device__ __forceinline__ void load_tokens(const void* p, long long stride, int first, int rows, int e, int width, bool inside, Raw<T, kV> (&r)[kSteps])
+{
+    if (inside) {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) r[i] = load_raw<T, kV>(row_of<T>(p, min(first + i, rows - 1), stride), e);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) r[i] = load_end<T, kV>(row_of<T>(p, min(first + i, rows - 1), stride), e, width);
+    }
+}
+
+template<int T>
+__device__ __forceinline__ void store_token(void* p, long long stride, int t, int e, int width, bool inside, const float (&v)[kV])
+{
+    Raw<T, kV> r;
+    r.set(v);
+    char* const row = row_of<T>(p, t, stride);
+    if (inside) store_raw<T, kV>(row, e, r);
+    else if (e < width) store_row<T, kV>(row, e, width, r);
+}
+
+// ---------------------------------------------------------------- forward
+struct ScanArgs {
+    const void* x;
+    const void* update;
+    const void* gate;
+    void* y;
+    const float* state;
+    float* final;
+    float* saved;               // [rows / kSteps, rounded up][width]: in front of every kSteps-th token
+    long long x_stride, update_stride, gate_stride, y_stride;
+    Sequences q;
+    Slots slots;
+    Exchange exchange;
+    int width;
+};
+
+// A workgroup takes kChunk tokens of kTile channels, a wave kSteps of them, which stay in registers as z and x between the pass that finds
+// what they do to a state and the one that forms the states: one trip to memory.
+template<int T, bool GATE>
+__global__ __launch_bounds__(kScanLanes) void scan_kernel(ScanArgs a)
+{
+    __shared__ ScanShared lds;
+    uint32_t chunk, tile;
+    take_number(a.exchange, lds, chunk, tile);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+    const int first = static_cast<int>(chunk) * kChunk + wave * kSteps;
+    const int e = static_cast<int>(tile) * kTile + lane * kV;
+    const bool inside = (static_cast<int>(tile) + 1) * kTile <= a.width;
+    Raw<T, kV> x[kSteps], u[kSteps], o[GATE ? kSteps : 1];
+    load_tokens<T>(a.x, a.x_stride, first, a.q.rows, e, a.width, inside, x);
+    load_tokens<T>(a.update, a.update_stride, first, a.q.rows, e, a.width, inside, u);
+    if constexpr (GATE) load_tokens<T>(a.gate, a.gate_stride, first, a.q.rows, e, a.width, inside, o);
+    const Borders b = borders_of(a.q, first);
+    if (threadIdx.x == 0) lds.fresh = b.begins & 1;
+    float z[kSteps][kV];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+        float v[kV], rest;
+        u[i].get(v);
+#pragma unroll
+        for (int k = 0; k < kV; ++k) gate_of<T>(v[k], z[i][k], rest);
+    }
+    float h[kV] = {}, Z[kV] = {};
+    const auto take = [&](int i) {
+        float v[kV];
+        x[i].get(v);
+#pragma unroll
+        for (int k = 0; k < kV; ++k) {
+            Z[k] += fmaf(-z[i][k], Z[k], z[i][k]);
+            h[k] = fmaf(z[i][k], v[k] - h[k], h[k]);
+        }
+    };
+    const bool plain = b.begins == 0 && b.active == kAll;
+    if (plain) {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) take(i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            if (!(b.active >> i & 1)) continue;
+            const bool begins = b.begins >> i & 1;
+            if (begins) load_state(a.state, a.state ? slot_of(a.slots, __builtin_amdgcn_readlane(b.sequence, i)) : -1, e, a.width, h);
+            take(i);
+            if (begins) {
+                // the second pass takes the state from here: by then `final`, which may be `state`, may have been written
+#pragma unroll
+                for (int k = 0; k < kV; ++k) {
+                    Z[k] = 1.0f;
+                    z[i][k] = h[k];
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kV; ++k) lds.ranges[wave][lane * kV + k] = Range{ Z[k], h[k] };
+    join_waves(a.exchange, lds, chunk, tile, a.width, [](int w) { return w; });
+#pragma unroll
+    for (int k = 0; k < kV; ++k) h[k] = lds.states[wave][lane * kV + k];
+    if (a.saved && first < a.q.rows) store_state(a.saved, first / kSteps, e, a.width, h);
+    const auto give = [&](int i) {
+        float v[kV];
+#pragma unroll
+        for (int k = 0; k < kV; ++k) v[k] = h[k];
+        if constexpr (GATE) {
+            float w[kV];
+            o[i].get(w);
+#pragma unroll
+            for (int k = 0; k < kV; ++k) v[k] = gated<T>(h[k], w[k]);
+        }
+        store_token<T>(a.y, a.y_stride, first + i, e, a.width, inside, v);
+    };
+    const auto step = [&](int i) {
+        float v[kV];
+        x[i].get(v);
+#pragma unroll
+        for (int k = 0; k < kV; ++k) h[k] = fmaf(z[i][k], v[k] - h[k], h[k]);
+    };
+    if (plain && b.ends == 0) {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            step(i);
+            give(i);
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+        if (!(b.active >> i & 1)) continue;
+        if (b.begins >> i & 1) {
+#pragma unroll
+            for (int k = 0; k < kV; ++k) h[k] = z[i][k];
+        } else {
+            step(i);
+        }
+        give(i);
+        if (a.final && (b.ends >> i & 1)) store_state(a.final, slot_of(a.slots, __builtin_amdgcn_readlane(b.sequence, i)), e, a.width, h);
+    }
+}
+
+// ---------------------------------------------------------------- backward
+//   G[t] = dy * g + (1 - z[t + 1]) * G[t + 1], g = gate / (1 + exp(-gate));  dx = z G;  dupdate = G (x - h[t - 1]) z (1 - z)
+//   dgate = dy h s (1 + gate (1 - s)), s = 1 / (1 + exp(-gate))
+// Along the tokens from the saved states for h, then against them for G: the carry C = (1 - z) G goes through a range as a state does.
+struct ScanBackwardArgs {
+    const void* dy;
+    const void* x;
+    const void* update;
+    const void* gate;
+    const float* saved;
+    void* dx;
+    void* dupdate;
+    void* dgate;
+    const float* state;
+    const float* d_final;
+    float* d_state;
+    long long dy_stride, x_stride, update_stride, gate_stride, dx_stride, dupdate_stride, dgate_stride;
+    Sequences q;
+    Slots slots;
+    Exchange exchange;
+    int width;
+};
+
+template<int T, bool GATE>
+__global__ __launch_bounds__(kScanLanes, 4) void scan_backward_kernel(ScanBackwardArgs a)
+{
+    __shared__ ScanShared lds;
+    uint32_t turn, tile;
+    take_number(a.exchange, lds, turn, tile);
+    const uint32_t chunk = a.exchange.chunks - 1 - turn;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
+    const int first = static_cast<int>(chunk) * kChunk + wave * kSteps;
+    const int e = static_cast<int>(tile) * kTile + lane * kV;
+    const bool inside = (static_cast<int>(tile) + 1) * kTile <= a.width;
+    Raw<T, kV> x[kSteps], u[kSteps], dy[kSteps], o[GATE ? kSteps : 1];
+    load_tokens<T>(a.update, a.update_stride, first, a.q.rows, e, a.width, inside, u);
+    load_tokens<T>(a.x, a.x_stride, first, a.q.rows, e, a.width, inside, x);
+    load_tokens<T>(a.dy, a.dy_stride, first, a.q.rows, e, a.width, inside, dy);
+    if constexpr (GATE) load_tokens<T>(a.gate, a.gate_stride, first, a.q.rows, e, a.width, inside, o);
+    float h[kV];
+    load_state(a.saved, first < a.q.rows ? first / kSteps : -1, e, a.width, h);
+    const Borders b = borders_of(a.q, first);
+    if (wave == kWaves - 1 && lane == 0) lds.fresh = b.ends >> (kSteps - 1) & 1;
+    float z[kSteps][kV], g[kSteps][kV], w[kSteps][kV];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+        const bool active = b.active >> i & 1;
+        if (b.begins >> i & 1) load_state(a.state, a.state ? slot_of(a.slots, __builtin_amdgcn_readlane(b.sequence, i)) : -1, e, a.width, h);
+        float v[kV], d[kV];
+        u[i].get(v);
+        x[i].get(d);
+        dy[i].get(g[i]);
+#pragma unroll
+        for (int k = 0; k < kV; ++k) {
+            float rest;
+            gate_of<T>(v[k], z[i][k], rest);
+            const float ahead = d[k] - h[k];
+            w[i][k] = ahead * (z[i][k] * rest);
+            h[k] = active ? fmaf(z[i][k], ahead, h[k]) : h[k];
+        }
+        if constexpr (GATE) {
+            float p[kV], dgate[kV];
+            o[i].get(p);
+#pragma unroll
+            for (int k = 0; k < kV; ++k) {
+                float s, rest;
+                gate_of<T>(p[k], s, rest);
+                dgate[k] = g[i][k] * h[k] * (s * fmaf(p[k], rest, 1.0f));
+                g[i][k] *= p[k] * s;
+            }
+            if (active) store_token<T>(a.dgate, a.dgate_stride, first + i, e, a.width, inside, dgate);
+        }
+        if (a.d_final && (b.ends >> i & 1)) {
+            float more[kV];
+            load_state(a.d_final, slot_of(a.slots, __builtin_amdgcn_readlane(b.sequence, i)), e, a.width, more);
+#pragma unroll
+            for (int k = 0; k < kV; ++k) g[i][k] += more[k];
+        }
+    }
+    float C[kV] = {}, Z[kV] = {};
+#pragma unroll
+    for (int i = kSteps - 1; i >= 0; --i) {
+        if (!(b.active >> i & 1)) continue;
+        const bool ends = b.ends >> i & 1;
+#pragma unroll
+        for (int k = 0; k < kV; ++k) {
+            const float G = ends ? g[i][k] : g[i][k] + C[k];
+            C[k] = fmaf(-z[i][k], G, G);
+            Z[k] = ends ? 1.0f : Z[k] + fmaf(-z[i][k], Z[k], z[i][k]);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kV; ++k) lds.ranges[wave][lane * kV + k] = Range{ Z[k], C[k] };
+    join_waves(a.exchange, lds, turn, tile, a.width, [](int k) { return kWaves - 1 - k; });
+#pragma unroll
+    for (int k = 0; k < kV; ++k) C[k] = lds.states[wave][lane * kV + k];
+#pragma unroll
+    for (int i = kSteps - 1; i >= 0; --i) {
+        if (!(b.active >> i & 1)) continue;
+        const bool ends = b.ends >> i & 1;
+        float dx[kV], du[kV];
+#pragma unroll
+        for (int k = 0; k < kV; ++k) {
+            const float G = ends ? g[i][k] : g[i][k] + C[k];
+            dx[k] = z[i][k] * G;
+            du[k] = w[i][k] * G;
+            C[k] = G - dx[k];
+        }
+        store_token<T>(a.dx, a.dx_stride, first + i, e, a.width, inside, dx);
+        store_token<T>(a.dupdate, a.dupdate_stride, first + i, e, a.width, inside, du);
+        if (a.d_state && (b.begins >> i & 1)) store_state(a.d_state, slot_of(a.slots, __builtin_amdgcn_readlane(b.sequence, i)), e, a.width, C);
+    }
+}
+
+// ---------------------------------------------------------------- one token of each sequence
+struct StepArgs {
+    const char* x;
+    const char* update;
+    const char* gate;
+    char* y;
+    float* state;
+    long long x_stride, update_stride, gate_stride, y_stride;
+    Slots slots;
+    uint32_t items;
+    FastDiv by_row;
+    int width;
+};
+
+template<int T, bool GATE>
+__global__ __launch_bounds__(kBlock) void scan_step_kernel(StepArgs a)
+{
+    constexpr int V = 4;
+    const uint32_t item = blockIdx.x * kBlock + threadIdx.x;
+    if (item >= a.items) return;
+    uint32_t row, vector;
+    a.by_row.divmod(item, row, vector);
+    const int e = static_cast<int>(vector) * V;
+    float x[V], u[V], o[V] = {}, h[V] = {};
+    load_row<T, V>(row_of<T>(a.x, row, a.x_stride), e, a.width).get(x);
+    load_row<T, V>(row_of<T>(a.update, row, a.update_stride), e, a.width).get(u);
+    if constexpr (GATE) load_row<T, V>(row_of<T>(a.gate, row, a.gate_stride), e, a.width).get(o);
+    const int slot = slot_of(a.slots, static_cast<int>(row));
+    float* const state = a.state + static_cast<size_t>(slot < 0 ? 0 : slot) * a.width;
+    if (slot >= 0) load_row<PXH_F32, V>(state, e, a.width).get(h);
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        float z, rest;
+        gate_of<T>(u[k], z, rest);
+        h[k] = fmaf(z, x[k] - h[k], h[k]);
+    }
+    if (slot >= 0) {
+        Raw<PXH_F32, V> r;
+        r.set(h);
+        store_row<PXH_F32, V>(state, e, a.width, r);
+    }
+    if constexpr (GATE) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) h[k] = gated<T>(h[k], o[k]);
+    }
+    Raw<T, V> r;
+    r.set(h);
+    store_row<T, V>(row_of<T>(a.y, row, a.y_stride), e, a.width, r);
+}
+
+// ---------------------------------------------------------------- host
+size_t chunks_of(long long rows) { return (static_cast<size_t>(rows) + kChunk - 1) / kChunk; }
+
+// The words' counter in front of them.
+constexpr size_t kCounterBytes = 256;
+
+int check_scan(const char* who, int type, long long rows, int width, int sequences, const int* starts, const int* slots, int slot_count, bool states)
+{
+    if (type != PXH_F32 && type != PXH_BF16 && type != PXH_F16) return fail_invalid("%s: type %d is not fp32, bf16 or half", who, type);
+    if (rows < 0 || rows > 1 << 30) return fail_invalid("%s: %lld rows", who, rows);
+    if (width <= 0 || width > 1 << 24) return fail_invalid("%s: rows of %d values", who, width);
+    if (sequences < 0 || sequences > 1 << 30 || (sequences == 0 && rows > 0)) return fail_invalid("%s: %d sequences", who, sequences);
+    if (!starts && sequences > 0 && rows % sequences) return fail_invalid("%s: %lld rows are not %d sequences of one length", who, rows, sequences);
+    if (slots && !states) return fail_invalid("%s: slots without states", who);
+    if (states && slot_count < 0) return fail_invalid("%s: %d slots", who, slot_count);
+    if (states && !slots && slot_count < sequences) return fail_invalid("%s: states of %d slots for %d sequences", who, slot_count, sequences);
+    return PXH_OK;
+}
+
+// Sequences of the call, and the words that its chunks exchange (none where every chunk begins and ends with a sequence).
+int start_scan(const char* who, long long rows, int width, int sequences, const int* starts, const Slots& slots, const float* from, float* to,
+               void* workspace, size_t workspace_bytes, Sequences& q, Exchange& x, uint32_t& groups, hipStream_t s)
+{
+    const long long length = starts || sequences == 0 ? 0 : rows / sequences;
+    q = Sequences{ starts, FastDiv(length > 0 ? static_cast<uint32_t>(length) : 1), sequences, static_cast<int>(rows) };
+    const size_t chunks = chunks_of(rows), tiles = (static_cast<size_t>(width) + kTile - 1) / kTile;
+    if (chunks * tiles * kScanLanes >= 1ull << 32) return fail_invalid("%s: too many rows of too many values", who);
+    groups = static_cast<uint32_t>(chunks * tiles);
+    x = Exchange{ nullptr, nullptr, static_cast<uint32_t>(chunks), FastDiv(static_cast<uint32_t>(tiles)) };
+    size_t count = 0;
+    if (chunks > 1 && (starts || kChunk % length)) {
+        void* ws = nullptr;
+        count = chunks * static_cast<size_t>(width);
+        if (int rc = resolve_workspace(workspace, workspace_bytes, kCounterBytes + count * sizeof(unsigned long long), &ws, s)) return rc;
+        x.counter = static_cast<uint32_t*>(ws);
+        x.words = reinterpret_cast<unsigned long long*>(static_cast<char*>(ws) + kCounterBytes);
+    }
+    // sequences may be without tokens where their lengths are given, or where there are none at all
+    if (to == from || sequences == 0 || !(starts || length == 0)) to = nullptr;
+    if (count || to) {
+        size_t blocks = (count + 4 * kBlock - 1) / (4 * kBlock);
+        if (to && blocks < static_cast<size_t>(sequences)) blocks = sequences;
+        if (blocks > 2048) blocks = 2048;
+        hipLaunchKernelGGL(scan_start_kernel, dim3(static_cast<unsigned>(blocks)), dim3(kBlock), 0, s, x.words, count, x.counter, q, slots, from, to, width);
+        return check_launch(who);
+    }
+    return PXH_OK;
+}
+
+}  // namespace
+}  // namespace pxh
+
+using namespace pxh;
+
+extern "C" {
+
+size_t pxh_gated_scan_workspace_bytes(long long rows, int width)
+{
+    if (rows <= 0 || width <= 0) return 0;
+    return kCounterBytes + chunks_of(rows) * static_cast<size_t>(width) * sizeof(unsigned long long);
+}
+
+int pxh_gated_scan_forward(const void* x, const void* update, const void* gate, void* y, const int* starts, const float* state, float* final,
+                           const int* slots, float* saved, int type, long long rows, int width, int sequences, int slot_count, long long x_stride,
+                           long long update_stride, long long gate_stride, long long y_stride, void* workspace, size_t workspace_bytes, void* stream)
+{
+    const char* who = "pxh_gated_scan_forward";
+    if (int rc = check_scan(who, type, rows, width, sequences, starts, slots, slot_count, state || final)) return rc;
+    if (rows > 0 && (!x || !update || !y)) return fail_invalid("%s: null pointer", who);
+    if (rows > 1 && (x_stride < width || update_stride < width || y_stride < width || (gate && gate_stride < width)))
+        return fail_invalid("%s: rows of %d values that overlap", who, width);
+    ScanArgs a{ x, update, gate, y, state, final, saved, x_stride, update_stride, gate_stride, y_stride, {}, Slots{ slots, slot_count }, {}, width };
+    uint32_t groups;
+    hipStream_t s = as_stream(stream);
+    if (int rc = start_scan(who, rows, width, sequences, starts, a.slots, state, final, workspace, workspace_bytes, a.q, a.exchange, groups, s)) return rc;
+    if (rows == 0) return PXH_OK;
+    dispatch_type(type, [&]<int T>() {
+        if (gate) hipLaunchKernelGGL((scan_kernel<T, true>), dim3(groups), dim3(kScanLanes), 0, s, a);
+        else hipLaunchKernelGGL((scan_kernel<T, false>), dim3(groups), dim3(kScanLanes), 0, s, a);
+    });
+    return check_launch(who);
+}
+
+int pxh_gated_scan_backward(const void* dy, const void* x, const void* update, const void* gate, const float* saved, void* dx, void* dupdate,
+                            void* dgate, const int* starts, const float* state, const float* d_final, float* d_state, const int* slots, int type,
+                            long long rows, int width, int sequences, int slot_count, long long dy_stride, long long x_stride,
+                            long long update_stride, long long gate_stride, long long dx_stride, long long dupdate_stride,
+                            long long dgate_stride, void* workspace, size_t workspace_bytes, void* stream)
+{
+    const char* who = "pxh_gated_scan_backward";
+    if (int rc = check_scan(who, type, rows, width, sequences, starts, slots, slot_count, state || d_final || d_state)) return rc;
+    if (!gate != !dgate) return fail_invalid("%s: gate and dgate go together", who);
+    if (rows > 0 && (!dy || !x || !update || !saved || !dx || !dupdate)) return fail_invalid("%s: null pointer", who);
+    if (rows > 1 && (dy_stride < width || x_stride < width || update_stride < width || dx_stride < width || dupdate_stride < width
+                     || (gate && (gate_stride < width || dgate_stride < width))))
+        return fail_invalid("%s: rows of %d values that overlap", who, width);
+    ScanBackwardArgs a{ dy, x, update, gate, saved, dx, dupdate, dgate, state, d_final, d_state, dy_stride, x_stride, update_stride, gate_stride,
+                        dx_stride, dupdate_stride, dgate_stride, {}, Slots{ slots, slot_count }, {}, width };
+    uint32_t groups;
+    hipStream_t s = as_stream(stream);
+    if (int rc = start_scan(who, rows, width, sequences, starts, a.slots, d_final, d_state, workspace, workspace_bytes, a.q, a.exchange, groups, s))
+        return rc;
+    if (rows == 0) return PXH_OK;
+    dispatch_type(type, [&]<int T>() {
+        if (gate) hipLaunchKernelGGL((scan_backward_kernel<T, true>), dim3(groups), dim3(kScanLanes), 0, s, a);
+        else hipLaunchKernelGGL((scan_backward_kernel<T, false>), dim3(groups), dim3(kScanLanes), 0, s, a);
+    });
+    return check_launch(who);
+}
+
+int pxh_gated_scan_step(const void* x, const void* update, const void* gate, void* y, float* state, const int* slots, int type, long long rows,
+                        int width, int slot_count, long long x_stride, long long update_stride, long long gate_stride, long long y_stride, void* stream)
+{
+    const char* who = "pxh_gated_scan_step";
+    if (int rc = check_scan(who, type, rows, width, static_cast<int>(rows), nullptr, slots, slot_count, true)) return rc;
+    if (rows == 0) return PXH_OK;
+    if (!x || !update || !y || (!state && slot_count > 0)) return fail_invalid("%s: null pointer", who);
+    if (rows > 1 && (x_stride < width || update_stride < width || y_stride < width || (gate && gate_stride < width)))
+        return fail_invalid("%s: rows of %d values that overlap", who, width);
+    const int vectors = (width + 3) / 4;
+    if (rows * vectors >= (1ll << 31) - kBlock) return fail_invalid("%s: too many rows of too many values", who);
+    const StepArgs a{ static_cast<const char*>(x), static_cast<const char*>(update), static_cast<const char*>(gate), static_cast<char*>(y), state, x_stride,
+                      update_stride, gate_stride, y_stride, Slots{ slots, slot_count }, static_cast<uint32_t>(rows * vectors), FastDiv(vectors), width };
+    const dim3 grid(grid_for(a.items, kBlock)), block(kBlock);
+    hipStream_t s = as_stream(stream);
+    dispatch_type(type, [&]<int T>() {
+        if (gate) hipLaunchKernelGGL((scan_step_kernel<T, true>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((scan_step_kernel<T, false>), grid, block, 0, s, a);
+    });
+    return check_launch(who);
+}
+
+}

@@ -910,6 +910,15 @@ def _layer(name, *args):
     return rc == 0
 
 
+def _given(t, name):
+    """A tensor that a call cannot do without."""
+    if t is None:
+        raise PxError("%s is required" % name)
+    if not isinstance(t, torch.Tensor):
+        _chk(t, name=name)
+    return t
+
+
 def _tokens(tokens, rows, name="tokens"):
     """(address, whether of 64 bits) of the rows' tokens."""
     if tokens is None:
@@ -962,8 +971,8 @@ def layer_norm_forward(x, y, weight, bias=None, residual=None, sum=None, mean=No
         return y
     rows, width, x_stride = _rows(x, "x")
     kind = _type(x, "x")
-    y_stride = _like(_tensor(y), "y", x.shape, x.dtype)
-    _vector(_tensor(weight), "weight", width, None)
+    y_stride = _like(_given(y, "y"), "y", x.shape, x.dtype)
+    _vector(_given(weight, "weight"), "weight", width, None)
     weight_kind = _type(weight, "weight")
     _vector(bias, "bias", width, weight.dtype)
     _per_row(rows, mean=mean, rstd=rstd)
@@ -985,7 +994,7 @@ def layer_norm_backward(dy, h, weight, mean, rstd, dx, dw, db=None, dsum=None, a
         return dx
     rows, width, dy_stride = _rows(dy, "dy")
     kind = _type(dy, "dy")
-    _vector(_tensor(weight), "weight", width, None)
+    _vector(_given(weight, "weight"), "weight", width, None)
     weight_kind = _type(weight, "weight")
     _per_row(rows, mean=mean, rstd=rstd)
     for name, t in (("dw", dw), ("db", db)):
@@ -995,6 +1004,97 @@ def layer_norm_backward(dy, h, weight, mean, rstd, dx, dw, db=None, dsum=None, a
     call("pxh_layer_norm_backward", ptr(dy), ptr(h), ptr(weight), ptr(mean), ptr(rstd), ptr(dsum), ptr(dx), ptr(dw), ptr(db), kind,
          weight_kind, rows, width, dy_stride, *strides, int(bool(accumulate)), *_space(workspace), _stream())
     return dx
+
+
+SCAN_SAVED = 16          # tokens from one saved state of a gated scan to the next
+
+
+def gated_scan_saved_like(x):
+    """What gated_scan_forward leaves for the backward pass of tokens like x: fp32, a state for every SCAN_SAVED of them."""
+    rows, width, _ = _rows(x, "x")
+    return torch.empty(-(-rows // SCAN_SAVED), width, device=x.device)
+
+
+def gated_scan_workspace_bytes(rows, width):
+    return int(capi.load().pxh_gated_scan_workspace_bytes(rows, width))
+
+
+def _states(count, width, slots, **states):
+    """Slots of the states of a call's sequences; 0 where there are none."""
+    slot_count = None
+    for name, t in states.items():
+        if t is None:
+            continue
+        _chk(t, name=name)
+        if t.dim() != 2 or t.shape[1] != width or slot_count not in (None, t.shape[0]):
+            raise PxError("%s must be [slots, %d], of as many slots as the others (got %s)" % (name, width, tuple(t.shape)))
+        slot_count = t.shape[0]
+    _vector(slots, "slots", count, torch.int32)
+    return slot_count or 0
+
+
+def _sequences(x, rows, starts, sequences):
+    if starts is not None:
+        _chk(starts, torch.int32, "starts")
+        if starts.numel() < 1:
+            raise PxError("starts holds one more value than there are sequences")
+        return starts.numel() - 1
+    if sequences is None:
+        sequences = x.shape[0] if x.dim() == 3 else 1 if rows else 0
+    return int(sequences)
+
+
+def gated_scan_forward(x, update, y, gate=None, starts=None, sequences=None, state=None, final=None, slots=None, saved=None, workspace=None):
+    """h[t] = h[t - 1] + sigmoid(update) * (x - h[t - 1]), channel by channel along the tokens of each sequence; y = h, or with a
+    gate h * gate * sigmoid(gate).  x, update, gate and y are [tokens, width], the sequences one behind the other: starts
+    (int32, one more than sequences) says where each begins and the last one ends, or all are of one length ([sequences, tokens, width],
+    or `sequences` of them).  state and final (fp32 [slots, width], they may be one tensor): what the sequences begin with and leave, sequence s
+    in row slots[s] (int32; one outside: none is kept), or s.  saved (gated_scan_saved_like(x)) is what the backward pass needs."""
+    if _layer("pxh_gated_scan_forward", x, update, y, gate, starts, sequences, state, final, slots, saved, workspace):
+        return y
+    rows, width, x_stride = _rows(x, "x")
+    kind = _type(x, "x")
+    strides = [_like(t, name, x.shape, x.dtype) for name, t in (("update", _given(update, "update")), ("gate", gate), ("y", _given(y, "y")))]
+    count = _sequences(x, rows, starts, sequences)
+    slot_count = _states(count, width, slots, state=state, final=final)
+    _vector(saved, "saved", -(-rows // SCAN_SAVED) * width)
+    _on_device(x=x, update=update, y=y, gate=gate, starts=starts, state=state, final=final, slots=slots, saved=saved, workspace=workspace)
+    call("pxh_gated_scan_forward", ptr(x), ptr(update), ptr(gate), ptr(y), ptr(starts), ptr(state), ptr(final), ptr(slots), ptr(saved), kind, rows,
+         width, count, slot_count, x_stride, *strides, *_space(workspace), _stream())
+    return y
+
+
+def gated_scan_backward(dy, x, update, saved, dx, dupdate, gate=None, dgate=None, starts=None, sequences=None, state=None, d_final=None,
+                        d_state=None, slots=None, workspace=None):
+    """The gradients of gated_scan_forward, from its inputs and what it saved.  state: what the sequences began with (not what a
+    forward pass in place has left there).  d_final: the gradient of final, d_state: that of state; they may be one tensor."""
+    if _layer("pxh_gated_scan_backward", dy, x, update, saved, dx, dupdate, gate, dgate, starts, sequences, state, d_final, d_state, slots, workspace):
+        return dx
+    rows, width, dy_stride = _rows(dy, "dy")
+    kind = _type(dy, "dy")
+    strides = [_like(t, name, dy.shape, dy.dtype) for name, t in (("x", _given(x, "x")), ("update", _given(update, "update")), ("gate", gate), ("dx", _given(dx, "dx")),
+                                                                  ("dupdate", _given(dupdate, "dupdate")), ("dgate", dgate))]
+    count = _sequences(dy, rows, starts, sequences)
+    slot_count = _states(count, width, slots, state=state, d_final=d_final, d_state=d_state)
+    _vector(saved, "saved", -(-rows // SCAN_SAVED) * width)
+    _on_device(dy=dy, x=x, update=update, saved=saved, dx=dx, dupdate=dupdate, gate=gate, dgate=dgate, starts=starts, state=state, d_final=d_final,
+               d_state=d_state, slots=slots, workspace=workspace)
+    call("pxh_gated_scan_backward", ptr(dy), ptr(x), ptr(update), ptr(gate), ptr(saved), ptr(dx), ptr(dupdate), ptr(dgate), ptr(starts), ptr(state),
+         ptr(d_final), ptr(d_state), ptr(slots), kind, rows, width, count, slot_count, dy_stride, *strides, *_space(workspace), _stream())
+    return dx
+
+
+def gated_scan_step(x, update, y, state, gate=None, slots=None):
+    """One new token for each of x's rows: gated_scan_forward for sequences of one token, with `state` in place."""
+    if _layer("pxh_gated_scan_step", x, update, y, state, gate, slots):
+        return y
+    rows, width, x_stride = _rows(x, "x")
+    kind = _type(x, "x")
+    strides = [_like(t, name, x.shape, x.dtype) for name, t in (("update", _given(update, "update")), ("gate", gate), ("y", _given(y, "y")))]
+    slot_count = _states(rows, width, slots, state=_given(state, "state"))
+    _on_device(x=x, update=update, y=y, state=state, gate=gate, slots=slots)
+    call("pxh_gated_scan_step", ptr(x), ptr(update), ptr(gate), ptr(y), ptr(state), ptr(slots), kind, rows, width, slot_count, x_stride, *strides, _stream())
+    return y
 
 
 DETECTION_DTYPE = workloads.DETECTION_DTYPE
