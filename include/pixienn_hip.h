@@ -751,6 +751,26 @@ int pxh_gated_scan_step(const void* x, const void* update, const void* gate, voi
                         long long rows, int width, int slot_count, long long x_stride, long long update_stride,
                         long long gate_stride, long long y_stride, void* stream);
 
+/* Beam search: of every item's `beams` beams (at most 64) the `count` best continuations (at most PXH_MOST_ALTERNATIVES), by
+ *   score[beam][token] = scores[beam] + scale * logits[beam][token] - log sum exp (scale * logits[beam])
+ * descending; of equal ones the lower beam's first, then the lower token.  logits: [batch * beams][vocab]; scores: [batch][beams], what the
+ * beams have come to.  A beam that is ended (nullable, [batch][beams], not 0) has one continuation, end_token with the score that it has.
+ * out_scores, parents (the beams) and tokens are [batch][count].  A score of minus infinity (a masked token, a beam that is not
+ * there yet) and one that is no number (a beam whose logits hold a NaN or plus infinity) are no continuations; the places for
+ * which there is none have a score of minus infinity, and -1 for parent and token.  Scores are formed and compared in 64 bits from sums in
+ * fp32, and rounded once.  out_scores may be scores where count is beams.
+ * workspace: pxh_beam_select_workspace_bytes(batch, beams, vocab, count), which serves fewer of each too, or NULL for the library's. */
+size_t pxh_beam_select_workspace_bytes(int batch, int beams, int vocab, int count);
+int pxh_beam_select(const void* logits, const float* scores, const unsigned char* ended, float* out_scores, int* parents,
+                    int* tokens, int type, int batch, int beams, int vocab, long long stride, int count, int end_token, float scale,
+                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* Tensors with a row for each beam, in the beams' new order, in place: row (item, k) becomes what row (item, parents[item][k]) was.
+ * A parent outside [0, beams) leaves the row as it is.  tensors, row_bytes and strides (bytes from row to row) are HOST arrays of
+ * `count`: the states of layers, histories of tokens, of any type; one launch for every 32 of them.  The tensors may not overlap. */
+int pxh_beam_reorder(int count, void* const* tensors, const long long* row_bytes, const long long* strides, const int* parents,
+                     int batch, int beams, void* stream);
+
 /* AdamW over all parameter tensors of a model at once, from a table kept on the device, with states in 32 or in 8 bits and the
  * gradients clipped by their common norm:
  *   norm = |d_scale * d|_2 over all tensors;  f = max_norm > 0 and norm > max_norm ? max_norm / norm : 1

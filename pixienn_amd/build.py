@@ -12,7 +12,7 @@ LIB = os.path.join(PKG, "libpixienn_hip.so")
 CALLS = os.path.join(PKG, "_calls.so")
 
 SOURCES = ["runtime.hip", "epilogue.hip", "resident_fwd.hip", "resident_bwd.hip", "grouped_bwd.hip", "elementwise.hip", "pool.hip", "yolo.hip", "nms.hip",
-           "rmsnorm.hip", "tokens.hip", "adamw.hip", "embedding.hip", "layernorm.hip", "scan.hip"]
+           "rmsnorm.hip", "tokens.hip", "adamw.hip", "embedding.hip", "layernorm.hip", "scan.hip", "beam.hip"]
 
 # -ffp-contract=off: the bit-exact kernels must not fuse a*b+c; packed fp32 VALU forms are
 # switched off for every kernel.

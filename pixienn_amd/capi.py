@@ -98,6 +98,8 @@ SIGNATURES = {
     "pxh_gated_scan_forward": [P, P, P, P, P, P, P, P, P, I, L, I, I, I, L, L, L, L, P, Z, P],
     "pxh_gated_scan_backward": [P, P, P, P, P, P, P, P, P, P, P, P, P, I, L, I, I, I, L, L, L, L, L, L, L, P, Z, P],
     "pxh_gated_scan_step": [P, P, P, P, P, P, I, L, I, I, L, L, L, L, P],
+    "pxh_beam_select": [P, P, P, P, P, P, I, I, I, I, L, I, I, F, P, Z, P],
+    "pxh_beam_reorder": [I, P, P, P, P, I, I, P],
     "pxh_token_logprobs_forward_train": [P, P, P, P, P, P, P, P, I, I, L, I, L, L, F, P],
 }
 _OTHER_RETURNS = {
@@ -120,6 +122,7 @@ _OTHER_RETURNS = {
     "pxh_embedding_workspace_bytes": (Z, [L, I]),
     "pxh_layer_norm_workspace_bytes": (Z, [L, I]),
     "pxh_gated_scan_workspace_bytes": (Z, [L, I]),
+    "pxh_beam_select_workspace_bytes": (Z, [I, I, I, I]),
 }
 # test hooks (pixienn_amd/csrc/pixienn_hip_test.h): exported, but not part of the C ABI
 _TEST_HOOKS = {

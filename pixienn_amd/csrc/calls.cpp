@@ -13,6 +13,7 @@
 #include <tuple>
 #include <type_traits>
 #include <utility>
+#include <vector>
 
 namespace {
 
@@ -622,6 +623,70 @@ PyObject* gated_scan_step(PyObject* self, PyObject* const* args, Py_ssize_t coun
     });
 }
 
+// A packed tensor of two dimensions.
+template<typename V>
+V* table_of(const Device& d, PyObject* o, at::ScalarType type, long long& rows, long long& columns)
+{
+    const at::Tensor& t = d.tensor(o);
+    if (t.dim() != 2 || (rows >= 0 && t.size(0) != rows) || (columns >= 0 && t.size(1) != columns)) throw NotHere{};
+    rows = t.size(0);
+    columns = t.size(1);
+    return d.packed<V>(o, rows * columns, type);
+}
+
+// (logits, scores, out_scores, parents, tokens, ended, end_token, scale, workspace)
+PyObject* beam_select(PyObject* self, PyObject* const* args, Py_ssize_t count)
+{
+    return on_device<&pxh_beam_select, 9>(self, args, count, [](PyObject* const* a, const Device& d, auto f) {
+        const Rows logits = needed(d.rows(a[0]));
+        long long batch = -1, beams = -1, best = -1;
+        const float* const scores = table_of<float>(d, a[1], at::kFloat, batch, beams);
+        float* const out = table_of<float>(d, a[2], at::kFloat, batch, best);
+        int* const parents = table_of<int>(d, a[3], at::kInt, batch, best);
+        int* const tokens = table_of<int>(d, a[4], at::kInt, batch, best);
+        if (logits.rows != batch * beams) throw NotHere{};
+        const unsigned char* ended = nullptr;
+        if (a[5] != Py_None) {
+            const at::ScalarType type = d.tensor(a[5]).scalar_type();
+            if (type != at::kBool && type != at::kByte) throw NotHere{};
+            ended = d.packed<unsigned char>(a[5], batch * beams, type);
+        }
+        const int end_token = argument<int>(a[6]), vocab = fits(logits.width);
+        const float scale = argument<float>(a[7]);
+        const Space space = d.space(a[8]);
+        const int items = fits(batch), of_item = fits(beams), continuations = fits(best);
+        return status([&] {
+            return f(logits.data, scores, ended, out, parents, tokens, logits.type, items, of_item, vocab, logits.stride, continuations, end_token, scale,
+                     space.data, space.bytes, d.stream);
+        });
+    });
+}
+
+// ([tensors], parents)
+PyObject* beam_reorder(PyObject* self, PyObject* const* args, Py_ssize_t count)
+{
+    return on_device<&pxh_beam_reorder, 2>(self, args, count, [](PyObject* const* a, const Device& d, auto f) {
+        if (!PyList_CheckExact(a[0])) throw NotHere{};
+        long long batch = -1, beams = -1;
+        const int* const parents = table_of<int>(d, a[1], at::kInt, batch, beams);
+        const Py_ssize_t n = PyList_GET_SIZE(a[0]);
+        std::vector<void*> data(n);
+        std::vector<long long> bytes(n), strides(n);
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            const at::Tensor& t = d.tensor(PyList_GET_ITEM(a[0], i));
+            if (t.dim() == 0 || t.size(0) != batch * beams) throw NotHere{};
+            const long long rows = t.size(0), size = static_cast<long long>(t.element_size());
+            bytes[i] = rows ? t.numel() / rows * size : 0;
+            if (t.is_contiguous()) strides[i] = bytes[i];
+            else if (t.dim() == 2 && (t.stride(1) == 1 || t.size(1) == 1)) strides[i] = rows > 1 ? t.stride(0) * size : bytes[i];
+            else throw NotHere{};
+            data[i] = t.data_ptr();
+        }
+        const int tensors = fits(n), items = fits(batch), of_item = fits(beams);
+        return status([&] { return f(tensors, data.data(), bytes.data(), strides.data(), parents, items, of_item, d.stream); });
+    });
+}
+
 #define FUNCTION(name) \
     PyMethodDef { "pxh_" #name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&name)), METH_FASTCALL, nullptr }
 
@@ -629,7 +694,8 @@ PyMethodDef functions[] = { FUNCTION(rms_norm_forward), FUNCTION(rms_norm_backwa
                             FUNCTION(token_logprobs_backward), FUNCTION(token_logprobs_forward_train) };
 
 PyMethodDef layers[] = { FUNCTION(embedding_forward), FUNCTION(embedding_backward), FUNCTION(layer_norm_forward), FUNCTION(layer_norm_backward),
-                         FUNCTION(gated_scan_forward), FUNCTION(gated_scan_backward), FUNCTION(gated_scan_step) };
+                         FUNCTION(gated_scan_forward), FUNCTION(gated_scan_backward), FUNCTION(gated_scan_step),
+                         FUNCTION(beam_select), FUNCTION(beam_reorder) };
 
 // bind_function(name, address) -> the callable that takes a Python function's own arguments and the stream, or None
 PyObject* bind_function(PyObject*, PyObject* args)

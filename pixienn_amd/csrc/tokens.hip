@@ -1,5 +1,6 @@
 // Log probabilities of given tokens, entropy, the most probable alternatives, and the gradient of the logits.
 #include "stream.h"
+#include "tokens.h"
 #include "typed.h"
 
 #include <cmath>
@@ -98,6 +99,7 @@ struct TokenArgs {
     const float* lse_in;
     const float* entropy_in;
     void* dlogits;
+    float2* row_sums;       // nullable: the rows' largest logits and sums
     long long rows, stride, d_stride;
     int vocab, wide, top;
     float scale;
@@ -584,8 +586,12 @@ __global__ __launch_bounds__(LANES, K == kThirdVectors ? 6 : 1) void token_logpr
     mine.load(logits, a.vocab, static_cast<int>(part) * p.vectors, p.vectors);
     const Sums s = group_join<LANES>(mine.template sums<ENTROPY>(logits, c), c, slots);
     RowResult result{};
-    if (whole) result = finish_row(a, row, s, target, given, threadIdx.x == 0);
-    else if (threadIdx.x == 0) p.sums[blockIdx.x] = s;
+    if (whole) {
+        result = finish_row(a, row, s, target, given, threadIdx.x == 0);
+        if (a.row_sums && threadIdx.x == 0) a.row_sums[row] = make_float2(s.peak, s.sum);
+    } else if (threadIdx.x == 0) {
+        p.sums[blockIdx.x] = s;
+    }
     if (a.top) {
         // a lane of NaNs has minus infinity for its peak, which need not be a value of the row: no floor comes from there
         const float peak = mine.peak * a.scale;
@@ -622,6 +628,7 @@ __global__ __launch_bounds__(kBlock) void token_join_few_kernel(TokenArgs a, Par
     if (lane < p.parts) s = p.sums[row * p.parts + lane];
     s = group_join<kWave>(s, c, nullptr);
     const RowResult result = finish_row(a, row, s, target, given, lane == 0);
+    if (a.row_sums && lane == 0) a.row_sums[row] = make_float2(s.peak, s.sum);
     int larger = 0;
     for (int j = 0; j < n; ++j) larger += key_of_lane(mine, j) > mine;
     if (lane < n && larger < a.top) {
@@ -649,6 +656,7 @@ __global__ __launch_bounds__(kBlock) void token_join_kernel(TokenArgs a, Parts p
     }
     s = group_join<kBlock>(s, c, slots);
     const RowResult result = finish_row(a, row, s, target, given, threadIdx.x == 0);
+    if (a.row_sums && threadIdx.x == 0) a.row_sums[row] = make_float2(s.peak, s.sum);
     if (a.top) {
         const unsigned long long* keys = p.keys + static_cast<size_t>(row) * p.parts * a.top;
         const int n = p.parts * a.top;
@@ -1118,6 +1126,7 @@ int by_rows(const TokenArgs& a, int type, const F& launch)
             if (*f) *f += done;
         for (const float** f: { &p.d_logp, &p.d_entropy, &p.lse_in, &p.entropy_in })
             if (*f) *f += done;
+        if (a.row_sums) p.row_sums += done;
         if (a.top) {
             p.top_logp += done * a.top;
             p.top_ids += done * a.top;
@@ -1141,6 +1150,20 @@ int check_tokens(const char* who, const void* logits, int type, int wide, long l
 }
 
 }  // namespace
+
+size_t token_rows_workspace_bytes(long long rows, int vocab, int top) { return pxh_token_logprobs_workspace_bytes(rows, vocab, top); }
+
+int token_rows(const char* who, const void* logits, int type, long long rows, int vocab, long long stride, int top, float scale,
+               float* values, int* ids, float2* sums, void* workspace, hipStream_t s)
+{
+    TokenArgs a{};
+    a.logits = logits; a.top_logp = values; a.top_ids = ids; a.row_sums = sums; a.rows = rows; a.stride = stride; a.vocab = vocab;
+    a.top = top; a.scale = scale;
+    int rc = PXH_OK;
+    dispatch_type(type, [&]<int T>() { rc = by_rows(a, T, [&](const TokenArgs& p) { return launch_forward<T, false>(who, p, workspace, s); }); });
+    return rc;
+}
+
 }  // namespace pxh
 
 using namespace pxh;

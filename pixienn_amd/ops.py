@@ -1097,6 +1097,64 @@ def gated_scan_step(x, update, y, state, gate=None, slots=None):
     return y
 
 
+def beam_select_workspace_bytes(batch, beams, vocab, count):
+    return int(capi.load().pxh_beam_select_workspace_bytes(batch, beams, vocab, count))
+
+
+def beam_select(logits, scores, out_scores, parents, tokens, ended=None, end_token=0, scale=1.0, workspace=None):
+    """Of every item's beams the best continuations: scores [batch, beams] (fp32) plus the log probabilities of logits [batch * beams,
+    vocab], times `scale`.  out_scores (fp32), parents (the beams) and tokens (int32) are [batch, count], descending, of equal ones
+    the lower beam's and the lower token first; -1 and minus infinity where there are fewer.  A beam that is ended ([batch, beams], bool)
+    has one continuation: end_token, with the score that it has."""
+    if _layer("pxh_beam_select", logits, scores, out_scores, parents, tokens, ended, end_token, scale, workspace):
+        return
+    rows, vocab, stride = _rows(logits, "logits")
+    kind = _type(logits, "logits")
+    for name, t, dtype in (("scores", scores, _F32), ("out_scores", out_scores, _F32), ("parents", parents, torch.int32), ("tokens", tokens, torch.int32)):
+        _chk(_given(t, name), dtype, name)
+        if t.dim() != 2:
+            raise PxError("%s must have two dimensions (got %s)" % (name, tuple(t.shape)))
+    batch, beams = scores.shape
+    if rows != batch * beams:
+        raise PxError("logits must have a row for each of %d x %d beams (got %d)" % (batch, beams, rows))
+    count = out_scores.shape[1]
+    for name, t in (("out_scores", out_scores), ("parents", parents), ("tokens", tokens)):
+        if tuple(t.shape) != (batch, count):
+            raise PxError("%s must be of shape %s (got %s)" % (name, (batch, count), tuple(t.shape)))
+    if ended is not None:
+        _vector(ended, "ended", rows, torch.uint8 if getattr(ended, "dtype", None) is torch.uint8 else torch.bool)
+    _on_device(logits=logits, scores=scores, out_scores=out_scores, parents=parents, tokens=tokens, ended=ended, workspace=workspace)
+    call("pxh_beam_select", ptr(logits), ptr(scores), ptr(ended), ptr(out_scores), ptr(parents), ptr(tokens), kind, batch, beams, vocab, stride, count,
+         int(end_token), float(scale), *_space(workspace), _stream())
+
+
+def beam_reorder(tensors, parents):
+    """Tensors of any type with a row for each beam ([batch * beams, ...]) in the beams' new order, in place: row (item, k) becomes
+    what row (item, parents[item, k]) was; a parent outside the beams (-1) leaves it as it is.  parents: int32 [batch, beams]."""
+    tensors = list(tensors)
+    if _layer("pxh_beam_reorder", tensors, parents):
+        return
+    _chk(_given(parents, "parents"), torch.int32, "parents")
+    if parents.dim() != 2:
+        raise PxError("parents must be [batch, beams] (got %s)" % (tuple(parents.shape),))
+    batch, beams = parents.shape
+    table = []
+    for t in tensors:
+        if not _given(t, "a tensor of beams").is_cuda:
+            _chk(t, t.dtype, "a tensor of beams")
+        if t.dim() == 0 or t.shape[0] != batch * beams:
+            raise PxError("a tensor of beams must have %d x %d rows (got %s)" % (batch, beams, tuple(t.shape)))
+        rows = t.reshape(t.shape[0], -1) if t.is_contiguous() and t.numel() else t
+        if t.numel() and (rows.dim() != 2 or rows.shape[1] > 1 and rows.stride(1) != 1):
+            raise PxError("a tensor of beams must have the values of a row next to each other")
+        size = t.element_size()
+        row_bytes = t.numel() // max(1, t.shape[0]) * size
+        table.append((t.data_ptr(), row_bytes, rows.stride(0) * size if t.shape[0] > 1 and t.numel() else row_bytes))
+    _on_device(parents=parents, **{"tensor %d of beams" % i: t for i, t in enumerate(tensors)})
+    arrays = [(ctypes.c_longlong * max(1, len(table)))(*column) for column in (zip(*table) if table else ((), (), ()))]
+    call("pxh_beam_reorder", len(table), *arrays, ptr(parents), batch, beams, _stream())
+
+
 DETECTION_DTYPE = workloads.DETECTION_DTYPE
 
 
