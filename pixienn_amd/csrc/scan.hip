@@ -49,13 +49,25 @@ __device__ __forceinline__ float gated(float h, float o)
     return y;
 }
 
-constexpr int kSteps = 16;              // tokens of a wave, and from one saved state to the next
-constexpr int kWaves = 8;               // of a workgroup, one behind the other along the tokens
-constexpr int kChunk = kSteps * kWaves; // tokens of a workgroup
-constexpr int kV = 2;                   // channels of a lane
-constexpr int kTile = kV * kWave;       // ... and of a workgroup
-constexpr int kScanLanes = kWaves * kWave;
-constexpr uint32_t kAll = (1u << kSteps) - 1;
+// Channels of a lane, four bytes of a row: 16 tokens of a few tensors and what is formed of them fit the registers.  And of a workgroup.
+template<int T>
+constexpr int kChannels = 4 / kSize<T>;
+template<int T>
+constexpr int kTileOf = kChannels<T> * kWave;
+constexpr int kSaved = PXH_SCAN_SAVED;  // tokens from one saved state to the next
+
+// Tokens of a wave, and waves of a workgroup, one behind the other along the tokens.
+template<int STEPS, int WAVES>
+struct Shape {
+    static constexpr int kSteps = STEPS, kWaves = WAVES, kChunk = STEPS * WAVES, kLanes = WAVES * kWave;
+    static constexpr uint32_t kAll = (1u << STEPS) - 1;
+    static_assert(kSaved % STEPS == 0 && kChunk % kSaved == 0, "a saved state is in front of a wave's tokens");
+};
+// Two workgroups of eight waves to a unit.  Chunks of 64 tokens pay twice for what a chunk costs whatever its length (a number, a word, a
+// look back: 8 x 4096 x 2048 bf16 with a gate 134 us where 128 take 105).  The gradients keep three values for each that they read:
+// waves of 16 tokens spill (430 us, and 180).
+using Forward = Shape<16, 8>;
+using Backward = Shape<8, 8>;
 
 // Where sequences begin: starts[sequences + 1], or all of one length.
 struct Sequences {
@@ -77,34 +89,40 @@ __device__ __forceinline__ int slot_of(const Slots& slots, int s)
     return slot >= 0 && slot < slots.count ? slot : -1;
 }
 
-// What the wave has to know of its tokens first .. first + kSteps: a bit each, for those that begin a sequence, end one, and lie in
+// What the wave has to know of its tokens first .. first + STEPS: a bit each, for those that begin a sequence, end one, and lie in
 // one; lane i knows the sequence of token i.
 struct Borders {
     uint32_t begins, ends, active;
     int sequence;
 };
 
+// The last of n ascending places that is not behind t, or -1.
+__device__ __forceinline__ int last_in_front(const int* starts, int n, int t)
+{
+    int low = 0;
+    while (n > 0) {
+        const int half = n / 2;
+        if (starts[low + half] <= t) {
+            low += half + 1;
+            n -= half + 1;
+        } else {
+            n = half;
+        }
+    }
+    return low - 1;
+}
+
+template<int STEPS>
 __device__ __forceinline__ Borders borders_of(const Sequences& q, int first)
 {
     const int lane = threadIdx.x % kWave;
     const int t = first + lane;
-    const bool mine = lane < kSteps && t < q.rows;
+    const bool mine = lane < STEPS && t < q.rows;
     bool begins = false, ends = false, active = false;
     int s = 0;
     if (mine) {
         if (q.starts) {
-            // the last sequence that begins at or in front of t
-            int low = 0, n = q.count + 1;
-            while (n > 0) {
-                const int half = n / 2;
-                if (q.starts[low + half] <= t) {
-                    low += half + 1;
-                    n -= half + 1;
-                } else {
-                    n = half;
-                }
-            }
-            s = low - 1;
+            s = last_in_front(q.starts, q.count + 1, t);
             if (s >= 0 && s < q.count) {
                 active = true;
                 begins = q.starts[s] == t;
@@ -124,6 +142,20 @@ __device__ __forceinline__ Borders borders_of(const Sequences& q, int first)
     return Borders{ static_cast<uint32_t>(__ballot(begins)), static_cast<uint32_t>(__ballot(ends)), static_cast<uint32_t>(__ballot(active)), s };
 }
 
+// Whether tokens first .. first + n are all there, and none of them begins a sequence, ends one or lies in none: then most of what a
+// workgroup has to look at, token by token, is not there.
+__device__ __forceinline__ bool lies_within_one(const Sequences& q, int first, int n)
+{
+    if (first + n > q.rows) return false;
+    if (!q.starts) {
+        uint32_t which, place;
+        q.length.divmod(first, which, place);
+        return place > 0 && place + n < q.length.d;
+    }
+    const int s = last_in_front(q.starts, q.count + 1, first);
+    return s >= 0 && s < q.count && q.starts[s] < first && q.starts[s + 1] > first + n && first + n < q.rows;
+}
+
 // ---------------------------------------------------------------- from chunk to chunk
 // Workgroups take numbers, chunk by chunk along the tokens (for the gradients against them).  Each leaves what its chunk does to a
 // state, channel by channel, as one 64-bit word, and once it knows the state in front of it the one behind it as a range with Z = 1.  It
@@ -133,7 +165,8 @@ __device__ __forceinline__ Borders borders_of(const Sequences& q, int first)
 // makes the exit unconditional all the same; where it was reached (two launches at once on one workspace, which the interface
 // forbids) the states are NaN.
 constexpr unsigned long long kNotThere = ~0ull;     // no range: a Z that is no number is left as 1, with its H
-constexpr int kWindow = 8;
+// (2 chunks: 105 us, 4: 107, 8: 111, for want of registers)
+constexpr int kWindow = 2;
 constexpr uint32_t kLooks = 1u << 22;
 
 struct Exchange {
@@ -189,39 +222,39 @@ __device__ __forceinline__ float look_back(const unsigned long long* words, uint
     return s;
 }
 
+template<int WAVES, int TILE>
 struct ScanShared {
-    Range ranges[kWaves][kTile];
-    float states[kWaves][kTile];        // in front of each wave's tokens
+    Range ranges[WAVES][TILE];
+    float states[WAVES][TILE];         // in front of each wave's tokens
+    float passed[WAVES][TILE];         // from wave to wave
     uint32_t number, fresh;             // fresh: no state reaches the chunk
 };
 
 // Takes the workgroup's number: chunk and tile.
-__device__ __forceinline__ void take_number(const Exchange& x, ScanShared& lds, uint32_t& chunk, uint32_t& tile)
+template<int WAVES, int TILE>
+__device__ __forceinline__ void take_number(const Exchange& x, ScanShared<WAVES, TILE>& lds, uint32_t& chunk, uint32_t& tile)
 {
     uint32_t number = blockIdx.x;
     if (x.words) {
         if (threadIdx.x == 0) lds.number = atomicAdd(x.counter, 1u);
         __syncthreads();
-        number = lds.number;
+        number = __builtin_amdgcn_readfirstlane(lds.number);
     }
     x.by_tiles.divmod(number, chunk, tile);
 }
 
-// From the waves' ranges, in the order `order(0 .. kWaves - 1)`, and the chunks in front of `chunk`: the state in front of every wave.
-template<typename Order>
-__device__ __forceinline__ void join_waves(const Exchange& x, ScanShared& lds, uint32_t chunk, uint32_t tile, int width, const Order& order)
+// From the waves' ranges, in the order `order(0 .. WAVES - 1)`, and the chunks in front of `chunk`: the state in front of every wave.
+template<int WAVES, int TILE, typename Order>
+__device__ __forceinline__ void join_waves(const Exchange& x, ScanShared<WAVES, TILE>& lds, uint32_t chunk, uint32_t tile, int width, const Order& order)
 {
     __syncthreads();
     const int c = threadIdx.x;
-    if (c < kTile) {            // whole waves
-        const int e = static_cast<int>(tile) * kTile + c;
+    if (c < TILE) {            // whole waves
+        const int e = static_cast<int>(tile) * TILE + c;
         const bool there = e < width;
-        Range own[kWaves], all{ 0.0f, 0.0f };
+        Range all{ 0.0f, 0.0f };
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            own[w] = lds.ranges[order(w)][c];
-            all = joined(all, own[w]);
-        }
+        for (int w = 0; w < WAVES; ++w) all = joined(all, lds.ranges[order(w)][c]);
         float s = 0.0f;
         if (x.words) {
             unsigned long long* const word = x.words + e;
@@ -235,9 +268,9 @@ __device__ __forceinline__ void join_waves(const Exchange& x, ScanShared& lds, u
             }
         }
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = 0; w < WAVES; ++w) {
             lds.states[order(w)][c] = s;
-            s = behind(s, own[w]);
+            s = behind(s, lds.ranges[order(w)][c]);
         }
     }
     __syncthreads();
@@ -261,43 +294,102 @@ __global__ __launch_bounds__(kBlock) void scan_start_kernel(unsigned long long* 
     }
 }
 
-// kV channels of a row of fp32 states.
-__device__ __forceinline__ void load_state(const float* states, int slot, int e, int width, float (&s)[kV])
+// V channels of a row of fp32 states.
+template<int V>
+__device__ __forceinline__ void load_state(const float* states, int slot, int e, int width, float (&s)[V])
 {
 #pragma unroll
-    for (int k = 0; k < kV; ++k) s[k] = states && slot >= 0 && e + k < width ? states[static_cast<size_t>(slot) * width + e + k] : 0.0f;
+    for (int k = 0; k < V; ++k) s[k] = states && slot >= 0 && e + k < width ? states[static_cast<size_t>(slot) * width + e + k] : 0.0f;
 }
 
-__device__ __forceinline__ void store_state(float* states, int slot, int e, int width, const float (&s)[kV])
+template<bool NT = false, int V>
+__device__ __forceinline__ void store_state(float* states, int slot, int e, int width, const float (&s)[V])
 {
-#pragma unroll
-    for (int k = 0; k < kV; ++k)
-        if (slot >= 0 && e + k < width) states[static_cast<size_t>(slot) * width + e + k] = s[k];
+    if (slot < 0 || e >= width) return;
+    Raw<PXH_F32, V> r;
+    r.set(s);
+    store_row<PXH_F32, V, NT>(states + static_cast<size_t>(slot) * width, e, width, r);
 }
 
-// The wave's kSteps tokens of a tensor, kV channels a lane; tokens behind the last row repeat it, channels behind the last one are
-// zeros.  No branch around a load.
-template<int T>
-__device__ __forceinline__ void load_tokens(const void* p, long long stride, int first, int rows, int e, int width, bool inside, Raw<T, kV> (&r)[kSteps])
+// Channels of a lane in rows of a tensor: a place that is the workgroup's and a byte offset of the lane's own, one for all rows.
+struct Columns {
+    int tile_first, e, width;       // the workgroup's first channel and the lane's
+    bool inside;                    // the workgroup's channels are all there
+};
+
+// The wave's tokens of a tensor, a word a lane; tokens behind the last row repeat it, channels behind the last one are zeros.  No
+// branch around a load: a lane at the end of a row reads the row's last word, and takes what is its own.
+template<int T, int STEPS>
+__device__ __forceinline__ void load_tokens(const void* p, long long stride, int first, int rows, const Columns& c, Raw<T, kChannels<T>> (&r)[STEPS])
 {
-    if (inside) {
+    constexpr int V = kChannels<T>;
+    const int last = rows - 1 - first;                  // of the wave's tokens; where none is there, all are the last row
+    const char* row = row_of<T>(p, last < 0 ? rows - 1 : first, stride);
+    const size_t step = static_cast<size_t>(stride) * kSize<T>;
+    if (c.inside) {
+        row += static_cast<size_t>(c.tile_first) * kSize<T>;
+        const uint32_t offset = static_cast<uint32_t>(c.e - c.tile_first) * kSize<T>;
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) r[i] = load_raw<T, kV>(row_of<T>(p, min(first + i, rows - 1), stride), e);
+        for (int i = 0; i < STEPS; ++i) {
+            r[i] = load_raw_at<T, V>(row, offset);
+            row += i < last ? step : 0;
+        }
+    } else if (c.width >= V) {
+        const int at = min(c.e, c.width - V), beyond = c.e - at;
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) {
+            r[i] = load_raw<T, V>(row, at);
+            row += i < last ? step : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) r[i].w[0] = beyond == 0 ? r[i].w[0] : V == 2 && beyond == 1 ? r[i].w[0] >> 16 : 0u;
     } else {
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) r[i] = load_end<T, kV>(row_of<T>(p, min(first + i, rows - 1), stride), e, width);
+        for (int i = 0; i < STEPS; ++i) {
+            float x[V] = {};
+            const float only = load_one<T>(row, 0);
+            x[0] = c.e == 0 ? only : 0.0f;
+            r[i].set(x);
+            row += i < last ? step : 0;
+        }
     }
 }
 
-template<int T>
-__device__ __forceinline__ void store_token(void* p, long long stride, int t, int e, int width, bool inside, const float (&v)[kV])
+// Values as they were read, to be unpacked again: unpacked they would be kept, in twice the registers.
+template<int T, int STEPS>
+__device__ __forceinline__ void as_read(Raw<T, kChannels<T>> (&r)[STEPS])
 {
-    Raw<T, kV> r;
-    r.set(v);
-    char* const row = row_of<T>(p, t, stride);
-    if (inside) store_raw<T, kV>(row, e, r);
-    else if (e < width) store_row<T, kV>(row, e, width, r);
+    if constexpr (T != PXH_F32) {
+#pragma unroll
+        for (int i = 0; i < STEPS; ++i) asm volatile("" : "+v"(r[i].w[0]));
+    }
 }
+
+// The rows of a tensor that a wave writes, one behind the other or against the tokens.
+template<int T, bool NT>
+struct Writer {
+    static constexpr int kV = kChannels<T>;
+    char* row;
+    long long step;
+    const Columns& c;
+
+    __device__ __forceinline__ Writer(void* p, long long stride, int first, const Columns& columns, bool against = false)
+        : row(row_of<T>(static_cast<char*>(p) + (columns.inside ? static_cast<size_t>(columns.tile_first) * kSize<T> : 0), first, stride)),
+          step(stride * kSize<T> * (against ? -1 : 1)), c(columns) {}
+
+    // RARE: not of all tokens, or not all channels
+    template<bool RARE>
+    __device__ __forceinline__ void put(bool active, const float (&v)[kV])
+    {
+        Raw<T, kV> r;
+        r.set(v);
+        if (!RARE || active) {
+            if (!RARE || c.inside) store_raw_at<T, kV, NT>(row, static_cast<uint32_t>(c.e - c.tile_first) * kSize<T>, r);
+            else if (c.e < c.width) store_row<T, kV, NT>(row, c.e, c.width, r);
+        }
+        row += step;
+    }
+};
 
 // ---------------------------------------------------------------- forward
 struct ScanArgs {
@@ -307,7 +399,7 @@ struct ScanArgs {
     void* y;
     const float* state;
     float* final;
-    float* saved;               // [rows / kSteps, rounded up][width]: in front of every kSteps-th token
+    float* saved;               // [rows / kSaved, rounded up][width]: in front of every kSaved-th token
     long long x_stride, update_stride, gate_stride, y_stride;
     Sequences q;
     Slots slots;
@@ -315,53 +407,50 @@ struct ScanArgs {
     int width;
 };
 
-// A workgroup takes kChunk tokens of kTile channels, a wave kSteps of them, which stay in registers as z and x between the pass that finds
+// A workgroup takes a chunk of tokens of kTile channels, a wave a few of them, which stay in registers as z and x between the pass that finds
 // what they do to a state and the one that forms the states: one trip to memory.
-template<int T, bool GATE>
-__global__ __launch_bounds__(kScanLanes) void scan_kernel(ScanArgs a)
+template<int T, bool GATE, bool NT>
+__global__ __launch_bounds__(Forward::kLanes, 4) void scan_kernel(ScanArgs a)
 {
-    __shared__ ScanShared lds;
+    constexpr int kSteps = Forward::kSteps, kChunk = Forward::kChunk, kV = kChannels<T>, kTile = kTileOf<T>;
+    __shared__ ScanShared<Forward::kWaves, kTile> lds;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
     uint32_t chunk, tile;
     take_number(a.exchange, lds, chunk, tile);
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
     const int first = static_cast<int>(chunk) * kChunk + wave * kSteps;
     const int e = static_cast<int>(tile) * kTile + lane * kV;
-    const bool inside = (static_cast<int>(tile) + 1) * kTile <= a.width;
+    const Columns columns{ static_cast<int>(tile) * kTile, e, a.width, (static_cast<int>(tile) + 1) * kTile <= a.width };
     Raw<T, kV> x[kSteps], u[kSteps], o[GATE ? kSteps : 1];
-    load_tokens<T>(a.x, a.x_stride, first, a.q.rows, e, a.width, inside, x);
-    load_tokens<T>(a.update, a.update_stride, first, a.q.rows, e, a.width, inside, u);
-    if constexpr (GATE) load_tokens<T>(a.gate, a.gate_stride, first, a.q.rows, e, a.width, inside, o);
-    const Borders b = borders_of(a.q, first);
-    if (threadIdx.x == 0) lds.fresh = b.begins & 1;
-    float z[kSteps][kV];
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-        float v[kV], rest;
-        u[i].get(v);
-#pragma unroll
-        for (int k = 0; k < kV; ++k) gate_of<T>(v[k], z[i][k], rest);
-    }
-    float h[kV] = {}, Z[kV] = {};
-    const auto take = [&](int i) {
-        float v[kV];
-        x[i].get(v);
-#pragma unroll
-        for (int k = 0; k < kV; ++k) {
-            Z[k] += fmaf(-z[i][k], Z[k], z[i][k]);
-            h[k] = fmaf(z[i][k], v[k] - h[k], h[k]);
-        }
-    };
-    const bool plain = b.begins == 0 && b.active == kAll;
-    if (plain) {
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) take(i);
-    } else {
+    load_tokens<T, kSteps>(a.x, a.x_stride, first, a.q.rows, columns, x);
+    load_tokens<T, kSteps>(a.update, a.update_stride, first, a.q.rows, columns, u);
+    const auto pass = [&]<bool RARE>() {
+        Borders b{ 0, 0, Forward::kAll, 0 };
+        if constexpr (RARE) b = borders_of<kSteps>(a.q, first);
+        if (threadIdx.x == 0) lds.fresh = b.begins & 1;
+        float z[kSteps][kV];
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
-            if (!(b.active >> i & 1)) continue;
-            const bool begins = b.begins >> i & 1;
+            float v[kV], rest;
+            u[i].get(v);
+#pragma unroll
+            for (int k = 0; k < kV; ++k) gate_of<T>(v[k], z[i][k], rest);
+        }
+        // into the updates' registers
+        if constexpr (GATE) load_tokens<T, kSteps>(a.gate, a.gate_stride, first, a.q.rows, columns, o);
+        float h[kV] = {}, Z[kV] = {};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const bool begins = RARE && (b.begins >> i & 1), active = !RARE || (b.active >> i & 1);
             if (begins) load_state(a.state, a.state ? slot_of(a.slots, __builtin_amdgcn_readlane(b.sequence, i)) : -1, e, a.width, h);
-            take(i);
+            float v[kV];
+            x[i].get(v);
+#pragma unroll
+            for (int k = 0; k < kV; ++k) {
+                if (RARE) z[i][k] = active ? z[i][k] : 0.0f;
+                const float ahead = active ? v[k] - h[k] : 0.0f;
+                Z[k] += fmaf(-z[i][k], Z[k], z[i][k]);
+                h[k] = fmaf(z[i][k], ahead, h[k]);
+            }
             if (begins) {
                 // the second pass takes the state from here: by then `final`, which may be `state`, may have been written
 #pragma unroll
@@ -371,51 +460,38 @@ __global__ __launch_bounds__(kScanLanes) void scan_kernel(ScanArgs a)
                 }
             }
         }
-    }
 #pragma unroll
-    for (int k = 0; k < kV; ++k) lds.ranges[wave][lane * kV + k] = Range{ Z[k], h[k] };
-    join_waves(a.exchange, lds, chunk, tile, a.width, [](int w) { return w; });
+        for (int k = 0; k < kV; ++k) lds.ranges[wave][lane * kV + k] = Range{ Z[k], h[k] };
+        join_waves(a.exchange, lds, chunk, tile, a.width, [](int w) { return w; });
+        as_read(x);
 #pragma unroll
-    for (int k = 0; k < kV; ++k) h[k] = lds.states[wave][lane * kV + k];
-    if (a.saved && first < a.q.rows) store_state(a.saved, first / kSteps, e, a.width, h);
-    const auto give = [&](int i) {
-        float v[kV];
-#pragma unroll
-        for (int k = 0; k < kV; ++k) v[k] = h[k];
-        if constexpr (GATE) {
-            float w[kV];
-            o[i].get(w);
-#pragma unroll
-            for (int k = 0; k < kV; ++k) v[k] = gated<T>(h[k], w[k]);
-        }
-        store_token<T>(a.y, a.y_stride, first + i, e, a.width, inside, v);
-    };
-    const auto step = [&](int i) {
-        float v[kV];
-        x[i].get(v);
-#pragma unroll
-        for (int k = 0; k < kV; ++k) h[k] = fmaf(z[i][k], v[k] - h[k], h[k]);
-    };
-    if (plain && b.ends == 0) {
+        for (int k = 0; k < kV; ++k) h[k] = lds.states[wave][lane * kV + k];
+        if (a.saved && first % kSaved == 0 && first < a.q.rows) store_state<NT>(a.saved, first / kSaved, e, a.width, h);
+        Writer<T, NT> y(a.y, a.y_stride, first, columns);
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
-            step(i);
-            give(i);
-        }
-        return;
-    }
+            const bool begins = RARE && (b.begins >> i & 1), active = !RARE || (b.active >> i & 1);
+            float v[kV];
+            x[i].get(v);
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-        if (!(b.active >> i & 1)) continue;
-        if (b.begins >> i & 1) {
+            for (int k = 0; k < kV; ++k) {
+                const float ahead = active ? v[k] - h[k] : 0.0f;
+                h[k] = begins ? z[i][k] : fmaf(z[i][k], ahead, h[k]);
+                v[k] = h[k];
+            }
+            if constexpr (GATE) {
+                float w[kV];
+                o[i].get(w);
 #pragma unroll
-            for (int k = 0; k < kV; ++k) h[k] = z[i][k];
-        } else {
-            step(i);
+                for (int k = 0; k < kV; ++k) v[k] = gated<T>(h[k], w[k]);
+            }
+            y.template put<RARE>(active, v);
+            if (RARE && a.final && (b.ends >> i & 1))
+                store_state(a.final, slot_of(a.slots, __builtin_amdgcn_readlane(b.sequence, i)), e, a.width, h);
         }
-        give(i);
-        if (a.final && (b.ends >> i & 1)) store_state(a.final, slot_of(a.slots, __builtin_amdgcn_readlane(b.sequence, i)), e, a.width, h);
-    }
+    };
+    if (columns.inside && lies_within_one(a.q, static_cast<int>(chunk) * kChunk, kChunk)) pass.template operator()<false>();
+    else pass.template operator()<true>();
 }
 
 // ---------------------------------------------------------------- backward
@@ -441,95 +517,158 @@ struct ScanBackwardArgs {
     int width;
 };
 
-template<int T, bool GATE>
-__global__ __launch_bounds__(kScanLanes, 4) void scan_backward_kernel(ScanBackwardArgs a)
+template<int T, bool GATE, bool NT>
+__global__ __launch_bounds__(Backward::kLanes, 4) void scan_backward_kernel(ScanBackwardArgs a)
 {
-    __shared__ ScanShared lds;
+    constexpr int kSteps = Backward::kSteps, kWaves = Backward::kWaves, kChunk = Backward::kChunk, kV = kChannels<T>, kTile = kTileOf<T>;
+    __shared__ ScanShared<kWaves, kTile> lds;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
     uint32_t turn, tile;
     take_number(a.exchange, lds, turn, tile);
     const uint32_t chunk = a.exchange.chunks - 1 - turn;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
     const int first = static_cast<int>(chunk) * kChunk + wave * kSteps;
     const int e = static_cast<int>(tile) * kTile + lane * kV;
-    const bool inside = (static_cast<int>(tile) + 1) * kTile <= a.width;
+    const Columns columns{ static_cast<int>(tile) * kTile, e, a.width, (static_cast<int>(tile) + 1) * kTile <= a.width };
     Raw<T, kV> x[kSteps], u[kSteps], dy[kSteps], o[GATE ? kSteps : 1];
-    load_tokens<T>(a.update, a.update_stride, first, a.q.rows, e, a.width, inside, u);
-    load_tokens<T>(a.x, a.x_stride, first, a.q.rows, e, a.width, inside, x);
-    load_tokens<T>(a.dy, a.dy_stride, first, a.q.rows, e, a.width, inside, dy);
-    if constexpr (GATE) load_tokens<T>(a.gate, a.gate_stride, first, a.q.rows, e, a.width, inside, o);
+    load_tokens<T, kSteps>(a.update, a.update_stride, first, a.q.rows, columns, u);
+    load_tokens<T, kSteps>(a.x, a.x_stride, first, a.q.rows, columns, x);
+    load_tokens<T, kSteps>(a.dy, a.dy_stride, first, a.q.rows, columns, dy);
+    if constexpr (GATE) load_tokens<T, kSteps>(a.gate, a.gate_stride, first, a.q.rows, columns, o);
     float h[kV];
-    load_state(a.saved, first < a.q.rows ? first / kSteps : -1, e, a.width, h);
-    const Borders b = borders_of(a.q, first);
-    if (wave == kWaves - 1 && lane == 0) lds.fresh = b.ends >> (kSteps - 1) & 1;
-    float z[kSteps][kV], g[kSteps][kV], w[kSteps][kV];
+    load_state(a.saved, first % kSaved == 0 && first < a.q.rows ? first / kSaved : -1, e, a.width, h);
+    const auto pass = [&]<bool RARE>() {
+        Borders b{ 0, 0, Backward::kAll, 0 };
+        if constexpr (RARE) b = borders_of<kSteps>(a.q, first);
+        if (wave == kWaves - 1 && lane == 0) lds.fresh = b.ends >> (kSteps - 1) & 1;
+        const auto begin = [&](int i) {
+            if (b.begins >> i & 1) load_state(a.state, a.state ? slot_of(a.slots, __builtin_amdgcn_readlane(b.sequence, i)) : -1, e, a.width, h);
+        };
+        float z[kSteps][kV], w[kSteps][kV], g[kSteps][kV];         // w: z (1 - z), then times x - h
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-        const bool active = b.active >> i & 1;
-        if (b.begins >> i & 1) load_state(a.state, a.state ? slot_of(a.slots, __builtin_amdgcn_readlane(b.sequence, i)) : -1, e, a.width, h);
-        float v[kV], d[kV];
-        u[i].get(v);
-        x[i].get(d);
-        dy[i].get(g[i]);
-#pragma unroll
-        for (int k = 0; k < kV; ++k) {
-            float rest;
-            gate_of<T>(v[k], z[i][k], rest);
-            const float ahead = d[k] - h[k];
-            w[i][k] = ahead * (z[i][k] * rest);
-            h[k] = active ? fmaf(z[i][k], ahead, h[k]) : h[k];
-        }
-        if constexpr (GATE) {
-            float p[kV], dgate[kV];
-            o[i].get(p);
+        for (int i = 0; i < kSteps; ++i) {
+            float v[kV];
+            u[i].get(v);
 #pragma unroll
             for (int k = 0; k < kV; ++k) {
-                float s, rest;
-                gate_of<T>(p[k], s, rest);
-                dgate[k] = g[i][k] * h[k] * (s * fmaf(p[k], rest, 1.0f));
-                g[i][k] *= p[k] * s;
+                float rest;
+                gate_of<T>(v[k], z[i][k], rest);
+                w[i][k] = z[i][k] * rest;
             }
-            if (active) store_token<T>(a.dgate, a.dgate_stride, first + i, e, a.width, inside, dgate);
         }
-        if (a.d_final && (b.ends >> i & 1)) {
-            float more[kV];
-            load_state(a.d_final, slot_of(a.slots, __builtin_amdgcn_readlane(b.sequence, i)), e, a.width, more);
+        if (RARE && b.active != Backward::kAll) {
+            // tokens of no sequence leave everything as it is
 #pragma unroll
-            for (int k = 0; k < kV; ++k) g[i][k] += more[k];
+            for (int i = 0; i < kSteps; ++i) {
+                const bool active = b.active >> i & 1;
+#pragma unroll
+                for (int k = 0; k < kV; ++k) z[i][k] = active ? z[i][k] : 0.0f;
+#pragma unroll
+                for (int k = 0; k < Raw<T, kV>::kWords; ++k) {
+                    x[i].w[k] = active ? x[i].w[k] : 0u;
+                    dy[i].w[k] = active ? dy[i].w[k] : 0u;
+                    if constexpr (GATE) o[i].w[k] = active ? o[i].w[k] : 0u;
+                }
+            }
         }
-    }
-    float C[kV] = {}, Z[kV] = {};
+        if constexpr (kSteps < kSaved) {
+            // a state is saved for every few waves: the others have theirs from the one in front
 #pragma unroll
-    for (int i = kSteps - 1; i >= 0; --i) {
-        if (!(b.active >> i & 1)) continue;
-        const bool ends = b.ends >> i & 1;
+            for (int part = 0; part + 1 < kSaved / kSteps; ++part) {
+                if (wave % (kSaved / kSteps) == part) {
+                    float was[kV];
 #pragma unroll
-        for (int k = 0; k < kV; ++k) {
-            const float G = ends ? g[i][k] : g[i][k] + C[k];
-            C[k] = fmaf(-z[i][k], G, G);
-            Z[k] = ends ? 1.0f : Z[k] + fmaf(-z[i][k], Z[k], z[i][k]);
+                    for (int k = 0; k < kV; ++k) was[k] = h[k];
+#pragma unroll
+                    for (int i = 0; i < kSteps; ++i) {
+                        if (RARE) begin(i);
+                        float v[kV];
+                        x[i].get(v);
+#pragma unroll
+                        for (int k = 0; k < kV; ++k) h[k] = fmaf(z[i][k], v[k] - h[k], h[k]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < kV; ++k) {
+                        lds.passed[wave + 1][lane * kV + k] = h[k];
+                        h[k] = was[k];
+                    }
+                }
+                __syncthreads();
+                as_read(x);
+                if (wave % (kSaved / kSteps) == part + 1) {
+#pragma unroll
+                    for (int k = 0; k < kV; ++k) h[k] = lds.passed[wave][lane * kV + k];
+                }
+            }
         }
-    }
+        Writer<T, NT> out(a.dgate, a.dgate_stride, first, columns);
 #pragma unroll
-    for (int k = 0; k < kV; ++k) lds.ranges[wave][lane * kV + k] = Range{ Z[k], C[k] };
-    join_waves(a.exchange, lds, turn, tile, a.width, [](int k) { return kWaves - 1 - k; });
+        for (int i = 0; i < kSteps; ++i) {
+            if (RARE) begin(i);
+            float d[kV];
+            x[i].get(d);
+            dy[i].get(g[i]);
 #pragma unroll
-    for (int k = 0; k < kV; ++k) C[k] = lds.states[wave][lane * kV + k];
+            for (int k = 0; k < kV; ++k) {
+                const float ahead = d[k] - h[k];
+                w[i][k] *= ahead;
+                h[k] = fmaf(z[i][k], ahead, h[k]);
+            }
+            if constexpr (GATE) {
+                float p[kV], dgate[kV];
+                o[i].get(p);
 #pragma unroll
-    for (int i = kSteps - 1; i >= 0; --i) {
-        if (!(b.active >> i & 1)) continue;
-        const bool ends = b.ends >> i & 1;
-        float dx[kV], du[kV];
+                for (int k = 0; k < kV; ++k) {
+                    float s, rest;
+                    gate_of<T>(p[k], s, rest);
+                    dgate[k] = g[i][k] * h[k] * (s * fmaf(p[k], rest, 1.0f));
+                    g[i][k] *= p[k] * s;
+                }
+                out.template put<RARE>(b.active >> i & 1, dgate);
+                __builtin_amdgcn_sched_barrier(0);      // a token's gate after the other's: all at once they want more registers than there are
+            }
+            if (RARE && a.d_final && (b.ends >> i & 1)) {
+                float more[kV];
+                load_state(a.d_final, slot_of(a.slots, __builtin_amdgcn_readlane(b.sequence, i)), e, a.width, more);
 #pragma unroll
-        for (int k = 0; k < kV; ++k) {
-            const float G = ends ? g[i][k] : g[i][k] + C[k];
-            dx[k] = z[i][k] * G;
-            du[k] = w[i][k] * G;
-            C[k] = G - dx[k];
+                for (int k = 0; k < kV; ++k) g[i][k] += more[k];
+            }
         }
-        store_token<T>(a.dx, a.dx_stride, first + i, e, a.width, inside, dx);
-        store_token<T>(a.dupdate, a.dupdate_stride, first + i, e, a.width, inside, du);
-        if (a.d_state && (b.begins >> i & 1)) store_state(a.d_state, slot_of(a.slots, __builtin_amdgcn_readlane(b.sequence, i)), e, a.width, C);
-    }
+        float C[kV] = {}, Z[kV] = {};
+#pragma unroll
+        for (int i = kSteps - 1; i >= 0; --i) {
+            const bool ends = RARE && (b.ends >> i & 1);
+#pragma unroll
+            for (int k = 0; k < kV; ++k) {
+                const float G = ends ? g[i][k] : g[i][k] + C[k];
+                C[k] = fmaf(-z[i][k], G, G);
+                Z[k] = ends ? 1.0f : Z[k] + fmaf(-z[i][k], Z[k], z[i][k]);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kV; ++k) lds.ranges[wave][lane * kV + k] = Range{ Z[k], C[k] };
+        join_waves(a.exchange, lds, turn, tile, a.width, [](int k) { return kWaves - 1 - k; });
+#pragma unroll
+        for (int k = 0; k < kV; ++k) C[k] = lds.states[wave][lane * kV + k];
+        Writer<T, NT> out_x(a.dx, a.dx_stride, first + kSteps - 1, columns, true), out_u(a.dupdate, a.dupdate_stride, first + kSteps - 1, columns, true);
+#pragma unroll
+        for (int i = kSteps - 1; i >= 0; --i) {
+            const bool ends = RARE && (b.ends >> i & 1), active = !RARE || (b.active >> i & 1);
+            float dx[kV], du[kV];
+#pragma unroll
+            for (int k = 0; k < kV; ++k) {
+                const float G = ends ? g[i][k] : g[i][k] + C[k];
+                dx[k] = z[i][k] * G;
+                du[k] = w[i][k] * G;
+                C[k] = G - dx[k];
+            }
+            out_x.template put<RARE>(active, dx);
+            out_u.template put<RARE>(active, du);
+            if (RARE && a.d_state && (b.begins >> i & 1))
+                store_state(a.d_state, slot_of(a.slots, __builtin_amdgcn_readlane(b.sequence, i)), e, a.width, C);
+        }
+    };
+    if (columns.inside && lies_within_one(a.q, static_cast<int>(chunk) * kChunk, kChunk)) pass.template operator()<false>();
+    else pass.template operator()<true>();
 }
 
 // ---------------------------------------------------------------- one token of each sequence
@@ -583,10 +722,17 @@ __global__ __launch_bounds__(kBlock) void scan_step_kernel(StepArgs a)
 }
 
 // ---------------------------------------------------------------- host
-size_t chunks_of(long long rows) { return (static_cast<size_t>(rows) + kChunk - 1) / kChunk; }
+size_t chunks_of(long long rows, int chunk) { return (static_cast<size_t>(rows) + chunk - 1) / chunk; }
 
 // The words' counter in front of them.
 constexpr size_t kCounterBytes = 256;
+
+// Whether `tensors` of the tokens' size do not fit the caches: then results are stored past them (8 x 4096 x 2048 bf16 without a gate, no
+// chunk waiting for another, 79 -> 61 us).
+bool streams(long long rows, int width, int type, int tensors)
+{
+    return static_cast<size_t>(rows) * static_cast<size_t>(width) * size_of(type) * tensors >= kStreamingBytes;
+}
 
 int check_scan(const char* who, int type, long long rows, int width, int sequences, const int* starts, const int* slots, int slot_count, bool states)
 {
@@ -602,13 +748,15 @@ int check_scan(const char* who, int type, long long rows, int width, int sequenc
 }
 
 // Sequences of the call, and the words that its chunks exchange (none where every chunk begins and ends with a sequence).
-int start_scan(const char* who, long long rows, int width, int sequences, const int* starts, const Slots& slots, const float* from, float* to,
+template<typename S>
+int start_scan(const char* who, int type, long long rows, int width, int sequences, const int* starts, const Slots& slots, const float* from, float* to,
                void* workspace, size_t workspace_bytes, Sequences& q, Exchange& x, uint32_t& groups, hipStream_t s)
 {
     const long long length = starts || sequences == 0 ? 0 : rows / sequences;
     q = Sequences{ starts, FastDiv(length > 0 ? static_cast<uint32_t>(length) : 1), sequences, static_cast<int>(rows) };
-    const size_t chunks = chunks_of(rows), tiles = (static_cast<size_t>(width) + kTile - 1) / kTile;
-    if (chunks * tiles * kScanLanes >= 1ull << 32) return fail_invalid("%s: too many rows of too many values", who);
+    constexpr int kChunk = S::kChunk;
+    const size_t chunks = chunks_of(rows, kChunk), tile = 4 / size_of(type) * kWave, tiles = (static_cast<size_t>(width) + tile - 1) / tile;
+    if (chunks * tiles * S::kLanes >= 1ull << 32) return fail_invalid("%s: too many rows of too many values", who);
     groups = static_cast<uint32_t>(chunks * tiles);
     x = Exchange{ nullptr, nullptr, static_cast<uint32_t>(chunks), FastDiv(static_cast<uint32_t>(tiles)) };
     size_t count = 0;
@@ -641,7 +789,7 @@ extern "C" {
 size_t pxh_gated_scan_workspace_bytes(long long rows, int width)
 {
     if (rows <= 0 || width <= 0) return 0;
-    return kCounterBytes + chunks_of(rows) * static_cast<size_t>(width) * sizeof(unsigned long long);
+    return kCounterBytes + chunks_of(rows, Forward::kChunk < Backward::kChunk ? Forward::kChunk : Backward::kChunk) * static_cast<size_t>(width) * sizeof(unsigned long long);
 }
 
 int pxh_gated_scan_forward(const void* x, const void* update, const void* gate, void* y, const int* starts, const float* state, float* final,
@@ -656,11 +804,13 @@ int pxh_gated_scan_forward(const void* x, const void* update, const void* gate, 
     ScanArgs a{ x, update, gate, y, state, final, saved, x_stride, update_stride, gate_stride, y_stride, {}, Slots{ slots, slot_count }, {}, width };
     uint32_t groups;
     hipStream_t s = as_stream(stream);
-    if (int rc = start_scan(who, rows, width, sequences, starts, a.slots, state, final, workspace, workspace_bytes, a.q, a.exchange, groups, s)) return rc;
+    if (int rc = start_scan<Forward>(who, type, rows, width, sequences, starts, a.slots, state, final, workspace, workspace_bytes, a.q, a.exchange, groups, s)) return rc;
     if (rows == 0) return PXH_OK;
     dispatch_type(type, [&]<int T>() {
-        if (gate) hipLaunchKernelGGL((scan_kernel<T, true>), dim3(groups), dim3(kScanLanes), 0, s, a);
-        else hipLaunchKernelGGL((scan_kernel<T, false>), dim3(groups), dim3(kScanLanes), 0, s, a);
+        const bool past = streams(rows, width, type, gate ? 4 : 3);
+        const auto kernel = gate ? (past ? &scan_kernel<T, true, true> : &scan_kernel<T, true, false>)
+                                 : (past ? &scan_kernel<T, false, true> : &scan_kernel<T, false, false>);
+        hipLaunchKernelGGL(kernel, dim3(groups), dim3(Forward::kLanes), 0, s, a);
     });
     return check_launch(who);
 }
@@ -682,12 +832,14 @@ int pxh_gated_scan_backward(const void* dy, const void* x, const void* update, c
                         dx_stride, dupdate_stride, dgate_stride, {}, Slots{ slots, slot_count }, {}, width };
     uint32_t groups;
     hipStream_t s = as_stream(stream);
-    if (int rc = start_scan(who, rows, width, sequences, starts, a.slots, d_final, d_state, workspace, workspace_bytes, a.q, a.exchange, groups, s))
+    if (int rc = start_scan<Backward>(who, type, rows, width, sequences, starts, a.slots, d_final, d_state, workspace, workspace_bytes, a.q, a.exchange, groups, s))
         return rc;
     if (rows == 0) return PXH_OK;
     dispatch_type(type, [&]<int T>() {
-        if (gate) hipLaunchKernelGGL((scan_backward_kernel<T, true>), dim3(groups), dim3(kScanLanes), 0, s, a);
-        else hipLaunchKernelGGL((scan_backward_kernel<T, false>), dim3(groups), dim3(kScanLanes), 0, s, a);
+        const bool past = streams(rows, width, type, gate ? 7 : 5);
+        const auto kernel = gate ? (past ? &scan_backward_kernel<T, true, true> : &scan_backward_kernel<T, true, false>)
+                                 : (past ? &scan_backward_kernel<T, false, true> : &scan_backward_kernel<T, false, false>);
+        hipLaunchKernelGGL(kernel, dim3(groups), dim3(Backward::kLanes), 0, s, a);
     });
     return check_launch(who);
 }
