@@ -54,6 +54,37 @@ __global__ __launch_bounds__(kBlock) void embedding_kernel(LookupArgs a)
 // The rows are sorted by token, those of one token in their own order; then every 32 consecutive ones are added up run by run, runs that go
 // on beyond their 32 in a launch behind it, part after part.  No order depends on which workgroup comes first.
 
+// -- zeros.  Sorting keeps a few units busy for some microseconds, in which the others write zeros to the table's first rows, whether
+// a row has their token or not; the rows behind those wait for the sums, which know which of them have none.
+struct Zeros {
+    char* d;
+    long long first, rows, stride_bytes, row_bytes;
+    FastDiv by_row;             // pieces of 16 bytes of a row
+    uint32_t groups;            // workgroups, each of kZeroPieces pieces a lane
+};
+
+constexpr int kZeroPieces = 8;
+
+template<int LANES>
+__device__ __forceinline__ void write_zeros(const Zeros& z, uint32_t group)
+{
+    typedef uint32_t words __attribute__((ext_vector_type(4), aligned(1)));
+    const uint32_t base = group * (LANES * kZeroPieces) + threadIdx.x;
+#pragma unroll
+    for (int j = 0; j < kZeroPieces; ++j) {
+        uint32_t row, piece;
+        z.by_row.divmod(base + j * LANES, row, piece);
+        if (row >= z.rows) return;
+        char* const at = z.d + (z.first + row) * z.stride_bytes + static_cast<size_t>(piece) * 16;
+        const long long left = z.row_bytes - static_cast<long long>(piece) * 16;
+        if (left >= 16) {
+            *global_memory<words>(at) = words{};
+        } else {
+            for (long long k = 0; k < left; k += 2) *global_memory<uint16_t>(at + k) = 0;
+        }
+    }
+}
+
 // -- sorting: tiles of 2048 rows by one workgroup each, then up to 32 sorted tiles at a time into one.
 constexpr int kTile = 2048, kSortLanes = 1024, kFanIn = 32;
 constexpr uint32_t kNoToken = ~0u;          // behind the last row: larger than any token
@@ -71,8 +102,12 @@ __device__ __forceinline__ void compare(Key& a, Key& b, bool up)
 
 template<typename Key>
 __global__ __launch_bounds__(kSortLanes) void sort_tile_kernel(const void* tokens, bool wide, long long rows, int vocab, uint32_t* sorted_tokens,
-                                                               uint32_t* sorted_rows)
+                                                               uint32_t* sorted_rows, uint32_t tiles, Zeros zeros)
 {
+    if (blockIdx.x >= tiles) {
+        write_zeros<kSortLanes>(zeros, blockIdx.x - tiles);
+        return;
+    }
     constexpr int kShift = sizeof(Key) == 4 ? 11 : 32;
     __shared__ Key keys[kTile];
     const long long first = static_cast<long long>(blockIdx.x) * kTile;
@@ -145,8 +180,73 @@ __device__ __forceinline__ uint32_t places_below(const uint32_t* sorted, uint32_
     return low;
 }
 
-// Up to kFanIn neighbouring tiles of `tile` rows into one: a row's place is the number of rows in front of it in each.
-__global__ __launch_bounds__(kBlock) void merge_tiles_kernel(const uint32_t* tokens, const uint32_t* rows, uint32_t* out_tokens, uint32_t* out_rows,
+// Up to kFanIn neighbouring tiles into one: a row's place is the number of rows in front of it in each, of those of the same token in the
+// tiles in front too.  A workgroup takes kMerged rows of one tile, and kSides tiles at a time into LDS (a step of a search in memory that
+// another XCD has written waits 0.7 us); each of its four parts searches two of them for every row.
+constexpr int kSides = 8, kMerged = 256, kMergeLanes = 1024, kParts = kMergeLanes / kMerged;
+
+__global__ __launch_bounds__(kMergeLanes) void merge_tiles_kernel(const uint32_t* tokens, const uint32_t* rows, uint32_t* out_tokens, uint32_t* out_rows,
+                                                                  uint32_t count)
+{
+    __shared__ uint32_t lists[kSides][kTile];
+    __shared__ uint32_t counts[kParts][kMerged];
+    const uint32_t begin = blockIdx.x * kMerged, own = begin / kTile, first = own / kFanIn * kFanIn;
+    const uint32_t tiles = count / kTile + (count % kTile != 0);
+    const uint32_t last = first + kFanIn < tiles ? first + kFanIn : tiles;
+    const uint32_t part = threadIdx.x / kMerged, i = begin + threadIdx.x % kMerged;
+    const uint32_t token = tokens[i < count ? i : 0], row = rows[i < count ? i : 0];
+    uint32_t below = 0;
+    for (uint32_t t = first; t < last; t += kSides) {
+        __syncthreads();
+        const uint32_t base = t * kTile;
+        // all of them asked for before the first is waited for; the list's memory goes on to the next 64 words
+        constexpr int kLoads = kSides * kTile / (4 * kMergeLanes);
+        typedef uint32_t words __attribute__((ext_vector_type(4)));
+        words w[kLoads];
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const uint32_t at = base + (j * kMergeLanes + threadIdx.x) * 4;
+            w[j] = *reinterpret_cast<const words*>(tokens + (at < count ? at : 0));
+        }
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+            const uint32_t at = (j * kMergeLanes + threadIdx.x) * 4;
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) w[j][k] = base + at + k < count ? w[j][k] : kNoToken;
+            *reinterpret_cast<words*>(&lists[0][0] + at) = w[j];
+        }
+        __syncthreads();
+        // step by step in all of the part's lists at once; a list behind the last one holds kNoToken, and nothing below a token
+        constexpr int kOwn = kSides / kParts;
+        uint32_t low[kOwn] = {};
+        const auto look = [&](uint32_t step) {
+            uint32_t seen[kOwn];
+#pragma unroll
+            for (int j = 0; j < kOwn; ++j) seen[j] = lists[part * kOwn + j][low[j] + step - 1];
+#pragma unroll
+            for (int j = 0; j < kOwn; ++j) low[j] += (t + part * kOwn + j < own ? seen[j] <= token : seen[j] < token) ? step : 0;
+        };
+#pragma unroll
+        for (uint32_t step = kTile / 2; step; step /= 2) look(step);
+        look(1);
+#pragma unroll
+        for (int j = 0; j < kOwn; ++j) {
+            const uint32_t list = t + part * kOwn + j;
+            below += list < last && list != own ? low[j] : 0;
+        }
+    }
+    counts[part][threadIdx.x % kMerged] = below;
+    __syncthreads();
+    if (part != 0 || i >= count) return;
+    uint32_t place = first * kTile + (i - own * kTile);
+#pragma unroll
+    for (int k = 0; k < kParts; ++k) place += counts[k][threadIdx.x];
+    out_tokens[place] = token;
+    out_rows[place] = row;
+}
+
+// The same for larger tiles, of more than 65536 rows, in memory.
+__global__ __launch_bounds__(kBlock) void merge_large_kernel(const uint32_t* tokens, const uint32_t* rows, uint32_t* out_tokens, uint32_t* out_rows,
                                                              uint32_t count, uint32_t tile)
 {
     const uint32_t i = blockIdx.x * kBlock + threadIdx.x;
@@ -163,7 +263,7 @@ __global__ __launch_bounds__(kBlock) void merge_tiles_kernel(const uint32_t* tok
 }
 
 // -- sums
-constexpr int kRun = 32;            // sorted rows that a workgroup adds up
+constexpr int kMostRun = 32, kLeastRun = 4;             // sorted rows that a workgroup adds up
 
 struct TableGradientArgs {
     const char* dy;
@@ -172,44 +272,59 @@ struct TableGradientArgs {
     const uint32_t* rows;
     float* partial;                 // [chunks][2][width]: of the run that goes on from the chunk before, of the one that goes on behind it
     long long dy_stride, d_stride;
-    uint32_t count, chunks;         // rows, and every kRun of them
+    uint32_t count, chunks;         // rows, and every `run` of them
+    int run;
+    uint32_t zeroed;                // rows of the table that hold zeros already
     int vocab, width, column_groups;
     float scale;
     bool accumulate;
 };
 
-template<int T, int D, int V>
-__device__ __forceinline__ void write_sum(const TableGradientArgs& a, uint32_t token, int e, const float (&sum)[V])
-{
-    constexpr int kPart = V * kSize<D> > 16 ? 16 / kSize<D> : V;
-    char* const d = row_of<D>(a.d, token, a.d_stride);
-#pragma unroll
-    for (int q = 0; q < V; q += kPart) {
-        if (e + q >= a.width) break;
-        float x[kPart] = {};
-        if (a.accumulate) load_row<D, kPart>(d, e + q, a.width).get(x);
-#pragma unroll
-        for (int k = 0; k < kPart; ++k) x[k] = fmaf(a.scale, sum[q + k], x[k]);
-        Raw<D, kPart> r;
-        r.set(x);
-        store_row<D, kPart>(d, e + q, a.width, r);
-    }
-}
+// V values of a row of the gradient, as many of them as one access takes at a time.
+template<int D, int V>
+struct TableRow {
+    static constexpr int kPart = V * kSize<D> > 16 ? 16 / kSize<D> : V, kParts = V / kPart;
+    Raw<D, kPart> r[kParts];
 
-// The first workgroups add up kRun sorted rows each (times column groups), the others, where the gradient is overwritten, write zeros to
+    __device__ __forceinline__ void load(const TableGradientArgs& a, uint32_t token, int e)
+    {
+        const char* const d = row_of<D>(a.d, token, a.d_stride);
+#pragma unroll
+        for (int q = 0; q < kParts; ++q)
+            if (e + q * kPart < a.width) r[q] = load_row<D, kPart>(d, e + q * kPart, a.width);
+    }
+
+    // the row with scale * sum added to what it holds
+    __device__ __forceinline__ void write(const TableGradientArgs& a, uint32_t token, int e, const float (&sum)[V])
+    {
+        char* const d = row_of<D>(a.d, token, a.d_stride);
+#pragma unroll
+        for (int q = 0; q < kParts; ++q) {
+            if (e + q * kPart >= a.width) break;
+            float x[kPart];
+            r[q].get(x);
+#pragma unroll
+            for (int k = 0; k < kPart; ++k) x[k] = fmaf(a.scale, sum[q * kPart + k], x[k]);
+            r[q].set(x);
+            store_row<D, kPart>(d, e + q * kPart, a.width, r[q]);
+        }
+    }
+};
+
+// The first workgroups add up a run of sorted rows each (times column groups), the others, where the gradient is overwritten, write zeros to
 // kZeroRows rows of the table each, where no row has their token.
 constexpr int kZeroRows = 32;
 
-template<int T, int D, int LANES>
-__global__ __launch_bounds__(LANES) void table_gradient_kernel(TableGradientArgs a, FastDiv by_columns)
+template<int T, int D, bool ADDS>
+__global__ __launch_bounds__(kBlock) void table_gradient_kernel(TableGradientArgs a, FastDiv by_columns)
 {
     constexpr int V = kVec<T>, kAhead = 8;
-    __shared__ uint32_t tokens[kRun + 2], rows[kRun];
+    __shared__ uint32_t tokens[kMostRun + 2], rows[kMostRun];
     uint32_t part, group;
     by_columns.divmod(blockIdx.x, part, group);
-    const int e = static_cast<int>(group * LANES + threadIdx.x) * V;
+    const int e = static_cast<int>(group * blockDim.x + threadIdx.x) * V;
     if (part >= a.chunks) {
-        const uint32_t first = (part - a.chunks) * kZeroRows;
+        const uint32_t first = a.zeroed + (part - a.chunks) * kZeroRows;
         if (threadIdx.x < kZeroRows) {
             const uint32_t token = first + threadIdx.x;
             bool empty = token < static_cast<uint32_t>(a.vocab);
@@ -231,10 +346,10 @@ __global__ __launch_bounds__(LANES) void table_gradient_kernel(TableGradientArgs
         }
         return;
     }
-    const uint32_t first = part * kRun;
-    const int n = static_cast<int>(a.count - first < static_cast<uint32_t>(kRun) ? a.count - first : kRun);
+    const uint32_t first = part * a.run;
+    const int n = static_cast<int>(a.count - first < static_cast<uint32_t>(a.run) ? a.count - first : a.run);
     // tokens[0] and tokens[n + 1]: those of the neighbours
-    for (int i = threadIdx.x; i < kRun + 2; i += LANES) {
+    for (int i = threadIdx.x; i < a.run + 2; i += blockDim.x) {
         const long long at = static_cast<long long>(first) + i - 1;
         tokens[i] = at >= 0 && at < a.count ? a.tokens[at] : kNoToken;
         if (i >= 1 && i <= n) rows[i - 1] = a.rows[at];
@@ -242,13 +357,16 @@ __global__ __launch_bounds__(LANES) void table_gradient_kernel(TableGradientArgs
     __syncthreads();
     if (e >= a.width) return;
     float sum[V] = {};
-    uint32_t begin = 0;             // place of the run's first row in the chunk
+    int begin = 0;                  // place of the run's first row in the chunk
     for (int base = 0; base < n; base += kAhead) {
         Raw<T, V> x[kAhead];
+        TableRow<D, V> old[ADDS ? kAhead : 1];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             const int i = min(base + j, n - 1);
             x[j] = load_row<T, V>(row_of<T>(a.dy, rows[i], a.dy_stride), e, a.width);
+            // what the run is added to, asked for with it
+            if (ADDS && tokens[i + 2] != tokens[i + 1] && tokens[i + 1] < static_cast<uint32_t>(a.vocab)) old[ADDS ? j : 0].load(a, tokens[i + 1], e);
         }
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
@@ -264,7 +382,8 @@ __global__ __launch_bounds__(LANES) void table_gradient_kernel(TableGradientArgs
             const bool goes_on_from = begin == 0 && tokens[0] == token;
             if (token < static_cast<uint32_t>(a.vocab)) {
                 if (ends && !goes_on_from) {
-                    write_sum<T, D, V>(a, token, e, sum);
+                    if (!ADDS) old[0] = TableRow<D, V>{};
+                    old[ADDS ? j : 0].write(a, token, e, sum);
                 } else {
                     float* const partial = a.partial + (static_cast<size_t>(part) * 2 + !goes_on_from) * a.width;
 #pragma unroll
@@ -285,7 +404,7 @@ __global__ __launch_bounds__(LANES) void table_gradient_kernel(TableGradientArgs
 
 // The runs that go on beyond a chunk, by the workgroup of the chunk in which they begin: 256 columns to a workgroup, whose waves share
 // the chunks.
-constexpr int kJoinLanes = 1024, kJoinColumns = 256;
+constexpr int kJoinLanes = 256, kJoinColumns = 256;
 
 template<int D>
 __global__ __launch_bounds__(kJoinLanes) void table_join_kernel(TableGradientArgs a, FastDiv by_columns)
@@ -294,21 +413,30 @@ __global__ __launch_bounds__(kJoinLanes) void table_join_kernel(TableGradientArg
     __shared__ float sums[kWaves][kJoinColumns];
     uint32_t part, group;
     by_columns.divmod(blockIdx.x, part, group);
-    const uint32_t first = part * kRun, next = first + kRun;
-    if (next >= a.count) return;
-    const uint32_t token = a.tokens[next];
-    if (token >= static_cast<uint32_t>(a.vocab) || a.tokens[next - 1] != token) return;
-    if (a.tokens[first] == token && first > 0 && a.tokens[first - 1] == token) return;       // begins further in front
-    // its end: the last chunk that has rows of it
-    const uint32_t end = next + places_below<true>(a.tokens + next, a.count - next, token);
-    const uint32_t last = (end - 1) / kRun;
+    const uint32_t first = part * a.run, next = first + a.run;
     const int wave = threadIdx.x / kWave, lane = threadIdx.x % kWave;
+    if (next >= a.count) return;
+    // the run's last chunk: those whose first row is of the token, looked at by as many lanes at once
+    const uint32_t in_front = first > 0 ? a.tokens[first - 1] : kNoToken, begin = a.tokens[first], before = a.tokens[next - 1];
+    const auto is_of = [&](uint32_t c, uint32_t token) { return c < a.chunks && a.tokens[c * a.run] == token; };
+    bool mine = is_of(part + 1 + lane, before);
+    const uint32_t token = before;
+    if (token >= static_cast<uint32_t>(a.vocab) || !__builtin_amdgcn_readfirstlane(mine)) return;
+    if (begin == token && in_front == token) return;       // begins further in front
+    uint32_t last = part;
+    for (;;) {
+        const unsigned long long no = ~__ballot(mine);
+        const int run = no ? __ffsll(no) - 1 : kWave;
+        last += run;
+        if (run < kWave) break;
+        mine = is_of(last + 1 + lane, token);
+    }
     const int e = static_cast<int>(group) * kJoinColumns + lane * 4;
     float sum[4] = {};
     if (e < a.width) {
         // part's second row of sums, then the first one of the chunks behind it
         const auto row = [&](uint32_t c) { return a.partial + (static_cast<size_t>(c) * 2 + (c == part)) * a.width; };
-        constexpr int kAhead = 4;
+        constexpr int kAhead = 8;
         uint32_t c = part + wave;
         for (; c + (kAhead - 1) * kWaves <= last; c += kAhead * kWaves) {
             Raw<PXH_F32, 4> x[kAhead];
@@ -329,12 +457,25 @@ __global__ __launch_bounds__(kJoinLanes) void table_join_kernel(TableGradientArg
     for (int k = 0; k < 4; ++k) sums[wave][lane * 4 + k] = sum[k];
     __syncthreads();
     if (wave != 0 || e >= a.width) return;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) sum[k] = 0.0f;
-    for (int w = 0; w < kWaves; ++w)
+    const int waves = last - part + 1 < static_cast<uint32_t>(kWaves) ? static_cast<int>(last - part + 1) : kWaves;
+    for (int w = 1; w < waves; ++w)
 #pragma unroll
         for (int k = 0; k < 4; ++k) sum[k] += sums[w][lane * 4 + k];
-    write_sum<D, D, 4>(a, token, e, sum);
+    TableRow<D, 4> d{};
+    if (a.accumulate) d.load(a, token, e);
+    d.write(a, token, e, sum);
+}
+
+// What the machine writes while it sorts: 8 us without, 11 with it.
+constexpr long long kZerosDuringSort = 48ll << 20;
+
+// Rows of a run: as many as leave a workgroup for each, and kEnoughChunks of them where there are rows for that.
+constexpr size_t kEnoughChunks = 768;
+int run_of(long long rows)
+{
+    int run = kMostRun;
+    while (run > kLeastRun && (rows + run / 2 - 1) / (run / 2) <= static_cast<long long>(kEnoughChunks)) run /= 2;
+    return run;
 }
 
 constexpr size_t align256(size_t b) { return (b + 255) & ~static_cast<size_t>(255); }
@@ -346,29 +487,26 @@ struct Space {
     {
         list = align256(static_cast<size_t>(rows) * 4);
         partial = 4 * list;
-        const size_t chunks = (static_cast<size_t>(rows) + kRun - 1) / kRun;
-        bytes = partial + align256(chunks * 2 * static_cast<size_t>(width) * sizeof(float));
+        // the fewest rows to a run are those of a call that makes few of them
+        const size_t chunks = (static_cast<size_t>(rows) + kMostRun - 1) / kMostRun, short_chunks = (static_cast<size_t>(rows) + kLeastRun - 1) / kLeastRun;
+        const size_t most = short_chunks < kEnoughChunks ? short_chunks : kEnoughChunks;
+        bytes = partial + align256((chunks > most ? chunks : most) * 2 * static_cast<size_t>(width) * sizeof(float));
     }
 };
-
-template<int T, int D, int LANES>
-void launch_sums(const TableGradientArgs& a, uint32_t groups, hipStream_t s)
-{
-    hipLaunchKernelGGL((table_gradient_kernel<T, D, LANES>), dim3(groups), dim3(LANES), 0, s, a, FastDiv(a.column_groups));
-}
 
 template<int T, int D>
 int launch_gradient(const char* who, TableGradientArgs a, hipStream_t s)
 {
+    // the vectors of a row in equal parts of at most kBlock (1025 fp32 values: 257 vectors are twice 192 lanes, not 256 and one)
     const int vectors = (a.width + kVec<T> - 1) / kVec<T>;
-    const int lanes = vectors <= 64 ? 64 : vectors <= 128 ? 128 : 256;
-    a.column_groups = (vectors + lanes - 1) / lanes;
-    const long long zero_groups = a.accumulate ? 0 : (static_cast<long long>(a.vocab) + kZeroRows - 1) / kZeroRows;
+    a.column_groups = (vectors + kBlock - 1) / kBlock;
+    const int lanes = ((vectors + a.column_groups - 1) / a.column_groups + kWave - 1) / kWave * kWave;
+    const long long zero_groups = (static_cast<long long>(a.vocab) - a.zeroed + kZeroRows - 1) / kZeroRows;
     const long long groups = (a.chunks + zero_groups) * a.column_groups;
     if (groups * lanes >= 1ll << 32 || groups >= 1ll << 31) return fail_invalid("%s: too many rows of too many values", who);
     if (groups == 0) return PXH_OK;
-    const auto go = lanes == 64 ? &launch_sums<T, D, 64> : lanes == 128 ? &launch_sums<T, D, 128> : &launch_sums<T, D, 256>;
-    go(a, static_cast<uint32_t>(groups), s);
+    const auto kernel = a.accumulate ? &table_gradient_kernel<T, D, true> : &table_gradient_kernel<T, D, false>;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(groups)), dim3(lanes), 0, s, a, FastDiv(a.column_groups));
     if (int rc = check_launch(who)) return rc;
     if (a.chunks <= 1) return PXH_OK;
     const int columns = (a.width + kJoinColumns - 1) / kJoinColumns;
@@ -444,11 +582,13 @@ int pxh_embedding_backward(const void* dy, const void* tokens, void* d, int type
     a.dy_stride = dy_stride;
     a.d_stride = d_stride;
     a.count = static_cast<uint32_t>(rows);
-    a.chunks = (a.count + kRun - 1) / kRun;
+    a.run = run_of(rows);
+    a.chunks = (a.count + a.run - 1) / a.run;
     a.vocab = vocab;
     a.width = width;
     a.scale = scale;
     a.accumulate = accumulate != 0;
+    a.zeroed = a.accumulate ? static_cast<uint32_t>(vocab) : 0;
     if (rows > 0) {
         const Space space(rows, width);
         void* ws = nullptr;
@@ -458,17 +598,31 @@ int pxh_embedding_backward(const void* dy, const void* tokens, void* d, int type
         for (int i = 0; i < 4; ++i) lists[i] = reinterpret_cast<uint32_t*>(base + i * space.list);
         a.partial = reinterpret_cast<float*>(base + space.partial);
         const uint32_t tiles = (a.count + kTile - 1) / kTile;
+        // zeros for a launch that takes some microseconds on a few units: `bytes` of them, from the rows that have none yet
+        const long long row_bytes = static_cast<long long>(width) * size_of(d_type), pieces = (row_bytes + 15) / 16;
+        const auto zeros = [&](long long bytes, int lanes) {
+            Zeros z{ a.d, a.zeroed, 0, d_stride * static_cast<long long>(size_of(d_type)), row_bytes, FastDiv(static_cast<uint32_t>(pieces)), 0 };
+            const long long left = vocab - static_cast<long long>(a.zeroed);
+            z.rows = bytes / row_bytes < left ? bytes / row_bytes : left;
+            z.groups = grid_for(static_cast<size_t>(z.rows) * pieces, static_cast<size_t>(lanes) * kZeroPieces);
+            a.zeroed += static_cast<uint32_t>(z.rows);
+            return z;
+        };
+        const Zeros during = zeros(kZerosDuringSort, kSortLanes);
         // token and place of the tile in 32 bits
-        if (vocab < (1 << 21) - 1)
-            hipLaunchKernelGGL((sort_tile_kernel<uint32_t>), dim3(tiles), dim3(kSortLanes), 0, s, tokens, wide_tokens != 0, rows, vocab, lists[0], lists[1]);
-        else
-            hipLaunchKernelGGL((sort_tile_kernel<unsigned long long>), dim3(tiles), dim3(kSortLanes), 0, s, tokens, wide_tokens != 0, rows, vocab, lists[0], lists[1]);
+        const auto sort = vocab < (1 << 21) - 1 ? &sort_tile_kernel<uint32_t> : &sort_tile_kernel<unsigned long long>;
+        hipLaunchKernelGGL(sort, dim3(tiles + during.groups), dim3(kSortLanes), 0, s, tokens, wide_tokens != 0, rows, vocab, lists[0], lists[1], tiles, during);
         if (int rc = check_launch(who)) return rc;
         int from = 0;
         for (unsigned long long tile = kTile; tile < a.count; tile *= kFanIn) {
             const int to = 2 - from;
-            hipLaunchKernelGGL(merge_tiles_kernel, dim3(grid_for(a.count, kBlock)), dim3(kBlock), 0, s, lists[from], lists[from + 1], lists[to],
-                               lists[to + 1], a.count, static_cast<uint32_t>(tile));
+            if (tile == kTile) {
+                hipLaunchKernelGGL(merge_tiles_kernel, dim3(grid_for(a.count, kMerged)), dim3(kMergeLanes), 0, s, lists[from], lists[from + 1], lists[to],
+                                   lists[to + 1], a.count);
+            } else {
+                hipLaunchKernelGGL(merge_large_kernel, dim3(grid_for(a.count, kBlock)), dim3(kBlock), 0, s, lists[from], lists[from + 1], lists[to],
+                                   lists[to + 1], a.count, static_cast<uint32_t>(tile));
+            }
             if (int rc = check_launch(who)) return rc;
             from = to;
         }
