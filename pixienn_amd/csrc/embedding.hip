@@ -61,6 +61,7 @@ struct Zeros {
     long long first, rows, stride_bytes, row_bytes;
     FastDiv by_row;             // pieces of 16 bytes of a row
     uint32_t groups;            // workgroups, each of kZeroPieces pieces a lane
+    bool past;                  // the caches
 };
 
 constexpr int kZeroPieces = 8;
@@ -78,7 +79,8 @@ __device__ __forceinline__ void write_zeros(const Zeros& z, uint32_t group)
         char* const at = z.d + (z.first + row) * z.stride_bytes + static_cast<size_t>(piece) * 16;
         const long long left = z.row_bytes - static_cast<long long>(piece) * 16;
         if (left >= 16) {
-            *global_memory<words>(at) = words{};
+            if (z.past) __builtin_nontemporal_store(words{}, global_memory<words>(at));
+            else *global_memory<words>(at) = words{};
         } else {
             for (long long k = 0; k < left; k += 2) *global_memory<uint16_t>(at + k) = 0;
         }
@@ -278,6 +280,7 @@ struct TableGradientArgs {
     int vocab, width, column_groups;
     float scale;
     bool accumulate;
+    bool past;                      // zeros past the caches
 };
 
 // V values of a row of the gradient, as many of them as one access takes at a time.
@@ -342,7 +345,10 @@ __global__ __launch_bounds__(kBlock) void table_gradient_kernel(TableGradientArg
             char* const d = row_of<D>(a.d, first + i, a.d_stride);
 #pragma unroll
             for (int q = 0; q < V; q += kPart)
-                if (e + q < a.width) store_row<D, kPart>(d, e + q, a.width, Raw<D, kPart>{});
+                if (e + q < a.width) {
+                    if (a.past) store_row<D, kPart, true>(d, e + q, a.width, Raw<D, kPart>{});
+                    else store_row<D, kPart>(d, e + q, a.width, Raw<D, kPart>{});
+                }
         }
         return;
     }
@@ -588,6 +594,7 @@ int pxh_embedding_backward(const void* dy, const void* tokens, void* d, int type
     a.width = width;
     a.scale = scale;
     a.accumulate = accumulate != 0;
+    a.past = static_cast<size_t>(vocab) * static_cast<size_t>(width) * size_of(d_type) >= kStreamingBytes;
     a.zeroed = a.accumulate ? static_cast<uint32_t>(vocab) : 0;
     if (rows > 0) {
         const Space space(rows, width);
@@ -601,7 +608,7 @@ int pxh_embedding_backward(const void* dy, const void* tokens, void* d, int type
         // zeros for a launch that takes some microseconds on a few units: `bytes` of them, from the rows that have none yet
         const long long row_bytes = static_cast<long long>(width) * size_of(d_type), pieces = (row_bytes + 15) / 16;
         const auto zeros = [&](long long bytes, int lanes) {
-            Zeros z{ a.d, a.zeroed, 0, d_stride * static_cast<long long>(size_of(d_type)), row_bytes, FastDiv(static_cast<uint32_t>(pieces)), 0 };
+            Zeros z{ a.d, a.zeroed, 0, d_stride * static_cast<long long>(size_of(d_type)), row_bytes, FastDiv(static_cast<uint32_t>(pieces)), 0, a.past };
             const long long left = vocab - static_cast<long long>(a.zeroed);
             z.rows = bytes / row_bytes < left ? bytes / row_bytes : left;
             z.groups = grid_for(static_cast<size_t>(z.rows) * pieces, static_cast<size_t>(lanes) * kZeroPieces);

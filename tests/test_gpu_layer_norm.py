@@ -157,7 +157,7 @@ def gradient(dy, h, weight, mean, rstd, dsum):
 
 
 @gpu
-@pytest.mark.parametrize("rows,width", SHAPES + [(1500, 300), (700, 2100)])
+@pytest.mark.parametrize("rows,width", SHAPES + [(1500, 300), (700, 2100), (600, 9003), (300, 16383), (500, 8191)])
 @pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("with_sum,pad,wide_weight,with_bias", [(False, 0, False, True), (True, 5, True, True), (True, 0, True, False)])
 def test_gradients_are_the_formula(ops, rows, width, kind, with_sum, pad, wide_weight, with_bias):
@@ -185,6 +185,11 @@ def test_gradients_are_the_formula(ops, rows, width, kind, with_sum, pad, wide_w
     ops.layer_norm_backward(dyi, h.contiguous(), weight, mean, rstd, dyi, dw, db=db, dsum=None if dsum is None else dsum.contiguous(),
                             accumulate=True, workspace=space)
     assert torch.equal(dyi, dx[:, :width])
+    if with_sum:
+        # and over dsum
+        over = dsum.clone().contiguous()
+        ops.layer_norm_backward(dy, h, weight, mean, rstd, over, torch.empty_like(dw), db=None, dsum=over)
+        assert torch.equal(over, dx[:, :width])
     assert torch.equal(dw, first + first) and (db is None or torch.equal(db, first_db + first_db))
 
 
