@@ -72,23 +72,30 @@ __global__ __launch_bounds__(kBlock) void beam_select_kernel(SelectArgs a)
         if (own == 0) continue;
         atomicAdd(&candidates, 1);
         const int beam = c / a.per;
-        int rank = c - beam * a.per;
-        for (int b = 0; b < a.beams && rank < a.count; ++b) {
-            if (b == beam) continue;
-            // how many of beam b's come first: of equal ones those of the lower beam
-            const unsigned long long* list = orders + b * a.per;
-            const unsigned long long least = b < beam ? own : own + 1;
-            int low = 0, left = a.per;
-            while (left > 0) {
-                const int half = left / 2;
-                if (list[low + half] >= least) {
-                    low += half + 1;
-                    left -= half + 1;
-                } else {
-                    left = half;
+        int rank = 0;
+        if (n <= kBlock) {
+            // few: how many come first, of equal ones those in front
+#pragma unroll 8
+            for (int o = 0; o < n; ++o) rank += orders[o] > own || (orders[o] == own && o < c);
+        } else {
+            rank = c - beam * a.per;
+            for (int b = 0; b < a.beams && rank < a.count; ++b) {
+                if (b == beam) continue;
+                // how many of beam b's come first: of equal ones those of the lower beam
+                const unsigned long long* list = orders + b * a.per;
+                const unsigned long long least = b < beam ? own : own + 1;
+                int low = 0, left = a.per;
+                while (left > 0) {
+                    const int half = left / 2;
+                    if (list[low + half] >= least) {
+                        low += half + 1;
+                        left -= half + 1;
+                    } else {
+                        left = half;
+                    }
                 }
+                rank += low;
             }
-            rank += low;
         }
         if (rank >= a.count) continue;
         const long long row = item * a.beams + beam, out = item * a.count + rank;
@@ -146,39 +153,48 @@ __global__ __launch_bounds__(kBlock) void beam_reorder_kernel(ReorderArgs a)
     const unsigned at = blockIdx.x - t.first;
     const long long item = at / t.parts;
     const long long first = static_cast<long long>(at % t.parts) * a.columns * 16;
+    char* const rows = t.data + item * a.beams * t.stride;
+    const int* const parents = a.parents + item * a.beams;
     const int pieces = a.beams * a.columns;
     typedef uint32_t words __attribute__((ext_vector_type(4), aligned(1)));
-    words held[kHeld];
-    char* to[kHeld];
-    int length[kHeld];
+    // all parents first, then all rows: one trip to memory each
+    int beam[kHeld], parent[kHeld];
 #pragma unroll
     for (int j = 0; j < kHeld; ++j) {
         const int piece = j * kBlock + threadIdx.x;
-        length[j] = 0;
-        if (piece >= pieces) continue;
-        const int beam = piece / a.columns;
-        const long long byte = first + static_cast<long long>(piece - beam * a.columns) * 16;
-        const int parent = a.parents[item * a.beams + beam];
-        if (byte >= t.bytes || parent == beam || parent < 0 || parent >= a.beams) continue;
-        const char* from = t.data + (item * a.beams + parent) * t.stride + byte;
-        to[j] = t.data + (item * a.beams + beam) * t.stride + byte;
-        length[j] = t.bytes - byte < 16 ? static_cast<int>(t.bytes - byte) : 16;
-        if (length[j] == 16) {
-            held[j] = *global_memory<words>(from);
-        } else {
+        beam[j] = piece < pieces ? piece / a.columns : 0;
+        parent[j] = parents[beam[j]];
+    }
+    words held[kHeld];
+    long long byte[kHeld];
+    bool moves[kHeld];
+    // a row's last piece is read as its last 16 bytes, and what is the piece's own is written
+    const long long last = t.bytes - 16;
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+        const int piece = j * kBlock + threadIdx.x;
+        byte[j] = first + static_cast<long long>(piece - beam[j] * a.columns) * 16;
+        moves[j] = piece < pieces && byte[j] < t.bytes && parent[j] != beam[j] && parent[j] >= 0 && parent[j] < a.beams;
+        const char* const from = rows + (moves[j] ? parent[j] : 0) * t.stride;
+        if (last >= 0) {
+            if (moves[j]) held[j] = *global_memory<words>(from + (byte[j] < last ? byte[j] : last));
+        } else if (moves[j]) {
             uint32_t w[4] = {};
-            for (int k = 0; k < length[j]; ++k) w[k / 4] |= static_cast<uint32_t>(*global_memory<unsigned char>(from + k)) << (8 * (k & 3));
+            for (int k = 0; k < t.bytes; ++k) w[k / 4] |= static_cast<uint32_t>(*global_memory<unsigned char>(from + k)) << (8 * (k & 3));
             held[j] = words{ w[0], w[1], w[2], w[3] };
         }
     }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < kHeld; ++j) {
-        if (length[j] == 16) {
-            *global_memory<words>(to[j]) = held[j];
-        } else {
-            for (int k = 0; k < length[j]; ++k) *global_memory<unsigned char>(to[j] + k) = static_cast<unsigned char>(held[j][k / 4] >> (8 * (k & 3)));
+        if (!moves[j]) continue;
+        char* const to = rows + beam[j] * t.stride + byte[j];
+        if (byte[j] <= last) {
+            *global_memory<words>(to) = held[j];
+            continue;
         }
+        const int left = static_cast<int>(t.bytes - byte[j]), skip = last >= 0 ? 16 - left : 0;
+        for (int k = 0; k < left; ++k) *global_memory<unsigned char>(to + k) = static_cast<unsigned char>(held[j][(k + skip) / 4] >> (8 * ((k + skip) & 3)));
     }
 }
 
