@@ -1,5 +1,5 @@
-"""A small next-token model trained and asked with the layers of token models: norm with the residual's addition, log probabilities
-with their gradient, AdamW over all tensors.
+"""A small next-token model trained and asked with the layers of token models: embeddings by token, norm with the residual's addition,
+log probabilities with their gradient, AdamW over all tensors.
 
     python examples/token_model.py [--steps 200] [--bits 8|32]
 
@@ -48,7 +48,8 @@ class TokenModel:
         return y, total, rstd
 
     def logits(self, tokens, keep=None):
-        h, branch = self.copy["embedding"][tokens], None
+        h, branch = torch.empty(len(tokens), self.width, device="cuda", dtype=BF16), None
+        ops.embedding_forward(self.copy["embedding"], tokens, h)
         for b in range(self.blocks):
             # the block's branch joins the stream in the next norm
             y, h, rstd = self._norm("norm%d" % b, h, branch)
@@ -83,7 +84,7 @@ class TokenModel:
             torch.mm(d_up.t(), y, out=self.d["up%d" % b])
             # what goes through the block and what goes past it
             ops.rms_norm_backward(d_up @ self.copy["up%d" % b], h, self.copy["norm%d" % b], rstd, d_stream, self.d["norm%d" % b], dsum=d_stream)
-        self.d["embedding"].zero_().index_add_(0, tokens, d_stream)
+        ops.embedding_backward(d_stream, tokens, self.d["embedding"])
         return logp.mean()
 
     def step(self, tokens, targets, lr):
