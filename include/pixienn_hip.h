@@ -724,7 +724,8 @@ int pxh_layer_norm_backward(const void* dy, const void* h, const void* weight, c
  * saved (nullable, fp32 [rows / PXH_SCAN_SAVED, rounded up][width]) receives h in front of every PXH_SCAN_SAVED-th row, which is what
  * the backward pass needs.  y may be x, update or gate where the strides are the same.
  * A result depends on its sequence alone up to the last bits of h, which depend on where in the rows the sequence lies, and the same
- * call gives the same bits.  Within a step h is rounded to 2^-23 of the larger of |h| and |x|.
+ * call gives the same bits.  Within a step h is rounded to 2^-23 of the larger of |h| and |x|.  Where h is infinite or no number, it is no
+ * number from the next token to the end of the sequence, as the formula has it.
  * workspace: pxh_gated_scan_workspace_bytes(rows, width), which serves fewer rows and shorter rows too, or NULL for the library's. */
 #define PXH_SCAN_SAVED 16
 size_t pxh_gated_scan_workspace_bytes(long long rows, int width);

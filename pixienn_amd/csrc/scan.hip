@@ -7,17 +7,25 @@ namespace pxh {
 namespace {
 
 // A range of tokens takes a state s to (1 - Z) * s + H.  1 - z is never kept: of a z of 2^-13 it has only half the digits in fp32, which
-// thousands of tokens would add up, while Z = z + z' - z z' has them all.  Z == 1 says that nothing in front of the range counts
-// any more; then the state behind it is H to the bit, whatever came before.
+// thousands of tokens would add up, while Z = z + z' - z z' has them all.  Z == 1 says that what was in front of the range is forgotten:
+// the state behind it is H, or no number where s is infinite or none.  A range in which a sequence begins has nothing in front of
+// it (kWhole): the state behind it is H to the bit.
 struct Range {
     float z, h;
 };
 
-__device__ __forceinline__ float behind(float s, Range r) { return r.z == 1.0f ? r.h : s + fmaf(-r.z, s, r.h); }
+constexpr float kWhole = 2.0f;
+
+__device__ __forceinline__ float behind(float s, Range r)
+{
+    const float by = r.z == 1.0f ? fmaf(0.0f, s, r.h) : s + fmaf(-r.z, s, r.h);
+    return r.z == kWhole ? r.h : by;
+}
 
 __device__ __forceinline__ Range joined(Range first, Range then)
 {
-    return Range{ then.z == 1.0f ? 1.0f : first.z + fmaf(-then.z, first.z, then.z), behind(first.h, then) };
+    const float z = then.z == 1.0f ? 1.0f : first.z + fmaf(-then.z, first.z, then.z);
+    return Range{ first.z == kWhole || then.z == kWhole ? kWhole : z, behind(first.h, then) };
 }
 
 // z = 1 / (1 + e) with e = exp(-u), and 1 - z to all its digits: e z where z is near 1.  16-bit values: the hardware's exp2 of the
@@ -64,16 +72,25 @@ struct Shape {
     static_assert(kSaved % STEPS == 0 && kChunk % kSaved == 0, "a saved state is in front of a wave's tokens");
 };
 // Two workgroups of eight waves to a unit.  Chunks of 64 tokens pay twice for what a chunk costs whatever its length (a number, a word, a
-// look back: 8 x 4096 x 2048 bf16 with a gate 134 us where 128 take 105).  The gradients keep three values for each that they read:
-// waves of 16 tokens spill (430 us, and 180).
+// look back: 8 x 4096 x 2048 bf16 with a gate 139 us where 128 take 116).  The gradients keep three values for each that they read:
+// waves of 16 tokens spill (430 us, and 193).
 using Forward = Shape<16, 8>;
 using Backward = Shape<8, 8>;
 
-// Where sequences begin: starts[sequences + 1], or all of one length.
+// Where sequences begin: starts[sequences + 1], or all of one length.  Of fewer than kFew sequences a wave's lanes keep all places, asked for
+// before the workgroup knows its chunk.
+constexpr int kFew = kWave - 1;
 struct Sequences {
     const int* starts;
     FastDiv length;
     int count, rows;
+
+    __device__ __forceinline__ bool few() const { return starts && count < kFew; }
+    __device__ __forceinline__ int kept() const
+    {
+        const int lane = threadIdx.x % kWave;
+        return few() && lane <= count ? starts[lane] : 0x7fffffff;
+    }
 };
 
 // States of sequences: a row of `width` fp32 for each slot.
@@ -112,68 +129,111 @@ __device__ __forceinline__ int last_in_front(const int* starts, int n, int t)
     return low - 1;
 }
 
+// The same for one t of the whole wave, 64 places at a time: 4000 sequences are two trips to memory, where halves are twelve.
+__device__ __forceinline__ int last_in_front_of_wave(const int* starts, int n, int t)
+{
+    const int lane = threadIdx.x % kWave;
+    int low = 0;
+    while (n > 0) {
+        const int step = (n + kWave - 1) / kWave, at = lane * step;
+        const int passed = __popcll(__ballot(at < n && starts[low + at] <= t));
+        if (passed == 0) break;
+        low += (passed - 1) * step + 1;
+        n = min(step - 1, n - (passed - 1) * step - 1);
+    }
+    return low - 1;
+}
+
+// `kept`: the lane's place, as Sequences keeps it.  All lanes of the wave.
 template<int STEPS>
-__device__ __forceinline__ Borders borders_of(const Sequences& q, int first)
+__device__ __forceinline__ Borders borders_of(const Sequences& q, int kept, int first)
 {
     const int lane = threadIdx.x % kWave;
     const int t = first + lane;
     const bool mine = lane < STEPS && t < q.rows;
     bool begins = false, ends = false, active = false;
     int s = 0;
-    if (mine) {
-        if (q.starts) {
-            s = last_in_front(q.starts, q.count + 1, t);
-            if (s >= 0 && s < q.count) {
-                active = true;
-                begins = q.starts[s] == t;
-                ends = q.starts[s + 1] == t + 1 || t + 1 == q.rows;
-            } else {
-                s = 0;
-            }
+    if (q.starts) {
+        int begin = 0, end = 0;
+        if (q.few()) {
+            s = -1;
+#pragma unroll
+            for (int half = kWave / 2; half; half /= 2) s = __shfl(kept, s + half) <= t ? s + half : s;
+            begin = __shfl(kept, max(s, 0));
+            end = __shfl(kept, s + 1);
         } else {
-            uint32_t which, place;
-            q.length.divmod(t, which, place);
-            s = static_cast<int>(which);
-            active = true;
-            begins = place == 0;
-            ends = place + 1 == q.length.d;
+            const int low = max(last_in_front_of_wave(q.starts, q.count + 1, first), 0);
+            const int among = last_in_front_of_wave(q.starts + low, q.count + 1 - low, first + STEPS - 1) + 1;
+            s = low + last_in_front(q.starts + low, among, t);
+            if (s >= 0 && s < q.count) {
+                begin = q.starts[s];
+                end = q.starts[s + 1];
+            }
         }
+        active = mine && s >= 0 && s < q.count;
+        begins = active && begin == t;
+        ends = active && (end == t + 1 || t + 1 == q.rows);
+        s = active ? s : 0;
+    } else if (mine) {
+        uint32_t which, place;
+        q.length.divmod(t, which, place);
+        s = static_cast<int>(which);
+        active = true;
+        begins = place == 0;
+        ends = place + 1 == q.length.d;
     }
     return Borders{ static_cast<uint32_t>(__ballot(begins)), static_cast<uint32_t>(__ballot(ends)), static_cast<uint32_t>(__ballot(active)), s };
 }
 
-// Whether tokens first .. first + n are all there, and none of them begins a sequence, ends one or lies in none: then most of what a
-// workgroup has to look at, token by token, is not there.
-__device__ __forceinline__ bool lies_within_one(const Sequences& q, int first, int n)
+// Whether tokens first .. first + n are all there and of one sequence, which may begin with the first and end with the last of them: then
+// most of what a workgroup has to look at, token by token, is not there.
+struct Whole {
+    bool there, begins, ends;
+    int sequence;
+};
+
+__device__ __forceinline__ Whole within_one(const Sequences& q, int kept, int first, int n)
 {
-    if (first + n > q.rows) return false;
+    if (first + n > q.rows) return Whole{ false, false, false, 0 };
     if (!q.starts) {
         uint32_t which, place;
         q.length.divmod(first, which, place);
-        return place > 0 && place + n < q.length.d;
+        return Whole{ place + n <= q.length.d, place == 0, place + n == q.length.d, static_cast<int>(which) };
     }
-    const int s = last_in_front(q.starts, q.count + 1, first);
-    return s >= 0 && s < q.count && q.starts[s] < first && q.starts[s + 1] > first + n && first + n < q.rows;
+    const int s = q.few() ? __popcll(__ballot(kept <= first)) - 1 : last_in_front_of_wave(q.starts, q.count + 1, first);
+    if (s < 0 || s >= q.count) return Whole{ false, false, false, 0 };
+    const int begin = q.few() ? __builtin_amdgcn_readlane(kept, s) : q.starts[s], end = q.few() ? __builtin_amdgcn_readlane(kept, s + 1) : q.starts[s + 1];
+    return Whole{ end >= first + n, begin == first, end == first + n || first + n == q.rows, s };
 }
 
 // ---------------------------------------------------------------- from chunk to chunk
 // Workgroups take numbers, chunk by chunk along the tokens (for the gradients against them).  Each leaves what its chunk does to a
-// state, channel by channel, as one 64-bit word, and once it knows the state in front of it the one behind it as a range with Z = 1.  It
-// looks back at the words of up to kWindow chunks, until one of them has Z = 1 and none nearer is missing, and goes on
-// from there: s + (H - Z s) chunk by chunk is the same to the bit wherever it begins.
+// state, channel by channel, as one 64-bit word; the last one of kGroup chunks leaves one for all of them, and once it knows the state in
+// front of the group, the state behind it as a whole range.  A chunk waits for the words of those in front of it in its group, which
+// wait for nobody, and for the state in front of the group: the words of up to kWindow groups, until one of them is whole and none nearer is
+// missing.  So the state has to go from hand to hand only once for kGroup * kWindow chunks.  A state is always put together in the same way,
+// whichever words were there first: the same call gives the same bits.
 // A workgroup waits for lower numbers only, which are running or done: the lowest of those running waits for none.  The bound on the looks
 // makes the exit unconditional all the same; where it was reached (two launches at once on one workspace, which the interface
 // forbids) the states are NaN.
 constexpr unsigned long long kNotThere = ~0ull;     // no range: a Z that is no number is left as 1, with its H
-// (2 chunks: 105 us, 4: 107, 8: 111, for want of registers)
-constexpr int kWindow = 2;
+// (65536 x 256 bf16, channels that remember: every chunk handing its state on 173 us, groups of 4 49, of 8 38, where the gradients of wide
+// calls spill: 8 x 4096 x 2048 with a gate 193 -> 244)
+constexpr int kGroup = 4, kWindow = 4;
 constexpr uint32_t kLooks = 1u << 22;
 
+// The chunks of the call: segments of as many chunks each, of which none needs another segment's.  Where all sequences have the same length, of
+// whole chunks, they are the segments, and numbers go round them: chunks that run together then wait for few of each other.
 struct Exchange {
-    unsigned long long* words;      // [chunks][width]; null where no chunk needs another's
+    unsigned long long* words;      // [segments * per][width]; null where no chunk needs another's
+    unsigned long long* groups;     // [segments * groups_per][width]
     uint32_t* counter;
-    uint32_t chunks;
-    FastDiv by_tiles;
+    uint32_t per, groups_per;       // of a segment
+    FastDiv by_tiles, by_segments;
+};
+
+struct Place {
+    uint32_t segment, chunk, tile;  // chunk: of the segment, in the order in which they wait for each other
 };
 
 __device__ __forceinline__ unsigned long long word_of(Range r)
@@ -191,24 +251,52 @@ __device__ __forceinline__ void leave_word(unsigned long long* at, Range r)
     __hip_atomic_store(at, word_of(r), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// The state behind the chunk in front of `chunk`, of one channel (there: one that exists); chunk > 0, all lanes of the wave.
-__device__ __forceinline__ float look_back(const unsigned long long* words, uint32_t chunk, size_t width, bool there)
+__device__ __forceinline__ unsigned long long see_word(const unsigned long long* at)
+{
+    return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// What the `count` chunks (fewer than kGroup) whose words begin at `words` do to a state, of one channel (there: one that exists); all lanes of
+// the wave.
+__device__ __forceinline__ Range of_group(const unsigned long long* words, uint32_t count, size_t width, bool there)
+{
+    unsigned long long w[kGroup - 1];
+    uint32_t looks = kLooks;
+    for (; looks; --looks) {
+        bool missing = false;
+#pragma unroll
+        for (int d = 0; d < kGroup - 1; ++d) {
+            w[d] = 0;                                   // a range of no tokens
+            if (there && static_cast<uint32_t>(d) < count) w[d] = see_word(words + d * width);
+        }
+#pragma unroll
+        for (int d = 0; d < kGroup - 1; ++d) missing = missing || w[d] == kNotThere;
+        if (!__any(missing)) break;
+        __builtin_amdgcn_s_sleep(1);
+    }
+    Range all = range_of(w[0]);
+#pragma unroll
+    for (int d = 1; d < kGroup - 1; ++d) all = joined(all, range_of(w[d]));
+    return looks ? all : Range{ kWhole, __builtin_nanf("") };
+}
+
+// The state in front of the group whose word is at `word`, the group'th of its segment, of one channel; all lanes of the wave.
+__device__ __forceinline__ float look_back(const unsigned long long* word, uint32_t group, size_t width, bool there)
 {
     unsigned long long w[kWindow];
     int found = -1;
     for (uint32_t looks = kLooks; looks; --looks) {
 #pragma unroll
         for (int d = 0; d < kWindow; ++d) {
-            w[d] = word_of(Range{ 1.0f, 0.0f });         // in front of the first chunk
-            if (there && chunk > static_cast<uint32_t>(d))
-                w[d] = __hip_atomic_load(words + (chunk - 1 - d) * width, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            w[d] = word_of(Range{ kWhole, 0.0f });       // in front of the first group
+            if (there && group > static_cast<uint32_t>(d)) w[d] = see_word(word - (d + 1) * width);
         }
         bool whole = true;
         found = -1;
 #pragma unroll
         for (int d = 0; d < kWindow; ++d) {
             whole = whole && w[d] != kNotThere;
-            if (whole && found < 0 && range_of(w[d]).z == 1.0f) found = d;
+            if (whole && found < 0 && range_of(w[d]).z == kWhole) found = d;
         }
         if (!__any(found < 0)) break;
         __builtin_amdgcn_s_sleep(1);
@@ -225,14 +313,15 @@ __device__ __forceinline__ float look_back(const unsigned long long* words, uint
 template<int WAVES, int TILE>
 struct ScanShared {
     Range ranges[WAVES][TILE];
-    float states[WAVES][TILE];         // in front of each wave's tokens
+    Range in_front[TILE];               // the chunks of the group in front of this one
+    float states[TILE];                 // in front of the group
+    float begun[TILE];                  // what the sequence begins with that begins with the chunk
     float passed[WAVES][TILE];         // from wave to wave
     uint32_t number, fresh;             // fresh: no state reaches the chunk
 };
 
-// Takes the workgroup's number: chunk and tile.
 template<int WAVES, int TILE>
-__device__ __forceinline__ void take_number(const Exchange& x, ScanShared<WAVES, TILE>& lds, uint32_t& chunk, uint32_t& tile)
+__device__ __forceinline__ Place take_number(const Exchange& x, ScanShared<WAVES, TILE>& lds)
 {
     uint32_t number = blockIdx.x;
     if (x.words) {
@@ -240,40 +329,52 @@ __device__ __forceinline__ void take_number(const Exchange& x, ScanShared<WAVES,
         __syncthreads();
         number = __builtin_amdgcn_readfirstlane(lds.number);
     }
-    x.by_tiles.divmod(number, chunk, tile);
+    Place p;
+    uint32_t rest;
+    x.by_tiles.divmod(number, rest, p.tile);
+    x.by_segments.divmod(rest, p.chunk, p.segment);
+    return p;
 }
 
-// From the waves' ranges, in the order `order(0 .. WAVES - 1)`, and the chunks in front of `chunk`: the state in front of every wave.
-template<int WAVES, int TILE, typename Order>
-__device__ __forceinline__ void join_waves(const Exchange& x, ScanShared<WAVES, TILE>& lds, uint32_t chunk, uint32_t tile, int width, const Order& order)
+// From the waves' ranges, in the order `order(0 .. WAVES - 1)`, of which the wave is number `turn`, and the chunks in front of the workgroup's: the
+// state in front of the wave, of its lane's channels.
+template<int WAVES, int TILE, int V, typename Order>
+__device__ __forceinline__ void join_waves(const Exchange& x, ScanShared<WAVES, TILE>& lds, const Place& p, int width, int turn, const Order& order,
+                                           float (&s)[V])
 {
     __syncthreads();
-    const int c = threadIdx.x;
-    if (c < TILE) {            // whole waves
-        const int e = static_cast<int>(tile) * TILE + c;
-        const bool there = e < width;
+    const int c = threadIdx.x % TILE, lane = threadIdx.x % kWave;
+    const int e = static_cast<int>(p.tile) * TILE + c;
+    const bool there = e < width;
+    if (x.words) {
+        const size_t pitch = static_cast<size_t>(width);
+        const uint32_t group = p.chunk / kGroup, place = p.chunk % kGroup;
+        const bool fresh = p.chunk == 0 || lds.fresh, last = p.chunk + 1 == x.per, ends_group = place == kGroup - 1 && !last;
+        unsigned long long* const of_groups = x.groups + (static_cast<size_t>(p.segment) * x.groups_per + group) * pitch + e;
         Range all{ 0.0f, 0.0f };
+        if (threadIdx.x < TILE) {            // whole waves
 #pragma unroll
-        for (int w = 0; w < WAVES; ++w) all = joined(all, lds.ranges[order(w)][c]);
-        float s = 0.0f;
-        if (x.words) {
-            unsigned long long* const word = x.words + e;
-            const bool leaves = there && chunk + 1 < x.chunks;
-            const bool fresh = chunk == 0 || lds.fresh;
-            if (fresh) all.z = 1.0f;
-            if (leaves) leave_word(word + chunk * static_cast<size_t>(width), all);
-            if (!fresh) {
-                s = look_back(word, chunk, width, there);
-                if (leaves && all.z != 1.0f) leave_word(word + chunk * static_cast<size_t>(width), Range{ 1.0f, behind(s, all) });
-            }
+            for (int w = 0; w < WAVES; ++w) all = joined(all, lds.ranges[order(w)][c]);
+            if (fresh) all.z = kWhole;
+            unsigned long long* const word = x.words + (static_cast<size_t>(p.segment) * x.per + p.chunk) * pitch + e;
+            if (there && !ends_group && !last) leave_word(word, all);
+            Range front{ fresh ? kWhole : 0.0f, fresh ? lds.begun[c] : 0.0f };
+            if (!fresh && place) front = of_group(word - place * pitch, place, pitch, there);
+            lds.in_front[c] = front;
+            all = joined(front, all);
+            if (there && ends_group) leave_word(of_groups, all);
+        } else if (threadIdx.x < 2 * TILE) {
+            lds.states[c] = fresh ? 0.0f : look_back(of_groups, group, pitch, there);
         }
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
-            lds.states[order(w)][c] = s;
-            s = behind(s, lds.ranges[order(w)][c]);
-        }
+        __syncthreads();
+        if (threadIdx.x < TILE && there && ends_group && all.z != kWhole) leave_word(of_groups, Range{ kWhole, behind(lds.states[c], all) });
     }
-    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < V; ++k) s[k] = x.words ? behind(lds.states[lane * V + k], lds.in_front[lane * V + k]) : lds.begun[lane * V + k];
+    for (int w = 0; w < turn; ++w) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) s[k] = behind(s[k], lds.ranges[order(w)][lane * V + k]);
+    }
 }
 
 // ---- the launch in front: empties the words, and hands the states of sequences without tokens on.
@@ -415,18 +516,20 @@ __global__ __launch_bounds__(Forward::kLanes, 4) void scan_kernel(ScanArgs a)
     constexpr int kSteps = Forward::kSteps, kChunk = Forward::kChunk, kV = kChannels<T>, kTile = kTileOf<T>;
     __shared__ ScanShared<Forward::kWaves, kTile> lds;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
-    uint32_t chunk, tile;
-    take_number(a.exchange, lds, chunk, tile);
-    const int first = static_cast<int>(chunk) * kChunk + wave * kSteps;
-    const int e = static_cast<int>(tile) * kTile + lane * kV;
-    const Columns columns{ static_cast<int>(tile) * kTile, e, a.width, (static_cast<int>(tile) + 1) * kTile <= a.width };
+    const int kept = a.q.kept();
+    const Place place = take_number(a.exchange, lds);
+    const int chunk_first = static_cast<int>(place.segment * a.exchange.per + place.chunk) * kChunk, first = chunk_first + wave * kSteps;
+    const int tile_first = static_cast<int>(place.tile) * kTile, e = tile_first + lane * kV;
+    const Columns columns{ tile_first, e, a.width, tile_first + kTile <= a.width };
     Raw<T, kV> x[kSteps], u[kSteps], o[GATE ? kSteps : 1];
     load_tokens<T, kSteps>(a.x, a.x_stride, first, a.q.rows, columns, x);
     load_tokens<T, kSteps>(a.update, a.update_stride, first, a.q.rows, columns, u);
+    const Whole whole = columns.inside ? within_one(a.q, kept, chunk_first, kChunk) : Whole{ false, false, false, 0 };
     const auto pass = [&]<bool RARE>() {
         Borders b{ 0, 0, Forward::kAll, 0 };
-        if constexpr (RARE) b = borders_of<kSteps>(a.q, first);
-        if (threadIdx.x == 0) lds.fresh = b.begins & 1;
+        if constexpr (RARE) b = borders_of<kSteps>(a.q, kept, first);
+        const bool begins_here = !RARE && whole.begins && wave == 0;
+        if (threadIdx.x == 0) lds.fresh = RARE ? b.begins & 1 : whole.begins;
         float z[kSteps][kV];
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
@@ -438,6 +541,11 @@ __global__ __launch_bounds__(Forward::kLanes, 4) void scan_kernel(ScanArgs a)
         // into the updates' registers
         if constexpr (GATE) load_tokens<T, kSteps>(a.gate, a.gate_stride, first, a.q.rows, columns, o);
         float h[kV] = {}, Z[kV] = {};
+        if (begins_here && a.state) load_state(a.state, slot_of(a.slots, whole.sequence), e, a.width, h);
+        if (wave == 0) {
+#pragma unroll
+            for (int k = 0; k < kV; ++k) lds.begun[lane * kV + k] = h[k];
+        }
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             const bool begins = RARE && (b.begins >> i & 1), active = !RARE || (b.active >> i & 1);
@@ -461,11 +569,9 @@ __global__ __launch_bounds__(Forward::kLanes, 4) void scan_kernel(ScanArgs a)
             }
         }
 #pragma unroll
-        for (int k = 0; k < kV; ++k) lds.ranges[wave][lane * kV + k] = Range{ Z[k], h[k] };
-        join_waves(a.exchange, lds, chunk, tile, a.width, [](int w) { return w; });
+        for (int k = 0; k < kV; ++k) lds.ranges[wave][lane * kV + k] = Range{ begins_here || (RARE && b.begins) ? kWhole : Z[k], h[k] };
+        join_waves(a.exchange, lds, place, a.width, wave, [](int w) { return w; }, h);
         as_read(x);
-#pragma unroll
-        for (int k = 0; k < kV; ++k) h[k] = lds.states[wave][lane * kV + k];
         if (a.saved && first % kSaved == 0 && first < a.q.rows) store_state<NT>(a.saved, first / kSaved, e, a.width, h);
         Writer<T, NT> y(a.y, a.y_stride, first, columns);
 #pragma unroll
@@ -489,8 +595,9 @@ __global__ __launch_bounds__(Forward::kLanes, 4) void scan_kernel(ScanArgs a)
             if (RARE && a.final && (b.ends >> i & 1))
                 store_state(a.final, slot_of(a.slots, __builtin_amdgcn_readlane(b.sequence, i)), e, a.width, h);
         }
+        if (!RARE && a.final && whole.ends && wave == Forward::kWaves - 1) store_state(a.final, slot_of(a.slots, whole.sequence), e, a.width, h);
     };
-    if (columns.inside && lies_within_one(a.q, static_cast<int>(chunk) * kChunk, kChunk)) pass.template operator()<false>();
+    if (whole.there) pass.template operator()<false>();
     else pass.template operator()<true>();
 }
 
@@ -523,12 +630,11 @@ __global__ __launch_bounds__(Backward::kLanes, 4) void scan_backward_kernel(Scan
     constexpr int kSteps = Backward::kSteps, kWaves = Backward::kWaves, kChunk = Backward::kChunk, kV = kChannels<T>, kTile = kTileOf<T>;
     __shared__ ScanShared<kWaves, kTile> lds;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave;
-    uint32_t turn, tile;
-    take_number(a.exchange, lds, turn, tile);
-    const uint32_t chunk = a.exchange.chunks - 1 - turn;
-    const int first = static_cast<int>(chunk) * kChunk + wave * kSteps;
-    const int e = static_cast<int>(tile) * kTile + lane * kV;
-    const Columns columns{ static_cast<int>(tile) * kTile, e, a.width, (static_cast<int>(tile) + 1) * kTile <= a.width };
+    const int kept = a.q.kept();
+    const Place place = take_number(a.exchange, lds);
+    const int chunk_first = static_cast<int>((place.segment + 1) * a.exchange.per - 1 - place.chunk) * kChunk, first = chunk_first + wave * kSteps;
+    const int tile_first = static_cast<int>(place.tile) * kTile, e = tile_first + lane * kV;
+    const Columns columns{ tile_first, e, a.width, tile_first + kTile <= a.width };
     Raw<T, kV> x[kSteps], u[kSteps], dy[kSteps], o[GATE ? kSteps : 1];
     load_tokens<T, kSteps>(a.update, a.update_stride, first, a.q.rows, columns, u);
     load_tokens<T, kSteps>(a.x, a.x_stride, first, a.q.rows, columns, x);
@@ -536,10 +642,15 @@ __global__ __launch_bounds__(Backward::kLanes, 4) void scan_backward_kernel(Scan
     if constexpr (GATE) load_tokens<T, kSteps>(a.gate, a.gate_stride, first, a.q.rows, columns, o);
     float h[kV];
     load_state(a.saved, first % kSaved == 0 && first < a.q.rows ? first / kSaved : -1, e, a.width, h);
+    const Whole whole = columns.inside ? within_one(a.q, kept, chunk_first, kChunk) : Whole{ false, false, false, 0 };
     const auto pass = [&]<bool RARE>() {
         Borders b{ 0, 0, Backward::kAll, 0 };
-        if constexpr (RARE) b = borders_of<kSteps>(a.q, first);
-        if (wave == kWaves - 1 && lane == 0) lds.fresh = b.ends >> (kSteps - 1) & 1;
+        if constexpr (RARE) b = borders_of<kSteps>(a.q, kept, first);
+        if (wave == kWaves - 1) {
+            if (lane == 0) lds.fresh = b.ends >> (kSteps - 1) & 1;
+#pragma unroll
+            for (int k = 0; k < kV; ++k) lds.begun[lane * kV + k] = 0.0f;
+        }
         const auto begin = [&](int i) {
             if (b.begins >> i & 1) load_state(a.state, a.state ? slot_of(a.slots, __builtin_amdgcn_readlane(b.sequence, i)) : -1, e, a.width, h);
         };
@@ -645,10 +756,8 @@ __global__ __launch_bounds__(Backward::kLanes, 4) void scan_backward_kernel(Scan
             }
         }
 #pragma unroll
-        for (int k = 0; k < kV; ++k) lds.ranges[wave][lane * kV + k] = Range{ Z[k], C[k] };
-        join_waves(a.exchange, lds, turn, tile, a.width, [](int k) { return kWaves - 1 - k; });
-#pragma unroll
-        for (int k = 0; k < kV; ++k) C[k] = lds.states[wave][lane * kV + k];
+        for (int k = 0; k < kV; ++k) lds.ranges[wave][lane * kV + k] = Range{ RARE && b.ends ? kWhole : Z[k], C[k] };
+        join_waves(a.exchange, lds, place, a.width, kWaves - 1 - wave, [](int k) { return kWaves - 1 - k; }, C);
         Writer<T, NT> out_x(a.dx, a.dx_stride, first + kSteps - 1, columns, true), out_u(a.dupdate, a.dupdate_stride, first + kSteps - 1, columns, true);
 #pragma unroll
         for (int i = kSteps - 1; i >= 0; --i) {
@@ -667,7 +776,7 @@ __global__ __launch_bounds__(Backward::kLanes, 4) void scan_backward_kernel(Scan
                 store_state(a.d_state, slot_of(a.slots, __builtin_amdgcn_readlane(b.sequence, i)), e, a.width, C);
         }
     };
-    if (columns.inside && lies_within_one(a.q, static_cast<int>(chunk) * kChunk, kChunk)) pass.template operator()<false>();
+    if (whole.there && !whole.begins && !whole.ends) pass.template operator()<false>();
     else pass.template operator()<true>();
 }
 
@@ -724,6 +833,9 @@ __global__ __launch_bounds__(kBlock) void scan_step_kernel(StepArgs a)
 // ---------------------------------------------------------------- host
 size_t chunks_of(long long rows, int chunk) { return (static_cast<size_t>(rows) + chunk - 1) / chunk; }
 
+// Words of chunks and groups: a segment of two chunks and more has half as many groups at most.
+size_t words_of(size_t chunks, int width) { return (chunks + chunks / 2 + 1) * static_cast<size_t>(width); }
+
 // The words' counter in front of them.
 constexpr size_t kCounterBytes = 256;
 
@@ -758,14 +870,18 @@ int start_scan(const char* who, int type, long long rows, int width, int sequenc
     const size_t chunks = chunks_of(rows, kChunk), tile = 4 / size_of(type) * kWave, tiles = (static_cast<size_t>(width) + tile - 1) / tile;
     if (chunks * tiles * S::kLanes >= 1ull << 32) return fail_invalid("%s: too many rows of too many values", who);
     groups = static_cast<uint32_t>(chunks * tiles);
-    x = Exchange{ nullptr, nullptr, static_cast<uint32_t>(chunks), FastDiv(static_cast<uint32_t>(tiles)) };
+    const bool apart = length > 0 && length % kChunk == 0 && sequences > 1;
+    const size_t segments = apart ? sequences : 1, per = chunks / segments, groups_per = (per + kGroup - 1) / kGroup;
+    x = Exchange{ nullptr, nullptr, nullptr, static_cast<uint32_t>(per), static_cast<uint32_t>(groups_per), FastDiv(static_cast<uint32_t>(tiles)),
+                  FastDiv(static_cast<uint32_t>(segments)) };
     size_t count = 0;
-    if (chunks > 1 && (starts || kChunk % length)) {
+    if (per > 1 && (starts || kChunk % length)) {
         void* ws = nullptr;
-        count = chunks * static_cast<size_t>(width);
-        if (int rc = resolve_workspace(workspace, workspace_bytes, kCounterBytes + count * sizeof(unsigned long long), &ws, s)) return rc;
+        count = segments * (per + groups_per) * static_cast<size_t>(width);
+        if (int rc = resolve_workspace(workspace, workspace_bytes, kCounterBytes + words_of(chunks, width) * sizeof(unsigned long long), &ws, s)) return rc;
         x.counter = static_cast<uint32_t*>(ws);
         x.words = reinterpret_cast<unsigned long long*>(static_cast<char*>(ws) + kCounterBytes);
+        x.groups = x.words + chunks * static_cast<size_t>(width);
     }
     // sequences may be without tokens where their lengths are given, or where there are none at all
     if (to == from || sequences == 0 || !(starts || length == 0)) to = nullptr;
@@ -789,7 +905,7 @@ extern "C" {
 size_t pxh_gated_scan_workspace_bytes(long long rows, int width)
 {
     if (rows <= 0 || width <= 0) return 0;
-    return kCounterBytes + chunks_of(rows, Forward::kChunk < Backward::kChunk ? Forward::kChunk : Backward::kChunk) * static_cast<size_t>(width) * sizeof(unsigned long long);
+    return kCounterBytes + words_of(chunks_of(rows, Forward::kChunk < Backward::kChunk ? Forward::kChunk : Backward::kChunk), width) * sizeof(unsigned long long);
 }
 
 int pxh_gated_scan_forward(const void* x, const void* update, const void* gate, void* y, const int* starts, const float* state, float* final,

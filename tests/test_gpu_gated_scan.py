@@ -255,6 +255,59 @@ def test_a_step_is_a_sequence_of_one_token(ops, rows, width, kind, gated, with_s
 
 @gpu
 @pytest.mark.parametrize("kind", list(TYPES))
+def test_what_is_no_number_is_not_forgotten(ops, kind):
+    """Updates after a few hundred of which nothing of a number is left: what is none stays, from chunk to chunk."""
+    dtype = TYPES[kind][0]
+    g = torch.Generator().manual_seed(6)
+    starts = [0, 50, 5050, 5100]
+    rows, width = starts[-1], 70
+    x, u, dy = draw(g, rows, width, dtype), draw(g, rows, width, dtype, 2.0), draw(g, rows, width, dtype, 0.1)
+    there = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    x[300, 3], x[301, 4], x[4000, 5], u[2000, 6] = float("nan"), float("inf"), float("-inf"), float("nan")
+    dy[4500, 7], dy[100, 8], dy[4900, 9] = float("nan"), float("inf"), float("-inf")
+    y, dx, du, saved = torch.empty_like(x), torch.empty_like(x), torch.empty_like(x), ops.gated_scan_saved_like(x)
+    ops.gated_scan_forward(x, u, y, starts=there, saved=saved)
+    ops.gated_scan_backward(dy, x, u, saved, dx, du, starts=there)
+    none = torch.zeros(rows, width, dtype=torch.bool)
+    none[300:5050, 3], none[302:5050, 4], none[4001:5050, 5], none[2000:5050, 6] = True, True, True, True
+    assert torch.equal(torch.isnan(y).cpu(), none)
+    got = torch.isnan(dx).cpu()
+    # against the tokens, to the sequence's first one: from there where it is no number, from the one in front of an infinite one
+    assert bool(got[50:4501, 7].all()) and not bool(got[4501:, 7].any()) and not bool(got[:50, 7].any())
+    for column, first in ((8, 100), (9, 4900)):
+        # (an infinite G times 1 - z is infinite where z < 1, and so is what is added to it: no number where signs meet or z is 1)
+        lost = ~torch.isfinite(dx[:, column].cpu())
+        assert bool(lost[50:first + 1].all()) and not bool(lost[first + 1:].any()) and not bool(lost[:50].any())
+
+
+@gpu
+@pytest.mark.parametrize("count", [62, 63, 64, 200, 5000])
+def test_many_ragged_sequences(ops, count):
+    """Some without a token, some of many: against each by itself, where only the last bits of h can differ."""
+    g = torch.Generator().manual_seed(count)
+    lengths = torch.randint(0, 40, (count,), generator=g)
+    lengths[count // 2], lengths[3], lengths[4] = 700, 0, 0
+    starts = torch.cat([torch.zeros(1, dtype=torch.long), lengths.cumsum(0)]) + 5
+    rows, width = int(starts[-1]) + 9, 66
+    x, u = draw(g, rows, width, torch.float32), draw(g, rows, width, torch.float32)
+    state = draw(g, count, width, torch.float32)
+    y, final = torch.full_like(x, 7.0), torch.empty_like(state)
+    ops.gated_scan_forward(x, u, y, starts=starts.int().cuda(), state=state, final=final)
+    z, h = torch.sigmoid(u.double()).cpu(), state.double().cpu()
+    want, xs = torch.full((rows, width), 7.0, dtype=torch.float64), x.double().cpu()
+    for t in range(int(lengths.max())):
+        on = (lengths > t).nonzero()[:, 0]
+        at = starts[on] + t
+        h[on] = h[on] + z[at] * (xs[at] - h[on])
+        want[at] = h[on]
+    # a step rounds h by 2^-23 of what is there at most, of which less than all is kept: 700 of them
+    bound = 700 * 2.0 ** -23 * 6
+    assert float((y.double().cpu() - want).abs().max()) < bound and float((final.double().cpu() - h).abs().max()) < bound
+    assert bool((y[:5] == 7).all()) and bool((y[-9:] == 7).all())
+
+
+@gpu
+@pytest.mark.parametrize("kind", list(TYPES))
 def test_what_is_no_number_stays_in_its_sequence_and_closed_gates_keep_the_state(ops, kind):
     dtype = TYPES[kind][0]
     g = torch.Generator().manual_seed(5)
