@@ -51,7 +51,7 @@ __global__ __launch_bounds__(kBlock) void embedding_kernel(LookupArgs a)
 
 // ---------------------------------------------------------------- backward
 //   d[v] (+)= scale * the sum over the rows r with token[r] = v of dy[r], in the rows' order
-// The rows are sorted by token, those of one token in their own order; then every 32 consecutive ones are added up run by run, runs that go
+// The rows are sorted by token, those of one token in their own order; then every 4 to 32 consecutive ones are added up run by run, runs that go
 // on beyond their 32 in a launch behind it, part after part.  No order depends on which workgroup comes first.
 
 // -- zeros.  Sorting keeps a few units busy for some microseconds, in which the others write zeros to the table's first rows, whether
@@ -87,9 +87,52 @@ __device__ __forceinline__ void write_zeros(const Zeros& z, uint32_t group)
     }
 }
 
-// -- sorting: tiles of 2048 rows by one workgroup each, then up to 32 sorted tiles at a time into one.
-constexpr int kTile = 2048, kSortLanes = 1024, kFanIn = 32;
+// -- sorting: tiles of 2048 rows by one workgroup each, then several sorted tiles at a time into one: all 32 of up to 65536
+// rows (65536 x 512 62 us for the whole call, and 66 with eight at a time), of more rows eight (2^20 x 64 265 us, and 385).
+constexpr int kTile = 2048, kSortLanes = 1024, kFanIn = 8, kMostTiles = 32;
 constexpr uint32_t kNoToken = ~0u;          // behind the last row: larger than any token
+
+// Few rows: a row's place is the number of rows in front of it, those of a lower token and those of the same one further in front, counted one by
+// one.  A workgroup takes kRanked rows; all tokens are in LDS, in kShares shares of a multiple of four, each counted for the kRanked rows by as many lanes.
+constexpr int kRanked = 16, kRankLanes = 1024, kShares = kRankLanes / kRanked;
+
+__global__ __launch_bounds__(kRankLanes) void rank_kernel(const void* tokens, bool wide, uint32_t rows, int vocab, uint32_t share, uint32_t* sorted_tokens,
+                                                          uint32_t* sorted_rows, uint32_t groups, Zeros zeros)
+{
+    if (blockIdx.x >= groups) {
+        write_zeros<kRankLanes>(zeros, blockIdx.x - groups);
+        return;
+    }
+    extern __shared__ uint32_t all[];               // [kShares][share]
+    __shared__ uint32_t places[kRanked];
+    if (threadIdx.x < kRanked) places[threadIdx.x] = 0;
+    for (uint32_t i = threadIdx.x; i < share * kShares; i += kRankLanes) all[i] = i < rows ? token_at(tokens, wide, i, vocab) : kNoToken;
+    __syncthreads();
+    const uint32_t row = blockIdx.x * kRanked + threadIdx.x % kRanked, from = threadIdx.x / kRanked * share;
+    const uint32_t token = all[row < rows ? row : 0];
+    // those in front count up to the token, those behind below it
+    typedef uint32_t words __attribute__((ext_vector_type(4)));
+    uint32_t count = 0;
+    const uint32_t first = blockIdx.x * kRanked;
+    if (first < from + share && first + kRanked > from) {
+        for (uint32_t j = from; j < from + share; ++j) count += all[j] < token + (j < row);
+    } else {
+        const uint32_t below = token + (from < first);
+#pragma unroll 4
+        for (uint32_t j = from; j < from + share; j += 4) {
+            const words w = *reinterpret_cast<const words*>(all + j);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) count += w[k] < below;
+        }
+    }
+#pragma unroll
+    for (int over = kRanked; over < kWave; over *= 2) count += __shfl_xor(count, over, kWave);
+    if (static_cast<int>(threadIdx.x) % kWave < kRanked) atomicAdd(places + threadIdx.x % kRanked, count);
+    __syncthreads();
+    if (threadIdx.x >= kRanked || row >= rows) return;
+    sorted_tokens[places[threadIdx.x]] = token;
+    sorted_rows[places[threadIdx.x]] = row;
+}
 
 // Bitonic sorting of 2048 keys, two to a lane: the token above the place in the tile, all of them different.
 template<typename Key>
@@ -164,15 +207,13 @@ __global__ __launch_bounds__(kSortLanes) void sort_tile_kernel(const void* token
     }
 }
 
-// Places of sorted[0 .. n) that hold less than `token`, or, with OR_EQUAL, not more.
-template<bool OR_EQUAL>
+// Places of sorted[0 .. n) that hold less than `token`.
 __device__ __forceinline__ uint32_t places_below(const uint32_t* sorted, uint32_t n, uint32_t token)
 {
     uint32_t low = 0;
     while (n > 0) {
         const uint32_t half = n / 2;
-        const uint32_t t = sorted[low + half];
-        if (OR_EQUAL ? t <= token : t < token) {
+        if (sorted[low + half] < token) {
             low += half + 1;
             n -= half + 1;
         } else {
@@ -182,27 +223,27 @@ __device__ __forceinline__ uint32_t places_below(const uint32_t* sorted, uint32_
     return low;
 }
 
-// Up to kFanIn neighbouring tiles into one: a row's place is the number of rows in front of it in each, of those of the same token in the
-// tiles in front too.  A workgroup takes kMerged rows of one tile, and kSides tiles at a time into LDS (a step of a search in memory that
-// another XCD has written waits 0.7 us); each of its four parts searches two of them for every row.
-constexpr int kSides = 8, kMerged = 256, kMergeLanes = 1024, kParts = kMergeLanes / kMerged;
+// `fan` neighbouring tiles into one: a row's place is the number of rows in front of it in each, of those of the same token in the tiles in
+// front too.  A workgroup takes kMerged rows of one tile, and kFanIn tiles at a time into LDS (a step of a search in memory that another
+// XCD has written waits 0.7 us); each of its four parts searches two of them for every row.
+constexpr int kMerged = 256, kMergeLanes = 1024, kParts = kMergeLanes / kMerged;
 
 __global__ __launch_bounds__(kMergeLanes) void merge_tiles_kernel(const uint32_t* tokens, const uint32_t* rows, uint32_t* out_tokens, uint32_t* out_rows,
-                                                                  uint32_t count)
+                                                                  uint32_t count, uint32_t fan)
 {
-    __shared__ uint32_t lists[kSides][kTile];
+    __shared__ uint32_t lists[kFanIn][kTile];
     __shared__ uint32_t counts[kParts][kMerged];
-    const uint32_t begin = blockIdx.x * kMerged, own = begin / kTile, first = own / kFanIn * kFanIn;
+    const uint32_t begin = blockIdx.x * kMerged, own = begin / kTile, first = own / fan * fan;
     const uint32_t tiles = count / kTile + (count % kTile != 0);
-    const uint32_t last = first + kFanIn < tiles ? first + kFanIn : tiles;
+    const uint32_t last = first + fan < tiles ? first + fan : tiles;
     const uint32_t part = threadIdx.x / kMerged, i = begin + threadIdx.x % kMerged;
     const uint32_t token = tokens[i < count ? i : 0], row = rows[i < count ? i : 0];
     uint32_t below = 0;
-    for (uint32_t t = first; t < last; t += kSides) {
+    for (uint32_t t = first; t < last; t += kFanIn) {
         __syncthreads();
         const uint32_t base = t * kTile;
         // all of them asked for before the first is waited for; the list's memory goes on to the next 64 words
-        constexpr int kLoads = kSides * kTile / (4 * kMergeLanes);
+        constexpr int kLoads = kFanIn * kTile / (4 * kMergeLanes);
         typedef uint32_t words __attribute__((ext_vector_type(4)));
         words w[kLoads];
 #pragma unroll
@@ -218,8 +259,8 @@ __global__ __launch_bounds__(kMergeLanes) void merge_tiles_kernel(const uint32_t
             *reinterpret_cast<words*>(&lists[0][0] + at) = w[j];
         }
         __syncthreads();
-        // step by step in all of the part's lists at once; a list behind the last one holds kNoToken, and nothing below a token
-        constexpr int kOwn = kSides / kParts;
+        // step by step in all of the part's lists at once; a list that is not there holds kNoToken, and nothing below a token
+        constexpr int kOwn = kFanIn / kParts;
         uint32_t low[kOwn] = {};
         const auto look = [&](uint32_t step) {
             uint32_t seen[kOwn];
@@ -247,19 +288,35 @@ __global__ __launch_bounds__(kMergeLanes) void merge_tiles_kernel(const uint32_t
     out_rows[place] = row;
 }
 
-// The same for larger tiles, of more than 65536 rows, in memory.
+// kFanIn larger tiles into one, in memory, step by step in all tiles at once.
 __global__ __launch_bounds__(kBlock) void merge_large_kernel(const uint32_t* tokens, const uint32_t* rows, uint32_t* out_tokens, uint32_t* out_rows,
                                                              uint32_t count, uint32_t tile)
 {
     const uint32_t i = blockIdx.x * kBlock + threadIdx.x;
     if (i >= count) return;
     const uint32_t own = i / tile, first = own / kFanIn * kFanIn;
-    const uint32_t tiles = count / tile + (count % tile != 0);
-    const uint32_t last = first + kFanIn < tiles ? first + kFanIn : tiles;
     const uint32_t token = tokens[i];
+    uint32_t low[kFanIn] = {}, n[kFanIn];
+#pragma unroll
+    for (uint32_t j = 0; j < kFanIn; ++j) {
+        const unsigned long long begin = static_cast<unsigned long long>(first + j) * tile;
+        n[j] = first + j == own || begin >= count ? 0 : count - begin < tile ? static_cast<uint32_t>(count - begin) : tile;
+    }
+    const auto look = [&](uint32_t step) {
+        uint32_t seen[kFanIn];
+#pragma unroll
+        for (uint32_t j = 0; j < kFanIn; ++j) {
+            const uint32_t at = low[j] + step - 1;
+            seen[j] = at < n[j] ? tokens[(first + j) * tile + at] : kNoToken;
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kFanIn; ++j) low[j] += (first + j < own ? seen[j] <= token : seen[j] < token) ? step : 0;
+    };
+    for (uint32_t step = tile / 2; step; step /= 2) look(step);
+    look(1);
     uint32_t place = first * tile + (i - own * tile);
-    for (uint32_t t = first; t < own; ++t) place += places_below<true>(tokens + t * tile, tile, token);
-    for (uint32_t t = own + 1; t < last; ++t) place += places_below<false>(tokens + t * tile, count - t * tile < tile ? count - t * tile : tile, token);
+#pragma unroll
+    for (int j = 0; j < kFanIn; ++j) place += low[j];
     out_tokens[place] = token;
     out_rows[place] = rows[i];
 }
@@ -332,7 +389,7 @@ __global__ __launch_bounds__(kBlock) void table_gradient_kernel(TableGradientArg
             const uint32_t token = first + threadIdx.x;
             bool empty = token < static_cast<uint32_t>(a.vocab);
             if (empty && a.count) {
-                const uint32_t at = places_below<false>(a.tokens, a.count, token);
+                const uint32_t at = places_below(a.tokens, a.count, token);
                 empty = at == a.count || a.tokens[at] != token;
             }
             rows[threadIdx.x] = empty;
@@ -475,6 +532,10 @@ __global__ __launch_bounds__(kJoinLanes) void table_join_kernel(TableGradientArg
 // What the machine writes while it sorts: 8 us without, 11 with it.
 constexpr long long kZerosDuringSort = 48ll << 20;
 
+// Counted up to here, sorted in tiles and merged beyond: one launch for two, and work that grows with the square of the rows (64 rows 14.6 -> 9.5 us
+// for the whole call, 4099 27.5 -> 22.6, 7000 30.3 -> 28.2, but 8192 30.7 -> 32.4).
+constexpr uint32_t kMostRanked = 7168;
+
 // Rows of a run: as many as leave a workgroup for each, and kEnoughChunks of them where there are rows for that.
 constexpr size_t kEnoughChunks = 768;
 int run_of(long long rows)
@@ -615,26 +676,37 @@ int pxh_embedding_backward(const void* dy, const void* tokens, void* d, int type
             a.zeroed += static_cast<uint32_t>(z.rows);
             return z;
         };
+        static_assert(kRankLanes == kSortLanes, "zeros are written by as many lanes");
         const Zeros during = zeros(kZerosDuringSort, kSortLanes);
-        // token and place of the tile in 32 bits
-        const auto sort = vocab < (1 << 21) - 1 ? &sort_tile_kernel<uint32_t> : &sort_tile_kernel<unsigned long long>;
-        hipLaunchKernelGGL(sort, dim3(tiles + during.groups), dim3(kSortLanes), 0, s, tokens, wide_tokens != 0, rows, vocab, lists[0], lists[1], tiles, during);
-        if (int rc = check_launch(who)) return rc;
-        int from = 0;
-        for (unsigned long long tile = kTile; tile < a.count; tile *= kFanIn) {
-            const int to = 2 - from;
-            if (tile == kTile) {
-                hipLaunchKernelGGL(merge_tiles_kernel, dim3(grid_for(a.count, kMerged)), dim3(kMergeLanes), 0, s, lists[from], lists[from + 1], lists[to],
-                                   lists[to + 1], a.count);
-            } else {
-                hipLaunchKernelGGL(merge_large_kernel, dim3(grid_for(a.count, kBlock)), dim3(kBlock), 0, s, lists[from], lists[from + 1], lists[to],
-                                   lists[to + 1], a.count, static_cast<uint32_t>(tile));
-            }
+        if (a.count <= kMostRanked) {
+            const uint32_t groups = (a.count + kRanked - 1) / kRanked, share = (a.count + 4 * kShares - 1) / (4 * kShares) * 4;
+            hipLaunchKernelGGL(rank_kernel, dim3(groups + during.groups), dim3(kRankLanes), share * kShares * sizeof(uint32_t), s, tokens, wide_tokens != 0,
+                               a.count, vocab, share, lists[0], lists[1], groups, during);
             if (int rc = check_launch(who)) return rc;
-            from = to;
+            a.tokens = lists[0];
+            a.rows = lists[1];
+        } else {
+            // token and place of the tile in 32 bits
+            const auto sort = vocab < (1 << 21) - 1 ? &sort_tile_kernel<uint32_t> : &sort_tile_kernel<unsigned long long>;
+            hipLaunchKernelGGL(sort, dim3(tiles + during.groups), dim3(kSortLanes), 0, s, tokens, wide_tokens != 0, rows, vocab, lists[0], lists[1], tiles, during);
+            if (int rc = check_launch(who)) return rc;
+            const uint32_t fan = tiles <= kMostTiles ? kMostTiles : kFanIn;
+            int from = 0;
+            for (unsigned long long tile = kTile; tile < a.count; tile *= tile == kTile ? fan : kFanIn) {
+                const int to = 2 - from;
+                if (tile == kTile) {
+                    hipLaunchKernelGGL(merge_tiles_kernel, dim3(grid_for(a.count, kMerged)), dim3(kMergeLanes), 0, s, lists[from], lists[from + 1], lists[to],
+                                       lists[to + 1], a.count, fan);
+                } else {
+                    hipLaunchKernelGGL(merge_large_kernel, dim3(grid_for(a.count, kBlock)), dim3(kBlock), 0, s, lists[from], lists[from + 1], lists[to],
+                                       lists[to + 1], a.count, static_cast<uint32_t>(tile));
+                }
+                if (int rc = check_launch(who)) return rc;
+                from = to;
+            }
+            a.tokens = lists[from];
+            a.rows = lists[from + 1];
         }
-        a.tokens = lists[from];
-        a.rows = lists[from + 1];
     }
     int rc = PXH_OK;
     dispatch_type(type, [&]<int T>() {
