@@ -16,6 +16,8 @@ __device__ __forceinline__ uint32_t token_at(const void* tokens, bool wide, long
 
 // ---------------------------------------------------------------- forward
 //   y[r] = scale * table[token[r]], zeros for a token outside the vocabulary
+// A vector a lane, rows one behind the other: bound by what is written and by the table's rows that the caches do not hold.  16384 x 4096
+// bf16 of a text's tokens 30.4 us: 134 MB written and the rows of a table of 410 MB read, the frequent ones once (268 MB, at 8.8 TB/s).
 struct LookupArgs {
     const char* table;
     const void* tokens;
@@ -52,7 +54,10 @@ __global__ __launch_bounds__(kBlock) void embedding_kernel(LookupArgs a)
 // ---------------------------------------------------------------- backward
 //   d[v] (+)= scale * the sum over the rows r with token[r] = v of dy[r], in the rows' order
 // The rows are sorted by token, those of one token in their own order; then every 4 to 32 consecutive ones are added up run by run, runs that go
-// on beyond their 32 in a launch behind it, part after part.  No order depends on which workgroup comes first.
+// on beyond those in a launch behind it, part after part.  No order depends on which workgroup comes first.
+// 16384 x 2048 bf16 into 32768 rows: sorting 11 us (with 48 MB of zeros), merging 5, sums and the other zeros 25 (153 MB at 6.2 TB/s), what goes
+// on from chunk to chunk 5; 59 us in all, with tensors that no cache holds (floor 31).  4099 x 1025 fp32 added to 10007 rows: places 7.5, sums
+// 9, chunk to chunk 6, 23 in all (floor 8): three launches, each a few trips to memory one behind the other.
 
 // -- zeros.  Sorting keeps a few units busy for some microseconds, in which the others write zeros to the table's first rows, whether
 // a row has their token or not; the rows behind those wait for the sums, which know which of them have none.
@@ -134,7 +139,8 @@ __global__ __launch_bounds__(kRankLanes) void rank_kernel(const void* tokens, bo
     sorted_rows[places[threadIdx.x]] = row;
 }
 
-// Bitonic sorting of 2048 keys, two to a lane: the token above the place in the tile, all of them different.
+// Bitonic sorting of 2048 keys, two to a lane: the token above the place in the tile, all of them different.  66 steps one behind the
+// other, of which 51 stay in a wave: 8 us, whatever the number of tiles.
 template<typename Key>
 __device__ __forceinline__ void compare(Key& a, Key& b, bool up)
 {
@@ -371,6 +377,7 @@ struct TableRow {
     }
 };
 
+// Bound by the memory: eight rows of a run are asked for at once, and as many workgroups run as units hold.
 // The first workgroups add up a run of sorted rows each (times column groups), the others, where the gradient is overwritten, write zeros to
 // kZeroRows rows of the table each, where no row has their token.
 constexpr int kZeroRows = 32;
@@ -466,7 +473,8 @@ __global__ __launch_bounds__(kBlock) void table_gradient_kernel(TableGradientArg
 }
 
 // The runs that go on beyond a chunk, by the workgroup of the chunk in which they begin: 256 columns to a workgroup, whose waves share
-// the chunks.
+// the chunks.  Most chunks have none: 5 us, a launch and two trips to memory (where all of 16384 rows
+// have one token the call takes 10 us more).
 constexpr int kJoinLanes = 256, kJoinColumns = 256;
 
 template<int D>
