@@ -256,27 +256,33 @@ int pxh_beam_reorder(int count, void* const* tensors, const long long* row_bytes
     if (beams < 1 || beams > kMostBeams) return fail_invalid("%s: %d beams (1 to %d)", who, beams, kMostBeams);
     if (batch == 0 || count == 0) return PXH_OK;
     if (!parents) return fail_invalid("%s: null pointer", who);
+    const int columns = kHeld * kBlock / beams;
+    const long long width = static_cast<long long>(columns) * 16;
+    // everything is looked at before the first launch
     for (int i = 0; i < count; ++i) {
         if (row_bytes[i] < 0 || row_bytes[i] > 1ll << 40) return fail_invalid("%s: rows of %lld bytes", who, row_bytes[i]);
         if (row_bytes[i] && !tensors[i]) return fail_invalid("%s: null pointer", who);
         if (strides[i] < row_bytes[i]) return fail_invalid("%s: rows of %lld bytes that overlap", who, row_bytes[i]);
+        if ((row_bytes[i] + width - 1) / width * batch >= 1 << 23) return fail_invalid("%s: %d rows of %lld bytes", who, batch * beams, row_bytes[i]);
+        for (int j = 0; j < i && row_bytes[i]; ++j)
+            if (tensors[j] == tensors[i] && row_bytes[j]) return fail_invalid("%s: tensors %d and %d are the same", who, j, i);
     }
     ReorderArgs a{};
     a.parents = parents;
     a.batch = batch;
     a.beams = beams;
-    a.columns = kHeld * kBlock / beams;
+    a.columns = columns;
     unsigned groups = 0;
     const auto launch = [&] {
-        if (groups) hipLaunchKernelGGL(beam_reorder_kernel, dim3(groups), dim3(kBlock), 0, as_stream(stream), a);
+        if (!groups) return static_cast<int>(PXH_OK);
+        hipLaunchKernelGGL(beam_reorder_kernel, dim3(groups), dim3(kBlock), 0, as_stream(stream), a);
         a.count = 0;
         groups = 0;
         return check_launch(who);
     };
     for (int i = 0; i < count; ++i) {
         if (row_bytes[i] == 0) continue;
-        const long long width = static_cast<long long>(a.columns) * 16, parts = (row_bytes[i] + width - 1) / width;
-        if (parts * batch >= 1 << 23) return fail_invalid("%s: %d rows of %lld bytes", who, batch * beams, row_bytes[i]);
+        const long long parts = (row_bytes[i] + width - 1) / width;
         const unsigned more = static_cast<unsigned>(parts * batch);
         if (a.count == kMostTensors || groups + more >= 1u << 24)
             if (int rc = launch()) return rc;

@@ -528,6 +528,7 @@ __global__ __launch_bounds__(Forward::kLanes, 4) void scan_kernel(ScanArgs a)
     Raw<T, kV> x[kSteps], u[kSteps], o[GATE ? kSteps : 1];
     load_tokens<T, kSteps>(a.x, a.x_stride, first, a.q.rows, columns, x);
     load_tokens<T, kSteps>(a.update, a.update_stride, first, a.q.rows, columns, u);
+    if constexpr (GATE) load_tokens<T, kSteps>(a.gate, a.gate_stride, first, a.q.rows, columns, o);
     const Whole whole = columns.inside ? within_one(a.q, kept, chunk_first, kChunk) : Whole{ false, false, false, 0 };
     const auto pass = [&]<bool RARE>() {
         Borders b{ 0, 0, Forward::kAll, 0 };
@@ -542,8 +543,6 @@ __global__ __launch_bounds__(Forward::kLanes, 4) void scan_kernel(ScanArgs a)
 #pragma unroll
             for (int k = 0; k < kV; ++k) gate_of<T>(v[k], z[i][k], rest);
         }
-        // into the updates' registers
-        if constexpr (GATE) load_tokens<T, kSteps>(a.gate, a.gate_stride, first, a.q.rows, columns, o);
         float h[kV] = {}, Z[kV] = {};
         if (begins_here && a.state) load_state(a.state, slot_of(a.slots, whole.sequence), e, a.width, h);
         if (wave == 0) {

@@ -1,5 +1,7 @@
 """The native calls that also look at the tensors' device, and what the entry points behind them refuse.  No device: a call ends before
 anything is launched."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -100,6 +102,16 @@ def test_the_entry_points_refuse():
         assert "pxh_beam_select" in refused(*select(**change)), change
     assert capi.call_raw(*select(batch=0)) == 0
     assert "pxh_beam_reorder" in refused("pxh_beam_reorder", 1, None, None, None, HERE, 2, 3, None)
+
+    def reorder(tensors=(HERE, 2 * HERE), row_bytes=(8, 8), strides=(8, 8), batch=2, beams=3, parents=HERE):
+        n = len(tensors)
+        return ("pxh_beam_reorder", n, (ctypes.c_void_p * n)(*tensors), (ctypes.c_longlong * n)(*row_bytes), (ctypes.c_longlong * n)(*strides),
+                parents, batch, beams, None)
+    # (the second tensor is looked at before the first is touched)
+    for change in (dict(row_bytes=(8, -1)), dict(strides=(8, 7)), dict(tensors=(HERE, None)), dict(tensors=(HERE, HERE)), dict(parents=None),
+                   dict(beams=0), dict(beams=65), dict(batch=-1), dict(batch=1 << 20, beams=64, row_bytes=(8, 1 << 20), strides=(8, 1 << 20))):
+        assert "pxh_beam_reorder" in refused(*reorder(**change)), change
+    assert capi.call_raw(*reorder(batch=0)) == 0 and capi.call_raw(*reorder(row_bytes=(0, 0), tensors=(None, None))) == 0
 
 
 def test_a_workspace_that_is_too_small_or_askew_is_refused():
