@@ -59,8 +59,8 @@ __global__ __launch_bounds__(kBlock) void embedding_kernel(LookupArgs a)
 // on from chunk to chunk 5; 59 us in all, with tensors that no cache holds (floor 31).  4099 x 1025 fp32 added to 10007 rows: places 7.5, sums
 // 9, chunk to chunk 6, 23 in all (floor 8): three launches, each a few trips to memory one behind the other.
 
-// -- zeros.  Sorting keeps a few units busy for some microseconds, in which the others write zeros to the table's first rows, whether
-// a row has their token or not; the rows behind those wait for the sums, which know which of them have none.
+// -- zeros.  Sorting keeps a few units busy for some microseconds, in which the others write zeros to the table's last rows, whether
+// a row has their token or not; the rows in front of those wait for the sums, which know which of them have none.
 struct Zeros {
     char* d;
     long long first, rows, stride_bytes, row_bytes;
@@ -339,7 +339,7 @@ struct TableGradientArgs {
     long long dy_stride, d_stride;
     uint32_t count, chunks;         // rows, and every `run` of them
     int run;
-    uint32_t zeroed;                // rows of the table that hold zeros already
+    uint32_t open;                  // the table's first rows, which hold no zeros yet
     int vocab, width, column_groups;
     float scale;
     bool accumulate;
@@ -391,10 +391,10 @@ __global__ __launch_bounds__(kBlock) void table_gradient_kernel(TableGradientArg
     by_columns.divmod(blockIdx.x, part, group);
     const int e = static_cast<int>(group * blockDim.x + threadIdx.x) * V;
     if (part >= a.chunks) {
-        const uint32_t first = a.zeroed + (part - a.chunks) * kZeroRows;
+        const uint32_t first = (part - a.chunks) * kZeroRows;
         if (threadIdx.x < kZeroRows) {
             const uint32_t token = first + threadIdx.x;
-            bool empty = token < static_cast<uint32_t>(a.vocab);
+            bool empty = token < a.open;
             if (empty && a.count) {
                 const uint32_t at = places_below(a.tokens, a.count, token);
                 empty = at == a.count || a.tokens[at] != token;
@@ -537,8 +537,10 @@ __global__ __launch_bounds__(kJoinLanes) void table_join_kernel(TableGradientArg
     d.write(a, token, e, sum);
 }
 
-// What the machine writes while it sorts: 8 us without, 11 with it.
-constexpr long long kZerosDuringSort = 48ll << 20;
+// What the machine writes while it sorts, from the table's end, whose tokens are the rare ones where they are numbered by their frequency (8192 x
+// 1024 bf16 into 131072 rows 71.1 us without, 64.0 so; 65536 x 512 into 32768 rows of fp32 65.6 and 60.9; but 16384 x 2048 into 32768 55.9 and
+// 60.8: there the sums leave the memory time for all zeros).
+constexpr long long kZerosDuringSort = 64ll << 20;
 
 // Counted up to here, sorted in tiles and merged beyond: one launch for two, and work that grows with the square of the rows (64 rows 14.6 -> 9.5 us
 // for the whole call, 4099 27.5 -> 22.6, 7000 30.3 -> 28.2, but 8192 30.7 -> 32.4).
@@ -576,7 +578,7 @@ int launch_gradient(const char* who, TableGradientArgs a, hipStream_t s)
     const int vectors = (a.width + kVec<T> - 1) / kVec<T>;
     a.column_groups = (vectors + kBlock - 1) / kBlock;
     const int lanes = ((vectors + a.column_groups - 1) / a.column_groups + kWave - 1) / kWave * kWave;
-    const long long zero_groups = (static_cast<long long>(a.vocab) - a.zeroed + kZeroRows - 1) / kZeroRows;
+    const long long zero_groups = (static_cast<long long>(a.open) + kZeroRows - 1) / kZeroRows;
     const long long groups = (a.chunks + zero_groups) * a.column_groups;
     if (groups * lanes >= 1ll << 32 || groups >= 1ll << 31) return fail_invalid("%s: too many rows of too many values", who);
     if (groups == 0) return PXH_OK;
@@ -664,7 +666,7 @@ int pxh_embedding_backward(const void* dy, const void* tokens, void* d, int type
     a.scale = scale;
     a.accumulate = accumulate != 0;
     a.past = static_cast<size_t>(vocab) * static_cast<size_t>(width) * size_of(d_type) >= kStreamingBytes;
-    a.zeroed = a.accumulate ? static_cast<uint32_t>(vocab) : 0;
+    a.open = a.accumulate ? 0 : static_cast<uint32_t>(vocab);
     if (rows > 0) {
         const Space space(rows, width);
         void* ws = nullptr;
@@ -677,12 +679,10 @@ int pxh_embedding_backward(const void* dy, const void* tokens, void* d, int type
         // zeros for a launch that takes some microseconds on a few units: `bytes` of them, from the rows that have none yet
         const long long row_bytes = static_cast<long long>(width) * size_of(d_type), pieces = (row_bytes + 15) / 16;
         const auto zeros = [&](long long bytes, int lanes) {
-            Zeros z{ a.d, a.zeroed, 0, d_stride * static_cast<long long>(size_of(d_type)), row_bytes, FastDiv(static_cast<uint32_t>(pieces)), 0, a.past };
-            const long long left = vocab - static_cast<long long>(a.zeroed);
-            z.rows = bytes / row_bytes < left ? bytes / row_bytes : left;
-            z.groups = grid_for(static_cast<size_t>(z.rows) * pieces, static_cast<size_t>(lanes) * kZeroPieces);
-            a.zeroed += static_cast<uint32_t>(z.rows);
-            return z;
+            const long long some = bytes / row_bytes < a.open ? bytes / row_bytes : a.open;
+            a.open -= static_cast<uint32_t>(some);
+            return Zeros{ a.d, a.open, some, d_stride * static_cast<long long>(size_of(d_type)), row_bytes, FastDiv(static_cast<uint32_t>(pieces)),
+                          grid_for(static_cast<size_t>(some) * pieces, static_cast<size_t>(lanes) * kZeroPieces), a.past };
         };
         static_assert(kRankLanes == kSortLanes, "zeros are written by as many lanes");
         const Zeros during = zeros(kZerosDuringSort, kSortLanes);
