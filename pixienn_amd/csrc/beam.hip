@@ -131,8 +131,9 @@ struct Space {
 // ---------------------------------------------------------------- reordering
 // In place: a workgroup takes columns of all beams of one item, each lane up to kHeld pieces of 16 bytes, which it reads from the parent's
 // row and, when all of the workgroup have read, writes.  Rows that stay where they are are neither read nor written for themselves.
-// Parents, then rows, then stores, one behind the other: nine tensors of one item of 4 beams 5.9 us, five of 64 items of 8 beams 9.3 (18 MB).
-constexpr int kHeld = 8, kMostTensors = 32;
+// Parents, then rows, then stores, one behind the other: nine tensors of one item of 4 beams 3.6 us, five of 64 items of 8 beams 6.3 (18 MB); 16
+// tensors of 1024 rows of 16 kB 53 (537 MB if every row moved; three of four do).  Eight pieces a lane: 8.1 and 55.
+constexpr int kHeld = 4, kMostTensors = 32;
 
 struct Tensor {
     char* data;
@@ -145,13 +146,14 @@ struct ReorderArgs {
     Tensor tensors[kMostTensors];
     const int* parents;
     int count, batch, beams, columns;   // columns: pieces of a row that a workgroup takes
+    FastDiv by_columns;
 };
 
 __global__ __launch_bounds__(kBlock) void beam_reorder_kernel(ReorderArgs a)
 {
-    int which = 0;
-    for (int i = 1; i < a.count; ++i)
-        if (blockIdx.x >= a.tensors[i].first) which = i;
+    // the last tensor that begins no further behind: all of them looked at in one trip
+    const int lane = threadIdx.x % kWave;
+    const int which = __popcll(__ballot(lane < a.count && blockIdx.x >= a.tensors[lane < a.count ? lane : 0].first)) - 1;
     const Tensor& t = a.tensors[which];
     const unsigned at = blockIdx.x - t.first;
     const long long item = at / t.parts;
@@ -165,7 +167,7 @@ __global__ __launch_bounds__(kBlock) void beam_reorder_kernel(ReorderArgs a)
 #pragma unroll
     for (int j = 0; j < kHeld; ++j) {
         const int piece = j * kBlock + threadIdx.x;
-        beam[j] = piece < pieces ? piece / a.columns : 0;
+        beam[j] = piece < pieces ? static_cast<int>(a.by_columns.div(piece)) : 0;
         parent[j] = parents[beam[j]];
     }
     words held[kHeld];
@@ -268,6 +270,7 @@ int pxh_beam_reorder(int count, void* const* tensors, const long long* row_bytes
             if (tensors[j] == tensors[i] && row_bytes[j]) return fail_invalid("%s: tensors %d and %d are the same", who, j, i);
     }
     ReorderArgs a{};
+    a.by_columns = FastDiv(columns);
     a.parents = parents;
     a.batch = batch;
     a.beams = beams;
