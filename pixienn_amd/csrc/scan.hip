@@ -64,18 +64,18 @@ template<int T>
 constexpr int kTileOf = kChannels<T> * kWave;
 constexpr int kSaved = PXH_SCAN_SAVED;  // tokens from one saved state to the next
 
-// Tokens of a wave, and waves of a workgroup, one behind the other along the tokens.
-template<int STEPS, int WAVES>
+// Tokens of a wave, waves of a workgroup, one behind the other along the tokens, and chunks (workgroups) of a group.
+template<int STEPS, int WAVES, int GROUP>
 struct Shape {
-    static constexpr int kSteps = STEPS, kWaves = WAVES, kChunk = STEPS * WAVES, kLanes = WAVES * kWave;
+    static constexpr int kSteps = STEPS, kWaves = WAVES, kGroup = GROUP, kChunk = STEPS * WAVES, kLanes = WAVES * kWave;
     static constexpr uint32_t kAll = (1u << STEPS) - 1;
     static_assert(kSaved % STEPS == 0 && kChunk % kSaved == 0, "a saved state is in front of a wave's tokens");
 };
 // Two workgroups of eight waves to a unit.  Chunks of 64 tokens pay twice for what a chunk costs whatever its length (a number, a word, a
 // look back: 8 x 4096 x 2048 bf16 with a gate 139 us where 128 take 116).  The gradients keep three values for each that they read:
 // waves of 16 tokens spill (430 us, and 193).
-using Forward = Shape<16, 8>;
-using Backward = Shape<8, 8>;
+using Forward = Shape<16, 8, 8>;
+using Backward = Shape<8, 8, 4>;
 
 // Where sequences begin: starts[sequences + 1], or all of one length.  Of fewer than kFew sequences a wave's lanes keep all places, asked for
 // before the workgroup knows its chunk.
@@ -208,18 +208,18 @@ __device__ __forceinline__ Whole within_one(const Sequences& q, int kept, int fi
 
 // ---------------------------------------------------------------- from chunk to chunk
 // Workgroups take numbers, chunk by chunk along the tokens (for the gradients against them).  Each leaves what its chunk does to a
-// state, channel by channel, as one 64-bit word; the last one of kGroup chunks leaves one for all of them, and once it knows the state in
+// state, channel by channel, as one 64-bit word; the last one of a group of chunks leaves one for all of them, and once it knows the state in
 // front of the group, the state behind it as a whole range.  A chunk waits for the words of those in front of it in its group, which
 // wait for nobody, and for the state in front of the group: the words of up to kWindow groups, until one of them is whole and none nearer is
-// missing.  So the state has to go from hand to hand only once for kGroup * kWindow chunks.  A state is always put together in the same way,
+// missing.  So the state has to go from hand to hand only once for kWindow groups.  A state is always put together in the same way,
 // whichever words were there first: the same call gives the same bits.
 // A workgroup waits for lower numbers only, which are running or done: the lowest of those running waits for none.  The bound on the looks
 // makes the exit unconditional all the same (a second or two); where it was reached (two launches at once on one workspace, which the
 // interface forbids) the states are NaN.
 constexpr unsigned long long kNotThere = ~0ull;     // no range: a Z that is no number is left as 1, with its H
-// (65536 x 256 bf16, channels that remember: every chunk handing its state on 173 us, groups of 4 49, of 8 38, where the gradients of wide
-// calls spill: 8 x 4096 x 2048 with a gate 193 -> 244)
-constexpr int kGroup = 4, kWindow = 4;
+// (65536 x 256 bf16, channels that remember: every chunk handing its state on 173 us, groups of 4 49, of 8 36.  Eight words more than the gradients
+// have registers for: 8 x 4096 x 2048 with a gate 193 us with groups of 4, 244 with groups of 8)
+constexpr int kWindow = 4;
 constexpr uint32_t kLooks = 1u << 20;
 
 // The chunks of the call: segments of as many chunks each, of which none needs another segment's.  Where all sequences have the same length, of
@@ -256,27 +256,28 @@ __device__ __forceinline__ unsigned long long see_word(const unsigned long long*
     return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// What the `count` chunks (fewer than kGroup) whose words begin at `words` do to a state, of one channel (there: one that exists); all lanes of
+// What the `count` chunks (fewer than GROUP) whose words begin at `words` do to a state, of one channel (there: one that exists); all lanes of
 // the wave.
+template<int GROUP>
 __device__ __forceinline__ Range of_group(const unsigned long long* words, uint32_t count, size_t width, bool there)
 {
-    unsigned long long w[kGroup - 1];
+    unsigned long long w[GROUP - 1];
     uint32_t looks = kLooks;
     for (; looks; --looks) {
         bool missing = false;
 #pragma unroll
-        for (int d = 0; d < kGroup - 1; ++d) {
+        for (int d = 0; d < GROUP - 1; ++d) {
             w[d] = 0;                                   // a range of no tokens
             if (there && static_cast<uint32_t>(d) < count) w[d] = see_word(words + d * width);
         }
 #pragma unroll
-        for (int d = 0; d < kGroup - 1; ++d) missing = missing || w[d] == kNotThere;
+        for (int d = 0; d < GROUP - 1; ++d) missing = missing || w[d] == kNotThere;
         if (!__any(missing)) break;
         __builtin_amdgcn_s_sleep(1);
     }
     Range all = range_of(w[0]);
 #pragma unroll
-    for (int d = 1; d < kGroup - 1; ++d) all = joined(all, range_of(w[d]));
+    for (int d = 1; d < GROUP - 1; ++d) all = joined(all, range_of(w[d]));
     return looks ? all : Range{ kWhole, __builtin_nanf("") };
 }
 
@@ -338,7 +339,7 @@ __device__ __forceinline__ Place take_number(const Exchange& x, ScanShared<WAVES
 
 // From the waves' ranges, in the order `order(0 .. WAVES - 1)`, of which the wave is number `turn`, and the chunks in front of the workgroup's: the
 // state in front of the wave, of its lane's channels.
-template<int WAVES, int TILE, int V, typename Order>
+template<int GROUP, int WAVES, int TILE, int V, typename Order>
 __device__ __forceinline__ void join_waves(const Exchange& x, ScanShared<WAVES, TILE>& lds, const Place& p, int width, int turn, const Order& order,
                                            float (&s)[V])
 {
@@ -348,8 +349,8 @@ __device__ __forceinline__ void join_waves(const Exchange& x, ScanShared<WAVES, 
     const bool there = e < width;
     if (x.words) {
         const size_t pitch = static_cast<size_t>(width);
-        const uint32_t group = p.chunk / kGroup, place = p.chunk % kGroup;
-        const bool fresh = p.chunk == 0 || lds.fresh, last = p.chunk + 1 == x.per, ends_group = place == kGroup - 1 && !last;
+        const uint32_t group = p.chunk / GROUP, place = p.chunk % GROUP;
+        const bool fresh = p.chunk == 0 || lds.fresh, last = p.chunk + 1 == x.per, ends_group = place == GROUP - 1 && !last;
         unsigned long long* const of_groups = x.groups + (static_cast<size_t>(p.segment) * x.groups_per + group) * pitch + e;
         Range all{ 0.0f, 0.0f };
         if (threadIdx.x < TILE) {            // whole waves
@@ -359,7 +360,7 @@ __device__ __forceinline__ void join_waves(const Exchange& x, ScanShared<WAVES, 
             unsigned long long* const word = x.words + (static_cast<size_t>(p.segment) * x.per + p.chunk) * pitch + e;
             if (there && !ends_group && !last) leave_word(word, all);
             Range front{ fresh ? kWhole : 0.0f, fresh ? lds.begun[c] : 0.0f };
-            if (!fresh && place) front = of_group(word - place * pitch, place, pitch, there);
+            if (!fresh && place) front = of_group<GROUP>(word - place * pitch, place, pitch, there);
             lds.in_front[c] = front;
             all = joined(front, all);
             if (there && ends_group) leave_word(of_groups, all);
@@ -573,7 +574,7 @@ __global__ __launch_bounds__(Forward::kLanes, 4) void scan_kernel(ScanArgs a)
         }
 #pragma unroll
         for (int k = 0; k < kV; ++k) lds.ranges[wave][lane * kV + k] = Range{ begins_here || (RARE && b.begins) ? kWhole : Z[k], h[k] };
-        join_waves(a.exchange, lds, place, a.width, wave, [](int w) { return w; }, h);
+        join_waves<Forward::kGroup>(a.exchange, lds, place, a.width, wave, [](int w) { return w; }, h);
         as_read(x);
         if (a.saved && first % kSaved == 0 && first < a.q.rows) store_state<NT>(a.saved, first / kSaved, e, a.width, h);
         Writer<T, NT> y(a.y, a.y_stride, first, columns);
@@ -763,7 +764,7 @@ __global__ __launch_bounds__(Backward::kLanes, 4) void scan_backward_kernel(Scan
         }
 #pragma unroll
         for (int k = 0; k < kV; ++k) lds.ranges[wave][lane * kV + k] = Range{ RARE && b.ends ? kWhole : Z[k], C[k] };
-        join_waves(a.exchange, lds, place, a.width, kWaves - 1 - wave, [](int k) { return kWaves - 1 - k; }, C);
+        join_waves<Backward::kGroup>(a.exchange, lds, place, a.width, kWaves - 1 - wave, [](int k) { return kWaves - 1 - k; }, C);
         Writer<T, NT> out_x(a.dx, a.dx_stride, first + kSteps - 1, columns, true), out_u(a.dupdate, a.dupdate_stride, first + kSteps - 1, columns, true);
 #pragma unroll
         for (int i = kSteps - 1; i >= 0; --i) {
@@ -877,7 +878,7 @@ int start_scan(const char* who, int type, long long rows, int width, int sequenc
     if (chunks * tiles * S::kLanes >= 1ull << 32) return fail_invalid("%s: too many rows of too many values", who);
     groups = static_cast<uint32_t>(chunks * tiles);
     const bool apart = length > 0 && length % kChunk == 0 && sequences > 1;
-    const size_t segments = apart ? sequences : 1, per = chunks / segments, groups_per = (per + kGroup - 1) / kGroup;
+    const size_t segments = apart ? sequences : 1, per = chunks / segments, groups_per = (per + S::kGroup - 1) / S::kGroup;
     x = Exchange{ nullptr, nullptr, nullptr, static_cast<uint32_t>(per), static_cast<uint32_t>(groups_per), FastDiv(static_cast<uint32_t>(tiles)),
                   FastDiv(static_cast<uint32_t>(segments)) };
     size_t count = 0;
