@@ -511,7 +511,7 @@ struct ScanArgs {
 
 // A workgroup takes a chunk of tokens of kTile channels, a wave a few of them, which stay in registers as z and x between the pass that finds
 // what they do to a state and the one that forms the states: one trip to memory.
-// 8 x 4096 x 2048 bf16 with a gate and what is saved 120 us (4.5 TB/s; a workgroup's 12 us are 1.4 for its number, 7 for its tokens, 2 for the
+// 8 x 4096 x 2048 bf16 with a gate and what is saved 112 us (4.8 TB/s; a workgroup's 14 us are 1.4 for its number, 6.6 for its tokens, 5 for the
 // states in front of it and 1.5 for the rest; chunks that wait for none 103), without a gate 80 (5.0 TB/s); 30011 x 2561 half in 31 sequences
 // 140 (rows that begin off a word's boundary, and tiles that share lines: 2560 values wide 112).
 template<int T, bool GATE, bool NT>
@@ -609,7 +609,7 @@ __global__ __launch_bounds__(Forward::kLanes, 4) void scan_kernel(ScanArgs a)
 //   G[t] = dy * g + (1 - z[t + 1]) * G[t + 1], g = gate / (1 + exp(-gate));  dx = z G;  dupdate = G (x - h[t - 1]) z (1 - z)
 //   dgate = dy h s (1 + gate (1 - s)), s = 1 / (1 + exp(-gate))
 // Along the tokens from the saved states for h, then against them for G: the carry C = (1 - z) G goes through a range as a state does.
-// 8 x 4096 x 2048 bf16 with a gate 187 us (939 MB at 5.0 TB/s): half as many tokens to a workgroup as forward, for want of registers, and the
+// 8 x 4096 x 2048 bf16 with a gate 188 us (939 MB at 5.0 TB/s): half as many tokens to a workgroup as forward, for want of registers, and the
 // same waits.
 struct ScanBackwardArgs {
     const void* dy;
@@ -866,9 +866,12 @@ int check_scan(const char* who, int type, long long rows, int width, int sequenc
     return PXH_OK;
 }
 
-// Sequences of the call, and the words that its chunks exchange (none where every chunk begins and ends with a sequence).
+// Sequences of the call, and the words that its chunks exchange (none where every chunk begins and ends with a sequence).  side_by_side: sequences
+// as segments, where they can be.  Most calls win by it (the gradients of 8 x 4096 x 2048 bf16 with a gate 198 -> 189 us, of 65536 x 256 in 16
+// sequences 61 -> 53; forward without a gate 84 -> 81), but forward with a gate those lose whose sequences lie 16 MB apart, which meet in the same
+// banks: 8 x 4096 x 2048 116 -> 127, 16 of them 203 -> 217, where 32 x 1024 x 2048 has 107 and 106, 8 x 8192 x 2048 206 and 197.
 template<typename S>
-int start_scan(const char* who, int type, long long rows, int width, int sequences, const int* starts, const Slots& slots, const float* from, float* to,
+int start_scan(const char* who, bool side_by_side, int type, long long rows, int width, int sequences, const int* starts, const Slots& slots, const float* from, float* to,
                void* workspace, size_t workspace_bytes, Sequences& q, Exchange& x, uint32_t& groups, hipStream_t s)
 {
     const long long length = starts || sequences == 0 ? 0 : rows / sequences;
@@ -877,7 +880,7 @@ int start_scan(const char* who, int type, long long rows, int width, int sequenc
     const size_t chunks = chunks_of(rows, kChunk), tile = 4 / size_of(type) * kWave, tiles = (static_cast<size_t>(width) + tile - 1) / tile;
     if (chunks * tiles * S::kLanes >= 1ull << 32) return fail_invalid("%s: too many rows of too many values", who);
     groups = static_cast<uint32_t>(chunks * tiles);
-    const bool apart = length > 0 && length % kChunk == 0 && sequences > 1;
+    const bool apart = side_by_side && length > 0 && length % kChunk == 0 && sequences > 1;
     const size_t segments = apart ? sequences : 1, per = chunks / segments, groups_per = (per + S::kGroup - 1) / S::kGroup;
     x = Exchange{ nullptr, nullptr, nullptr, static_cast<uint32_t>(per), static_cast<uint32_t>(groups_per), FastDiv(static_cast<uint32_t>(tiles)),
                   FastDiv(static_cast<uint32_t>(segments)) };
@@ -927,7 +930,7 @@ int pxh_gated_scan_forward(const void* x, const void* update, const void* gate, 
     ScanArgs a{ x, update, gate, y, state, final, saved, x_stride, update_stride, gate_stride, y_stride, {}, Slots{ slots, slot_count }, {}, width };
     uint32_t groups;
     hipStream_t s = as_stream(stream);
-    if (int rc = start_scan<Forward>(who, type, rows, width, sequences, starts, a.slots, state, final, workspace, workspace_bytes, a.q, a.exchange, groups, s)) return rc;
+    if (int rc = start_scan<Forward>(who, !gate, type, rows, width, sequences, starts, a.slots, state, final, workspace, workspace_bytes, a.q, a.exchange, groups, s)) return rc;
     if (rows == 0) return PXH_OK;
     dispatch_type(type, [&]<int T>() {
         const bool past = streams(rows, width, type, gate ? 4 : 3);
@@ -955,7 +958,7 @@ int pxh_gated_scan_backward(const void* dy, const void* x, const void* update, c
                         dx_stride, dupdate_stride, dgate_stride, {}, Slots{ slots, slot_count }, {}, width };
     uint32_t groups;
     hipStream_t s = as_stream(stream);
-    if (int rc = start_scan<Backward>(who, type, rows, width, sequences, starts, a.slots, d_final, d_state, workspace, workspace_bytes, a.q, a.exchange, groups, s))
+    if (int rc = start_scan<Backward>(who, true, type, rows, width, sequences, starts, a.slots, d_final, d_state, workspace, workspace_bytes, a.q, a.exchange, groups, s))
         return rc;
     if (rows == 0) return PXH_OK;
     dispatch_type(type, [&]<int T>() {
