@@ -55,8 +55,8 @@ __global__ __launch_bounds__(kBlock) void embedding_kernel(LookupArgs a)
 //   d[v] (+)= scale * the sum over the rows r with token[r] = v of dy[r], in the rows' order
 // The rows are sorted by token, those of one token in their own order; then every 4 to 32 consecutive ones are added up run by run, runs that go
 // on beyond those in a launch behind it, part after part.  No order depends on which workgroup comes first.
-// 16384 x 2048 bf16 into 32768 rows: sorting 11 us (with 48 MB of zeros), merging 5, sums and the other zeros 25 (153 MB at 6.2 TB/s), what goes
-// on from chunk to chunk 5; 59 us in all, with tensors that no cache holds (floor 31).  4099 x 1025 fp32 added to 10007 rows: places 7.5, sums
+// 16384 x 2048 bf16 into 32768 rows: sorting 11 us (with 64 MB of zeros), merging 5, sums and the other zeros 31 (137 MB at 4.4 TB/s), what goes
+// on from chunk to chunk 6; 53 us in all, with tensors that no cache holds (floor 31).  4099 x 1025 fp32 added to 10007 rows: places 7.5, sums
 // 9, chunk to chunk 6, 23 in all (floor 8): three launches, each a few trips to memory one behind the other.
 
 // -- zeros.  Sorting keeps a few units busy for some microseconds, in which the others write zeros to the table's last rows, whether
@@ -343,7 +343,7 @@ struct TableGradientArgs {
     int vocab, width, column_groups;
     float scale;
     bool accumulate;
-    bool past;                      // zeros past the caches
+    bool past;                      // rows, sums and zeros past the caches
 };
 
 // V values of a row of the gradient, as many of them as one access takes at a time.
@@ -361,6 +361,7 @@ struct TableRow {
     }
 
     // the row with scale * sum added to what it holds
+    template<bool NT>
     __device__ __forceinline__ void write(const TableGradientArgs& a, uint32_t token, int e, const float (&sum)[V])
     {
         char* const d = row_of<D>(a.d, token, a.d_stride);
@@ -372,7 +373,7 @@ struct TableRow {
 #pragma unroll
             for (int k = 0; k < kPart; ++k) x[k] = fmaf(a.scale, sum[q * kPart + k], x[k]);
             r[q].set(x);
-            store_row<D, kPart>(d, e + q * kPart, a.width, r[q]);
+            store_row<D, kPart, NT>(d, e + q * kPart, a.width, r[q]);
         }
     }
 };
@@ -382,7 +383,7 @@ struct TableRow {
 // kZeroRows rows of the table each, where no row has their token.
 constexpr int kZeroRows = 32;
 
-template<int T, int D, bool ADDS>
+template<int T, int D, bool ADDS, bool NT>
 __global__ __launch_bounds__(kBlock) void table_gradient_kernel(TableGradientArgs a, FastDiv by_columns)
 {
     constexpr int V = kVec<T>, kAhead = 8;
@@ -409,10 +410,7 @@ __global__ __launch_bounds__(kBlock) void table_gradient_kernel(TableGradientArg
             char* const d = row_of<D>(a.d, first + i, a.d_stride);
 #pragma unroll
             for (int q = 0; q < V; q += kPart)
-                if (e + q < a.width) {
-                    if (a.past) store_row<D, kPart, true>(d, e + q, a.width, Raw<D, kPart>{});
-                    else store_row<D, kPart>(d, e + q, a.width, Raw<D, kPart>{});
-                }
+                if (e + q < a.width) store_row<D, kPart, NT>(d, e + q, a.width, Raw<D, kPart>{});
         }
         return;
     }
@@ -434,7 +432,7 @@ __global__ __launch_bounds__(kBlock) void table_gradient_kernel(TableGradientArg
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             const int i = min(base + j, n - 1);
-            x[j] = load_row<T, V>(row_of<T>(a.dy, rows[i], a.dy_stride), e, a.width);
+            x[j] = load_row<T, V, NT>(row_of<T>(a.dy, rows[i], a.dy_stride), e, a.width);
             // what the run is added to, asked for with it
             if (ADDS && tokens[i + 2] != tokens[i + 1] && tokens[i + 1] < static_cast<uint32_t>(a.vocab)) old[ADDS ? j : 0].load(a, tokens[i + 1], e);
         }
@@ -453,7 +451,7 @@ __global__ __launch_bounds__(kBlock) void table_gradient_kernel(TableGradientArg
             if (token < static_cast<uint32_t>(a.vocab)) {
                 if (ends && !goes_on_from) {
                     if (!ADDS) old[0] = TableRow<D, V>{};
-                    old[ADDS ? j : 0].write(a, token, e, sum);
+                    old[ADDS ? j : 0].template write<NT && !ADDS>(a, token, e, sum);
                 } else {
                     float* const partial = a.partial + (static_cast<size_t>(part) * 2 + !goes_on_from) * a.width;
 #pragma unroll
@@ -534,24 +532,31 @@ __global__ __launch_bounds__(kJoinLanes) void table_join_kernel(TableGradientArg
         for (int k = 0; k < 4; ++k) sum[k] += sums[w][lane * 4 + k];
     TableRow<D, 4> d{};
     if (a.accumulate) d.load(a, token, e);
-    d.write(a, token, e, sum);
+    d.template write<false>(a, token, e, sum);
 }
 
-// What the machine writes while it sorts, from the table's end, whose tokens are the rare ones where they are numbered by their frequency (8192 x
-// 1024 bf16 into 131072 rows 71.1 us without, 64.0 so; 65536 x 512 into 32768 rows of fp32 65.6 and 60.9; but 16384 x 2048 into 32768 55.9 and
-// 60.8: there the sums leave the memory time for all zeros).
+// What the machine writes while it sorts, from the table's end, whose tokens are the rare ones where they are numbered by their frequency (16384 x
+// 2048 bf16 into 32768 rows 62 us without, 53 so; 65536 x 512 into 32768 rows of fp32 63 and 57).
 constexpr long long kZerosDuringSort = 64ll << 20;
 
 // Counted up to here, sorted in tiles and merged beyond: one launch for two, and work that grows with the square of the rows (64 rows 14.6 -> 9.5 us
 // for the whole call, 4099 27.5 -> 22.6, 7000 30.3 -> 28.2, but 8192 30.7 -> 32.4).
 constexpr uint32_t kMostRanked = 7168;
 
-// Rows of a run: as many as leave a workgroup for each, and kEnoughChunks of them where there are rows for that.
-constexpr size_t kEnoughChunks = 768;
-int run_of(long long rows)
+// Workgroups for the columns of a row.
+int column_groups_of(int width, int type)
+{
+    const int v = 16 / static_cast<int>(size_of(type)), vectors = (width + v - 1) / v;
+    return (vectors + kBlock - 1) / kBlock;
+}
+
+// Rows of a run: as few as still leave no more than kEnoughChunks workgroups, five to a unit (16384 x 2048 bf16 into 32768 rows with 1024 of
+// them 53 us, with 512 56; x 4096, where each takes half the columns, with 1024 92 and with 2048 97.  All of one token it costs: 73, and 61).
+constexpr size_t kEnoughChunks = 1280;
+int run_of(long long rows, int groups)
 {
     int run = kMostRun;
-    while (run > kLeastRun && (rows + run / 2 - 1) / (run / 2) <= static_cast<long long>(kEnoughChunks)) run /= 2;
+    while (run > kLeastRun && (rows + run / 2 - 1) / (run / 2) * groups <= static_cast<long long>(kEnoughChunks)) run /= 2;
     return run;
 }
 
@@ -576,13 +581,13 @@ int launch_gradient(const char* who, TableGradientArgs a, hipStream_t s)
 {
     // the vectors of a row in equal parts of at most kBlock (1025 fp32 values: 257 vectors are twice 192 lanes, not 256 and one)
     const int vectors = (a.width + kVec<T> - 1) / kVec<T>;
-    a.column_groups = (vectors + kBlock - 1) / kBlock;
     const int lanes = ((vectors + a.column_groups - 1) / a.column_groups + kWave - 1) / kWave * kWave;
     const long long zero_groups = (static_cast<long long>(a.open) + kZeroRows - 1) / kZeroRows;
     const long long groups = (a.chunks + zero_groups) * a.column_groups;
     if (groups * lanes >= 1ll << 32 || groups >= 1ll << 31) return fail_invalid("%s: too many rows of too many values", who);
     if (groups == 0) return PXH_OK;
-    const auto kernel = a.accumulate ? &table_gradient_kernel<T, D, true> : &table_gradient_kernel<T, D, false>;
+    const auto kernel = a.accumulate ? a.past ? &table_gradient_kernel<T, D, true, true> : &table_gradient_kernel<T, D, true, false>
+                        : a.past ? &table_gradient_kernel<T, D, false, true> : &table_gradient_kernel<T, D, false, false>;
     hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(groups)), dim3(lanes), 0, s, a, FastDiv(a.column_groups));
     if (int rc = check_launch(who)) return rc;
     if (a.chunks <= 1) return PXH_OK;
@@ -659,13 +664,15 @@ int pxh_embedding_backward(const void* dy, const void* tokens, void* d, int type
     a.dy_stride = dy_stride;
     a.d_stride = d_stride;
     a.count = static_cast<uint32_t>(rows);
-    a.run = run_of(rows);
+    a.column_groups = column_groups_of(width, type);
+    a.run = run_of(rows, a.column_groups);
     a.chunks = (a.count + a.run - 1) / a.run;
     a.vocab = vocab;
     a.width = width;
     a.scale = scale;
     a.accumulate = accumulate != 0;
-    a.past = static_cast<size_t>(vocab) * static_cast<size_t>(width) * size_of(d_type) >= kStreamingBytes;
+    // what is read and written does not fit the caches (131072 x 1024 bf16 into 50001 rows 133 us through them, 119 past them)
+    a.past = (static_cast<size_t>(rows) * size_of(type) + (accumulate ? 0 : static_cast<size_t>(vocab)) * size_of(d_type)) * static_cast<size_t>(width) >= kStreamingBytes;
     a.open = a.accumulate ? 0 : static_cast<uint32_t>(vocab);
     if (rows > 0) {
         const Space space(rows, width);
