@@ -57,6 +57,9 @@ __device__ __forceinline__ float gated(float h, float o)
     return y;
 }
 
+// What goes past the caches.
+enum { kNone, kResults, kAll };
+
 // Channels of a lane, four bytes of a row: 16 tokens of a few tensors and what is formed of them fit the registers.  And of a workgroup.
 template<int T>
 constexpr int kChannels = 4 / kSize<T>;
@@ -421,7 +424,7 @@ struct Columns {
 
 // The wave's tokens of a tensor, a word a lane; tokens behind the last row repeat it, channels behind the last one are zeros.  No
 // branch around a load: a lane at the end of a row reads the row's last word, and takes what is its own.
-template<int T, int STEPS>
+template<int T, int STEPS, bool NT>
 __device__ __forceinline__ void load_tokens(const void* p, long long stride, int first, int rows, const Columns& c, Raw<T, kChannels<T>> (&r)[STEPS])
 {
     constexpr int V = kChannels<T>;
@@ -433,14 +436,14 @@ __device__ __forceinline__ void load_tokens(const void* p, long long stride, int
         const uint32_t offset = static_cast<uint32_t>(c.e - c.tile_first) * kSize<T>;
 #pragma unroll
         for (int i = 0; i < STEPS; ++i) {
-            r[i] = load_raw_at<T, V>(row, offset);
+            r[i] = load_raw_at<T, V, NT>(row, offset);
             row += i < last ? step : 0;
         }
     } else if (c.width >= V) {
         const int at = min(c.e, c.width - V), beyond = c.e - at;
 #pragma unroll
         for (int i = 0; i < STEPS; ++i) {
-            r[i] = load_raw<T, V>(row, at);
+            r[i] = load_raw<T, V, NT>(row, at);
             row += i < last ? step : 0;
         }
 #pragma unroll
@@ -511,10 +514,10 @@ struct ScanArgs {
 
 // A workgroup takes a chunk of tokens of kTile channels, a wave a few of them, which stay in registers as z and x between the pass that finds
 // what they do to a state and the one that forms the states: one trip to memory.
-// 8 x 4096 x 2048 bf16 with a gate and what is saved 112 us (4.8 TB/s; a workgroup's 14 us are 1.4 for its number, 6.6 for its tokens, 5 for the
-// states in front of it and 1.5 for the rest; chunks that wait for none 103), without a gate 80 (5.0 TB/s); 30011 x 2561 half in 31 sequences
+// 8 x 4096 x 2048 bf16 with a gate and what is saved 111 us (4.8 TB/s; a workgroup's 14 us are 1.4 for its number, 6.6 for its tokens, 5 for the
+// states in front of it and 1.5 for the rest; chunks that wait for none 98), without a gate 80 (5.0 TB/s); 30011 x 2561 half in 31 sequences
 // 140 (rows that begin off a word's boundary, and tiles that share lines: 2560 values wide 112).
-template<int T, bool GATE, bool NT>
+template<int T, bool GATE, int PAST>
 __global__ __launch_bounds__(Forward::kLanes, 4) void scan_kernel(ScanArgs a)
 {
     constexpr int kSteps = Forward::kSteps, kChunk = Forward::kChunk, kV = kChannels<T>, kTile = kTileOf<T>;
@@ -527,9 +530,9 @@ __global__ __launch_bounds__(Forward::kLanes, 4) void scan_kernel(ScanArgs a)
     const int tile_first = static_cast<int>(place.tile) * kTile, e = tile_first + lane * kV;
     const Columns columns{ tile_first, e, a.width, tile_first + kTile <= a.width };
     Raw<T, kV> x[kSteps], u[kSteps], o[GATE ? kSteps : 1];
-    load_tokens<T, kSteps>(a.x, a.x_stride, first, a.q.rows, columns, x);
-    load_tokens<T, kSteps>(a.update, a.update_stride, first, a.q.rows, columns, u);
-    if constexpr (GATE) load_tokens<T, kSteps>(a.gate, a.gate_stride, first, a.q.rows, columns, o);
+    load_tokens<T, kSteps, PAST == kAll>(a.x, a.x_stride, first, a.q.rows, columns, x);
+    load_tokens<T, kSteps, PAST == kAll>(a.update, a.update_stride, first, a.q.rows, columns, u);
+    if constexpr (GATE) load_tokens<T, kSteps, PAST == kAll>(a.gate, a.gate_stride, first, a.q.rows, columns, o);
     const Whole whole = columns.inside ? within_one(a.q, kept, chunk_first, kChunk) : Whole{ false, false, false, 0 };
     const auto pass = [&]<bool RARE>() {
         Borders b{ 0, 0, Forward::kAll, 0 };
@@ -576,8 +579,8 @@ __global__ __launch_bounds__(Forward::kLanes, 4) void scan_kernel(ScanArgs a)
         for (int k = 0; k < kV; ++k) lds.ranges[wave][lane * kV + k] = Range{ begins_here || (RARE && b.begins) ? kWhole : Z[k], h[k] };
         join_waves<Forward::kGroup>(a.exchange, lds, place, a.width, wave, [](int w) { return w; }, h);
         as_read(x);
-        if (a.saved && first % kSaved == 0 && first < a.q.rows) store_state<NT>(a.saved, first / kSaved, e, a.width, h);
-        Writer<T, NT> y(a.y, a.y_stride, first, columns);
+        if (a.saved && first % kSaved == 0 && first < a.q.rows) store_state<PAST != kNone>(a.saved, first / kSaved, e, a.width, h);
+        Writer<T, PAST != kNone> y(a.y, a.y_stride, first, columns);
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             const bool begins = RARE && (b.begins >> i & 1), active = !RARE || (b.active >> i & 1);
@@ -609,7 +612,7 @@ __global__ __launch_bounds__(Forward::kLanes, 4) void scan_kernel(ScanArgs a)
 //   G[t] = dy * g + (1 - z[t + 1]) * G[t + 1], g = gate / (1 + exp(-gate));  dx = z G;  dupdate = G (x - h[t - 1]) z (1 - z)
 //   dgate = dy h s (1 + gate (1 - s)), s = 1 / (1 + exp(-gate))
 // Along the tokens from the saved states for h, then against them for G: the carry C = (1 - z) G goes through a range as a state does.
-// 8 x 4096 x 2048 bf16 with a gate 188 us (939 MB at 5.0 TB/s): half as many tokens to a workgroup as forward, for want of registers, and the
+// 8 x 4096 x 2048 bf16 with a gate 187 us (939 MB at 5.0 TB/s): half as many tokens to a workgroup as forward, for want of registers, and the
 // same waits.
 struct ScanBackwardArgs {
     const void* dy;
@@ -630,7 +633,7 @@ struct ScanBackwardArgs {
     int width;
 };
 
-template<int T, bool GATE, bool NT>
+template<int T, bool GATE, int PAST>
 __global__ __launch_bounds__(Backward::kLanes, 4) void scan_backward_kernel(ScanBackwardArgs a)
 {
     constexpr int kSteps = Backward::kSteps, kWaves = Backward::kWaves, kChunk = Backward::kChunk, kV = kChannels<T>, kTile = kTileOf<T>;
@@ -643,10 +646,10 @@ __global__ __launch_bounds__(Backward::kLanes, 4) void scan_backward_kernel(Scan
     const int tile_first = static_cast<int>(place.tile) * kTile, e = tile_first + lane * kV;
     const Columns columns{ tile_first, e, a.width, tile_first + kTile <= a.width };
     Raw<T, kV> x[kSteps], u[kSteps], dy[kSteps], o[GATE ? kSteps : 1];
-    load_tokens<T, kSteps>(a.update, a.update_stride, first, a.q.rows, columns, u);
-    load_tokens<T, kSteps>(a.x, a.x_stride, first, a.q.rows, columns, x);
-    load_tokens<T, kSteps>(a.dy, a.dy_stride, first, a.q.rows, columns, dy);
-    if constexpr (GATE) load_tokens<T, kSteps>(a.gate, a.gate_stride, first, a.q.rows, columns, o);
+    load_tokens<T, kSteps, PAST == kAll>(a.update, a.update_stride, first, a.q.rows, columns, u);
+    load_tokens<T, kSteps, PAST == kAll>(a.x, a.x_stride, first, a.q.rows, columns, x);
+    load_tokens<T, kSteps, PAST == kAll>(a.dy, a.dy_stride, first, a.q.rows, columns, dy);
+    if constexpr (GATE) load_tokens<T, kSteps, PAST == kAll>(a.gate, a.gate_stride, first, a.q.rows, columns, o);
     float h[kV];
     load_state(a.saved, first % kSaved == 0 && first < a.q.rows ? first / kSaved : -1, e, a.width, h);
     const Whole whole = columns.inside ? within_one(a.q, kept, chunk_first, kChunk) : Whole{ false, false, false, 0 };
@@ -718,7 +721,7 @@ __global__ __launch_bounds__(Backward::kLanes, 4) void scan_backward_kernel(Scan
                 }
             }
         }
-        Writer<T, NT> out(a.dgate, a.dgate_stride, first, columns);
+        Writer<T, PAST != kNone> out(a.dgate, a.dgate_stride, first, columns);
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             if (RARE) begin(i);
@@ -765,7 +768,7 @@ __global__ __launch_bounds__(Backward::kLanes, 4) void scan_backward_kernel(Scan
 #pragma unroll
         for (int k = 0; k < kV; ++k) lds.ranges[wave][lane * kV + k] = Range{ RARE && b.ends ? kWhole : Z[k], C[k] };
         join_waves<Backward::kGroup>(a.exchange, lds, place, a.width, kWaves - 1 - wave, [](int k) { return kWaves - 1 - k; }, C);
-        Writer<T, NT> out_x(a.dx, a.dx_stride, first + kSteps - 1, columns, true), out_u(a.dupdate, a.dupdate_stride, first + kSteps - 1, columns, true);
+        Writer<T, PAST != kNone> out_x(a.dx, a.dx_stride, first + kSteps - 1, columns, true), out_u(a.dupdate, a.dupdate_stride, first + kSteps - 1, columns, true);
 #pragma unroll
         for (int i = kSteps - 1; i >= 0; --i) {
             const bool ends = RARE && (b.ends >> i & 1), active = !RARE || (b.active >> i & 1);
@@ -840,17 +843,28 @@ __global__ __launch_bounds__(kBlock) void scan_step_kernel(StepArgs a)
 // ---------------------------------------------------------------- host
 size_t chunks_of(long long rows, int chunk) { return (static_cast<size_t>(rows) + chunk - 1) / chunk; }
 
+constexpr int kLine = 128;             // bytes
+
 // Words of chunks and groups: a segment of two chunks and more has half as many groups at most.
 size_t words_of(size_t chunks, int width) { return (chunks + chunks / 2 + 1) * static_cast<size_t>(width); }
 
 // The words' counter in front of them.
 constexpr size_t kCounterBytes = 256;
 
-// Whether `tensors` of the tokens' size do not fit the caches: then results are stored past them (8 x 4096 x 2048 bf16 without a gate, no
-// chunk waiting for another, 79 -> 61 us).
-bool streams(long long rows, int width, int type, int tensors)
+// What goes past the caches: nothing where `tensors` of the tokens' size fit them, else the results (8 x 4096 x 2048 bf16 without a gate, no chunk waiting for
+// another, 79 -> 61 us), and, where rows begin with lines, so that no line is read for two tiles, what is read (its gradients with a gate 194 -> 188 us,
+// 65536 x 1024 in one sequence 169 -> 167; rows that do not: 30080 x 2561 half 238 -> 244).
+int past_caches(long long rows, int width, int type, int tensors, long long strides)
 {
-    return static_cast<size_t>(rows) * static_cast<size_t>(width) * size_of(type) * tensors >= kStreamingBytes;
+    if (static_cast<size_t>(rows) * static_cast<size_t>(width) * size_of(type) * tensors < kStreamingBytes) return kNone;
+    return strides * static_cast<long long>(size_of(type)) % kLine ? kResults : kAll;
+}
+
+// pick(constant) for one of the two or three that a kernel is built for.
+template<typename F>
+auto for_past(int past, const F& pick)
+{
+    return past == kAll ? pick.template operator()<kAll>() : past == kResults ? pick.template operator()<kResults>() : pick.template operator()<kNone>();
 }
 
 int check_scan(const char* who, int type, long long rows, int width, int sequences, const int* starts, const int* slots, int slot_count, bool states)
@@ -933,9 +947,10 @@ int pxh_gated_scan_forward(const void* x, const void* update, const void* gate, 
     if (int rc = start_scan<Forward>(who, !gate, type, rows, width, sequences, starts, a.slots, state, final, workspace, workspace_bytes, a.q, a.exchange, groups, s)) return rc;
     if (rows == 0) return PXH_OK;
     dispatch_type(type, [&]<int T>() {
-        const bool past = streams(rows, width, type, gate ? 4 : 3);
-        const auto kernel = gate ? (past ? &scan_kernel<T, true, true> : &scan_kernel<T, true, false>)
-                                 : (past ? &scan_kernel<T, false, true> : &scan_kernel<T, false, false>);
+        // (without a gate what is read stays: 8 x 4096 x 2048 bf16 81 us, and 91)
+        const int past = past_caches(rows, width, type, gate ? 4 : 3, x_stride | update_stride | gate_stride);
+        const auto kernel = gate ? for_past(past, []<int PAST>() { return &scan_kernel<T, true, PAST>; })
+                                 : past != kNone ? &scan_kernel<T, false, kResults> : &scan_kernel<T, false, kNone>;
         hipLaunchKernelGGL(kernel, dim3(groups), dim3(Forward::kLanes), 0, s, a);
     });
     return check_launch(who);
@@ -962,9 +977,9 @@ int pxh_gated_scan_backward(const void* dy, const void* x, const void* update, c
         return rc;
     if (rows == 0) return PXH_OK;
     dispatch_type(type, [&]<int T>() {
-        const bool past = streams(rows, width, type, gate ? 7 : 5);
-        const auto kernel = gate ? (past ? &scan_backward_kernel<T, true, true> : &scan_backward_kernel<T, true, false>)
-                                 : (past ? &scan_backward_kernel<T, false, true> : &scan_backward_kernel<T, false, false>);
+        const int past = past_caches(rows, width, type, gate ? 7 : 5, x_stride | update_stride | dy_stride | (gate ? gate_stride : 0));
+        const auto kernel = gate ? for_past(past, []<int PAST>() { return &scan_backward_kernel<T, true, PAST>; })
+                                 : for_past(past, []<int PAST>() { return &scan_backward_kernel<T, false, PAST>; });
         hipLaunchKernelGGL(kernel, dim3(groups), dim3(Backward::kLanes), 0, s, a);
     });
     return check_launch(who);
