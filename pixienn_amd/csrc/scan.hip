@@ -45,16 +45,29 @@ __device__ __forceinline__ void gate_of(float u, float& z, float& rest)
     rest = z < 0.5f ? 1.0f - z : e * z;
 }
 
-// h times the gate's factor o s, rounded to fp32 before it is rounded to the type: the compiler would round some products to half at
-// once, and a step would not have the bits of the forward pass.
+// h times the gate's factor o s.
 template<int T>
 __device__ __forceinline__ float gated(float h, float o)
 {
     float s, rest;
     gate_of<T>(o, s, rest);
-    float y = h * (o * s);
-    if constexpr (T == PXH_F16) asm("" : "+v"(y));
-    return y;
+    return h * (o * s);
+}
+
+// A result, rounded to fp32 before it is rounded to the type: the compiler would round some products and sums to half at once, here and not there,
+// and a chunk at a row's end would not have the bits of the others, nor a step those of the forward pass.
+template<int T, int V>
+__device__ __forceinline__ Raw<T, V> result_of(const float (&x)[V])
+{
+    float v[V];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+        v[k] = x[k];
+        if constexpr (T == PXH_F16) asm("" : "+v"(v[k]));
+    }
+    Raw<T, V> r;
+    r.set(v);
+    return r;
 }
 
 // What goes past the caches.
@@ -486,8 +499,7 @@ struct Writer {
     template<bool RARE>
     __device__ __forceinline__ void put(bool active, const float (&v)[kV])
     {
-        Raw<T, kV> r;
-        r.set(v);
+        const Raw<T, kV> r = result_of<T>(v);
         if (!RARE || active) {
             if (!RARE || c.inside) store_raw_at<T, kV, NT>(row, static_cast<uint32_t>(c.e - c.tile_first) * kSize<T>, r);
             else if (c.e < c.width) store_row<T, kV, NT>(row, c.e, c.width, r);
@@ -835,9 +847,7 @@ __global__ __launch_bounds__(kBlock) void scan_step_kernel(StepArgs a)
 #pragma unroll
         for (int k = 0; k < V; ++k) h[k] = gated<T>(h[k], o[k]);
     }
-    Raw<T, V> r;
-    r.set(h);
-    store_row<T, V>(row_of<T>(a.y, row, a.y_stride), e, a.width, r);
+    store_row<T, V>(row_of<T>(a.y, row, a.y_stride), e, a.width, result_of<T>(h));
 }
 
 // ---------------------------------------------------------------- host

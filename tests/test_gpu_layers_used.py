@@ -187,3 +187,52 @@ def test_long_rows_of_beams_and_many_logits():
     want, at = (t[:beams] for t in last.flatten().sort(descending=True, stable=True))
     assert float((best[-1].double() - want).abs().max()) < 1e-5
     assert (parents[-1].long() * vocab + tokens[-1]).tolist() == at.tolist()
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("width,dtype", [(1664, torch.bfloat16), (1666, torch.float16), (832, torch.float32)])
+def test_scans_past_the_caches_are_those_of_fewer_channels(gated, ragged, width, dtype):
+    """Channels have nothing to do with each other: some of them by themselves, in a call that the caches hold, have the same bits."""
+    g = torch.Generator(device="cuda").manual_seed(8)
+    rows = 16384
+    make = lambda: torch.empty(rows, width, device="cuda", dtype=dtype).normal_(generator=g)  # noqa: E731
+    x, update, gate, dy = make(), make() - 3, make() if gated else None, make()
+    assert rows * width * x.element_size() * 3 >= 128 << 20
+    how = dict(starts=torch.tensor([0, 1, 77, 5000, 5000, 12345, rows - 40], device="cuda", dtype=torch.int32)) if ragged else dict(sequences=4)
+
+    def run(columns):
+        x_, u_, dy_ = (t[:, columns].contiguous() for t in (x, update, dy))
+        o_ = gate[:, columns].contiguous() if gated else None
+        y, dx, du = (torch.full_like(x_, 7.0) for _ in range(3))
+        do, saved = torch.full_like(x_, 7.0) if gated else None, ops.gated_scan_saved_like(x_)
+        ops.gated_scan_forward(x_, u_, y, gate=o_, saved=saved, **how)
+        ops.gated_scan_backward(dy_, x_, u_, saved, dx, du, gate=o_, dgate=do, **how)
+        return [t for t in (y, dx, du, do) if t is not None]
+
+    whole = run(slice(None))
+    for columns in (slice(0, 64), slice(width - 130, width)):
+        for a, b in zip(whole, run(columns)):
+            assert torch.equal(a[:, columns], b)
+
+
+@pytest.mark.parametrize("rows,vocab,width,out,accumulate", [(9000, 20000, 3584, torch.bfloat16, False), (40000, 3000, 2000, torch.float32, False),
+                                                             (40000, 30000, 1001, torch.float32, True), (40000, 30000, 1800, torch.bfloat16, True)])
+def test_table_gradients_past_the_caches(rows, vocab, width, out, accumulate):
+    g = torch.Generator(device="cuda").manual_seed(9)
+    dy = torch.empty(rows, width, device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    tokens = (torch.rand(rows, device="cuda", generator=g) ** 4 * (vocab + 3)).long()
+    assert (rows * 2 + (0 if accumulate else vocab * out.itemsize)) * width >= 128 << 20 or accumulate
+    d = torch.empty(vocab, width, device="cuda", dtype=out).normal_(generator=g) if accumulate else torch.full((vocab, width), 7.0, device="cuda", dtype=out)
+    was = d.clone() if accumulate else torch.zeros_like(d)
+    ops.embedding_backward(dy, tokens, d, 0.5, accumulate=accumulate)
+    for columns in (slice(0, 40), slice(width - 40, width)):
+        there = tokens < vocab
+        part, who = dy[there][:, columns].double(), tokens[there]
+        zeros = lambda: torch.zeros(vocab, part.shape[1], device="cuda", dtype=torch.float64)  # noqa: E731
+        total, size = zeros().index_add_(0, who, part) * 0.5, zeros().index_add_(0, who, part.abs()) * 0.5
+        count = torch.zeros(vocab, 1, device="cuda", dtype=torch.float64).index_add_(0, who, torch.ones(len(who), 1, device="cuda", dtype=torch.float64))
+        want = was[:, columns].double() + total
+        # a rounding of 2^-24 of what is there for each addition, and half a step of the type
+        bound = (count + 2) * 2.0 ** -24 * (size + was[:, columns].double().abs()) + want.abs() * torch.finfo(out).eps / 2
+        assert bool(((d[:, columns].double() - want).abs() <= bound).all())
