@@ -103,6 +103,7 @@ struct TokenArgs {
     long long rows, stride, d_stride;
     int vocab, wide, top;
     float scale;
+    float order_scale;      // what the logits are ordered times: the scale, or one, so that none meet in a rounded product
 };
 
 // The place of a row's token, -1 where none is given.
@@ -594,7 +595,7 @@ __global__ __launch_bounds__(LANES, K == kThirdVectors ? 6 : 1) void token_logpr
     }
     if (a.top) {
         // a lane of NaNs has minus infinity for its peak, which need not be a value of the row: no floor comes from there
-        const float peak = mine.peak * a.scale;
+        const float peak = mine.peak * a.order_scale;
         const auto put = [&](int place, unsigned long long key) {
             if (whole) {
                 a.top_ids[static_cast<long long>(row) * a.top + place] = static_cast<int>(~static_cast<uint32_t>(key));
@@ -604,10 +605,10 @@ __global__ __launch_bounds__(LANES, K == kThirdVectors ? 6 : 1) void token_logpr
             }
         };
         const int begin = mine.first * kVec<T>;
-        const auto largest = [&] { return mine.largest_key(a.scale); };
-        const auto above = [&](unsigned long long floor, const auto& f) { mine.above(a.scale, floor, f); };
-        const auto each = [&](const auto& f) { mine.each(logits, a.vocab, a.scale, f); };
-        const auto masked = [&](int i) { return key_of_masked(load_one<T>(logits, begin + i) * a.scale, begin + i); };
+        const auto largest = [&] { return mine.largest_key(a.order_scale); };
+        const auto above = [&](unsigned long long floor, const auto& f) { mine.above(a.order_scale, floor, f); };
+        const auto each = [&](const auto& f) { mine.each(logits, a.vocab, a.order_scale, f); };
+        const auto masked = [&](int i) { return key_of_masked(load_one<T>(logits, begin + i) * a.order_scale, begin + i); };
         select_largest<LANES, true>(a.top, mine.end(a.vocab) - begin, peak > -INFINITY ? order_of(peak) : 0u, largest, above, each, masked, put, selection);
     }
 }
@@ -681,7 +682,7 @@ __global__ __launch_bounds__(kBlock) void token_join_kernel(TokenArgs a, Parts p
                 if (key >> 32 >= floor >> 32) f(key);
             });
         };
-        const auto masked = [&](int i) { return key_of_masked(load_one<T>(logits, i) * a.scale, i); };
+        const auto masked = [&](int i) { return key_of_masked(load_one<T>(logits, i) * a.order_scale, i); };
         const auto put = [&](int place, unsigned long long key) {
             a.top_ids[row * a.top + place] = static_cast<int>(~static_cast<uint32_t>(key));
             a.top_logp[row * a.top + place] = result.logp(value_of(key));
@@ -1158,7 +1159,7 @@ int token_rows(const char* who, const void* logits, int type, long long rows, in
 {
     TokenArgs a{};
     a.logits = logits; a.top_logp = values; a.top_ids = ids; a.row_sums = sums; a.rows = rows; a.stride = stride; a.vocab = vocab;
-    a.top = top; a.scale = scale;
+    a.top = top; a.scale = scale; a.order_scale = 1.0f;
     int rc = PXH_OK;
     dispatch_type(type, [&]<int T>() { rc = by_rows(a, T, [&](const TokenArgs& p) { return launch_forward<T, false>(who, p, workspace, s); }); });
     return rc;
@@ -1193,7 +1194,7 @@ int pxh_token_logprobs_forward(const void* logits, const void* targets, float* l
     TokenArgs a{};
     a.logits = logits; a.targets = targets; a.logp = logp; a.entropy = entropy; a.lse = lse;
     a.top_logp = top_logp; a.top_ids = top_ids; a.rows = rows; a.stride = stride; a.vocab = vocab; a.wide = wide_targets;
-    a.top = top; a.scale = scale;
+    a.top = top; a.scale = a.order_scale = scale;
     hipStream_t s = as_stream(stream);
     int rc = PXH_OK;
     if (rows == 0) return PXH_OK;

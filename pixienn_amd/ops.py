@@ -1104,7 +1104,7 @@ def beam_select_workspace_bytes(batch, beams, vocab, count):
 def beam_select(logits, scores, out_scores, parents, tokens, ended=None, end_token=0, scale=1.0, workspace=None):
     """Of every item's beams the best continuations: scores [batch, beams] (fp32) plus the log probabilities of logits [batch * beams,
     vocab], times `scale`.  out_scores (fp32), parents (the beams) and tokens (int32) are [batch, count], descending, of equal ones
-    the lower beam's and the lower token first; -1 and minus infinity where there are fewer.  A beam that is ended ([batch, beams], bool)
+    the lower beam's, the larger logit's and the lower token first; -1 and minus infinity where there are fewer.  A beam that is ended ([batch, beams], bool)
     has one continuation: end_token, with the score that it has."""
     if _layer("pxh_beam_select", logits, scores, out_scores, parents, tokens, ended, end_token, scale, workspace):
         return
