@@ -757,7 +757,7 @@ int pxh_gated_scan_step(const void* x, const void* update, const void* gate, voi
  * descending; of equal ones the lower beam's first, in a beam the larger logit's, then the lower token.  logits: [batch * beams][vocab];
  * scores: [batch][beams], what the beams have come to.  A beam that is ended (nullable, [batch][beams], not 0) has one continuation,
  * end_token with the score that it has.  out_scores, parents (the beams) and tokens are [batch][count].  A score of minus infinity (a
- * masked token, a beam that is not there yet) and one that is no number (a beam whose logits hold a NaN or plus
+ * masked token, a beam that is not there yet, a sum below the fp32 numbers) and one that is no number (a beam whose logits hold a NaN or plus
  * infinity) are no continuations; the places for which there is none have a score of minus infinity, and -1 for parent and token.  Scores
  * are formed and compared in 64 bits, the logits times the scale too, from sums in fp32, and rounded once.  out_scores may be scores where
  * count is beams.

@@ -28,10 +28,10 @@ struct SelectArgs {
     float scale;
 };
 
-// One number that orders scores, 0 for what is no candidate: minus infinity and what is no number.
+// One number that orders scores, 0 for what is no candidate: minus infinity, as it is left or before, and what is no number.
 __device__ __forceinline__ unsigned long long order_of(double score)
 {
-    if (!(score > -INFINITY)) return 0;
+    if (!(static_cast<float>(score) > -INFINITY)) return 0;
     const unsigned long long bits = static_cast<unsigned long long>(__double_as_longlong(score + 0.0));
     return bits >> 63 ? ~bits : bits | 1ull << 63;
 }

@@ -89,3 +89,20 @@ def test_the_type_s_lowest_and_largest_values_times_a_scale(ops, vocab, dtype):
         # two of the largest share it
         assert tokens[1, :2].tolist() == [1, vocab - 1] and parents[1, :2].tolist() == [0, 0]
         assert bool(((best[1, :2] + 2.0 + math.log(2)).abs() < 124 * U).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("vocab", [5, 2500, 300000])
+@pytest.mark.parametrize("scale", [1.0, 1.3, 3e4])
+def test_what_is_left_as_minus_infinity_is_no_continuation(ops, vocab, dtype, scale):
+    """Beside two of the type's largest value the others have next to nothing: a number, or less than those of fp32 are."""
+    lowest, largest = torch.finfo(dtype).min, torch.finfo(dtype).max
+    logits = torch.full((1, vocab), lowest, dtype=dtype)
+    logits[0, 1], logits[0, vocab - 1] = largest, largest
+    below = (float(lowest) - float(largest)) * float(np.float32(scale))
+    third = float(torch.tensor(below - math.log(2) - 2.0, dtype=torch.float64).float())
+    there = third > -math.inf
+    assert there == (dtype is torch.float16)
+    best, parents, tokens = run(ops, logits, torch.tensor([[-2.0]]), 3, scale)
+    assert tokens[0].tolist() == [1, vocab - 1, 0 if there else -1] and parents[0].tolist() == [0, 0, 0 if there else -1]
+    assert float(best[0, 2]) == third
