@@ -576,25 +576,33 @@ struct Space {
     }
 };
 
+// Workgroups that add up the runs and write zeros, with their lanes, and those that put together what goes on from chunk to chunk.
+struct Grids {
+    long long sums, joins;
+    int lanes, join_columns;
+
+    Grids(const TableGradientArgs& a, int type)
+    {
+        // the vectors of a row in equal parts of at most kBlock (1025 fp32 values: 257 vectors are twice 192 lanes, not 256 and one)
+        const int v = 16 / static_cast<int>(size_of(type)), vectors = (a.width + v - 1) / v;
+        lanes = ((vectors + a.column_groups - 1) / a.column_groups + kWave - 1) / kWave * kWave;
+        sums = (a.chunks + (static_cast<long long>(a.open) + kZeroRows - 1) / kZeroRows) * a.column_groups;
+        join_columns = (a.width + kJoinColumns - 1) / kJoinColumns;
+        joins = a.chunks > 1 ? static_cast<long long>(a.chunks - 1) * join_columns : 0;
+    }
+    bool too_many() const { return sums * lanes >= 1ll << 32 || sums >= 1ll << 31 || joins * kJoinLanes >= 1ll << 32; }
+};
+
 template<int T, int D>
-int launch_gradient(const char* who, TableGradientArgs a, hipStream_t s)
+int launch_gradient(const char* who, TableGradientArgs a, const Grids& grids, hipStream_t s)
 {
-    // the vectors of a row in equal parts of at most kBlock (1025 fp32 values: 257 vectors are twice 192 lanes, not 256 and one)
-    const int vectors = (a.width + kVec<T> - 1) / kVec<T>;
-    const int lanes = ((vectors + a.column_groups - 1) / a.column_groups + kWave - 1) / kWave * kWave;
-    const long long zero_groups = (static_cast<long long>(a.open) + kZeroRows - 1) / kZeroRows;
-    const long long groups = (a.chunks + zero_groups) * a.column_groups;
-    if (groups * lanes >= 1ll << 32 || groups >= 1ll << 31) return fail_invalid("%s: too many rows of too many values", who);
-    if (groups == 0) return PXH_OK;
+    if (grids.sums == 0) return PXH_OK;
     const auto kernel = a.accumulate ? a.past ? &table_gradient_kernel<T, D, true, true> : &table_gradient_kernel<T, D, true, false>
                         : a.past ? &table_gradient_kernel<T, D, false, true> : &table_gradient_kernel<T, D, false, false>;
-    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(groups)), dim3(lanes), 0, s, a, FastDiv(a.column_groups));
+    hipLaunchKernelGGL(kernel, dim3(static_cast<uint32_t>(grids.sums)), dim3(grids.lanes), 0, s, a, FastDiv(a.column_groups));
     if (int rc = check_launch(who)) return rc;
-    if (a.chunks <= 1) return PXH_OK;
-    const int columns = (a.width + kJoinColumns - 1) / kJoinColumns;
-    const long long joins = static_cast<long long>(a.chunks - 1) * columns;
-    if (joins * kJoinLanes >= 1ll << 32) return fail_invalid("%s: too many rows of too many values", who);
-    hipLaunchKernelGGL((table_join_kernel<D>), dim3(static_cast<uint32_t>(joins)), dim3(kJoinLanes), 0, s, a, FastDiv(columns));
+    if (grids.joins == 0) return PXH_OK;
+    hipLaunchKernelGGL((table_join_kernel<D>), dim3(static_cast<uint32_t>(grids.joins)), dim3(kJoinLanes), 0, s, a, FastDiv(grids.join_columns));
     return check_launch(who);
 }
 
@@ -674,6 +682,19 @@ int pxh_embedding_backward(const void* dy, const void* tokens, void* d, int type
     // what is read and written does not fit the caches (131072 x 1024 bf16 into 50001 rows 133 us through them, 119 past them)
     a.past = (static_cast<size_t>(rows) * size_of(type) + (accumulate ? 0 : static_cast<size_t>(vocab)) * size_of(d_type)) * static_cast<size_t>(width) >= kStreamingBytes;
     a.open = a.accumulate ? 0 : static_cast<uint32_t>(vocab);
+    // zeros for a launch that takes some microseconds on a few units: `bytes` of them, from the rows that have none yet
+    const long long row_bytes = static_cast<long long>(width) * size_of(d_type), pieces = (row_bytes + 15) / 16;
+    const auto zeros = [&](long long bytes, int lanes) {
+        const long long some = bytes / row_bytes < a.open ? bytes / row_bytes : a.open;
+        a.open -= static_cast<uint32_t>(some);
+        return Zeros{ a.d, a.open, some, d_stride * static_cast<long long>(size_of(d_type)), row_bytes, FastDiv(static_cast<uint32_t>(pieces)),
+                      grid_for(static_cast<size_t>(some) * pieces, static_cast<size_t>(lanes) * kZeroPieces), a.past };
+    };
+    static_assert(kRankLanes == kSortLanes, "zeros are written by as many lanes");
+    const Zeros during = rows > 0 ? zeros(kZerosDuringSort, kSortLanes) : Zeros{};
+    // looked at before the first launch
+    const Grids grids(a, type);
+    if (grids.too_many()) return fail_invalid("%s: too many rows of too many values", who);
     if (rows > 0) {
         const Space space(rows, width);
         void* ws = nullptr;
@@ -683,16 +704,6 @@ int pxh_embedding_backward(const void* dy, const void* tokens, void* d, int type
         for (int i = 0; i < 4; ++i) lists[i] = reinterpret_cast<uint32_t*>(base + i * space.list);
         a.partial = reinterpret_cast<float*>(base + space.partial);
         const uint32_t tiles = (a.count + kTile - 1) / kTile;
-        // zeros for a launch that takes some microseconds on a few units: `bytes` of them, from the rows that have none yet
-        const long long row_bytes = static_cast<long long>(width) * size_of(d_type), pieces = (row_bytes + 15) / 16;
-        const auto zeros = [&](long long bytes, int lanes) {
-            const long long some = bytes / row_bytes < a.open ? bytes / row_bytes : a.open;
-            a.open -= static_cast<uint32_t>(some);
-            return Zeros{ a.d, a.open, some, d_stride * static_cast<long long>(size_of(d_type)), row_bytes, FastDiv(static_cast<uint32_t>(pieces)),
-                          grid_for(static_cast<size_t>(some) * pieces, static_cast<size_t>(lanes) * kZeroPieces), a.past };
-        };
-        static_assert(kRankLanes == kSortLanes, "zeros are written by as many lanes");
-        const Zeros during = zeros(kZerosDuringSort, kSortLanes);
         if (a.count <= kMostRanked) {
             const uint32_t groups = (a.count + kRanked - 1) / kRanked, share = (a.count + 4 * kShares - 1) / (4 * kShares) * 4;
             hipLaunchKernelGGL(rank_kernel, dim3(groups + during.groups), dim3(kRankLanes), share * kShares * sizeof(uint32_t), s, tokens, wide_tokens != 0,
@@ -725,8 +736,8 @@ int pxh_embedding_backward(const void* dy, const void* tokens, void* d, int type
     }
     int rc = PXH_OK;
     dispatch_type(type, [&]<int T>() {
-        if (d_type == T) rc = launch_gradient<T, T>(who, a, s);
-        else rc = launch_gradient<T, PXH_F32>(who, a, s);
+        if (d_type == T) rc = launch_gradient<T, T>(who, a, grids, s);
+        else rc = launch_gradient<T, PXH_F32>(who, a, grids, s);
     });
     return rc;
 }
