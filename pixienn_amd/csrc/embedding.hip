@@ -55,6 +55,8 @@ __global__ __launch_bounds__(kBlock) void embedding_kernel(LookupArgs a)
 //   d[v] (+)= scale * the sum over the rows r with token[r] = v of dy[r], in the rows' order
 // The rows are sorted by token, those of one token in their own order; then every 4 to 32 consecutive ones are added up run by run, runs that go
 // on beyond those in a launch behind it, part after part.  No order depends on which workgroup comes first.
+// What comes out of the workspace is looked at before it is a place: where another call writes to the same one at the same time, which the
+// interface forbids, the results have no meaning, but nothing beyond the tensors and the workspace is touched.
 // 16384 x 2048 bf16 into 32768 rows: sorting 11 us (with 64 MB of zeros), merging 5, sums and the other zeros 31 (137 MB at 4.4 TB/s), what goes
 // on from chunk to chunk 6; 53 us in all, with tensors that no cache holds (floor 31).  4099 x 1025 fp32 added to 10007 rows: places 7.5, sums
 // 9, chunk to chunk 6, 23 in all (floor 8): three launches, each a few trips to memory one behind the other.
@@ -290,6 +292,7 @@ __global__ __launch_bounds__(kMergeLanes) void merge_tiles_kernel(const uint32_t
     uint32_t place = first * kTile + (i - own * kTile);
 #pragma unroll
     for (int k = 0; k < kParts; ++k) place += counts[k][threadIdx.x];
+    if (place >= count) return;             // lists that another call writes
     out_tokens[place] = token;
     out_rows[place] = row;
 }
@@ -323,6 +326,7 @@ __global__ __launch_bounds__(kBlock) void merge_large_kernel(const uint32_t* tok
     uint32_t place = first * tile + (i - own * tile);
 #pragma unroll
     for (int j = 0; j < kFanIn; ++j) place += low[j];
+    if (place >= count) return;             // lists that another call writes
     out_tokens[place] = token;
     out_rows[place] = rows[i];
 }
@@ -420,7 +424,7 @@ __global__ __launch_bounds__(kBlock) void table_gradient_kernel(TableGradientArg
     for (int i = threadIdx.x; i < a.run + 2; i += blockDim.x) {
         const long long at = static_cast<long long>(first) + i - 1;
         tokens[i] = at >= 0 && at < a.count ? a.tokens[at] : kNoToken;
-        if (i >= 1 && i <= n) rows[i - 1] = a.rows[at];
+        if (i >= 1 && i <= n) rows[i - 1] = min(a.rows[at], a.count - 1);
     }
     __syncthreads();
     if (e >= a.width) return;
