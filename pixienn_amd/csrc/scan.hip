@@ -890,12 +890,19 @@ int check_scan(const char* who, int type, long long rows, int width, int sequenc
     return PXH_OK;
 }
 
-// Sequences of the call, and the words that its chunks exchange (none where every chunk begins and ends with a sequence).  side_by_side: sequences
-// as segments, where they can be.  Most calls win by it (the gradients of 8 x 4096 x 2048 bf16 with a gate 198 -> 189 us, of 65536 x 256 in 16
-// sequences 61 -> 53; forward without a gate 84 -> 81), but forward with a gate those lose whose sequences lie 16 MB apart, which meet in the same
-// banks: 8 x 4096 x 2048 116 -> 127, 16 of them 203 -> 217, where 32 x 1024 x 2048 has 107 and 106, 8 x 8192 x 2048 206 and 197.
+// Distances that sequences side by side are kept away from, of rows and of sequences.
+constexpr long long kRowsApart = 4096, kSequencesApart = 8 << 20;
+
+// Sequences of the call, and the words that its chunks exchange (none where every chunk begins and ends with a sequence).  Sequences of one
+// length and of whole chunks are segments, side by side: gradients of 8 x 4096 x 2048 bf16 with a gate 195 -> 184 us, without 154 -> 136, forward without one
+// 83.8 -> 81.8, with one 8 x 3968 x 2048 107 -> 102.5, 8 x 4224 x 2048 113 -> 108, 16 x 4096 x 1024 117 -> 107, 64 x 512 x 2048 108 -> 100.  Not so forward with a
+// gate where rows lie multiples of 4 kB apart and sequences multiples of 8 MB (`row_bytes`, the distances of the rows that are read, or-ed; 0 where that does not
+// matter): 8 x 4096 x 2048 112 -> 116, 16 x 2048 x 2048 109 -> 117, 16 x 2048 x 4096 197 -> 224, 8 x 4096 x 1024 fp32 104 -> 114, columns of a product three times as
+// wide 111 -> 116.  There they go one behind the other, which costs the longer ones of such distances some (8 x 8192 x 2048 194 -> 203).  The gradients have no such
+// distance: of 36 shapes four lose more than 5 % by it (8 x 2048 x 2048 fp32 177 -> 202, without a gate 134 -> 157), and others at the same distance win as much.
+// Where groups of chunks begin with sequences either way, the bits are the same either way: rows at another distance have the same results.
 template<typename S>
-int start_scan(const char* who, bool side_by_side, int type, long long rows, int width, int sequences, const int* starts, const Slots& slots, const float* from, float* to,
+int start_scan(const char* who, long long row_bytes, int type, long long rows, int width, int sequences, const int* starts, const Slots& slots, const float* from, float* to,
                void* workspace, size_t workspace_bytes, Sequences& q, Exchange& x, uint32_t& groups, hipStream_t s)
 {
     const long long length = starts || sequences == 0 ? 0 : rows / sequences;
@@ -904,7 +911,8 @@ int start_scan(const char* who, bool side_by_side, int type, long long rows, int
     const size_t chunks = chunks_of(rows, kChunk), tile = 4 / size_of(type) * kWave, tiles = (static_cast<size_t>(width) + tile - 1) / tile;
     if (chunks * tiles * S::kLanes >= 1ull << 32) return fail_invalid("%s: too many rows of too many values", who);
     groups = static_cast<uint32_t>(chunks * tiles);
-    const bool apart = side_by_side && length > 0 && length % kChunk == 0 && sequences > 1;
+    const bool meet = row_bytes && row_bytes % kRowsApart == 0 && length * row_bytes % kSequencesApart == 0 && length % (kChunk * S::kGroup) == 0;
+    const bool apart = !meet && length > 0 && length % kChunk == 0 && sequences > 1;
     const size_t segments = apart ? sequences : 1, per = chunks / segments, groups_per = (per + S::kGroup - 1) / S::kGroup;
     x = Exchange{ nullptr, nullptr, nullptr, static_cast<uint32_t>(per), static_cast<uint32_t>(groups_per), FastDiv(static_cast<uint32_t>(tiles)),
                   FastDiv(static_cast<uint32_t>(segments)) };
@@ -954,7 +962,8 @@ int pxh_gated_scan_forward(const void* x, const void* update, const void* gate, 
     ScanArgs a{ x, update, gate, y, state, final, saved, x_stride, update_stride, gate_stride, y_stride, {}, Slots{ slots, slot_count }, {}, width };
     uint32_t groups;
     hipStream_t s = as_stream(stream);
-    if (int rc = start_scan<Forward>(who, !gate, type, rows, width, sequences, starts, a.slots, state, final, workspace, workspace_bytes, a.q, a.exchange, groups, s)) return rc;
+    const long long row_bytes = gate ? (x_stride | update_stride | gate_stride) * static_cast<long long>(size_of(type)) : 0;
+    if (int rc = start_scan<Forward>(who, row_bytes, type, rows, width, sequences, starts, a.slots, state, final, workspace, workspace_bytes, a.q, a.exchange, groups, s)) return rc;
     if (rows == 0) return PXH_OK;
     dispatch_type(type, [&]<int T>() {
         // (without a gate what is read stays: 8 x 4096 x 2048 bf16 81 us, and 91)
@@ -983,7 +992,7 @@ int pxh_gated_scan_backward(const void* dy, const void* x, const void* update, c
                         dx_stride, dupdate_stride, dgate_stride, {}, Slots{ slots, slot_count }, {}, width };
     uint32_t groups;
     hipStream_t s = as_stream(stream);
-    if (int rc = start_scan<Backward>(who, true, type, rows, width, sequences, starts, a.slots, d_final, d_state, workspace, workspace_bytes, a.q, a.exchange, groups, s))
+    if (int rc = start_scan<Backward>(who, 0, type, rows, width, sequences, starts, a.slots, d_final, d_state, workspace, workspace_bytes, a.q, a.exchange, groups, s))
         return rc;
     if (rows == 0) return PXH_OK;
     dispatch_type(type, [&]<int T>() {
