@@ -10,8 +10,8 @@ namespace {
 // are found row by row (as the alternatives of a token), and a workgroup for each item puts its beams' together.  Scores are formed and compared
 // in 64 bits from the logits as they are, so that in a beam the larger logit always comes first; a beam's sum of exponentials is of fp32, and
 // continuations of different beams that are nearer than its error (some vocab / 64 roundings) may change places.
-// The rows' launch is bound by the logits (512 x 50001 half 16 us, 3.2 TB/s), this one by its trips to memory, ids, then logits: 5.3 us for 64
-// items of 8 beams with 8 continuations, 3.1 for one of 4 with 4.
+// The rows' launch is bound by the logits (512 x 50001 half 16.5 us, 3.1 TB/s), this one by its trips to memory, ids, then logits: 5.2 us for 64
+// items of 8 beams with 8 continuations, 3.2 for one of 4 with 4.
 constexpr int kMostBeams = 64;
 
 struct SelectArgs {

@@ -17,7 +17,7 @@ __device__ __forceinline__ uint32_t token_at(const void* tokens, bool wide, long
 // ---------------------------------------------------------------- forward
 //   y[r] = scale * table[token[r]], zeros for a token outside the vocabulary
 // A vector a lane, rows one behind the other: bound by what is written and by the table's rows that the caches do not hold.  16384 x 4096
-// bf16 of a text's tokens 30.4 us: 134 MB written and the rows of a table of 410 MB read, the frequent ones once (268 MB, at 8.8 TB/s).
+// bf16 of a text's tokens 30.4 us: 134 MB written and 76 MB read, a row of the table once however many places have its token (7.0 TB/s).
 struct LookupArgs {
     const char* table;
     const void* tokens;
@@ -57,9 +57,9 @@ __global__ __launch_bounds__(kBlock) void embedding_kernel(LookupArgs a)
 // on beyond those in a launch behind it, part after part.  No order depends on which workgroup comes first.
 // What comes out of the workspace is looked at before it is a place: where another call writes to the same one at the same time, which the
 // interface forbids, the results have no meaning, but nothing beyond the tensors and the workspace is touched.
-// 16384 x 2048 bf16 into 32768 rows: sorting 11 us (with 64 MB of zeros), merging 5, sums and the other zeros 31 (137 MB at 4.4 TB/s), what goes
-// on from chunk to chunk 6; 53 us in all, with tensors that no cache holds (floor 31).  4099 x 1025 fp32 added to 10007 rows: places 7.5, sums
-// 9, chunk to chunk 6, 23 in all (floor 8): three launches, each a few trips to memory one behind the other.
+// 16384 x 2048 bf16 into 32768 rows: sorting 11.5 us (with 64 MB of zeros), merging 5.3, sums and the other zeros 29.6 (153 MB at 5.2 TB/s), what
+// goes on from chunk to chunk 7.5; 53 us in all, with tensors that no cache holds (floor 31).  4099 x 1025 fp32 added to 10007 rows: places 7.6,
+// sums 9.6, chunk to chunk 5.7, 23 in all (floor 8): three launches, each a few trips to memory one behind the other.
 
 // -- zeros.  Sorting keeps a few units busy for some microseconds, in which the others write zeros to the table's last rows, whether
 // a row has their token or not; the rows in front of those wait for the sums, which know which of them have none.
@@ -142,7 +142,7 @@ __global__ __launch_bounds__(kRankLanes) void rank_kernel(const void* tokens, bo
 }
 
 // Bitonic sorting of 2048 keys, two to a lane: the token above the place in the tile, all of them different.  66 steps one behind the
-// other, of which 51 stay in a wave: 8 us, whatever the number of tiles.
+// other, of which 56 stay in a wave: 11.5 us with the zeros beside it, whatever the number of tiles.
 template<typename Key>
 __device__ __forceinline__ void compare(Key& a, Key& b, bool up)
 {
@@ -475,7 +475,7 @@ __global__ __launch_bounds__(kBlock) void table_gradient_kernel(TableGradientArg
 }
 
 // The runs that go on beyond a chunk, by the workgroup of the chunk in which they begin: 256 columns to a workgroup, whose waves share
-// the chunks.  Most chunks have none: 5 us, a launch and two trips to memory (where all of 16384 rows
+// the chunks.  Most chunks have none: 7.5 us of 16384 x 2048, 5.7 of 4099 x 1025, a launch and two trips to memory (where all of 16384 rows
 // have one token the call takes 10 us more).
 constexpr int kJoinLanes = 256, kJoinColumns = 256;
 

@@ -73,8 +73,9 @@ struct Weights {
 // lane stay in registers from the sum over the squares of what is left without the mean (not a difference of two sums, which loses what a
 // large mean leaves of the digits) to the result; up to two of them with their weights, asked for with the row.  K == 0: a row of any
 // width, which is read three times.
-// Bound by the memory, and by a launch where there is little of it: 2111 x 5001 fp32 with a bias 15.8 us (84 MB at 5.3 TB/s; row ends value by
-// value 19.8), 8000 x 5001 60 (5.4 TB/s), 16 x 4096 bf16 with residual and bias 4.5.
+// Bound by the memory, and by a launch where there is little of it: 16384 x 4096 bf16 with residual and bias 91 us (537 MB at 5.9 TB/s), without a
+// residual 50 (5.3 TB/s); 2111 x 5001 fp32 with a bias 17.1, of which the kernel is 15.7 (85 MB at 5.4 TB/s; with row ends value by value it
+// was 4 more), 16 x 4096 bf16 with residual and bias 4.5.
 template<int T, bool WIDE, bool SHARED, int K, bool NT>
 __global__ __launch_bounds__(SHARED ? kMostWaves * kWave : kBlock) void layer_norm_kernel(LayerNormArgs a)
 {
@@ -293,7 +294,7 @@ __device__ __forceinline__ float2 two_sums(float a, float b, float2* slot)
 
 // dx of every row, and the part of dw and db that this worker's rows give: a worker (a wave, or a workgroup) takes every workers-th row, and
 // asks for the next one before it waits for the sums over this one.  Bound by the memory: 16384 x 4096 bf16 with dsum, dw and db 90.5 us with the
-// sums behind it (537 MB at 5.9 TB/s), 2048 x 16384 58 (4.6 TB/s: sixteen waves wait for one sum, and none is loaded ahead).
+// sums behind it (546 MB with the workers' sums, at 6.0 TB/s), 2048 x 16384 58 (4.6 TB/s: sixteen waves wait for one sum, and none is loaded ahead).
 template<int T, bool WIDE, bool SHARED, int K, bool NT>
 __global__ __launch_bounds__(SHARED ? kMostWaves * kWave : kBlock) void layer_norm_backward_kernel(LayerNormBackwardArgs a, int workers)
 {
@@ -429,7 +430,8 @@ __global__ __launch_bounds__(SHARED ? kMostWaves * kWave : kBlock) void layer_no
     }
 }
 
-// Rows of any width: dx alone, the row is read twice (1024 x 32768 bf16 with dsum 92 us, at 2.9 TB/s).
+// Rows of any width: dx alone, the row is read twice (1024 x 32768 bf16 with dsum 58 us, 405 MB at 7.0 TB/s, some of it from the caches; with the
+// sums in front of it, 29, and behind it, 5, the call takes 103 with tensors that no cache holds).
 template<int T>
 __global__ __launch_bounds__(1024) void layer_norm_backward_wide_kernel(LayerNormBackwardArgs a, long long first)
 {

@@ -526,9 +526,10 @@ struct ScanArgs {
 
 // A workgroup takes a chunk of tokens of kTile channels, a wave a few of them, which stay in registers as z and x between the pass that finds
 // what they do to a state and the one that forms the states: one trip to memory.
-// 8 x 4096 x 2048 bf16 with a gate and what is saved 111 us (4.8 TB/s; a workgroup's 14 us are 1.4 for its number, 6.6 for its tokens, 5 for the
-// states in front of it and 1.5 for the rest; chunks that wait for none 98), without a gate 80 (5.0 TB/s); 30011 x 2561 half in 31 sequences
-// 140 (rows that begin off a word's boundary, and tiles that share lines: 2560 values wide 112).
+// 8 x 4096 x 2048 bf16 with a gate and what is saved 111 us: 108 in this kernel, in which 578 MB move (5.4 TB/s) and the vector units have work for
+// 53; of sequences of 256 tokens, where a chunk waits for one other at most, 99.  Without a gate 91, and 82 where the caches hold some of it
+// from the call before.  30011 x 2561 half in 31 sequences 142: 618 MB where 461 would do, for the lines that two tiles share, as rows begin
+// off them (2560 values wide 112).  75 scalar registers (53 in fp32) are kept in lanes of vector registers; what that costs is not known.
 template<int T, bool GATE, int PAST>
 __global__ __launch_bounds__(Forward::kLanes, 4) void scan_kernel(ScanArgs a)
 {
@@ -624,8 +625,8 @@ __global__ __launch_bounds__(Forward::kLanes, 4) void scan_kernel(ScanArgs a)
 //   G[t] = dy * g + (1 - z[t + 1]) * G[t + 1], g = gate / (1 + exp(-gate));  dx = z G;  dupdate = G (x - h[t - 1]) z (1 - z)
 //   dgate = dy h s (1 + gate (1 - s)), s = 1 / (1 + exp(-gate))
 // Along the tokens from the saved states for h, then against them for G: the carry C = (1 - z) G goes through a range as a state does.
-// 8 x 4096 x 2048 bf16 with a gate 187 us (939 MB at 5.0 TB/s): half as many tokens to a workgroup as forward, for want of registers, and the
-// same waits.
+// 8 x 4096 x 2048 bf16 with a gate 189 us: 183 in this kernel, in which 993 MB move (5.4 TB/s) and the vector units have work for 99.  Half as many
+// tokens to a workgroup as forward, for want of registers, and the same waits.  30011 x 2561 half in 31 sequences 255: 1056 MB where 788 would do.
 struct ScanBackwardArgs {
     const void* dy;
     const void* x;
@@ -899,7 +900,7 @@ constexpr long long kRowsApart = 4096, kSequencesApart = 8 << 20;
 // gate where rows lie multiples of 4 kB apart and sequences multiples of 8 MB (`row_bytes`, the distances of the rows that are read, or-ed; 0 where that does not
 // matter): 8 x 4096 x 2048 112 -> 116, 16 x 2048 x 2048 109 -> 117, 16 x 2048 x 4096 197 -> 224, 8 x 4096 x 1024 fp32 104 -> 114, columns of a product three times as
 // wide 111 -> 116.  There they go one behind the other, which costs the longer ones of such distances some (8 x 8192 x 2048 194 -> 203).  The gradients have no such
-// distance: of 36 shapes four lose more than 5 % by it (8 x 2048 x 2048 fp32 177 -> 202, without a gate 134 -> 157), and others at the same distance win as much.
+// distance: of 71 shapes one loses more than 5 % with a gate (8 x 2048 x 2048 fp32 177 -> 202) and four without, and others at the same distances win as much.
 // Where groups of chunks begin with sequences either way, the bits are the same either way: rows at another distance have the same results.
 template<typename S>
 int start_scan(const char* who, long long row_bytes, int type, long long rows, int width, int sequences, const int* starts, const Slots& slots, const float* from, float* to,
